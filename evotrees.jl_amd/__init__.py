@@ -19,9 +19,11 @@ import numpy as np
 
 from . import _lib
 from ._lib import EvtError, Handle, TreeArrays, make_params, splitmix_mask  # noqa: F401
+from .class_losses import class_logp, class_logp_grad, distill_loss, policy_loss, preference_loss
 
 __all__ = ["EvoTreeRegressor", "EvoTreeCount", "EvoTreeClassifier", "EvoTreeMLE", "EvoTree", "Tree", "fit", "predict", "predict_leaf_idx", "init",
-           "grow_evotree", "update", "okay_to_continue", "get_edges", "get_edges_table", "binarize_table", "check_args", "CallBack", "init_logger", "update_logger", "EvtError"]
+           "grow_evotree", "update", "okay_to_continue", "get_edges", "get_edges_table", "binarize_table", "check_args", "CallBack", "init_logger", "update_logger", "EvtError",
+           "class_logp", "class_logp_grad", "distill_loss", "policy_loss", "preference_loss"]
 
 _GPU_DEVICES = ("gpu", "rocm", "amd", "hip")
 _EXP_LINK = ("poisson", "gamma", "tweedie")

@@ -31,6 +31,7 @@ EXPORTS = [
     "evt_set_option", "evt_synchronize", "evt_copy_bandwidth", "evt_read_bandwidth", "evt_predict_static",
     "evt_lds_atomic_rate", "evt_global_atomic_rate", "evt_trim", "evt_binarize", "evt_bin_columns", "evt_order_stats",
     "evt_model_create", "evt_model_destroy", "evt_model_predict",
+    "evt_class_logp", "evt_class_logp_grad", "evt_distill_loss", "evt_policy_loss", "evt_preference_loss",
 ]
 
 
@@ -48,6 +49,11 @@ class EvtParams(C.Structure):
 class EvtTreeOut(C.Structure):
     _fields_ = [("feat", C.c_void_p), ("cond_bin", C.c_void_p), ("w", C.c_void_p), ("gain", C.c_void_p),
                 ("pred", C.c_void_p), ("split", C.c_void_p)]
+
+
+class EvtScores(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("row_stride", C.c_int64), ("grad", C.c_void_p), ("grad_stride", C.c_int64), ("nrows", C.c_int64),
+                ("nclass", C.c_int32), ("dtype", C.c_int32), ("temperature", C.c_double)]
 
 
 _lib = None
@@ -117,6 +123,11 @@ def load():
         "evt_read_bandwidth": [i64, i32, vp],
         "evt_lds_atomic_rate": [i32, i32, i32, vp, vp],
         "evt_global_atomic_rate": [i32, i32, i32, vp],
+        "evt_class_logp": [vp, C.POINTER(EvtScores), vp, i32, vp, vp, i32],
+        "evt_class_logp_grad": [vp, C.POINTER(EvtScores), vp, i32, vp, vp, i32],
+        "evt_distill_loss": [vp, C.POINTER(EvtScores), vp, i32, vp, i32, i32, vp, vp, i32],
+        "evt_policy_loss": [vp, C.POINTER(EvtScores), vp, i32, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, vp, vp, i32],
+        "evt_preference_loss": [vp, C.POINTER(EvtScores), vp, i32, vp, i32, vp, vp, C.c_double, C.c_double, C.c_double, i32, vp, vp, vp, i32],
         "evt_predict_static": [vp, i64, i32, vp, vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, i32, vp, vp],
     }
     for name, args in sigs.items():

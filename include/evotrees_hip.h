@@ -89,7 +89,8 @@ enum {
 enum { EVT_TREE_BINARY = 0, EVT_TREE_OBLIVIOUS = 1 };
 
 /* element types of a feature matrix (the first two) and of a table's column */
-enum { EVT_F32 = 0, EVT_F64 = 1, EVT_I8 = 2, EVT_I16 = 3, EVT_I32 = 4, EVT_I64 = 5, EVT_U8 = 6, EVT_U16 = 7, EVT_U32 = 8, EVT_U64 = 9 };
+enum { EVT_F32 = 0, EVT_F64 = 1, EVT_I8 = 2, EVT_I16 = 3, EVT_I32 = 4, EVT_I64 = 5, EVT_U8 = 6, EVT_U16 = 7, EVT_U32 = 8, EVT_U64 = 9,
+       EVT_BF16 = 10, EVT_F16 = 11 /* class scores only (evt_scores) */ };
 
 /* A column of a table in host memory: row i at data + i * stride bytes (a Bool column is EVT_U8). */
 typedef struct {
@@ -385,6 +386,66 @@ int evt_predict_static(void *stream, int64_t nobs, int32_t nfeats, const uint8_t
                        int32_t loss, int32_t K, int32_t ntrees, int64_t total_nodes, const int64_t *tree_off_dev,
                        const int64_t *feat_dev, const uint8_t *cond_bin_dev, const float *pred_dev, const uint8_t *split_dev,
                        int32_t apply_link, float *out_dev, int32_t *status_dev);
+
+/* ---- losses over rows of class scores ---------------------------------------------------
+ * No counterpart in the reference, whose mlogloss takes one label a row: what a model of many classes trains on beside it - a language
+ * model's tokens (thousands of classes) as well as a classifier's rows.  Stateless and device-only, as evt_predict_static is: every pointer is
+ * device memory on the device that is current on the calling thread, the work is queued on `stream` and the call returns without waiting; nothing is
+ * allocated, copied or synchronised, so calls may overlap and be captured.  The pointers' memory types are queried unless flags holds EVT_STATIC_TRUSTED.
+ *
+ * With z = x / temperature, q = softmax(z) over a row's nclass scores and log q its logarithm:
+ *  - Scores are EVT_F32, EVT_BF16 or EVT_F16, a row's side by side, rows row_stride elements apart (any alignment; 0: one row for all).
+ *    Differences, exponentials and sums are 32-bit, losses 64-bit until they are written; a gradient is rounded once, to the scores' type.
+ *  - A score of -inf is a class that cannot be: q = 0, no gradient through it.  A row of nothing else has log q = -inf and q = 0 everywhere.
+ *    A NaN or +inf makes its row's results NaN, and no other's.
+ *  - Labels and ids count from 0 (EVT_I32 or EVT_I64).  A negative label leaves its row out: loss, logp and gradient are 0 and the row is not read.
+ *    One of nclass or more makes the row's results NaN.  A row of weight 0 has no loss and no gradient, whatever its scores.
+ *  - grad NULL: no gradient.  It may be the scores' own memory (grad == x with equal strides; each row is read before it is written); elsewhere
+ *    it must not overlap them.  Elements between nclass and grad_stride stay as they are.
+ *  - Results do not depend on the grid or the order of blocks: equal calls give equal bits. */
+typedef struct {
+    const void *x;       /* nrows x nclass scores */
+    int64_t row_stride;
+    void *grad;          /* of x's type, or NULL */
+    int64_t grad_stride; /* >= nclass */
+    int64_t nrows;       /* 0 .. 2^31 - 1; 0: the call does nothing */
+    int32_t nclass;      /* >= 1 */
+    int32_t dtype;
+    double temperature;  /* > 0 */
+} evt_scores;
+
+/* logp[i] = log q[i, labels[i]], and stats[2 i], stats[2 i + 1] = the row's maximum of x and sum of exp((x - maximum) / temperature) (both 0
+ * for a row left out), which the gradient takes: grad[i, :] = dlogp[i] (onehot(labels[i]) - q[i, :]) / temperature.  A row with dlogp 0 is not read. */
+int evt_class_logp(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, float *logp, float *stats, int32_t flags);
+int evt_class_logp_grad(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const float *stats, const float *dlogp,
+                        int32_t flags);
+
+/* Distillation from a teacher that kept its n_top best classes of each row (1 .. 1024): top_ids and top_scores are nrows x n_top, an id below 0 is no
+ * entry, and an id may come twice.  With p = softmax(top_scores / temperature) over a row's entries and w = weights[i] (NULL: 1):
+ *   loss[i] = w temperature^2 sum_j p_j (log p_j - log q[id_j]),   grad[i, c] = w temperature (q_c - sum of p_j with id_j == c).
+ * A row without entries, or with none above -inf, is left out. */
+int evt_distill_loss(void *stream, const evt_scores *s, const void *top_ids, int32_t id_dtype, const void *top_scores, int32_t top_dtype,
+                     int32_t n_top, const float *weights, float *loss, int32_t flags);
+
+/* The clipped policy loss of every token: with r = exp(logp - old_logp), A = advantages[i], b = ref_logp - logp and w = weights[i] (NULL: 1),
+ *   loss[i] = w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(b) - b - 1)),
+ *   grad[i, :] = dloss/dlogp (onehot(label) - q) / temperature,  dloss/dlogp = w (-r A where the first term is the smaller or both are equal, else 0;
+ *   + kl_coef (1 - exp(b))).
+ * An advantage of 0 has no share in the first term whatever r is.  ref_logp may be NULL with kl_coef 0, and is not read then. */
+int evt_policy_loss(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const float *old_logp, const float *advantages,
+                    const float *ref_logp, const float *weights, double clip_low, double clip_high, double kl_coef, float *loss, float *logp,
+                    int32_t flags);
+
+/* The preference loss of n_pairs pairs of sequences packed one behind the other: sequence k has the rows offsets[k] .. offsets[k + 1] - 1
+ * (2 n_pairs + 1 ascending row numbers), the chosen one of pair p is sequence p and the rejected one n_pairs + p.  seq_logp[k] is the sum of its rows' log
+ * q[label] - of those with a label - or with average their mean (0 of none), ref_logp[k] the reference model's, and with w = weights[p] (NULL: 1)
+ *   h = beta ((seq_logp[p] - seq_logp[n_pairs + p]) - (ref_logp[p] - ref_logp[n_pairs + p])) - margin,
+ *   loss[p] = w (-(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)).
+ * The gradient of sum_p loss[p] is written for every row: 0 for those in front of the first and behind the last sequence.  A pair whose
+ * offsets do not ascend or leave the rows gets NaN.  work: 4 nrows floats that the call may write.  label_smoothing in [0, 0.5]. */
+int evt_preference_loss(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
+                        const float *ref_logp, const float *weights, double beta, double label_smoothing, double margin, int32_t average,
+                        float *loss, float *seq_logp, float *work, int32_t flags);
 
 /* ---- measurement ---------------------------------------------------------------------
  * Kernel classes timed with HIP events on the handle's stream when profiling is on.  Kernels that do the work of several classes

@@ -10,209 +10,551 @@
 // Scores are 16 or 32 bits wide; differences, exponentials, sums and losses are 32-bit, a gradient is rounded once, when it is written.
 #include "scores.h"
 #include <math.h>
-#include <utility>
+#include <type_traits>
 
 typedef _Float16 half_t;
 typedef __bf16 bf16_t;
 
-// (m, s): the maximum of some scores and the sum of their exp((x - m) / T).  Scores of -inf count nothing, a NaN or +inf makes s a NaN.
+// Sixteen bytes of scores as they lie in memory, at any address their type allows.
+template <typename T>
+struct Piece {
+    static constexpr int E = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Raw {
+        uint32_t w[4];
+    };
+    Raw r;
+    __device__ __forceinline__ void load(const T *p) { r = *(const Raw *)p; }
+    __device__ __forceinline__ void store(T *p) const { *(Raw *)p = r; }
+    // o elements behind a base: a 32-bit offset is an operand of the access where a pointer is two registers for every piece
+    __device__ __forceinline__ void load(const T *p, uint32_t o) { r = *(const Raw *)((const char *)p + o * (uint32_t)sizeof(T)); }
+    __device__ __forceinline__ void store(T *p, uint32_t o) const { *(Raw *)((char *)p + o * (uint32_t)sizeof(T)) = r; }
+    __device__ __forceinline__ void get(float *f) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) f[k] = __uint_as_float(r.w[k]);
+        } else if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                f[2 * k] = __uint_as_float(r.w[k] << 16);
+                f[2 * k + 1] = __uint_as_float(r.w[k] & 0xffff0000u);
+            }
+        } else {
+            typedef half_t h2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const h2 v = __builtin_bit_cast(h2, r.w[k]);
+                f[2 * k] = (float)v[0];
+                f[2 * k + 1] = (float)v[1];
+            }
+        }
+    }
+    __device__ __forceinline__ void set(const float *f) { // rounds to nearest
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) r.w[k] = __float_as_uint(f[k]);
+        } else {
+            typedef T t2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const t2 v = {(T)f[2 * k], (T)f[2 * k + 1]};
+                r.w[k] = __builtin_bit_cast(uint32_t, v);
+            }
+        }
+    }
+};
+
+// (m, s): the maximum of some scores, at least the lowest finite number, and the sum of their exp((x - m) / T).  Scores of -inf count nothing, a
+// NaN or +inf makes s a NaN, and s is 0 where every score is -inf.
 struct MaxSum {
     float m, s;
 };
-__device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
+#define LOWEST (-3.402823466e38f)
+__device__ __forceinline__ float exp_of(float x, float m, float mul) { return __builtin_amdgcn_exp2f((x - m) * mul); }
 __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float mul) {
-    const float m = fmaxf(a.m, b.m), z = finite_or_zero(m);
-    return {m, a.s * __builtin_amdgcn_exp2f((a.m - z) * mul) + b.s * __builtin_amdgcn_exp2f((b.m - z) * mul)};
+    const float m = fmaxf(a.m, b.m);
+    return {m, a.s * exp_of(a.m, m, mul) + b.s * exp_of(b.m, m, mul)};
 }
-__device__ __forceinline__ MaxSum wave_join(MaxSum a, float mul) {
+// a with E more scores
+template <int E>
+__device__ __forceinline__ MaxSum take(MaxSum a, const float *f, float mul) {
+    float m = a.m;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) a = join(a, {__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, mul);
+    for (int k = 0; k < E; k++) m = fmaxf(m, f[k]);
+    float s[E];
+#pragma unroll
+    for (int k = 0; k < E; k++) s[k] = exp_of(f[k], m, mul);
+#pragma unroll
+    for (int w = E / 2; w > 0; w /= 2)
+#pragma unroll
+        for (int k = 0; k < w; k++) s[k] += s[k + w];
+    return {m, a.s * exp_of(a.m, m, mul) + s[0]};
+}
+__device__ __forceinline__ MaxSum lanes_join(MaxSum a, int lanes, float mul) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) a = join(a, {__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, mul);
     return a;
 }
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+__device__ __forceinline__ float lanes_sum(float v, int lanes) {
+    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
     return v;
 }
-template <int WAVES>
-__device__ __forceinline__ MaxSum block_join(MaxSum a, float mul) {
-    __shared__ MaxSum s_a[WAVES];
-    a = wave_join(a, mul);
-    if ((threadIdx.x & 63) == 0) s_a[threadIdx.x >> 6] = a;
-    __syncthreads();
-    a = s_a[0];
+
+// The threads that share a row: G lanes of a wavefront, or W whole wavefronts, a block.  LANES of them, the first, look after a teacher's entries.
+template <int G>
+struct Lanes {
+    static constexpr int SIZE = G, LANES = G, ROWS = 256 / G, THREADS = 256;
+    __device__ static int rank() { return threadIdx.x & (G - 1); }
+    __device__ static int slot() { return threadIdx.x / G; } // of the block's rows
+    __device__ static void sync() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ static MaxSum all(MaxSum a, float mul) { // the group's joined; what its lanes wrote to shared memory before can be read
+        a = lanes_join(a, G, mul);
+        sync();
+        return a;
+    }
+};
+template <int W>
+struct Waves {
+    static constexpr int SIZE = 64 * W, LANES = 64, ROWS = 1, THREADS = 64 * W;
+    __device__ static int rank() { return threadIdx.x; }
+    __device__ static int slot() { return 0; }
+    __device__ static void sync() { __syncthreads(); }
+    __device__ static MaxSum all(MaxSum a, float mul) {
+        __shared__ MaxSum s_a[W];
+        a = lanes_join(a, 64, mul);
+        if ((threadIdx.x & 63) == 0) s_a[threadIdx.x >> 6] = a;
+        __syncthreads();
+        a = s_a[0];
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) a = join(a, s_a[w], mul);
-    __syncthreads();
-    return a;
-}
-template <int WAVES>
-__device__ __forceinline__ float block_sum(float v) {
-    __shared__ float s_v[WAVES];
-    v = wave_sum(v);
-    if ((threadIdx.x & 63) == 0) s_v[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = s_v[0];
-#pragma unroll
-    for (int w = 1; w < WAVES; w++) v += s_v[w];
-    __syncthreads();
-    return v;
-}
+        for (int w = 1; w < W; w++) a = join(a, s_a[w], mul);
+        return a;
+    }
+};
 
 __device__ __forceinline__ int64_t load_id(const void *p, int wide, int64_t i) { return wide ? ((const int64_t *)p)[i] : ((const int32_t *)p)[i]; }
 __device__ __forceinline__ float load_score(const void *p, int type, int64_t i) {
     return type == EVT_F32 ? ((const float *)p)[i] : type == EVT_BF16 ? (float)((const bf16_t *)p)[i] : (float)((const half_t *)p)[i];
 }
 
+// log(s) to 3e-8: the exponent's share in 64 bits, the mantissa's, of at most 0.35, in 32.  (In 32 bits altogether a sum over a large vocabulary costs
+// 5e-7, in 64 a block of sixteen wavefronts about 4 us a row.)
+__device__ __forceinline__ double log_sum(float s) {
+    int k;
+    float f = frexpf(s, &k);
+    if (f < 0.70710678f) f += f, k--;
+    return (double)k * 0.6931471805599453 + (double)logf(f);
+}
 // A row of score x at its label: its log-probability.  Nothing is left of a row whose scores are all -inf: every class has probability 0.
 // 64 bits for the two terms: a policy's ratio is compared with its bounds.
 __device__ __forceinline__ double row_logp(const ScoreArgs &a, MaxSum r, float x) {
     if (r.s == 0.0f) return -INFINITY;
-    return (double)(x - finite_or_zero(r.m)) * a.inv_t - log((double)r.s);
+    return (double)(x - r.m) * a.inv_t - log_sum(r.s);
 }
 __device__ __forceinline__ float inverse_sum(MaxSum r) { return r.s == 0.0f ? 0.0f : 1.0f / r.s; }
 
-// The policy loss of a token and its derivative by logp: -min(r A, clip(r) A) + kl (exp(ref - logp) - (ref - logp) - 1), r = exp(logp - old).
+// The policy loss of a token and its derivative by logp: -min(r A, clip(r) A) + kl (exp(b) - b - 1), r = exp(logp - old), b = ref - logp.
+// The differences are 64-bit, and the side of the bounds that r is on is found from them: a ratio next to a bound has a whole row's gradient or none.
 // An advantage of zero has no share in it, however far apart the two policies are, a weight of zero no loss.
 __device__ __forceinline__ void policy_row(const ScoreArgs &a, int64_t row, float w, double logp, float &loss, float &slope) {
     double l = 0.0, d = 0.0;
-    const double adv = a.adv[row];
-    if (adv != 0.0) {
-        const double r = exp(logp - (double)a.old_logp[row]);
-        const double lo = 1.0 - a.clip_lo, hi = 1.0 + a.clip_hi;
-        const double held = (r < lo ? lo : r > hi ? hi : r) * adv, free = r * adv; // a NaN stays one
-        l = free <= held ? -free : -held;
-        d = free <= held ? -free : 0.0;
-        if (free != free) l = d = free;
+    const float adv = a.adv[row];
+    if (adv != 0.0f) {
+        const double gap = logp - (double)a.old_logp[row];
+        const double free = -(double)expf((float)gap) * adv;
+        if (adv > 0.0f ? gap > a.log_hi : gap < a.log_lo) l = -(adv > 0.0f ? a.hi : a.lo) * adv;
+        else l = d = free; // a NaN too
     }
     if (a.kl != 0.0) {
         const double back = (double)a.ref_logp[row] - logp;
-        const double e = expm1(back);
-        l += a.kl * (e - back);
+        const float b = (float)back, e = expm1f(b);
+        // e - b cancels where the policies are close: there the series up to b^7 / 7!, the rest of which is under 2^-26 of it
+        const float rest = fabsf(b) < 0.25f ? b * b * (0.5f + b * (1.0f / 6 + b * (1.0f / 24 + b * (1.0f / 120 + b * (1.0f / 720 + b * (1.0f / 5040)))))) : e - b;
+        l += a.kl * rest;
         d -= a.kl * e;
     }
-    loss = w == 0.0f ? 0.0f : (float)((double)w * l);
-    slope = w == 0.0f ? 0.0f : (float)((double)w * d);
+    loss = w == 0.0f ? 0.0f : (float)(w * l);
+    slope = w == 0.0f ? 0.0f : (float)(w * d);
 }
 
-// One block to a row, two passes over its scores: the simplest form.
-template <typename T, int OP>
-__global__ __launch_bounds__(256) void k_scores(ScoreArgs a) {
-    constexpr int WAVES = 4;
-    const int64_t row = blockIdx.x;
-    const int t = threadIdx.x, V = a.V;
+// What an operator makes of a labelled row's (m, s): its values are written by the thread that `writes`; the slope dloss / dx_label + ... = dloss /
+// dlogp / T is returned (SC_LOGP: 0).
+template <int OP>
+__device__ __forceinline__ float labelled_row(const ScoreArgs &a, int64_t row, bool bad, MaxSum r, float x_label, float given, bool writes) {
+    if (OP == SC_GRAD) return bad ? NAN : (float)(given * a.inv_t);
+    const double logp = bad ? NAN : row_logp(a, r, x_label);
+    float slope = 0.0f;
+    if (OP == SC_POLICY) {
+        float loss;
+        policy_row(a, row, a.weights ? a.weights[row] : 1.0f, logp, loss, slope);
+        slope = (float)(slope * a.inv_t);
+        if (writes) a.loss[row] = loss;
+    }
+    if (writes) {
+        a.logp[row] = (float)logp;
+        if (OP == SC_LOGP && a.stats) {
+            a.stats[2 * row] = r.s == 0.0f ? -INFINITY : r.m;
+            a.stats[2 * row + 1] = r.s;
+        }
+        if (OP == SC_LOGP && a.slope) a.slope[row] = 0.0f;
+    }
+    return slope;
+}
+template <int OP>
+__device__ __forceinline__ void left_out(const ScoreArgs &a, int64_t row) {
+    if (OP == SC_DISTILL || OP == SC_POLICY) a.loss[row] = 0.0f;
+    if (OP == SC_LOGP || OP == SC_POLICY) a.logp[row] = 0.0f;
+    if (OP == SC_LOGP && a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
+    if (OP == SC_LOGP && a.slope) a.slope[row] = 0.0f;
+}
+
+// A gradient of 0 for V classes
+template <typename T>
+__device__ __forceinline__ void clear_row(T *g, int V, int rank, int size) {
+    constexpr int E = Piece<T>::E;
+    Piece<T> p;
+    p.r = {};
+    const int n = V / E;
+    for (int v = rank; v < n; v += size) p.store(g + (size_t)v * E);
+    for (int c = n * E + rank; c < V; c += size) g[c] = (T)0.0f;
+}
+
+// E classes' gradients: fq * exp((x - m) / T), and at the label, if it is among them, slope (1 - q)
+template <int E>
+__device__ __forceinline__ void gradients(float *f, MaxSum r, float fq, float mul, int label_at, float slope, float inv) {
+    float e[E];
+#pragma unroll
+    for (int k = 0; k < E; k++) e[k] = exp_of(f[k], r.m, mul);
+#pragma unroll
+    for (int k = 0; k < E; k++) f[k] = fq * e[k];
+    if ((unsigned)label_at < (unsigned)E) {
+#pragma unroll
+        for (int k = 0; k < E; k++) f[k] = k == label_at ? slope * (1.0f - e[k] * inv) : f[k];
+    }
+}
+
+// A row to a group of threads.  The first NV pieces of every thread stay in registers between the two passes over the row, the rest
+// (rows of more classes than the largest form holds) is read again.  V is at least a piece's: the last one reaches back over classes of the one before it.
+template <typename T, int OP, int NV, class G>
+__global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
+    constexpr int E = Piece<T>::E;
+    extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs for each of the block's rows, then scores
+    __shared__ int s_state[G::ROWS];         // SC_DISTILL: 1 a teacher, 2 and an id of no class
+    const int64_t row = (int64_t)blockIdx.x * G::ROWS + G::slot();
+    if (G::ROWS > 1 && row >= a.N) return;
+    const int t = G::rank(), V = a.V;
     const T *x = (const T *)a.x + row * a.xs;
     T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
-    const float w = a.weights ? a.weights[row] : 1.0f;
-    __shared__ float s_p[OP == SC_DISTILL ? EVT_SCORES_MAX_TOP : 1], s_x[OP == SC_DISTILL ? EVT_SCORES_MAX_TOP : 1];
-    __shared__ int32_t s_id[OP == SC_DISTILL ? EVT_SCORES_MAX_TOP : 1];
-    bool live = OP != SC_DISTILL || w != 0.0f, bad = false;
+    const float mul = a.exp_mul;
+    float w = 1.0f, x_label = 0.0f, given = 0.0f;
+    bool live = true, bad = false;
     int64_t label = -1;
-    float x_label = 0.0f, slope = 0.0f;
-    MaxSum teacher = {-INFINITY, 0.0f};
-    if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
     if (OP == SC_DISTILL) {
-        if (live) { // uniform
-            bool mine = false;
-            for (int j = t; j < a.n_top; j += 256) {
-                const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
-                const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
-                mine |= id >= V;
-                s_id[j] = id < 0 || id >= V ? -1 : (int32_t)id;
-                s_x[j] = id < 0 || id >= V ? 0.0f : (float)x[id];
-                s_p[j] = s;
-                teacher = join(teacher, {s, s == -INFINITY ? 0.0f : s - s + 1.0f}, a.exp_mul);
-            }
-            bad = __syncthreads_or(mine);
-            teacher = block_join<WAVES>(teacher, a.exp_mul);
-            live = teacher.s != 0.0f; // a NaN is live
-        }
+        w = a.weights ? a.weights[row] : 1.0f;
+        live = w != 0.0f;
     } else {
         label = load_id(a.labels, a.label64, row);
-        live = live && label >= 0;
+        live = label >= 0;
+        if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
         if (OP == SC_GRAD && live) {
-            slope = a.slope[row];
-            live = slope != 0.0f; // nothing asked of it: not read
+            given = a.slope[row];
+            live = given != 0.0f; // nothing asked of it: not read
         }
         bad = live && label >= V;
         if (live && !bad) x_label = (float)x[label];
     }
     if (!live) { // the row has no part in the loss
-        if (t == 0) {
-            if (OP != SC_GRAD && OP != SC_LOGP) a.loss[row] = 0.0f;
-            if (OP == SC_LOGP || OP == SC_POLICY) a.logp[row] = 0.0f;
-            if (OP == SC_LOGP && a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
-            if (OP == SC_LOGP && a.slope) a.slope[row] = 0.0f;
-        }
-        if (OP != SC_LOGP && g)
-            for (int c = t; c < V; c += 256) g[c] = (T)0.0f;
+        if (t == 0) left_out<OP>(a, row);
+        if (OP != SC_LOGP && g) clear_row(g, V, t, G::SIZE);
         return;
     }
-    MaxSum r = {-INFINITY, 0.0f};
-    if (OP == SC_GRAD) r = {a.stats[2 * row], a.stats[2 * row + 1]};
-    else {
-        for (int c = t; c < V; c += 256) {
-            const float v = (float)x[c];
-            r = join(r, {v, v == -INFINITY ? 0.0f : v - v + 1.0f}, a.exp_mul); // 1, or a NaN for a score that is none
-        }
-        r = block_join<WAVES>(r, a.exp_mul);
+    Piece<T> p[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int o = (t + i * G::SIZE) * E;
+        p[i].load(x, o + E <= V ? o : V - E); // past the row's end: the last piece, which counts once
     }
-    const float z = finite_or_zero(r.m), inv = inverse_sum(r);
-    float factor = 0.0f; // of q
-    if (OP == SC_DISTILL) {
-        const double log_ts = log((double)teacher.s);
-        const double log_s = r.s == 0.0f ? 0.0 : log((double)r.s);
-        const float tz = finite_or_zero(teacher.m);
-        float sum = 0.0f;
-        for (int j = t; j < a.n_top; j += 256) {
-            const float d = s_p[j] - tz, p = __builtin_amdgcn_exp2f(d * a.exp_mul) / teacher.s;
-            if (s_id[j] >= 0 && p != 0.0f) {
-                const double lq = r.s == 0.0f ? -INFINITY : (double)(s_x[j] - z) * a.inv_t - log_s;
-                sum += p * (float)((double)d * a.inv_t - log_ts - lq);
-            }
-            s_p[j] = p;
+    int2 *const s_top = (int2 *)s_dyn + (size_t)G::slot() * a.n_top;
+    float *const s_x = (float *)((int2 *)s_dyn + (size_t)G::ROWS * a.n_top) + (size_t)G::slot() * a.n_top;
+    MaxSum teacher = {LOWEST, 0.0f};
+    if (OP == SC_DISTILL && t < G::LANES) {
+        bool none = false;
+        for (int j = t; j < a.n_top; j += G::LANES) {
+            const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
+            const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
+            const bool in = id >= 0 && id < V;
+            none |= id >= V;
+            s_top[j] = {in ? (int)id : -1, __float_as_int(s)};
+            s_x[j] = in ? (float)x[id] : 0.0f;
+            teacher = take<1>(teacher, &s, mul);
         }
-        sum = block_sum<WAVES>(sum);
-        if (t == 0) a.loss[row] = bad ? NAN : w * a.t2_mul * sum;
-        factor = bad ? NAN : w * a.t_mul;
-    } else if (OP == SC_GRAD) {
-        slope = bad ? NAN : (float)(slope * a.inv_t);
-        factor = -slope;
+        teacher = lanes_join(teacher, G::LANES, mul);
+        for (int o = G::LANES >> 1; o > 0; o >>= 1) none |= __shfl_xor((int)none, o) != 0;
+        if (t == 0) s_state[G::slot()] = teacher.s == 0.0f ? 0 : none ? 2 : 1; // a sum that is no number is a teacher
+        for (int j = t; j < a.n_top; j += G::LANES) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) / teacher.s);
+    }
+    MaxSum r = {LOWEST, 0.0f};
+    if (OP == SC_GRAD) {
+        r = {fmaxf(a.stats[2 * row], LOWEST), a.stats[2 * row + 1]};
     } else {
-        const double logp = bad ? NAN : row_logp(a, r, x_label);
-        if (OP == SC_POLICY) {
-            float loss;
-            policy_row(a, row, w, logp, loss, slope);
-            slope = (float)(slope * a.inv_t);
-            factor = -slope;
-            if (t == 0) a.loss[row] = loss;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int o = (t + i * G::SIZE) * E;
+            if (o < V) {
+                float f[E];
+                p[i].get(f);
+                if (o + E > V) { // classes that the piece before has counted
+#pragma unroll
+                    for (int k = 0; k < E; k++) f[k] = k < o + E - V ? -INFINITY : f[k];
+                }
+                r = take<E>(r, f, mul);
+            }
         }
-        if (t == 0) {
-            a.logp[row] = (float)logp;
-            if (OP == SC_LOGP && a.stats) a.stats[2 * row] = r.m, a.stats[2 * row + 1] = r.s;
-            if (OP == SC_LOGP && a.slope) a.slope[row] = 0.0f;
+        int64_t o = (int64_t)(t + NV * G::SIZE) * E;
+        for (; o + 3 * G::SIZE * E + E <= V; o += 4 * G::SIZE * E) { // four pieces in flight
+            Piece<T> q[4];
+            float f[E];
+#pragma unroll
+            for (int i = 0; i < 4; i++) q[i].load(x + o + i * G::SIZE * E);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                q[i].get(f);
+                r = take<E>(r, f, mul);
+            }
         }
+        for (; o < V; o += G::SIZE * E) {
+            float f[E];
+            if (o + E <= V) {
+                Piece<T> q;
+                q.load(x + o);
+                q.get(f);
+            } else {
+#pragma unroll
+                for (int k = 0; k < E; k++) f[k] = o + k < V ? (float)x[o + k] : -INFINITY;
+            }
+            r = take<E>(r, f, mul);
+        }
+        r = G::all(r, mul);
+    }
+    const float inv = inverse_sum(r);
+    float fq, slope = 0.0f, factor = 0.0f;
+    if (OP == SC_DISTILL) {
+        const int state = s_state[G::slot()];
+        if (state == 0) {
+            if (t == 0) left_out<OP>(a, row);
+            if (g) clear_row(g, V, t, G::SIZE);
+            return;
+        }
+        if (t < G::LANES) {
+            const double log_ts = log_sum(teacher.s), log_s = log_sum(r.s);
+            float sum = 0.0f;
+            for (int j = t; j < a.n_top; j += G::LANES) {
+                const int2 e = s_top[j];
+                const float pj = __int_as_float(e.y);
+                if (e.x >= 0 && pj != 0.0f) {
+                    const float tj = load_score(a.top, a.top_type, row * a.n_top + j);
+                    const double lq = r.s == 0.0f ? -INFINITY : (double)(s_x[j] - r.m) * a.inv_t - log_s;
+                    sum += pj * (float)((double)(tj - teacher.m) * a.inv_t - log_ts - lq);
+                }
+            }
+            sum = lanes_sum(sum, G::LANES);
+            if (t == 0) a.loss[row] = state == 2 ? NAN : w * a.t2_mul * sum;
+        }
+        factor = state == 2 ? NAN : w * a.t_mul;
+    } else {
+        slope = labelled_row<OP>(a, row, bad, r, x_label, given, t == 0);
+        if (OP == SC_POLICY && slope == 0.0f && g) { // clipped, or of no weight
+            clear_row(g, V, t, G::SIZE);
+            return;
+        }
+        factor = -slope;
     }
     if (OP == SC_LOGP || !g) return;
-    if (OP == SC_POLICY && slope == 0.0f) { // clipped
-        __syncthreads(); // every thread has read its label's score
-        for (int c = t; c < V; c += 256) g[c] = (T)0.0f;
+    fq = factor * inv;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        int o = (t + i * G::SIZE) * E;
+        if (o < V) {
+            o = o + E <= V ? o : V - E;
+            float f[E];
+            p[i].get(f);
+            gradients<E>(f, r, fq, mul, OP == SC_DISTILL ? -1 : (int)(label - o), slope, inv);
+            p[i].set(f);
+            p[i].store(g, o);
+        }
+    }
+    for (int64_t o = (int64_t)(t + NV * G::SIZE) * E; o < V; o += G::SIZE * E) {
+        float f[E];
+        if (o + E <= V) {
+            Piece<T> q;
+            q.load(x + o);
+            q.get(f);
+            gradients<E>(f, r, fq, mul, OP == SC_DISTILL ? -1 : (int)(label - o), slope, inv);
+            q.set(f);
+            q.store(g + o);
+        } else { // not reaching back: in place, the classes in front are gradients already
+            for (int64_t c = o; c < V; c++) {
+                f[0] = (float)x[c];
+                gradients<1>(f, r, fq, mul, OP == SC_DISTILL ? -1 : (int)(label - c), slope, inv);
+                g[c] = (T)f[0];
+            }
+        }
+    }
+    if (OP == SC_DISTILL) { // the teacher's classes again, behind the others' stores
+        G::sync();
+        for (int j = t; j < a.n_top; j += G::SIZE) {
+            const int id = s_top[j].x;
+            if (id < 0) continue;
+            float pj = 0.0f; // an id that comes twice has both shares
+            for (int i = 0; i < a.n_top; i++) {
+                const int2 e = s_top[i];
+                pj += e.x == id ? __int_as_float(e.y) : 0.0f;
+            }
+            g[id] = (T)(factor * (exp_of(s_x[j], r.m, mul) * inv - pj));
+        }
+    }
+}
+
+// A row to a thread: up to KM classes.
+template <typename T, int OP, int KM>
+__global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (row >= a.N) return;
+    const int V = a.V;
+    const T *x = (const T *)a.x + row * a.xs;
+    T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
+    const float mul = a.exp_mul;
+    float w = 1.0f, given = 0.0f;
+    bool live = true, bad = false;
+    int64_t label = -1;
+    if (OP == SC_DISTILL) {
+        w = a.weights ? a.weights[row] : 1.0f;
+        live = w != 0.0f;
+    } else {
+        label = load_id(a.labels, a.label64, row);
+        live = label >= 0;
+        if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
+        if (OP == SC_GRAD && live) {
+            given = a.slope[row];
+            live = given != 0.0f;
+        }
+        bad = live && label >= V;
+    }
+    float f[KM], p[KM]; // p: the teacher's share of each class
+    MaxSum teacher = {LOWEST, 0.0f};
+    if (OP == SC_DISTILL && live) {
+        for (int j = 0; j < a.n_top; j++) {
+            const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
+            const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
+            bad |= id >= V;
+            teacher = take<1>(teacher, &s, mul);
+        }
+        live = teacher.s != 0.0f;
+    }
+    if (!live) {
+        left_out<OP>(a, row);
+        if (OP != SC_LOGP && g)
+            for (int c = 0; c < V; c++) g[c] = (T)0.0f;
         return;
     }
-    const float fq = factor * inv;
-    __syncthreads(); // every score of another thread's class has been read
-    for (int c = t; c < V; c += 256) g[c] = (T)(fq * __builtin_amdgcn_exp2f(((float)x[c] - z) * a.exp_mul));
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < KM; k++) f[k] = (float)x[k < V ? k : V - 1];
+#pragma unroll
+    for (int k = 0; k < KM; k++) f[k] = k < V ? f[k] : -INFINITY;
+    MaxSum r = {LOWEST, 0.0f};
+    if (OP == SC_GRAD) r = {fmaxf(a.stats[2 * row], LOWEST), a.stats[2 * row + 1]};
+    else r = take<KM>(r, f, mul);
+    const float inv = inverse_sum(r);
+    float factor, slope = 0.0f;
     if (OP == SC_DISTILL) {
-        for (int j = t; j < a.n_top; j += 256) {
-            const int32_t id = s_id[j];
-            if (id < 0) continue;
-            float p = 0.0f; // an id that comes twice has both shares
-            for (int i = 0; i < a.n_top; i++) p += s_id[i] == id ? s_p[i] : 0.0f;
-            g[id] = (T)(factor * (__builtin_amdgcn_exp2f((s_x[j] - z) * a.exp_mul) * inv - p));
+#pragma unroll
+        for (int k = 0; k < KM; k++) p[k] = 0.0f;
+        const double log_ts = log_sum(teacher.s), log_s = log_sum(r.s);
+        float sum = 0.0f;
+        for (int j = 0; j < a.n_top; j++) {
+            const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
+            if (id < 0 || id >= V) continue;
+            const float tj = load_score(a.top, a.top_type, row * a.n_top + j);
+            const float pj = exp_of(tj, teacher.m, mul) / teacher.s;
+            float xj = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KM; k++) {
+                p[k] += k == (int)id ? pj : 0.0f;
+                xj = k == (int)id ? f[k] : xj;
+            }
+            if (pj != 0.0f) {
+                const double lq = r.s == 0.0f ? -INFINITY : (double)(xj - r.m) * a.inv_t - log_s;
+                sum += pj * (float)((double)(tj - teacher.m) * a.inv_t - log_ts - lq);
+            }
         }
-    } else if (t == 0 && !bad) {
-        g[label] = (T)(slope * (1.0f - __builtin_amdgcn_exp2f((x_label - z) * a.exp_mul) * inv));
+        a.loss[row] = bad ? NAN : w * a.t2_mul * sum;
+        factor = bad ? NAN : w * a.t_mul;
+    } else {
+        float x_label = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KM; k++) x_label = k == (int)label ? f[k] : x_label;
+        slope = labelled_row<OP>(a, row, bad, r, x_label, given, true);
+        factor = -slope;
+    }
+    if (OP == SC_LOGP || !g) return;
+    if (OP == SC_POLICY && slope == 0.0f) {
+        for (int c = 0; c < V; c++) g[c] = (T)0.0f;
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < KM; k++) {
+        const float q = exp_of(f[k], r.m, mul) * inv;
+        const float v = OP == SC_DISTILL ? factor * (q - p[k]) : k == (int)label ? slope * (1.0f - q) : factor * q;
+        if (k < V) g[k] = (T)v;
+    }
+}
+
+// The gradient of given slopes, where rows are long: nothing is joined, a block has a part of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, int parts) {
+    constexpr int E = Piece<T>::E, PART = 256 * 4 * E;
+    const int64_t blocks = a.N * parts;
+    for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
+        const int64_t row = b / parts;
+        const int64_t c0 = (b - row * parts) * PART;
+        const T *x = (const T *)a.x + row * a.xs + c0;
+        T *g = (T *)a.g + row * a.gs + c0;
+        const int V = (int)(a.V - c0 < PART ? a.V - c0 : PART), t = threadIdx.x;
+        const int64_t label = load_id(a.labels, a.label64, row);
+        float given = 0.0f;
+        bool live = label >= 0;
+        if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
+        if (live) given = a.slope[row];
+        if (given == 0.0f) {
+            clear_row(g, V, t, 256);
+            continue;
+        }
+        const MaxSum r = {fmaxf(a.stats[2 * row], LOWEST), a.stats[2 * row + 1]};
+        const float inv = inverse_sum(r), slope = label >= a.V ? NAN : (float)(given * a.inv_t), fq = -slope * inv;
+        const int64_t at = label - c0; // of the label, in this part if at all
+        Piece<T> p[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int o = (t + i * 256) * E;
+            if (o + E <= V) p[i].load(x + o);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int o = (t + i * 256) * E;
+            float f[E];
+            if (o + E <= V) {
+                p[i].get(f);
+                gradients<E>(f, r, fq, a.exp_mul, (int)(at - o), slope, inv);
+                p[i].set(f);
+                p[i].store(g + o);
+            }
+        }
+        const int c = V / E * E + t; // behind the last whole piece
+        if (c < V) {
+            float f = (float)x[c];
+            gradients<1>(&f, r, fq, a.exp_mul, (int)(at - c), slope, inv);
+            g[c] = (T)f;
+        }
     }
 }
 
@@ -276,12 +618,52 @@ __global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, int pairs, c
     }
 }
 
+// LAUNCH of the form that a row of n pieces takes
+template <typename T, int OP, int NV, class G>
+static void launch_rows(hipStream_t s, const ScoreArgs &a) {
+    const size_t lds = OP == SC_DISTILL ? (size_t)G::ROWS * a.n_top * 12 : 0;
+    hipLaunchKernelGGL((k_rows<T, OP, NV, G>), dim3((unsigned)((a.N + G::ROWS - 1) / G::ROWS)), dim3(G::THREADS), lds, s, a);
+}
+template <typename T, int OP>
+static void launch_typed(hipStream_t s, const ScoreArgs &a) {
+    constexpr int E = Piece<T>::E;
+    const int64_t n = ((int64_t)a.V + E - 1) / E;
+    if (a.V <= 16) {
+        const dim3 grid((unsigned)((a.N + 255) / 256)), block(256);
+        if (a.V <= 4) hipLaunchKernelGGL((k_few_classes<T, OP, 4>), grid, block, 0, s, a);
+        else if (a.V <= 8) hipLaunchKernelGGL((k_few_classes<T, OP, 8>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((k_few_classes<T, OP, 16>), grid, block, 0, s, a);
+        return;
+    }
+    if (n <= 256) {
+        // a group's rows share a block's memory with their teachers
+        const int top = OP == SC_DISTILL ? a.n_top : 0;
+        if (n <= 8 && top <= 64) return launch_rows<T, OP, 1, Lanes<8>>(s, a);
+        if (n <= 16 && top <= 128) return launch_rows<T, OP, 1, Lanes<16>>(s, a);
+        if (n <= 32 && top <= 256) return launch_rows<T, OP, 1, Lanes<32>>(s, a);
+        if (n <= 64) return launch_rows<T, OP, 1, Lanes<64>>(s, a);
+        return launch_rows<T, OP, 4, Lanes<64>>(s, a);
+    }
+    if constexpr (OP == SC_GRAD) {
+        const int64_t parts = (n + 1023) / 1024, blocks = a.N * parts;
+        hipLaunchKernelGGL(k_slope_rows<T>, dim3((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30))), dim3(256), 0, s, a, (int)parts);
+    } else {
+        if (n <= 1024) return launch_rows<T, OP, 4, Waves<4>>(s, a);
+        if (OP != SC_LOGP && a.g) { // the row stays in registers
+            if constexpr (OP != SC_LOGP) {
+                if (n <= 2048) return launch_rows<T, OP, 2, Waves<16>>(s, a);
+                if (n > 8192) return launch_rows<T, OP, 16, Waves<16>>(s, a);
+                if (n > 4096) return launch_rows<T, OP, 8, Waves<16>>(s, a);
+            }
+        }
+        return launch_rows<T, OP, 4, Waves<16>>(s, a);
+    }
+}
 template <int OP>
 static int launch_scores(hipStream_t s, const ScoreArgs &a, int dtype) {
-    const dim3 grid((unsigned)a.N), block(256);
-    if (dtype == EVT_F32) hipLaunchKernelGGL((k_scores<float, OP>), grid, block, 0, s, a);
-    else if (dtype == EVT_BF16) hipLaunchKernelGGL((k_scores<bf16_t, OP>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((k_scores<half_t, OP>), grid, block, 0, s, a);
+    if (dtype == EVT_F32) launch_typed<float, OP>(s, a);
+    else if (dtype == EVT_BF16) launch_typed<bf16_t, OP>(s, a);
+    else launch_typed<half_t, OP>(s, a);
     HIPCHK(hipGetLastError());
     return EVT_OK;
 }
@@ -416,8 +798,10 @@ extern "C" int evt_policy_loss(void *stream, const evt_scores *s, const void *la
     a.adv = advantages;
     a.ref_logp = ref_logp;
     a.weights = weights;
-    a.clip_lo = clip_low;
-    a.clip_hi = clip_high;
+    a.lo = 1.0 - clip_low;
+    a.hi = 1.0 + clip_high;
+    a.log_lo = log(1.0 - clip_low); // -inf of 1: no lower bound
+    a.log_hi = log1p(clip_high);
     a.kl = kl_coef;
     a.loss = loss;
     a.logp = logp;

@@ -29,5 +29,6 @@ struct ScoreArgs {
     float t_mul, t2_mul; // temperature and its square
     // SC_POLICY
     const float *old_logp, *adv, *ref_logp;
-    double clip_lo, clip_hi, kl;
+    double log_lo, log_hi; // the bounds of logp - old_logp
+    double lo, hi, kl;
 };

@@ -21,128 +21,136 @@ __all__ = ["class_logp", "class_logp_grad", "distill_loss", "policy_loss", "pref
 
 _F32, _I32, _I64, _BF16, _F16 = 0, 4, 5, 10, 11
 _TRUSTED = 2  # EVT_STATIC_TRUSTED: the tensors say where they are
+_INF = float("inf")
 _torch = None
 
 
 def _load():
-    """torch and the codes of its types; imported with the first call, a fit needs none."""
-    global _torch, _FLOATS, _INTS, _new
-    if _torch is None:
-        import torch
-        _FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
-        _INTS = {torch.int32: _I32, torch.int64: _I64}
-        _new = torch.empty
-        _torch = torch
-    return _torch
+    """torch, the codes of its types and what a call needs of it; imported with the first call, a fit needs none."""
+    global _torch, _FLOATS, _INTS, _F32S, _I32S, _new, _like, _device, _stream
+    import torch
+    _F32S = {torch.float32: _F32}
+    _FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
+    _I32S = {torch.int32: _I32}
+    _INTS = {torch.int32: _I32, torch.int64: _I64}
+    _new, _like = torch.empty, torch.empty_like
+    _device = torch.cuda.current_device
+    # the current stream's handle without a Stream object around it, 1.1 us less a call
+    _stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _torch = torch
 
 
-def _scores(name, x):
-    torch = _load()
-    if not isinstance(x, torch.Tensor):
-        raise TypeError("%s must be a torch tensor, got %s" % (name, type(x).__name__))
-    if x.dtype not in _FLOATS:
-        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (name, x.dtype))
-    if x.dim() != 2:
-        raise ValueError("%s must be a (rows, classes) matrix, got shape %s" % (name, tuple(x.shape)))
-    if x.shape[1] < 1 or x.shape[1] > 0x7FFFFFFF or x.shape[0] > 0x7FFFFFFF:
-        raise ValueError("%s must have 1 to 2^31 - 1 classes and at most 2^31 - 1 rows, got shape %s" % (name, tuple(x.shape)))
-    if x.stride(1) != 1 and x.shape[1] > 1:
-        raise ValueError("the classes of %s must lie side by side, got strides %s" % (name, x.stride()))
-
-
-def _check(name, v, x, shape, kinds, what):
+def _bad(name, v, x, shape, kinds):
+    """Says what is wrong with a tensor that is not as its call needs it."""
     if not isinstance(v, _torch.Tensor):
         raise TypeError("%s must be a torch tensor, got %s" % (name, type(v).__name__))
     if v.dtype not in kinds:
-        raise TypeError("%s must be %s, got %s" % (name, what, v.dtype))
+        raise TypeError("%s must be %s, got %s" % (name, " or ".join(str(k)[6:] for k in kinds), v.dtype))
     if tuple(v.shape) != shape:
         raise ValueError("%s must have shape %s, got %s" % (name, shape, tuple(v.shape)))
-    if not v.is_contiguous():
-        raise ValueError("%s must be contiguous" % name)
     if v.device != x.device:
         raise ValueError("%s is on %s, the scores are on %s" % (name, v.device, x.device))
-
-
-def _floats(name, v, x, n):
-    _check(name, v, x, (n,), (_torch.float32,), "float32")
-
-
-def _labels(name, v, x):
-    _check(name, v, x, (x.shape[0],), _INTS, "int32 or int64")
+    raise ValueError("%s must be contiguous" % name)
 
 
 def _number(name, v, low, high, open_low=False):
     v = float(v)
-    if not (low < v if open_low else low <= v) or not v <= high or v == float("inf"):
+    if not (low < v if open_low else low <= v) or not v <= high or v == _INF:
         raise ValueError("%s must be finite and in %s%s, %s], got %s" % (name, "(" if open_low else "[", low, high, v))
     return v
 
 
-def _gradient(x, want, out):
-    """The tensor the gradient goes to, None for none."""
-    if out is None:
-        return _new(x.shape, dtype=x.dtype, device=x.device) if want else None
-    if not want:
-        raise ValueError("out was given, but no gradient is asked for")
-    if not isinstance(out, _torch.Tensor) or out.dtype != x.dtype or out.shape != x.shape or out.device != x.device:
-        raise ValueError("out must be a tensor like the scores: %s, %s, on %s" % (tuple(x.shape), x.dtype, x.device))
-    if (out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
-        raise ValueError("the rows of out must lie side by side or apart, got strides %s" % (out.stride(),))
-    return out
-
-
 class _Call:
-    """The scores as the library takes them, and the device and stream of the call."""
+    """A call on some scores: the checks of what belongs to them, and the launch on their device's current stream."""
+    __slots__ = ("x", "kind", "rows", "device", "temperature")
 
     def __init__(self, x, temperature):
-        self.x, self.temperature = x, _number("temperature", temperature, 0.0, float("inf"), True)
+        if _torch is None:
+            _load()
+        if not isinstance(x, _torch.Tensor):
+            raise TypeError("the scores must be a torch tensor, got %s" % type(x).__name__)
+        kind = _FLOATS.get(x.dtype)
+        if kind is None:
+            raise TypeError("the scores must be float32, bfloat16 or float16, got %s" % x.dtype)
+        if x.dim() != 2:
+            raise ValueError("the scores must be a (rows, classes) matrix, got shape %s" % (tuple(x.shape),))
+        rows, classes = x.shape
+        if not 1 <= classes <= 0x7FFFFFFF or rows > 0x7FFFFFFF:
+            raise ValueError("the scores must have 1 to 2^31 - 1 classes and at most 2^31 - 1 rows, got shape %s" % (tuple(x.shape),))
+        if x.stride(1) != 1 and classes > 1:
+            raise ValueError("the scores of a row must lie side by side, got strides %s" % (x.stride(),))
+        self.x, self.kind, self.rows, self.device = x, kind, rows, x.get_device()
+        self.temperature = _number("temperature", temperature, 0.0, _INF, True)
+
+    def check(self, name, v, shape, kinds):
+        """v's address, and its type's code by way of `kinds`."""
+        try:
+            if v.dtype in kinds and v.shape == shape and v.is_contiguous() and v.get_device() == self.device:
+                return v.data_ptr()
+        except AttributeError:
+            pass
+        _bad(name, v, self.x, shape, kinds)
+
+    def floats(self, name, v):
+        return self.check(name, v, (self.rows,), _F32S)
+
+    def optional(self, name, v, n):
+        return None if v is None else self.check(name, v, (n,), _F32S)
+
+    def gradient(self, want, out):
+        """The tensor the gradient goes to, None for none."""
+        x = self.x
+        if out is None:
+            if not want:
+                return None
+            return _like(x, memory_format=_torch.contiguous_format)
+        if not want:
+            raise ValueError("out was given, but no gradient is asked for")
+        if not isinstance(out, _torch.Tensor) or out.dtype != x.dtype or out.shape != x.shape or out.device != x.device:
+            raise ValueError("out must be a tensor like the scores: %s, %s, on %s" % (tuple(x.shape), x.dtype, x.device))
+        if (out.stride(1) != 1 and out.shape[1] > 1) or (out.shape[0] > 1 and out.stride(0) < out.shape[1]):
+            raise ValueError("the rows of out must lie side by side or apart, got strides %s" % (out.stride(),))
+        return out
+
+    def values(self, *shape):
+        return _new(shape, dtype=_torch.float32, device=self.x.device)
 
     def run(self, name, grad, *args):
-        x = self.x
-        if not x.is_cuda:
+        x, dev = self.x, self.device
+        if dev < 0:
             raise ValueError("the scores must be on a GPU, got %s" % x.device)
-        s = _lib.EvtScores(x.data_ptr(), x.stride(0) if x.shape[0] > 1 else x.shape[1], None if grad is None else grad.data_ptr(),
-                           0 if grad is None else grad.stride(0) if x.shape[0] > 1 else x.shape[1], x.shape[0], x.shape[1], _FLOATS[x.dtype], self.temperature)
+        rows, classes = x.shape
+        s = _lib.EvtScores(x.data_ptr(), x.stride(0) if rows > 1 else classes, None if grad is None else grad.data_ptr(),
+                           0 if grad is None else grad.stride(0) if rows > 1 else classes, rows, classes, self.kind, self.temperature)
         call = getattr(_lib.load(), name)
-        dev = x.device.index
-        if dev == _torch.cuda.current_device():
-            _lib.check(call(_torch.cuda.current_stream(dev).cuda_stream, C.byref(s), *args, _TRUSTED))
+        if dev == _device():
+            rc = call(_stream(dev), C.byref(s), *args, _TRUSTED)
         else:
             with _torch.cuda.device(dev):
-                _lib.check(call(_torch.cuda.current_stream(dev).cuda_stream, C.byref(s), *args, _TRUSTED))
-
-
-def _at(v):
-    return None if v is None else v.data_ptr()
-
-
-def _made(x, *shape):
-    return _new(shape, dtype=_torch.float32, device=x.device)
+                rc = call(_stream(dev), C.byref(s), *args, _TRUSTED)
+        if rc:
+            _lib.check(rc)
 
 
 def class_logp(logits, labels, temperature=1.0):
     """Log-probability of every row's label under softmax(logits / temperature), and each row's maximum and sum of exponentials, which
     class_logp_grad takes: tensors (rows,) and (rows, 2), both float32.  Both are 0 for a row whose label is negative."""
-    _scores("logits", logits)
     call = _Call(logits, temperature)
-    _labels("labels", labels, logits)
-    rows = logits.shape[0]
-    logp, stats = _made(logits, rows), _made(logits, rows, 2)
-    call.run("evt_class_logp", None, labels.data_ptr(), _INTS[labels.dtype], logp.data_ptr(), stats.data_ptr())
+    rows = call.rows
+    at = call.check("labels", labels, (rows,), _INTS)
+    logp, stats = call.values(rows), call.values(rows, 2)
+    call.run("evt_class_logp", None, at, _INTS[labels.dtype], logp.data_ptr(), stats.data_ptr())
     return logp, stats
 
 
 def class_logp_grad(logits, labels, stats, dlogp, temperature=1.0, out=None):
     """Gradient of sum(dlogp * class_logp(logits, labels, temperature)[0]) by the logits, of the logits' type.  stats: what class_logp
     returned for the same logits and temperature."""
-    _scores("logits", logits)
     call = _Call(logits, temperature)
-    _labels("labels", labels, logits)
-    rows = logits.shape[0]
-    _check("stats", stats, logits, (rows, 2), (_torch.float32,), "float32")
-    _floats("dlogp", dlogp, logits, rows)
-    grad = _gradient(logits, True, out)
-    call.run("evt_class_logp_grad", grad, labels.data_ptr(), _INTS[labels.dtype], stats.data_ptr(), dlogp.data_ptr())
+    at = call.check("labels", labels, (call.rows,), _INTS)
+    stats_at, dlogp_at = call.check("stats", stats, (call.rows, 2), _F32S), call.floats("dlogp", dlogp)
+    grad = call.gradient(True, out)
+    call.run("evt_class_logp_grad", grad, at, _INTS[labels.dtype], stats_at, dlogp_at)
     return grad
 
 
@@ -151,20 +159,16 @@ def distill_loss(logits, top_ids, top_logits, temperature=1.0, weights=None, gra
     softmax(logits / temperature)), and the gradient of the sum of all rows' losses by the logits (None with grad=False).
 
     top_ids, top_logits: (rows, n_top), at most 1024 entries; a negative id is no entry.  top_logits may be float32, bfloat16 or float16."""
-    _scores("logits", logits)
     call = _Call(logits, temperature)
-    rows = logits.shape[0]
+    rows = call.rows
     if not isinstance(top_ids, _torch.Tensor) or top_ids.dim() != 2 or not 1 <= top_ids.shape[1] <= 1024:
         raise ValueError("top_ids must be a (rows, n_top) tensor with n_top from 1 to 1024")
     shape = (rows, top_ids.shape[1])
-    _check("top_ids", top_ids, logits, shape, _INTS, "int32 or int64")
-    _check("top_logits", top_logits, logits, shape, _FLOATS, "float32, bfloat16 or float16")
-    if weights is not None:
-        _floats("weights", weights, logits, rows)
-    g = _gradient(logits, grad, out)
-    loss = _made(logits, rows)
-    call.run("evt_distill_loss", g, top_ids.data_ptr(), _INTS[top_ids.dtype], top_logits.data_ptr(), _FLOATS[top_logits.dtype], shape[1], _at(weights),
-             loss.data_ptr())
+    ids_at, top_at = call.check("top_ids", top_ids, shape, _INTS), call.check("top_logits", top_logits, shape, _FLOATS)
+    weights_at = call.optional("weights", weights, rows)
+    g = call.gradient(grad, out)
+    loss = call.values(rows)
+    call.run("evt_distill_loss", g, ids_at, _INTS[top_ids.dtype], top_at, _FLOATS[top_logits.dtype], shape[1], weights_at, loss.data_ptr())
     return loss, g
 
 
@@ -175,24 +179,18 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, clip_low=0
     With r = exp(logp - old_logp) the loss is weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(b) - b - 1)), A the
     advantage and b = ref_logp - logp.  A negative action marks a padded row: its loss, log-probability and gradient are 0.  A weight of 0 leaves
     the log-probability."""
-    _scores("logits", logits)
     call = _Call(logits, temperature)
-    rows = logits.shape[0]
-    _labels("actions", actions, logits)
-    _floats("old_logp", old_logp, logits, rows)
-    _floats("advantages", advantages, logits, rows)
-    clip_low, clip_high = _number("clip_low", clip_low, 0.0, 1.0), _number("clip_high", clip_high, 0.0, float("inf"))
-    kl_coef = _number("kl_coef", kl_coef, 0.0, float("inf"))
-    if ref_logp is not None:
-        _floats("ref_logp", ref_logp, logits, rows)
-    elif kl_coef:
+    at = call.check("actions", actions, (call.rows,), _INTS)
+    old_at, advantages_at = call.floats("old_logp", old_logp), call.floats("advantages", advantages)
+    clip_low, clip_high = _number("clip_low", clip_low, 0.0, 1.0), _number("clip_high", clip_high, 0.0, _INF)
+    kl_coef = _number("kl_coef", kl_coef, 0.0, _INF)
+    ref_at, weights_at = call.optional("ref_logp", ref_logp, call.rows), call.optional("weights", weights, call.rows)
+    if ref_at is None and kl_coef:
         raise ValueError("kl_coef needs ref_logp")
-    if weights is not None:
-        _floats("weights", weights, logits, rows)
-    g = _gradient(logits, grad, out)
-    loss, logp = _made(logits, rows), _made(logits, rows)
-    call.run("evt_policy_loss", g, actions.data_ptr(), _INTS[actions.dtype], old_logp.data_ptr(), advantages.data_ptr(), _at(ref_logp), _at(weights),
-             clip_low, clip_high, kl_coef, loss.data_ptr(), logp.data_ptr())
+    g = call.gradient(grad, out)
+    loss, logp = _like(old_logp), _like(old_logp)
+    call.run("evt_policy_loss", g, at, _INTS[actions.dtype], old_at, advantages_at, ref_at, weights_at, clip_low, clip_high, kl_coef,
+             loss.data_ptr(), logp.data_ptr())
     return loss, logp, g
 
 
@@ -206,22 +204,18 @@ def preference_loss(logits, labels, offsets, ref_logp, beta=0.1, label_smoothing
     With h = beta ((chosen - rejected) - (ref chosen - ref rejected)) - margin a pair's loss is weights * (-(1 - label_smoothing) log sigmoid(h)
     - label_smoothing log sigmoid(-h)).  Rows of no sequence get a gradient of 0; offsets that do not ascend or leave the rows
     make their pair's results NaN."""
-    _scores("logits", logits)
     call = _Call(logits, temperature)
-    rows = logits.shape[0]
-    _labels("labels", labels, logits)
+    at = call.check("labels", labels, (call.rows,), _INTS)
     if not isinstance(offsets, _torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:
         raise ValueError("offsets must be a vector of an odd number of row numbers, at least 3: one more than there are sequences")
-    _check("offsets", offsets, logits, tuple(offsets.shape), (_torch.int32,), "int32")
     seqs = offsets.shape[0] - 1
-    _floats("ref_logp", ref_logp, logits, seqs)
-    beta = _number("beta", beta, 0.0, float("inf"), True)
+    offsets_at, ref_at = call.check("offsets", offsets, (seqs + 1,), _I32S), call.check("ref_logp", ref_logp, (seqs,), _F32S)
+    beta = _number("beta", beta, 0.0, _INF, True)
     label_smoothing = _number("label_smoothing", label_smoothing, 0.0, 0.5)
-    margin = _number("margin", margin, -float("inf"), float("inf"))
-    if weights is not None:
-        _floats("weights", weights, logits, seqs // 2)
-    g = _gradient(logits, grad, out)
-    loss, seq_logp, work = _made(logits, seqs // 2), _made(logits, seqs), _made(logits, 4 * rows)
-    call.run("evt_preference_loss", g, labels.data_ptr(), _INTS[labels.dtype], offsets.data_ptr(), seqs // 2, ref_logp.data_ptr(), _at(weights),
-             beta, label_smoothing, margin, 1 if average else 0, loss.data_ptr(), seq_logp.data_ptr(), work.data_ptr())
+    margin = _number("margin", margin, -_INF, _INF)
+    weights_at = call.optional("weights", weights, seqs // 2)
+    g = call.gradient(grad, out)
+    loss, seq_logp, work = call.values(seqs // 2), _like(ref_logp), call.values(4 * call.rows)
+    call.run("evt_preference_loss", g, at, _INTS[labels.dtype], offsets_at, seqs // 2, ref_at, weights_at, beta, label_smoothing, margin,
+             1 if average else 0, loss.data_ptr(), seq_logp.data_ptr(), work.data_ptr())
     return loss, seq_logp, g

@@ -70,10 +70,6 @@ struct MaxSum {
 };
 #define LOWEST (-3.402823466e38f)
 __device__ __forceinline__ float exp_of(float x, float m, float mul) { return __builtin_amdgcn_exp2f((x - m) * mul); }
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float mul) {
-    const float m = fmaxf(a.m, b.m);
-    return {m, a.s * exp_of(a.m, m, mul) + b.s * exp_of(b.m, m, mul)};
-}
 // a with E more scores
 template <int E>
 __device__ __forceinline__ MaxSum take(MaxSum a, const float *f, float mul) {
@@ -89,13 +85,41 @@ __device__ __forceinline__ MaxSum take(MaxSum a, const float *f, float mul) {
         for (int k = 0; k < w; k++) s[k] += s[k + w];
     return {m, a.s * exp_of(a.m, m, mul) + s[0]};
 }
-__device__ __forceinline__ MaxSum lanes_join(MaxSum a, int lanes, float mul) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) a = join(a, {__shfl_xor(a.m, o), __shfl_xor(a.s, o)}, mul);
-    return a;
+// Reductions over G neighbouring lanes whose result every one of them has: by moves within rows of sixteen lanes and gfx950's swaps of rows between two
+// registers, a few cycles a step where a trip through the LDS crossbar is a hundred (8 rows of 32 768 classes: XX -> YY us a launch).
+template <int CTRL>
+__device__ __forceinline__ float moved(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false));
 }
-__device__ __forceinline__ float lanes_sum(float v, int lanes) {
-    for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+template <int G, typename F>
+__device__ __forceinline__ float over_lanes(float v, F &&f) {
+    if (G >= 2) v = f(v, moved<0xB1>(v));   // quad_perm: lane ^ 1
+    if (G >= 4) v = f(v, moved<0x4E>(v));   // quad_perm: lane ^ 2
+    if (G >= 8) v = f(v, moved<0x141>(v));  // row_half_mirror: the other four of eight
+    if (G >= 16) v = f(v, moved<0x140>(v)); // row_mirror: the other eight of sixteen
+    if (G >= 32) {
+        const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    }
+    if (G >= 64) {
+        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = f(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    }
     return v;
+}
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v) {
+    return over_lanes<G>(v, [](float x, float y) { return x + y; });
+}
+template <int G>
+__device__ __forceinline__ MaxSum lanes_join(MaxSum a, float mul) {
+    const float m = over_lanes<G>(a.m, [](float x, float y) { return fmaxf(x, y); });
+    return {m, lanes_sum<G>(a.s * exp_of(a.m, m, mul))};
+}
+template <int G>
+__device__ __forceinline__ bool lanes_any(bool v) {
+    const uint64_t set = __ballot(v);
+    return G == 64 ? set != 0 : ((set >> (threadIdx.x & 63 & ~(G - 1))) & ((1ull << (G & 63)) - 1)) != 0;
 }
 
 // The threads that share a row: G lanes of a wavefront, or W whole wavefronts, a block.  LANES of them, the first, look after a teacher's entries.
@@ -109,7 +133,7 @@ struct Lanes {
         __builtin_amdgcn_wave_barrier();
     }
     __device__ static MaxSum all(MaxSum a, float mul) { // the group's joined; what its lanes wrote to shared memory before can be read
-        a = lanes_join(a, G, mul);
+        a = lanes_join<G>(a, mul);
         sync();
         return a;
     }
@@ -122,13 +146,10 @@ struct Waves {
     __device__ static void sync() { __syncthreads(); }
     __device__ static MaxSum all(MaxSum a, float mul) {
         __shared__ MaxSum s_a[W];
-        a = lanes_join(a, 64, mul);
+        a = lanes_join<64>(a, mul);
         if ((threadIdx.x & 63) == 0) s_a[threadIdx.x >> 6] = a;
         __syncthreads();
-        a = s_a[0];
-#pragma unroll
-        for (int w = 1; w < W; w++) a = join(a, s_a[w], mul);
-        return a;
+        return lanes_join<W>(s_a[threadIdx.x & (W - 1)], mul);
     }
 };
 
@@ -249,6 +270,15 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     float w = 1.0f, x_label = 0.0f, given = 0.0f;
     bool live = true, bad = false;
     int64_t label = -1;
+    Piece<T> p[NV];
+    const auto load_row = [&]() {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int o = (t + i * G::SIZE) * E;
+            p[i].load(x, o + E <= V ? o : V - E); // past the row's end: the last piece, which counts once
+        }
+    };
+    if (a.early) load_row(); // whether the row counts or not
     if (OP == SC_DISTILL) {
         w = a.weights ? a.weights[row] : 1.0f;
         live = w != 0.0f;
@@ -268,17 +298,13 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         if (OP != SC_LOGP && g) clear_row(g, V, t, G::SIZE);
         return;
     }
-    Piece<T> p[NV];
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int o = (t + i * G::SIZE) * E;
-        p[i].load(x, o + E <= V ? o : V - E); // past the row's end: the last piece, which counts once
-    }
+    if (!a.early) load_row();
     int2 *const s_top = (int2 *)s_dyn + (size_t)G::slot() * a.n_top;
     float *const s_x = (float *)((int2 *)s_dyn + (size_t)G::ROWS * a.n_top) + (size_t)G::slot() * a.n_top;
     MaxSum teacher = {LOWEST, 0.0f};
     if (OP == SC_DISTILL && t < G::LANES) {
         bool none = false;
+#pragma unroll 1
         for (int j = t; j < a.n_top; j += G::LANES) {
             const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
             const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
@@ -288,9 +314,10 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
             s_x[j] = in ? (float)x[id] : 0.0f;
             teacher = take<1>(teacher, &s, mul);
         }
-        teacher = lanes_join(teacher, G::LANES, mul);
-        for (int o = G::LANES >> 1; o > 0; o >>= 1) none |= __shfl_xor((int)none, o) != 0;
+        teacher = lanes_join<G::LANES>(teacher, mul);
+        none = lanes_any<G::LANES>(none);
         if (t == 0) s_state[G::slot()] = teacher.s == 0.0f ? 0 : none ? 2 : 1; // a sum that is no number is a teacher
+#pragma unroll 1
         for (int j = t; j < a.n_top; j += G::LANES) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) / teacher.s);
     }
     MaxSum r = {LOWEST, 0.0f};
@@ -348,6 +375,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         if (t < G::LANES) {
             const double log_ts = log_sum(teacher.s), log_s = log_sum(r.s);
             float sum = 0.0f;
+#pragma unroll 1
             for (int j = t; j < a.n_top; j += G::LANES) {
                 const int2 e = s_top[j];
                 const float pj = __int_as_float(e.y);
@@ -357,7 +385,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
                     sum += pj * (float)((double)(tj - teacher.m) * a.inv_t - log_ts - lq);
                 }
             }
-            sum = lanes_sum(sum, G::LANES);
+            sum = lanes_sum<G::LANES>(sum);
             if (t == 0) a.loss[row] = state == 2 ? NAN : w * a.t2_mul * sum;
         }
         factor = state == 2 ? NAN : w * a.t_mul;
@@ -620,7 +648,8 @@ __global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, int pairs, c
 
 // LAUNCH of the form that a row of n pieces takes
 template <typename T, int OP, int NV, class G>
-static void launch_rows(hipStream_t s, const ScoreArgs &a) {
+static void launch_rows(hipStream_t s, ScoreArgs a) {
+    a.early = a.N <= 512;
     const size_t lds = OP == SC_DISTILL ? (size_t)G::ROWS * a.n_top * 12 : 0;
     hipLaunchKernelGGL((k_rows<T, OP, NV, G>), dim3((unsigned)((a.N + G::ROWS - 1) / G::ROWS)), dim3(G::THREADS), lds, s, a);
 }

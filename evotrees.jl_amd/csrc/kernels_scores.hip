@@ -260,7 +260,10 @@ template <typename T, int OP, int NV, class G>
 __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     constexpr int E = Piece<T>::E;
     extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs for each of the block's rows, then scores
-    __shared__ int s_state[G::ROWS];         // SC_DISTILL: 1 a teacher, 2 and an id of no class
+    __shared__ int s_state[G::ROWS];         // SC_DISTILL: 1 a teacher, 2 and an id of no class, 4 an id that may come twice
+    // a bit for every class of a group's row: which the teacher has named (a block's row has too many)
+    constexpr int WORDS = G::ROWS > 1 && OP == SC_DISTILL ? (G::SIZE * NV * E + 31) / 32 : 1;
+    __shared__ uint32_t s_named[G::ROWS * WORDS];
     const int64_t row = (int64_t)blockIdx.x * G::ROWS + G::slot();
     if (G::ROWS > 1 && row >= a.N) return;
     const int t = G::rank(), V = a.V;
@@ -275,7 +278,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int o = (t + i * G::SIZE) * E;
-            p[i].load(x, o + E <= V ? o : V - E); // past the row's end: the last piece, which counts once
+            if (i * G::SIZE * E < V) p[i].load(x, o + E <= V ? o : V - E); // past the row's end: the last piece, which counts once
         }
     };
     if (a.early) load_row(); // whether the row counts or not
@@ -303,7 +306,12 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     float *const s_x = (float *)((int2 *)s_dyn + (size_t)G::ROWS * a.n_top) + (size_t)G::slot() * a.n_top;
     MaxSum teacher = {LOWEST, 0.0f};
     if (OP == SC_DISTILL && t < G::LANES) {
-        bool none = false;
+        bool none = false, twice = G::ROWS == 1;
+        uint32_t *const named = s_named + G::slot() * WORDS;
+        if (G::ROWS > 1) {
+            for (int k = t; k < WORDS; k += G::LANES) named[k] = 0u;
+            G::sync();
+        }
 #pragma unroll 1
         for (int j = t; j < a.n_top; j += G::LANES) {
             const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
@@ -312,13 +320,18 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
             none |= id >= V;
             s_top[j] = {in ? (int)id : -1, __float_as_int(s)};
             s_x[j] = in ? (float)x[id] : 0.0f;
+            if (G::ROWS > 1 && in) {
+                const uint32_t bit = 1u << (id & 31);
+                twice |= (atomicOr(named + (id >> 5), bit) & bit) != 0;
+            }
             teacher = take<1>(teacher, &s, mul);
         }
         teacher = lanes_join<G::LANES>(teacher, mul);
         none = lanes_any<G::LANES>(none);
-        if (t == 0) s_state[G::slot()] = teacher.s == 0.0f ? 0 : none ? 2 : 1; // a sum that is no number is a teacher
+        twice = lanes_any<G::LANES>(twice);
+        if (t == 0) s_state[G::slot()] = teacher.s == 0.0f ? 0 : (none ? 2 : 1) | (twice ? 4 : 0); // a sum that is no number is a teacher
 #pragma unroll 1
-        for (int j = t; j < a.n_top; j += G::LANES) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) / teacher.s);
+        for (int j = t; j < a.n_top; j += G::LANES) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) * (1.0f / teacher.s));
     }
     MaxSum r = {LOWEST, 0.0f};
     if (OP == SC_GRAD) {
@@ -365,6 +378,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     }
     const float inv = inverse_sum(r);
     float fq, slope = 0.0f, factor = 0.0f;
+    bool twice = false;
     if (OP == SC_DISTILL) {
         const int state = s_state[G::slot()];
         if (state == 0) {
@@ -373,22 +387,20 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
             return;
         }
         if (t < G::LANES) {
-            const double log_ts = log_sum(teacher.s), log_s = log_sum(r.s);
+            // log p_j - log q_j = ((t_j - t_max) - (x_j - m)) / T + log(S / S_teacher), and the p_j add up to 1
+            const double logs = r.s == 0.0f ? 0.0 : log_sum(r.s) - log_sum(teacher.s);
             float sum = 0.0f;
 #pragma unroll 1
             for (int j = t; j < a.n_top; j += G::LANES) {
                 const int2 e = s_top[j];
                 const float pj = __int_as_float(e.y);
-                if (e.x >= 0 && pj != 0.0f) {
-                    const float tj = load_score(a.top, a.top_type, row * a.n_top + j);
-                    const double lq = r.s == 0.0f ? -INFINITY : (double)(s_x[j] - r.m) * a.inv_t - log_s;
-                    sum += pj * (float)((double)(tj - teacher.m) * a.inv_t - log_ts - lq);
-                }
+                if (e.x >= 0 && pj != 0.0f) sum += pj * ((load_score(a.top, a.top_type, row * a.n_top + j) - teacher.m) - (s_x[j] - r.m));
             }
             sum = lanes_sum<G::LANES>(sum);
-            if (t == 0) a.loss[row] = state == 2 ? NAN : w * a.t2_mul * sum;
+            if (t == 0) a.loss[row] = state & 2 ? NAN : w * a.t2_mul * (float)((double)sum * a.inv_t + logs);
         }
-        factor = state == 2 ? NAN : w * a.t_mul;
+        factor = state & 2 ? NAN : w * a.t_mul;
+        twice = (state & 4) != 0;
     } else {
         slope = labelled_row<OP>(a, row, bad, r, x_label, given, t == 0);
         if (OP == SC_POLICY && slope == 0.0f && g) { // clipped, or of no weight
@@ -433,10 +445,13 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         for (int j = t; j < a.n_top; j += G::SIZE) {
             const int id = s_top[j].x;
             if (id < 0) continue;
-            float pj = 0.0f; // an id that comes twice has both shares
-            for (int i = 0; i < a.n_top; i++) {
-                const int2 e = s_top[i];
-                pj += e.x == id ? __int_as_float(e.y) : 0.0f;
+            float pj = __int_as_float(s_top[j].y);
+            if (twice) { // an id that comes twice has both shares
+                pj = 0.0f;
+                for (int i = 0; i < a.n_top; i++) {
+                    const int2 e = s_top[i];
+                    pj += e.x == id ? __int_as_float(e.y) : 0.0f;
+                }
             }
             g[id] = (T)(factor * (exp_of(s_x[j], r.m, mul) * inv - pj));
         }
@@ -469,15 +484,16 @@ __global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
         bad = live && label >= V;
     }
     float f[KM], p[KM]; // p: the teacher's share of each class
-    MaxSum teacher = {LOWEST, 0.0f};
+    float most = LOWEST;
     if (OP == SC_DISTILL && live) {
+        live = false;
         for (int j = 0; j < a.n_top; j++) {
             const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
             const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
             bad |= id >= V;
-            teacher = take<1>(teacher, &s, mul);
+            live |= s != -INFINITY;
+            most = fmaxf(most, s);
         }
-        live = teacher.s != 0.0f;
     }
     if (!live) {
         left_out<OP>(a, row);
@@ -497,25 +513,26 @@ __global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
     if (OP == SC_DISTILL) {
 #pragma unroll
         for (int k = 0; k < KM; k++) p[k] = 0.0f;
-        const double log_ts = log_sum(teacher.s), log_s = log_sum(r.s);
-        float sum = 0.0f;
+        float sum = 0.0f, total = 0.0f;
         for (int j = 0; j < a.n_top; j++) {
             const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
             if (id < 0 || id >= V) continue;
-            const float tj = load_score(a.top, a.top_type, row * a.n_top + j);
-            const float pj = exp_of(tj, teacher.m, mul) / teacher.s;
+            const float d = load_score(a.top, a.top_type, row * a.n_top + j) - most, e = __builtin_amdgcn_exp2f(d * mul);
             float xj = 0.0f;
 #pragma unroll
             for (int k = 0; k < KM; k++) {
-                p[k] += k == (int)id ? pj : 0.0f;
+                p[k] += k == (int)id ? e : 0.0f;
                 xj = k == (int)id ? f[k] : xj;
             }
-            if (pj != 0.0f) {
-                const double lq = r.s == 0.0f ? -INFINITY : (double)(xj - r.m) * a.inv_t - log_s;
-                sum += pj * (float)((double)(tj - teacher.m) * a.inv_t - log_ts - lq);
-            }
+            total += e;
+            if (e != 0.0f) sum += e * (d - (xj - r.m));
         }
-        a.loss[row] = bad ? NAN : w * a.t2_mul * sum;
+        const float one = 1.0f / total;
+#pragma unroll
+        for (int k = 0; k < KM; k++) p[k] *= one;
+        // as in k_rows; both sums are between 1 and a small number
+        const float logs = r.s == 0.0f ? 0.0f : logf(r.s * one);
+        a.loss[row] = bad ? NAN : w * a.t2_mul * ((float)(sum * one * a.inv_t) + logs);
         factor = bad ? NAN : w * a.t_mul;
     } else {
         float x_label = 0.0f;
@@ -657,35 +674,38 @@ template <typename T, int OP>
 static void launch_typed(hipStream_t s, const ScoreArgs &a) {
     constexpr int E = Piece<T>::E;
     const int64_t n = ((int64_t)a.V + E - 1) / E;
-    if (a.V <= 16) {
+    if (a.V < E) {
         const dim3 grid((unsigned)((a.N + 255) / 256)), block(256);
-        if (a.V <= 4) hipLaunchKernelGGL((k_few_classes<T, OP, 4>), grid, block, 0, s, a);
-        else if (a.V <= 8) hipLaunchKernelGGL((k_few_classes<T, OP, 8>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((k_few_classes<T, OP, 16>), grid, block, 0, s, a);
+        hipLaunchKernelGGL((k_few_classes<T, OP, E>), grid, block, 0, s, a);
         return;
     }
     if (n <= 256) {
-        // a group's rows share a block's memory with their teachers
+        // lanes to a row: four pieces each, and no more teachers than a block's memory holds (48 KB)
         const int top = OP == SC_DISTILL ? a.n_top : 0;
-        if (n <= 8 && top <= 64) return launch_rows<T, OP, 1, Lanes<8>>(s, a);
-        if (n <= 16 && top <= 128) return launch_rows<T, OP, 1, Lanes<16>>(s, a);
-        if (n <= 32 && top <= 256) return launch_rows<T, OP, 1, Lanes<32>>(s, a);
-        if (n <= 64) return launch_rows<T, OP, 1, Lanes<64>>(s, a);
+        if (n <= 4 && top <= 16) return launch_rows<T, OP, 4, Lanes<1>>(s, a);
+        if (n <= 8 && top <= 32) return launch_rows<T, OP, 4, Lanes<2>>(s, a);
+        if (n <= 16 && top <= 64) return launch_rows<T, OP, 4, Lanes<4>>(s, a);
+        if (n <= 32 && top <= 128) return launch_rows<T, OP, 4, Lanes<8>>(s, a);
+        if (n <= 64 && top <= 256) return launch_rows<T, OP, 4, Lanes<16>>(s, a);
+        if (n <= 128 && top <= 512) return launch_rows<T, OP, 4, Lanes<32>>(s, a);
         return launch_rows<T, OP, 4, Lanes<64>>(s, a);
     }
     if constexpr (OP == SC_GRAD) {
         const int64_t parts = (n + 1023) / 1024, blocks = a.N * parts;
         hipLaunchKernelGGL(k_slope_rows<T>, dim3((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30))), dim3(256), 0, s, a, (int)parts);
     } else {
-        if (n <= 1024) return launch_rows<T, OP, 4, Waves<4>>(s, a);
-        if (OP != SC_LOGP && a.g) { // the row stays in registers
-            if constexpr (OP != SC_LOGP) {
-                if (n <= 2048) return launch_rows<T, OP, 2, Waves<16>>(s, a);
-                if (n > 8192) return launch_rows<T, OP, 16, Waves<16>>(s, a);
-                if (n > 4096) return launch_rows<T, OP, 8, Waves<16>>(s, a);
-            }
+        const bool few = a.N <= 256;
+        if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
+        if (OP == SC_LOGP || !a.g) return few ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 4, Waves<4>>(s, a);
+        // the row stays in registers
+        if constexpr (OP != SC_LOGP) {
+            if (few) return n <= 4096 ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 16, Waves<16>>(s, a);
+            if (n <= 1024) return launch_rows<T, OP, 4, Waves<4>>(s, a);
+            if (n <= 2048) return launch_rows<T, OP, 8, Waves<4>>(s, a);
+            if (n <= 4096) return launch_rows<T, OP, 16, Waves<4>>(s, a);
+            if (n <= 8192) return launch_rows<T, OP, 16, Waves<8>>(s, a);
+            return launch_rows<T, OP, 16, Waves<16>>(s, a);
         }
-        return launch_rows<T, OP, 4, Waves<16>>(s, a);
     }
 }
 template <int OP>

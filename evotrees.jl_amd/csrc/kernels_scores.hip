@@ -86,7 +86,7 @@ __device__ __forceinline__ MaxSum take(MaxSum a, const float *f, float mul) {
     return {m, a.s * exp_of(a.m, m, mul) + s[0]};
 }
 // Reductions over G neighbouring lanes whose result every one of them has: by moves within rows of sixteen lanes and gfx950's swaps of rows between two
-// registers, a few cycles a step where a trip through the LDS crossbar is a hundred (8 rows of 32 768 classes: XX -> YY us a launch).
+// registers, a few cycles a step where a trip through the LDS crossbar is a hundred (with the scores requested early, 8 rows of 32 768 classes take 4.8 us for 6.3).
 template <int CTRL>
 __device__ __forceinline__ float moved(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false));
@@ -122,10 +122,10 @@ __device__ __forceinline__ bool lanes_any(bool v) {
     return G == 64 ? set != 0 : ((set >> (threadIdx.x & 63 & ~(G - 1))) & ((1ull << (G & 63)) - 1)) != 0;
 }
 
-// The threads that share a row: G lanes of a wavefront, or W whole wavefronts, a block.  LANES of them, the first, look after a teacher's entries.
+// The threads that share a row: G lanes of a wavefront, or W whole wavefronts, a block.
 template <int G>
 struct Lanes {
-    static constexpr int SIZE = G, LANES = G, ROWS = 256 / G, THREADS = 256;
+    static constexpr int SIZE = G, ROWS = 256 / G, THREADS = 256;
     __device__ static int rank() { return threadIdx.x & (G - 1); }
     __device__ static int slot() { return threadIdx.x / G; } // of the block's rows
     __device__ static void sync() {
@@ -140,7 +140,7 @@ struct Lanes {
 };
 template <int W>
 struct Waves {
-    static constexpr int SIZE = 64 * W, LANES = 64, ROWS = 1, THREADS = 64 * W;
+    static constexpr int SIZE = 64 * W, ROWS = 1, THREADS = 64 * W;
     __device__ static int rank() { return threadIdx.x; }
     __device__ static int slot() { return 0; }
     __device__ static void sync() { __syncthreads(); }
@@ -259,11 +259,9 @@ __device__ __forceinline__ void gradients(float *f, MaxSum r, float fq, float mu
 template <typename T, int OP, int NV, class G>
 __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     constexpr int E = Piece<T>::E;
-    extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs for each of the block's rows, then scores
-    __shared__ int s_state[G::ROWS];         // SC_DISTILL: 1 a teacher, 2 and an id of no class, 4 an id that may come twice
-    // a bit for every class of a group's row: which the teacher has named (a block's row has too many)
-    constexpr int WORDS = G::ROWS > 1 && OP == SC_DISTILL ? (G::SIZE * NV * E + 31) / 32 : 1;
-    __shared__ uint32_t s_named[G::ROWS * WORDS];
+    static_assert(OP != SC_DISTILL || G::ROWS == 1, "k_distill_short has the others");
+    extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs, then the scores of these classes
+    __shared__ int s_state;                  // SC_DISTILL: 1 a teacher, 2 with an id of no class
     const int64_t row = (int64_t)blockIdx.x * G::ROWS + G::slot();
     if (G::ROWS > 1 && row >= a.N) return;
     const int t = G::rank(), V = a.V;
@@ -302,36 +300,26 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         return;
     }
     if (!a.early) load_row();
-    int2 *const s_top = (int2 *)s_dyn + (size_t)G::slot() * a.n_top;
-    float *const s_x = (float *)((int2 *)s_dyn + (size_t)G::ROWS * a.n_top) + (size_t)G::slot() * a.n_top;
+    int2 *const s_top = (int2 *)s_dyn;
+    float *const s_x = (float *)(s_top + a.n_top);
     MaxSum teacher = {LOWEST, 0.0f};
-    if (OP == SC_DISTILL && t < G::LANES) {
-        bool none = false, twice = G::ROWS == 1;
-        uint32_t *const named = s_named + G::slot() * WORDS;
-        if (G::ROWS > 1) {
-            for (int k = t; k < WORDS; k += G::LANES) named[k] = 0u;
-            G::sync();
-        }
+    if (OP == SC_DISTILL && t < 64) { // the first wavefront looks after the teacher while the row is on its way
+        bool none = false;
 #pragma unroll 1
-        for (int j = t; j < a.n_top; j += G::LANES) {
+        for (int j = t; j < a.n_top; j += 64) {
             const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
             const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
             const bool in = id >= 0 && id < V;
             none |= id >= V;
             s_top[j] = {in ? (int)id : -1, __float_as_int(s)};
             s_x[j] = in ? (float)x[id] : 0.0f;
-            if (G::ROWS > 1 && in) {
-                const uint32_t bit = 1u << (id & 31);
-                twice |= (atomicOr(named + (id >> 5), bit) & bit) != 0;
-            }
             teacher = take<1>(teacher, &s, mul);
         }
-        teacher = lanes_join<G::LANES>(teacher, mul);
-        none = lanes_any<G::LANES>(none);
-        twice = lanes_any<G::LANES>(twice);
-        if (t == 0) s_state[G::slot()] = teacher.s == 0.0f ? 0 : (none ? 2 : 1) | (twice ? 4 : 0); // a sum that is no number is a teacher
+        teacher = lanes_join<64>(teacher, mul);
+        none = __any(none);
+        if (t == 0) s_state = teacher.s == 0.0f ? 0 : none ? 2 : 1; // a sum that is no number is a teacher
 #pragma unroll 1
-        for (int j = t; j < a.n_top; j += G::LANES) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) * (1.0f / teacher.s));
+        for (int j = t; j < a.n_top; j += 64) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) * (1.0f / teacher.s));
     }
     MaxSum r = {LOWEST, 0.0f};
     if (OP == SC_GRAD) {
@@ -378,29 +366,27 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     }
     const float inv = inverse_sum(r);
     float fq, slope = 0.0f, factor = 0.0f;
-    bool twice = false;
     if (OP == SC_DISTILL) {
-        const int state = s_state[G::slot()];
+        const int state = s_state;
         if (state == 0) {
             if (t == 0) left_out<OP>(a, row);
             if (g) clear_row(g, V, t, G::SIZE);
             return;
         }
-        if (t < G::LANES) {
+        if (t < 64) {
             // log p_j - log q_j = ((t_j - t_max) - (x_j - m)) / T + log(S / S_teacher), and the p_j add up to 1
             const double logs = r.s == 0.0f ? 0.0 : log_sum(r.s) - log_sum(teacher.s);
             float sum = 0.0f;
 #pragma unroll 1
-            for (int j = t; j < a.n_top; j += G::LANES) {
+            for (int j = t; j < a.n_top; j += 64) {
                 const int2 e = s_top[j];
                 const float pj = __int_as_float(e.y);
                 if (e.x >= 0 && pj != 0.0f) sum += pj * ((load_score(a.top, a.top_type, row * a.n_top + j) - teacher.m) - (s_x[j] - r.m));
             }
-            sum = lanes_sum<G::LANES>(sum);
-            if (t == 0) a.loss[row] = state & 2 ? NAN : w * a.t2_mul * (float)((double)sum * a.inv_t + logs);
+            sum = lanes_sum<64>(sum);
+            if (t == 0) a.loss[row] = state == 2 ? NAN : w * a.t2_mul * (float)((double)sum * a.inv_t + logs);
         }
-        factor = state & 2 ? NAN : w * a.t_mul;
-        twice = (state & 4) != 0;
+        factor = state == 2 ? NAN : w * a.t_mul;
     } else {
         slope = labelled_row<OP>(a, row, bad, r, x_label, given, t == 0);
         if (OP == SC_POLICY && slope == 0.0f && g) { // clipped, or of no weight
@@ -445,112 +431,231 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         for (int j = t; j < a.n_top; j += G::SIZE) {
             const int id = s_top[j].x;
             if (id < 0) continue;
-            float pj = __int_as_float(s_top[j].y);
-            if (twice) { // an id that comes twice has both shares
-                pj = 0.0f;
-                for (int i = 0; i < a.n_top; i++) {
-                    const int2 e = s_top[i];
-                    pj += e.x == id ? __int_as_float(e.y) : 0.0f;
-                }
+            float pj = 0.0f; // an id that comes twice has both shares
+            for (int i = 0; i < a.n_top; i++) {
+                const int2 e = s_top[i];
+                pj += e.x == id ? __int_as_float(e.y) : 0.0f;
             }
             g[id] = (T)(factor * (exp_of(s_x[j], r.m, mul) * inv - pj));
         }
     }
 }
 
-// A row to a thread: up to KM classes.
-template <typename T, int OP, int KM>
+// A row to a thread: fewer classes than a piece has.
+template <typename T, int OP>
 __global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
+    constexpr int KM = Piece<T>::E;
     const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (row >= a.N) return;
     const int V = a.V;
     const T *x = (const T *)a.x + row * a.xs;
     T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
-    const float mul = a.exp_mul;
-    float w = 1.0f, given = 0.0f;
-    bool live = true, bad = false;
-    int64_t label = -1;
-    if (OP == SC_DISTILL) {
-        w = a.weights ? a.weights[row] : 1.0f;
-        live = w != 0.0f;
-    } else {
-        label = load_id(a.labels, a.label64, row);
-        live = label >= 0;
-        if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
-        if (OP == SC_GRAD && live) {
-            given = a.slope[row];
-            live = given != 0.0f;
-        }
-        bad = live && label >= V;
+    const int64_t label = load_id(a.labels, a.label64, row);
+    float given = 0.0f;
+    bool live = label >= 0;
+    if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
+    if (OP == SC_GRAD && live) {
+        given = a.slope[row];
+        live = given != 0.0f;
     }
-    float f[KM], p[KM]; // p: the teacher's share of each class
-    float most = LOWEST;
-    if (OP == SC_DISTILL && live) {
-        live = false;
-        for (int j = 0; j < a.n_top; j++) {
-            const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
-            const float s = id < 0 ? -INFINITY : load_score(a.top, a.top_type, row * a.n_top + j);
-            bad |= id >= V;
-            live |= s != -INFINITY;
-            most = fmaxf(most, s);
-        }
-    }
+    const bool bad = live && label >= V;
     if (!live) {
         left_out<OP>(a, row);
-        if (OP != SC_LOGP && g)
-            for (int c = 0; c < V; c++) g[c] = (T)0.0f;
+        if (OP != SC_LOGP && g) clear_row(g, V, 0, 1);
         return;
     }
+    float f[KM], x_label = 0.0f;
 #pragma unroll
     for (int k = 0; k < KM; k++) f[k] = (float)x[k < V ? k : V - 1];
 #pragma unroll
-    for (int k = 0; k < KM; k++) f[k] = k < V ? f[k] : -INFINITY;
+    for (int k = 0; k < KM; k++) {
+        f[k] = k < V ? f[k] : -INFINITY;
+        x_label = k == (int)label ? f[k] : x_label;
+    }
     MaxSum r = {LOWEST, 0.0f};
     if (OP == SC_GRAD) r = {fmaxf(a.stats[2 * row], LOWEST), a.stats[2 * row + 1]};
-    else r = take<KM>(r, f, mul);
-    const float inv = inverse_sum(r);
-    float factor, slope = 0.0f;
-    if (OP == SC_DISTILL) {
-#pragma unroll
-        for (int k = 0; k < KM; k++) p[k] = 0.0f;
-        float sum = 0.0f, total = 0.0f;
-        for (int j = 0; j < a.n_top; j++) {
-            const int64_t id = load_id(a.ids, a.id64, row * a.n_top + j);
-            if (id < 0 || id >= V) continue;
-            const float d = load_score(a.top, a.top_type, row * a.n_top + j) - most, e = __builtin_amdgcn_exp2f(d * mul);
-            float xj = 0.0f;
-#pragma unroll
-            for (int k = 0; k < KM; k++) {
-                p[k] += k == (int)id ? e : 0.0f;
-                xj = k == (int)id ? f[k] : xj;
-            }
-            total += e;
-            if (e != 0.0f) sum += e * (d - (xj - r.m));
-        }
-        const float one = 1.0f / total;
-#pragma unroll
-        for (int k = 0; k < KM; k++) p[k] *= one;
-        // as in k_rows; both sums are between 1 and a small number
-        const float logs = r.s == 0.0f ? 0.0f : logf(r.s * one);
-        a.loss[row] = bad ? NAN : w * a.t2_mul * ((float)(sum * one * a.inv_t) + logs);
-        factor = bad ? NAN : w * a.t_mul;
-    } else {
-        float x_label = 0.0f;
-#pragma unroll
-        for (int k = 0; k < KM; k++) x_label = k == (int)label ? f[k] : x_label;
-        slope = labelled_row<OP>(a, row, bad, r, x_label, given, true);
-        factor = -slope;
-    }
+    else r = take<KM>(r, f, a.exp_mul);
+    const float inv = inverse_sum(r), slope = labelled_row<OP>(a, row, bad, r, x_label, given, true);
     if (OP == SC_LOGP || !g) return;
-    if (OP == SC_POLICY && slope == 0.0f) {
-        for (int c = 0; c < V; c++) g[c] = (T)0.0f;
+    if (OP == SC_POLICY && slope == 0.0f) return clear_row(g, V, 0, 1);
+    gradients<KM>(f, r, -slope * inv, a.exp_mul, (int)label, slope, inv);
+#pragma unroll
+    for (int k = 0; k < KM; k++)
+        if (k < V) g[k] = (T)f[k];
+}
+
+// Distillation of rows that a group of lanes holds.  The entries of the block's rows are one stretch of memory: the block copies them to shared memory
+// in whole lines (read by each row's lanes they are a line an entry: 8M rows of 16 bfloat16 classes and 16 entries 1.85 -> 0.50 ms), and a row's
+// teacher is spread over all its classes there, so that no gradient is written twice.
+template <typename T, int NV, class G>
+__global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top_magic) {
+    constexpr int E = Piece<T>::E;
+    constexpr bool FEW = NV == 0; // V < E: every lane has the whole row, and shares the teacher's entries
+    extern __shared__ unsigned char s_dyn[];
+    const int V = a.V, k1 = a.n_top, ks = k1 | 1, vs = (V + 2) | 1; // odd distances: rows that lanes read side by side start in different banks
+    int2 *const s_all = (int2 *)s_dyn; // (class, V for no entry, V + 1 for no class; score)
+    float *const s_share = (float *)(s_all + G::ROWS * ks);
+    const int64_t row0 = (int64_t)blockIdx.x * G::ROWS, row = row0 + G::slot();
+    const int t = G::rank();
+    const bool in_range = row < a.N;
+    const T *x = (const T *)a.x + (in_range ? row : a.N - 1) * a.xs;
+    T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
+    const float mul = a.exp_mul;
+    const float w = !in_range ? 0.0f : a.weights ? a.weights[row] : 1.0f;
+    Piece<T> p[FEW ? 1 : NV];
+    float few[FEW ? E : 1];
+    if constexpr (FEW) {
+#pragma unroll
+        for (int k = 0; k < E; k++) few[k] = (float)x[k < V ? k : V - 1];
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int o = (t + i * G::SIZE) * E;
+            if (i * G::SIZE * E < V) p[i].load(x, o + E <= V ? o : V - E);
+        }
+    }
+    {
+        const int64_t at = row0 * k1, left = (a.N - row0) * k1;
+        const int n = (int)(left < G::ROWS * k1 ? left : G::ROWS * k1);
+        for (int e0 = threadIdx.x; e0 < n; e0 += 1024) { // four entries in flight
+            int64_t id[4];
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) id[i] = load_id(a.ids, a.id64, at + (e0 + 256 * i < n ? e0 + 256 * i : n - 1));
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] = load_score(a.top, a.top_type, at + (e0 + 256 * i < n ? e0 + 256 * i : n - 1));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int e = e0 + 256 * i, r = k1 == 1 ? e : (int)__umulhi((uint32_t)e, top_magic); // e / n_top
+                if (e < n) s_all[r * ks + e - r * k1] = {id[i] < 0 ? V : id[i] < V ? (int)id[i] : V + 1, __float_as_int(id[i] < 0 ? -INFINITY : v[i])};
+            }
+        }
+        for (int e = threadIdx.x; e < G::ROWS * vs; e += 256) s_share[e] = 0.0f;
+    }
+    __syncthreads();
+    if (w == 0.0f) {
+        if (in_range) {
+            if (t == 0) left_out<SC_DISTILL>(a, row);
+            if (g) clear_row(g, V, t, G::SIZE);
+        }
         return;
     }
+    int2 *const s_top = s_all + G::slot() * ks;
+    float *const share = s_share + G::slot() * vs;
+    MaxSum r = {LOWEST, 0.0f};
+    if constexpr (FEW) {
 #pragma unroll
-    for (int k = 0; k < KM; k++) {
-        const float q = exp_of(f[k], r.m, mul) * inv;
-        const float v = OP == SC_DISTILL ? factor * (q - p[k]) : k == (int)label ? slope * (1.0f - q) : factor * q;
-        if (k < V) g[k] = (T)v;
+        for (int k = 0; k < E; k++) few[k] = k < V ? few[k] : -INFINITY;
+        r = take<E>(r, few, mul);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int o = (t + i * G::SIZE) * E;
+            if (o < V) {
+                float f[E];
+                p[i].get(f);
+                if (o + E > V) {
+#pragma unroll
+                    for (int k = 0; k < E; k++) f[k] = k < o + E - V ? -INFINITY : f[k];
+                }
+                r = take<E>(r, f, mul);
+            }
+        }
+        r = lanes_join<G::SIZE>(r, mul);
+    }
+    // The teacher's entries, four at a time, for each is a trip to shared memory or two: their maximum while each leaves its number at its class, then
+    // exp of each in the number's place - another number there is an entry of the same class.  (Added up there by float atomics, 165 cycles a
+    // wavefront each, 8M rows of 7 classes and entries take 347 us for 237.)
+    float most = LOWEST, total = 0.0f, sum = 0.0f;
+    bool none = false, twice = false;
+    for (int j0 = t; j0 < k1; j0 += 4 * G::SIZE) {
+        int2 e[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[i] = s_top[j0 + i * G::SIZE < k1 ? j0 + i * G::SIZE : j0];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            most = fmaxf(most, __int_as_float(e[i].y));
+            none |= e[i].x == V + 1;
+            if (j0 + i * G::SIZE < k1) share[e[i].x] = __int_as_float(j0 + i * G::SIZE);
+        }
+    }
+    G::sync();
+    most = over_lanes<G::SIZE>(most, [](float a, float b) { return fmaxf(a, b); });
+    for (int j0 = t; j0 < k1; j0 += 4 * G::SIZE) {
+        int2 e[4];
+        float at[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) e[i] = s_top[j0 + i * G::SIZE < k1 ? j0 + i * G::SIZE : j0];
+#pragma unroll
+        for (int i = 0; i < 4; i++) at[i] = share[e[i].x];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (j0 + i * G::SIZE < k1) {
+                const float d = __int_as_float(e[i].y) - most, u = __builtin_amdgcn_exp2f(d * mul);
+                total += u;
+                sum += u != 0.0f ? u * d : 0.0f;
+                share[e[i].x] = u;
+                twice |= e[i].x < V && __float_as_int(at[i]) != j0 + i * G::SIZE;
+            }
+        }
+    }
+    total = lanes_sum<G::SIZE>(total);
+    sum = lanes_sum<G::SIZE>(sum);
+    none = lanes_any<G::SIZE>(none);
+    if (total == 0.0f) { // no entry; a total that is no number is one
+        if (t == 0) left_out<SC_DISTILL>(a, row);
+        if (g) clear_row(g, V, t, G::SIZE);
+        return;
+    }
+    if (lanes_any<G::SIZE>(twice)) { // a class that comes twice has both shares, added up in their order
+        G::sync();
+        for (int j = t; j < k1; j += G::SIZE) {
+            const int id = s_top[j].x;
+            if (id >= V) continue;
+            float u = 0.0f;
+            for (int i = 0; i < k1; i++) {
+                const int2 e = s_top[i];
+                u += e.x == id ? __builtin_amdgcn_exp2f((__int_as_float(e.y) - most) * mul) : 0.0f;
+            }
+            share[id] = u;
+        }
+    }
+    G::sync();
+    const float one = 1.0f / total, factor = none ? NAN : w * a.t_mul, fq = factor * inverse_sum(r), fp = factor * one;
+    float cross = 0.0f; // the sum of share (x - m)
+    if constexpr (FEW) {
+#pragma unroll
+        for (int k = 0; k < E; k++) {
+            const float u = share[k < V ? k : V - 1];
+            if (k < V && u != 0.0f) cross += u * (few[k] - r.m);
+            if (g && k < V && t == 0) g[k] = (T)(fq * exp_of(few[k], r.m, mul) - fp * u);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            int o = (t + i * G::SIZE) * E;
+            if (o < V) {
+                const int twofold = o + E <= V ? 0 : o + E - V; // classes of the piece before
+                o = o + E <= V ? o : V - E;
+                float f[E];
+                p[i].get(f);
+#pragma unroll
+                for (int k = 0; k < E; k++) {
+                    const float u = share[o + k], d = f[k] - r.m;
+                    cross += u != 0.0f && k >= twofold ? u * d : 0.0f; // not 0 times infinity
+                    f[k] = fq * __builtin_amdgcn_exp2f(d * mul) - fp * u;
+                }
+                if (g) {
+                    p[i].set(f);
+                    p[i].store(g, o);
+                }
+            }
+        }
+        cross = lanes_sum<G::SIZE>(cross);
+    }
+    if (t == 0) {
+        const double logs = r.s == 0.0f ? 0.0 : log_sum(r.s * one);
+        a.loss[row] = none ? NAN : w * a.t2_mul * (float)((double)((sum - cross) * one) * a.inv_t + logs);
     }
 }
 
@@ -663,39 +768,59 @@ __global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, int pairs, c
     }
 }
 
-// LAUNCH of the form that a row of n pieces takes
 template <typename T, int OP, int NV, class G>
-static void launch_rows(hipStream_t s, ScoreArgs a) {
+static int launch_rows(hipStream_t s, ScoreArgs a) {
     a.early = a.N <= 512;
-    const size_t lds = OP == SC_DISTILL ? (size_t)G::ROWS * a.n_top * 12 : 0;
+    const size_t lds = OP == SC_DISTILL ? (size_t)a.n_top * 12 : 0;
     hipLaunchKernelGGL((k_rows<T, OP, NV, G>), dim3((unsigned)((a.N + G::ROWS - 1) / G::ROWS)), dim3(G::THREADS), lds, s, a);
+    return EVT_OK;
+}
+// Distillation of short rows: true where the lanes hold a row of n pieces and a block's memory its teachers, 52 KB so that a unit has three blocks
+template <typename T, int NV, class G>
+static bool launch_distill(hipStream_t s, const ScoreArgs &a, int64_t n) {
+    const size_t lds = G::ROWS * ((size_t)(a.n_top | 1) * 8 + (size_t)((a.V + 2) | 1) * 4);
+    if ((NV ? a.V < Piece<T>::E || n > (int64_t)G::SIZE * NV : a.V >= Piece<T>::E) || (lds > 53248 && G::SIZE < 64) || lds > 65536) return false;
+    const uint32_t magic = a.n_top > 1 ? (uint32_t)(((1ull << 32) + a.n_top - 1) / a.n_top) : 0u; // exact for e / n_top, e * n_top < 2^32
+    hipLaunchKernelGGL((k_distill_short<T, NV, G>), dim3((unsigned)((a.N + G::ROWS - 1) / G::ROWS)), dim3(256), lds, s, a, magic);
+    return true;
 }
 template <typename T, int OP>
-static void launch_typed(hipStream_t s, const ScoreArgs &a) {
+static int launch_typed(hipStream_t s, const ScoreArgs &a) {
     constexpr int E = Piece<T>::E;
     const int64_t n = ((int64_t)a.V + E - 1) / E;
-    if (a.V < E) {
-        const dim3 grid((unsigned)((a.N + 255) / 256)), block(256);
-        hipLaunchKernelGGL((k_few_classes<T, OP, E>), grid, block, 0, s, a);
-        return;
-    }
-    if (n <= 256) {
-        // lanes to a row: four pieces each, and no more teachers than a block's memory holds (48 KB)
-        const int top = OP == SC_DISTILL ? a.n_top : 0;
-        if (n <= 4 && top <= 16) return launch_rows<T, OP, 4, Lanes<1>>(s, a);
-        if (n <= 8 && top <= 32) return launch_rows<T, OP, 4, Lanes<2>>(s, a);
-        if (n <= 16 && top <= 64) return launch_rows<T, OP, 4, Lanes<4>>(s, a);
-        if (n <= 32 && top <= 128) return launch_rows<T, OP, 4, Lanes<8>>(s, a);
-        if (n <= 64 && top <= 256) return launch_rows<T, OP, 4, Lanes<16>>(s, a);
-        if (n <= 128 && top <= 512) return launch_rows<T, OP, 4, Lanes<32>>(s, a);
-        return launch_rows<T, OP, 4, Lanes<64>>(s, a);
+    if constexpr (OP == SC_DISTILL) {
+        if (launch_distill<T, 0, Lanes<1>>(s, a, n) || launch_distill<T, 0, Lanes<8>>(s, a, n) || launch_distill<T, 0, Lanes<64>>(s, a, n) ||
+            launch_distill<T, 4, Lanes<1>>(s, a, n) || launch_distill<T, 4, Lanes<2>>(s, a, n) || launch_distill<T, 4, Lanes<4>>(s, a, n) ||
+            launch_distill<T, 4, Lanes<8>>(s, a, n) || launch_distill<T, 4, Lanes<16>>(s, a, n) || launch_distill<T, 4, Lanes<32>>(s, a, n) ||
+            launch_distill<T, 4, Lanes<64>>(s, a, n))
+            return EVT_OK;
+        if (a.V < E) {
+            evt_set_error("no form for %d classes and %d entries", a.V, a.n_top); // k_rows' last piece would start in front of the row
+            return EVT_ERR_INTERNAL;
+        }
+    } else {
+        if (a.V < E) {
+            hipLaunchKernelGGL((k_few_classes<T, OP>), dim3((unsigned)((a.N + 255) / 256)), dim3(256), 0, s, a);
+            return EVT_OK;
+        }
+        // lanes to a row: four pieces each
+        if (n <= 4) return launch_rows<T, OP, 4, Lanes<1>>(s, a);
+        if (n <= 8) return launch_rows<T, OP, 4, Lanes<2>>(s, a);
+        if (n <= 16) return launch_rows<T, OP, 4, Lanes<4>>(s, a);
+        if (n <= 32) return launch_rows<T, OP, 4, Lanes<8>>(s, a);
+        if (n <= 64) return launch_rows<T, OP, 4, Lanes<16>>(s, a);
+        if (n <= 128) return launch_rows<T, OP, 4, Lanes<32>>(s, a);
+        if (n <= 256) return launch_rows<T, OP, 4, Lanes<64>>(s, a);
     }
     if constexpr (OP == SC_GRAD) {
         const int64_t parts = (n + 1023) / 1024, blocks = a.N * parts;
         hipLaunchKernelGGL(k_slope_rows<T>, dim3((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30))), dim3(256), 0, s, a, (int)parts);
+        return EVT_OK;
     } else {
         const bool few = a.N <= 256;
-        if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
+        if constexpr (OP != SC_DISTILL) {
+            if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
+        }
         if (OP == SC_LOGP || !a.g) return few ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 4, Waves<4>>(s, a);
         // the row stays in registers
         if constexpr (OP != SC_LOGP) {
@@ -710,11 +835,9 @@ static void launch_typed(hipStream_t s, const ScoreArgs &a) {
 }
 template <int OP>
 static int launch_scores(hipStream_t s, const ScoreArgs &a, int dtype) {
-    if (dtype == EVT_F32) launch_typed<float, OP>(s, a);
-    else if (dtype == EVT_BF16) launch_typed<bf16_t, OP>(s, a);
-    else launch_typed<half_t, OP>(s, a);
+    const int r = dtype == EVT_F32 ? launch_typed<float, OP>(s, a) : dtype == EVT_BF16 ? launch_typed<bf16_t, OP>(s, a) : launch_typed<half_t, OP>(s, a);
     HIPCHK(hipGetLastError());
-    return EVT_OK;
+    return r;
 }
 
 // ---- entry points ---------------------------------------------------------------------------

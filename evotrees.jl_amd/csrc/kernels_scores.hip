@@ -276,7 +276,9 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             const int o = (t + i * G::SIZE) * E;
-            if (i * G::SIZE * E < V) p[i].load(x, o + E <= V ? o : V - E); // past the row's end: the last piece, which counts once
+            // past the row's end: the last piece, which counts once.  Lanes leave out what no lane has; between the loads of a block the branches cost
+            // more than the loads (8192 x 131072 bf16: 1020 for 790 us)
+            if (G::ROWS == 1 || i * G::SIZE * E < V) p[i].load(x, o + E <= V ? o : V - E);
         }
     };
     if (a.early) load_row(); // whether the row counts or not
@@ -821,7 +823,7 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
         if constexpr (OP != SC_DISTILL) {
             if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
         }
-        if (OP == SC_LOGP || !a.g) return few ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 4, Waves<4>>(s, a);
+        if (OP == SC_LOGP || !a.g) return few || n >= 8192 ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 4, Waves<4>>(s, a);
         // the row stays in registers
         if constexpr (OP != SC_LOGP) {
             if (few) return n <= 4096 ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 16, Waves<16>>(s, a);

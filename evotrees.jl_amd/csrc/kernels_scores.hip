@@ -24,10 +24,22 @@ struct Piece {
     };
     Raw r;
     __device__ __forceinline__ void load(const T *p) { r = *(const Raw *)p; }
-    __device__ __forceinline__ void store(T *p) const { *(Raw *)p = r; }
+    // past: by the caches.  A gradient that the last of them (256 MB) cannot hold only drives out what the next pass reads (8 pairs, 5003 x 32 768 bf16, loss and
+    // gradient again and again: the first pass over the scores 67 us, 39 so); a smaller one stays for its reader
+    __device__ __forceinline__ void store(T *p, bool past) const {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+        const u4 v = {r.w[0], r.w[1], r.w[2], r.w[3]};
+        if (past) {
+            asm volatile(""); // in front and behind, so that the two stores stay apart: joined, the hint is lost
+            __builtin_nontemporal_store(v, (u4 *)p);
+            asm volatile("");
+        } else {
+            *(u4 *)p = v;
+        }
+    }
     // o elements behind a base: a 32-bit offset is an operand of the access where a pointer is two registers for every piece
     __device__ __forceinline__ void load(const T *p, uint32_t o) { r = *(const Raw *)((const char *)p + o * (uint32_t)sizeof(T)); }
-    __device__ __forceinline__ void store(T *p, uint32_t o) const { *(Raw *)((char *)p + o * (uint32_t)sizeof(T)) = r; }
+    __device__ __forceinline__ void store(T *p, uint32_t o, bool past) const { store((T *)((char *)p + o * (uint32_t)sizeof(T)), past); }
     __device__ __forceinline__ void get(float *f) const {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -231,12 +243,12 @@ __device__ __forceinline__ void left_out(const ScoreArgs &a, int64_t row) {
 
 // A gradient of 0 for V classes
 template <typename T>
-__device__ __forceinline__ void clear_row(T *g, int V, int rank, int size) {
+__device__ __forceinline__ void clear_row(T *g, int V, int rank, int size, bool past) {
     constexpr int E = Piece<T>::E;
     Piece<T> p;
     p.r = {};
     const int n = V / E;
-    for (int v = rank; v < n; v += size) p.store(g + (size_t)v * E);
+    for (int v = rank; v < n; v += size) p.store(g + (size_t)v * E, past);
     for (int c = n * E + rank; c < V; c += size) g[c] = (T)0.0f;
 }
 
@@ -268,6 +280,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     const T *x = (const T *)a.x + row * a.xs;
     T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
     const float mul = a.exp_mul;
+    const bool past = a.past;
     float w = 1.0f, x_label = 0.0f, given = 0.0f;
     bool live = true, bad = false;
     int64_t label = -1;
@@ -302,7 +315,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     }
     if (!live) { // the row has no part in the loss
         if (t == 0) left_out<OP>(a, row);
-        if (OP != SC_LOGP && g) clear_row(g, V, t, G::SIZE);
+        if (OP != SC_LOGP && g) clear_row(g, V, t, G::SIZE, past);
         return;
     }
     if (!a.early) load_row();
@@ -377,7 +390,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         const int state = s_state;
         if (state == 0) {
             if (t == 0) left_out<OP>(a, row);
-            if (g) clear_row(g, V, t, G::SIZE);
+            if (g) clear_row(g, V, t, G::SIZE, past);
             return;
         }
         if (t < 64) {
@@ -397,7 +410,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     } else {
         slope = labelled_row<OP>(a, row, bad, r, x_label, given, t == 0);
         if (OP == SC_POLICY && slope == 0.0f && g) { // clipped, or of no weight
-            clear_row(g, V, t, G::SIZE);
+            clear_row(g, V, t, G::SIZE, past);
             return;
         }
         factor = -slope;
@@ -413,7 +426,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
             p[i].get(f);
             gradients<E>(f, r, fq, mul, OP == SC_DISTILL ? -1 : (int)(label - o), slope, inv);
             p[i].set(f);
-            p[i].store(g, o);
+            p[i].store(g, o, past);
         }
     }
     for (int64_t o = base + (int64_t)(t + NV * G::SIZE) * E; o < V; o += G::SIZE * E) {
@@ -424,7 +437,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
             q.get(f);
             gradients<E>(f, r, fq, mul, OP == SC_DISTILL ? -1 : (int)(label - o), slope, inv);
             q.set(f);
-            q.store(g + o);
+            q.store(g + o, past);
         } else { // not reaching back: in place, the classes in front are gradients already
             for (int64_t c = o; c < V; c++) {
                 f[0] = (float)x[c];
@@ -468,7 +481,7 @@ __global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
     const bool bad = live && label >= V;
     if (!live) {
         left_out<OP>(a, row);
-        if (OP != SC_LOGP && g) clear_row(g, V, 0, 1);
+        if (OP != SC_LOGP && g) clear_row(g, V, 0, 1, false);
         return;
     }
     float f[KM], x_label = 0.0f;
@@ -484,7 +497,7 @@ __global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
     else r = take<KM>(r, f, a.exp_mul);
     const float inv = inverse_sum(r), slope = labelled_row<OP>(a, row, bad, r, x_label, given, true);
     if (OP == SC_LOGP || !g) return;
-    if (OP == SC_POLICY && slope == 0.0f) return clear_row(g, V, 0, 1);
+    if (OP == SC_POLICY && slope == 0.0f) return clear_row(g, V, 0, 1, false);
     gradients<KM>(f, r, -slope * inv, a.exp_mul, (int)label, slope, inv);
 #pragma unroll
     for (int k = 0; k < KM; k++)
@@ -508,6 +521,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
     const T *x = (const T *)a.x + (in_range ? row : a.N - 1) * a.xs;
     T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
     const float mul = a.exp_mul;
+    const bool past = a.past;
     const float w = !in_range ? 0.0f : a.weights ? a.weights[row] : 1.0f;
     Piece<T> p[FEW ? 1 : NV];
     float few[FEW ? E : 1];
@@ -543,7 +557,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
     if (w == 0.0f) {
         if (in_range) {
             if (t == 0) left_out<SC_DISTILL>(a, row);
-            if (g) clear_row(g, V, t, G::SIZE);
+            if (g) clear_row(g, V, t, G::SIZE, past);
         }
         return;
     }
@@ -611,7 +625,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
     none = lanes_any<G::SIZE>(none);
     if (total == 0.0f) { // no entry; a total that is no number is one
         if (t == 0) left_out<SC_DISTILL>(a, row);
-        if (g) clear_row(g, V, t, G::SIZE);
+        if (g) clear_row(g, V, t, G::SIZE, past);
         return;
     }
     if (lanes_any<G::SIZE>(twice)) { // a class that comes twice has both shares, added up in their order
@@ -654,7 +668,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
                 }
                 if (g) {
                     p[i].set(f);
-                    p[i].store(g, o);
+                    p[i].store(g, o, past);
                 }
             }
         }
@@ -671,6 +685,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, int parts) {
     constexpr int E = Piece<T>::E, PART = 256 * 4 * E;
     const int64_t blocks = a.N * parts;
+    const bool past = a.past;
     for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
         const int64_t row = b / parts;
         const int64_t c0 = (b - row * parts) * PART;
@@ -683,7 +698,7 @@ __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, int parts) {
         if (a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
         if (live) given = a.slope[row];
         if (given == 0.0f) {
-            clear_row(g, V, t, 256);
+            clear_row(g, V, t, 256, past);
             continue;
         }
         const MaxSum r = {fmaxf(a.stats[2 * row], LOWEST), a.stats[2 * row + 1]};
@@ -703,7 +718,7 @@ __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, int parts) {
                 p[i].get(f);
                 gradients<E>(f, r, fq, a.exp_mul, (int)(at - o), slope, inv);
                 p[i].set(f);
-                p[i].store(g + o);
+                p[i].store(g + o, past);
             }
         }
         const int c = V / E * E + t; // behind the last whole piece
@@ -894,6 +909,7 @@ static int take_scores(const evt_scores *s, bool grad_needed, int32_t flags, Sco
     a.exp_mul = (float)(1.4426950408889634 / s->temperature);
     a.t_mul = (float)s->temperature;
     a.t2_mul = (float)(s->temperature * s->temperature);
+    a.past = (double)a.N * a.V * size > 256e6;
     return check_device(flags, s->x, s->grad);
 }
 static int take_labels(const void *labels, int32_t dtype, ScoreArgs &a) {

@@ -13,6 +13,7 @@ struct ScoreArgs {
     int64_t xs, gs; // elements from row to row
     int64_t N;
     int32_t V;
+    int32_t past;   // the gradient is stored past the caches
     int32_t early;  // few rows: a row's scores are requested before it is known whether it counts
     double inv_t;   // 1 / temperature
     float exp_mul;  // log2(e) / temperature: exp(d / T) = exp2(d * exp_mul)

@@ -21,7 +21,7 @@ from . import _lib
 from ._lib import EvtError, Handle, TreeArrays, make_params, splitmix_mask  # noqa: F401
 from .class_losses import class_logp, class_logp_grad, distill_loss, policy_loss, preference_loss
 
-__all__ = ["EvoTreeRegressor", "EvoTreeCount", "EvoTreeClassifier", "EvoTreeMLE", "EvoTree", "Tree", "fit", "predict", "predict_leaf_idx", "init",
+__all__ = ["EvoTreeRegressor", "EvoTreeCount", "EvoTreeClassifier", "EvoTreeMLE", "EvoTree", "Tree", "Teacher", "fit", "predict", "predict_leaf_idx", "init",
            "grow_evotree", "update", "okay_to_continue", "get_edges", "get_edges_table", "binarize_table", "check_args", "CallBack", "init_logger", "update_logger", "EvtError",
            "class_logp", "class_logp_grad", "distill_loss", "policy_loss", "preference_loss"]
 
@@ -126,6 +126,15 @@ class EvoTreeMLE(_Learner):
     _losses = ("gaussian_mle", "logistic_mle")
     _metrics = ("gaussian_mle", "logistic_mle")
     _defaults = dict(_Learner._defaults, loss="gaussian_mle", min_weight=8.0)
+
+
+class Teacher:
+    """What a classifier is fitted to in place of its target's labels (`fit(..., teacher=)`): the classes another model thinks best of every row and their
+    scores (logits), as distill_loss takes them.  ids, logits: (rows, n_top); an id is a position among the target's sorted levels, from 0,
+    and one below 0 is no entry.  The labels still give the levels, the bias and the metric."""
+
+    def __init__(self, ids, logits, temperature=1.0):
+        self.ids, self.logits, self.temperature = ids, logits, float(temperature)
 
 
 class Tree(TreeArrays):
@@ -409,10 +418,12 @@ class Cache:
 
 
 def init(config, x_train, y_train=None, w_train=None, offset_train=None, feature_names=None, device=None, target_name=None, weight_name=None,
-         offset_name=None):
+         offset_name=None, teacher=None):
     """init / init_core for the GPU device (src/init.jl:236-339; ext/EvoTreesKernelAbstractionsExt/init.jl:1-151).  x_train is a
     matrix (with y_train, w_train, offset_train) or a table (with target_name, weight_name, offset_name)."""
     _device_check(config.device if device is None else device)
+    if teacher is not None and config.loss != "mlogloss":
+        raise ValueError("a teacher needs the mlogloss loss, got %s" % config.loss)
     rng = np.random.default_rng(config.seed)
     table = _is_table(x_train)
     if table:
@@ -457,6 +468,8 @@ def init(config, x_train, y_train=None, w_train=None, offset_train=None, feature
     h.set_feature_meta(feattypes, mono)
     _set_levels(h, config)
     h.set_target(y32, w, mu, offset)
+    if teacher is not None:
+        h.set_teacher(teacher.ids, teacher.logits, teacher.temperature)
     info = dict(nrounds=0, feature_names=feature_names, target_levels=target_levels, target_isordered=False, edges=edges, featbins=featbins,
                 feattypes=feattypes)
     nfs = int(np.ceil(config.colsample * F))
@@ -612,20 +625,21 @@ def update_logger(logger, it, metric):
 
 def fit(config, dtrain=None, x_train=None, y_train=None, w_train=None, offset_train=None, x_eval=None, y_eval=None, w_eval=None, offset_eval=None,
         feature_names=None, print_every_n=9999, device=None, verbosity=1, return_cache=False, target_name=None, weight_name=None,
-        offset_name=None, deval=None):
+        offset_name=None, deval=None, teacher=None):
     """fit(params; x_train, y_train, ..., x_eval, y_eval, ...), src/fit.jl:388-437, and the Tables form
-    fit(params, dtrain; target_name, feature_names, weight_name, offset_name, deval), src/fit.jl:302-345."""
+    fit(params, dtrain; target_name, feature_names, weight_name, offset_name, deval), src/fit.jl:302-345.  teacher: a Teacher, which a
+    classifier is fitted to instead of the labels."""
     if dtrain is not None:
         if not _is_table(dtrain):
             raise AssertionError("fit(params, dtrain) only accepts Tables compatible input for `dtrain` (a DataFrame or a dict of columns)")
         m, cache = init(config, dtrain, feature_names=feature_names, device=device, target_name=target_name, weight_name=weight_name,
-                        offset_name=offset_name)
+                        offset_name=offset_name, teacher=teacher)
         m.info["target_names"] = [str(t) for t in target_name] if isinstance(target_name, (list, tuple)) else [str(target_name)]
         x_eval, y_eval = None, None
     else:
         if x_train is None or y_train is None:
             raise TypeError("x_train and y_train are required")
-        m, cache = init(config, x_train, y_train, w_train=w_train, offset_train=offset_train, feature_names=feature_names, device=device)
+        m, cache = init(config, x_train, y_train, w_train=w_train, offset_train=offset_train, feature_names=feature_names, device=device, teacher=teacher)
     logger, cb = None, None
     try:
         if dtrain is not None and deval is not None:
@@ -677,7 +691,7 @@ def okay_to_continue(config, m, cache):
     return a == b and config.nrounds >= m.info["nrounds"]
 
 
-def update(config, m, cache, x_train=None, y_train=None, w_train=None):
+def update(config, m, cache, x_train=None, y_train=None, w_train=None, teacher=None):
     """MMI.update, src/MLJ.jl:38-57: warm restart on the handle the first fit kept (`fit(..., return_cache=True)`);
     any change other than a larger nrounds refits from scratch."""
     if okay_to_continue(config, m, cache):
@@ -686,7 +700,7 @@ def update(config, m, cache, x_train=None, y_train=None, w_train=None):
         cache.config = config
         return m, cache
     cache.handle.close()
-    return fit(config, x_train=x_train, y_train=y_train, w_train=w_train, return_cache=True)
+    return fit(config, x_train=x_train, y_train=y_train, w_train=w_train, return_cache=True, teacher=teacher)
 
 
 def binarize(x, edges):

@@ -31,7 +31,7 @@ EXPORTS = [
     "evt_set_option", "evt_synchronize", "evt_copy_bandwidth", "evt_read_bandwidth", "evt_predict_static",
     "evt_lds_atomic_rate", "evt_global_atomic_rate", "evt_trim", "evt_binarize", "evt_bin_columns", "evt_order_stats",
     "evt_model_create", "evt_model_destroy", "evt_model_predict",
-    "evt_class_logp", "evt_class_logp_grad", "evt_distill_loss", "evt_policy_loss", "evt_preference_loss",
+    "evt_set_teacher", "evt_class_logp", "evt_class_logp_grad", "evt_distill_loss", "evt_policy_loss", "evt_preference_loss",
 ]
 
 
@@ -84,6 +84,7 @@ def load():
         "evt_set_target": [vp, vp, vp, vp, vp],
         "evt_set_feature_meta": [vp, vp, vp],
         "evt_set_alphas": [vp, vp, i32],
+        "evt_set_teacher": [vp, vp, vp, i32, C.c_double],
         "evt_update_grads": [vp],
         "evt_set_grads": [vp, vp],
         "evt_grow_tree": [vp, vp, C.c_uint8, vp, i32, C.POINTER(EvtParams), C.POINTER(EvtTreeOut)],
@@ -123,11 +124,11 @@ def load():
         "evt_read_bandwidth": [i64, i32, vp],
         "evt_lds_atomic_rate": [i32, i32, i32, vp, vp],
         "evt_global_atomic_rate": [i32, i32, i32, vp],
-        "evt_class_logp": [vp, C.POINTER(EvtScores), vp, i32, vp, vp, i32],
-        "evt_class_logp_grad": [vp, C.POINTER(EvtScores), vp, i32, vp, vp, i32],
-        "evt_distill_loss": [vp, C.POINTER(EvtScores), vp, i32, vp, i32, i32, vp, vp, i32],
-        "evt_policy_loss": [vp, C.POINTER(EvtScores), vp, i32, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, vp, vp, i32],
-        "evt_preference_loss": [vp, C.POINTER(EvtScores), vp, i32, vp, i32, vp, vp, C.c_double, C.c_double, C.c_double, i32, vp, vp, vp, i32],
+        "evt_class_logp": [vp, vp, vp, i32, vp, vp, i32],
+        "evt_class_logp_grad": [vp, vp, vp, i32, vp, vp, i32],
+        "evt_distill_loss": [vp, vp, vp, i32, vp, i32, i32, vp, vp, i32],
+        "evt_policy_loss": [vp, vp, vp, i32, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, vp, vp, i32],
+        "evt_preference_loss": [vp, vp, vp, i32, vp, i32, vp, vp, C.c_double, C.c_double, C.c_double, i32, vp, vp, vp, i32],
         "evt_predict_static": [vp, i64, i32, vp, vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, i32, vp, vp],
     }
     for name, args in sigs.items():
@@ -361,6 +362,22 @@ class Handle:
         ft = None if feattypes is None else np.ascontiguousarray(feattypes, np.uint8)
         mo = None if monotone is None else np.ascontiguousarray(monotone, np.int32)
         check(load().evt_set_feature_meta(self._h, ptr(ft), ptr(mo)))
+
+    def set_teacher(self, ids, scores, temperature=1.0):
+        """ids, scores: (N, n_top) classes from 0 (below 0: none) and their scores, which the gradients of mlogloss are computed from then; None
+        for both: from the labels again."""
+        if ids is None and scores is None:
+            check(load().evt_set_teacher(self._h, None, None, 0, 1.0))
+            return
+        ids = np.asarray(ids)
+        if ids.dtype.kind not in "iu":
+            raise ValueError("a teacher's ids must be whole numbers")
+        if ids.ndim != 2 or ids.shape[0] != self.N or np.shape(scores) != ids.shape:
+            raise ValueError("a teacher's ids and scores must both be %d x n_top" % self.N)
+        if ids.size and (ids.max() >= self.K):
+            raise ValueError("a teacher's ids must be below the number of classes (%d)" % self.K)
+        ids, scores = np.ascontiguousarray(np.maximum(ids, -1), np.int32), np.ascontiguousarray(scores, np.float32)
+        check(load().evt_set_teacher(self._h, ptr(ids), ptr(scores), ids.shape[1], float(temperature)))
 
     def update_grads(self):
         check(load().evt_update_grads(self._h))

@@ -23,17 +23,18 @@ _F32, _I32, _I64, _BF16, _F16 = 0, 4, 5, 10, 11
 _TRUSTED = 2  # EVT_STATIC_TRUSTED: the tensors say where they are
 _INF = float("inf")
 _torch = None
+_makers = {}  # by device
 
 
 def _load():
     """torch, the codes of its types and what a call needs of it; imported with the first call, a fit needs none."""
-    global _torch, _FLOATS, _INTS, _F32S, _I32S, _new, _like, _device, _stream
+    global _torch, _FLOATS, _INTS, _F32S, _I32S, _like, _device, _stream
     import torch
     _F32S = {torch.float32: _F32}
     _FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
     _I32S = {torch.int32: _I32}
     _INTS = {torch.int32: _I32, torch.int64: _I64}
-    _new, _like = torch.empty, torch.empty_like
+    _like = torch.empty_like
     _device = torch.cuda.current_device
     # the current stream's handle without a Stream object around it, 1.1 us less a call
     _stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -113,7 +114,13 @@ class _Call:
         return out
 
     def values(self, *shape):
-        return _new(shape, dtype=_torch.float32, device=self.x.device)
+        """A float32 tensor on the call's device, by way of one that is there: 0.3 us less than torch.empty with a type and a device."""
+        make = _makers.get(self.device)
+        if make is None:
+            make = _torch.empty(0, dtype=_torch.float32, device=self.x.device).new_empty
+            if self.device >= 0:
+                _makers[self.device] = make
+        return make(shape)
 
     def run(self, name, grad, *args):
         x, dev = self.x, self.device

@@ -1,5 +1,6 @@
 // C ABI of libevotrees_hip.so: handle lifecycle, uploads, the per-tree level loop, read-back.
 #include "grad_math.h"
+#include "scores.h"
 #include "upload.h"
 #include "walk_rule.h"
 
@@ -186,7 +187,7 @@ extern "C" int evt_destroy(evt_handle c) {
                     c->hist, c->seg_start, c->seg_len, c->status, c->node_sum, c->tree_blob, c->tree.packed, c->js, c->jsmap, c->feattypes, c->mono, c->absmax, c->qexp_buf[0], c->qexp_buf[1], c->qbits,
                     c->qscale_buf[0], c->qscale_buf[1], c->planes, c->metric_partial, c->errflag, c->ogains, c->sbest, c->scan_count, c->is_id, c->pt_nodes, c->mask_next,
                     c->small_nid[0], c->small_nid[1], c->small_head[0], c->small_head[1], c->small_left[0], c->small_left[1], c->small_acc,
-                    c->alphas, c->alphas_f, c->qkeys_a, c->qkeys_b, c->qtemp};
+                    c->alphas, c->alphas_f, c->qkeys_a, c->qkeys_b, c->qtemp, c->teach_ids, c->teach_scores};
     if (c->copy_stream) (void)hipStreamSynchronize(c->copy_stream);
     for (void *p : ptrs) dev_give(p);
     for (int l = 0; l < 2; l++) {
@@ -279,6 +280,7 @@ extern "C" int evt_create(int64_t nobs, int32_t nfeats, int32_t nbins, int32_t K
     memset(c->lvl, 0, sizeof(c->lvl));
     c->js = nullptr; c->jsmap = nullptr; c->feattypes = nullptr; c->mono = nullptr; c->absmax = nullptr; c->absmax_cur = 0; c->absmax_other = 1; c->absmax_spare = 2; c->grad_next = nullptr; c->path_off = 0; c->metric_host = nullptr; c->metric_queued = false; c->slot_path[0] = c->slot_path[1] = false; c->qexp = nullptr; c->qbits = nullptr;
     c->alphas = nullptr; c->alphas_f = nullptr; c->qkeys_a = c->qkeys_b = nullptr; c->qtemp = nullptr; c->qtemp_bytes = 0;
+    c->teach_ids = nullptr; c->teach_scores = nullptr; c->teach_n = 0; c->teach_temperature = 1.0;
     c->n_alphas = 1;
     for (int k = 0; k < EVT_MAX_K; k++) c->h_alphas[k] = 0.5;
     c->qscale = nullptr; c->qexp_buf[0] = c->qexp_buf[1] = nullptr; c->qscale_buf[0] = c->qscale_buf[1] = nullptr; c->q_cur = c->q_tree = 0; c->quant_pending = false;
@@ -712,6 +714,49 @@ extern "C" int evt_set_alphas(evt_handle c, const double *alphas, int32_t n) {
     HIPCHK(upload_alphas(c));
     HIPCHK(hipStreamSynchronize(c->stream));
     c->have_grads = false; // the gradients of the quantile losses depend on the levels
+    c->grads_ready = false;
+    return EVT_OK;
+    });
+}
+
+extern "C" int evt_set_teacher(evt_handle c, const int32_t *ids, const float *scores, int32_t n_top, double temperature) {
+    return guarded([&]() -> int {
+    CTXCHK(c);
+    ARGCHK(c->loss == EVT_LOSS_MLOGLOSS, "a teacher needs the mlogloss loss");
+    ARGCHK(n_top >= 0 && n_top <= EVT_SCORES_MAX_TOP, "n_top must be in [0, 1024]");
+    ARGCHK(n_top == 0 || (ids && scores), "ids and scores must not be NULL");
+    ARGCHK(n_top == 0 || (temperature > 0.0 && temperature < INFINITY), "temperature must be positive and finite");
+    int32_t *ti = nullptr;
+    float *ts = nullptr;
+    if (n_top) {
+        const size_t words = (size_t)c->N * n_top;
+        ti = static_cast<int32_t *>(dev_take(words * sizeof(int32_t)));
+        ts = ti ? static_cast<float *>(dev_take(words * sizeof(float))) : nullptr;
+        int r = ts ? EVT_OK : EVT_ERR_NOMEM;
+        hipError_t e = hipSuccess;
+        if (r == EVT_OK) e = hipMemcpyAsync(ti, ids, words * sizeof(int32_t), hipMemcpyDefault, c->stream);
+        if (r == EVT_OK && e == hipSuccess) e = hipMemcpyAsync(ts, scores, words * sizeof(float), hipMemcpyDefault, c->stream);
+        if (e != hipSuccess) {
+            evt_set_error("evt_set_teacher: %s", hipGetErrorString(e));
+            r = EVT_ERR_HIP;
+        }
+        if (r == EVT_OK) r = launch_validate_teacher(c, ti, ts, n_top);
+        if (r == EVT_OK) r = check_errflag(c, "a teacher's ids must be below the number of classes and its scores numbers below infinity");
+        if (r != EVT_OK) { // the teacher there was stays
+            (void)hipStreamSynchronize(c->stream);
+            dev_give(ti);
+            dev_give(ts);
+            return r;
+        }
+    }
+    HIPCHK(hipStreamSynchronize(c->stream)); // kernels queued earlier read the old teacher
+    dev_give(c->teach_ids);
+    dev_give(c->teach_scores);
+    c->teach_ids = ti;
+    c->teach_scores = ts;
+    c->teach_n = n_top;
+    c->teach_temperature = n_top ? temperature : 1.0;
+    c->have_grads = false;
     c->grads_ready = false;
     return EVT_OK;
     });

@@ -178,6 +178,11 @@ struct evt_ctx {
     unsigned long long *qkeys_a, *qkeys_b; // [N] (node, residual) keys, unsorted / sorted
     void *qtemp;
     size_t qtemp_bytes;
+    // mlogloss with a teacher (evt_set_teacher): teach_n entries a row, 0 for none
+    int32_t *teach_ids;
+    float *teach_scores;
+    int32_t teach_n;
+    double teach_temperature;
     int32_t *qexp;     // [EVT_MC_MAX_NK]; points into qexp_buf: the tables of the gradients quantised last
     int32_t *qbits;    // [EVT_MC_MAX_NK]
     double *qscale;    // [2 * EVT_MC_MAX_NK]: decode scale per global channel, then encode multiplier per gradient row
@@ -469,6 +474,7 @@ uint32_t *absmax_set(evt_ctx *c, int which);
 int launch_apply_pending(evt_ctx *c);
 int launch_set_weight_row(evt_ctx *c, const float *w_dev);
 int launch_validate_classes(evt_ctx *c);
+int launch_validate_teacher(evt_ctx *c, const int32_t *ids, const float *scores, int n_top);
 int launch_init_pred(evt_ctx *c, const float *mu_dev, const float *offset_dev);
 // data layout
 int launch_transpose_validate(evt_ctx *c);

@@ -313,6 +313,20 @@ __global__ __launch_bounds__(256) void k_validate_classes(const float *__restric
     }
     if (bad) atomicOr(errflag, 1);
 }
+// A teacher's entries (evt_set_teacher): ids below K, scores that are numbers and not +inf.
+__global__ __launch_bounds__(256) void k_validate_teacher(const int32_t *__restrict__ ids, const float *__restrict__ scores, int64_t n, int K, int32_t *errflag) {
+    bool bad = false;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) bad |= ids[i] >= K || (ids[i] >= 0 && !(scores[i] < INFINITY));
+    if (bad) atomicOr(errflag, 1);
+}
+int launch_validate_teacher(evt_ctx *c, const int32_t *ids, const float *scores, int n_top) {
+    const int64_t n = c->N * n_top;
+    int64_t nb = (n + 255) / 256;
+    if (nb > 2048) nb = 2048;
+    hipLaunchKernelGGL(k_validate_teacher, dim3((unsigned)nb), dim3(256), 0, c->stream, ids, scores, n, c->K, c->errflag);
+    HIPCHK(hipGetLastError());
+    return EVT_OK;
+}
 int launch_validate_classes(evt_ctx *c) {
     int64_t nb = (c->N + 255) / 256;
     if (nb > 2048) nb = 2048;

@@ -8,6 +8,7 @@
 // first thing the next gradient pass does (4 B of node id read and 4K B written more per row) - or in
 // k_apply_leaf when something else needs the predictions first.
 #include "grad_math.h"
+#include "scores.h"
 #include <algorithm>
 
 // Maxima of any number of outputs (mx[k] and mx[EVT_MAX_K + k]: gradient row k and K + k), by a whole block of 256 threads: a thread raises a
@@ -197,6 +198,73 @@ __global__ __launch_bounds__(256) void k_grads_mlogloss(float *__restrict__ pred
     raise_maxima(mx, K, absmax);
 }
 
+// mlogloss with a teacher: the gradients are distill_loss's, T (q - p) w with q = softmax(pred / T), written into the gradient matrix by its kernel
+// (kernels_scores.hip); this pass adds the second-order rows T^2 d2KL / dpred^2 = q (1 - q) w and raises the maxima of both.
+template <int KM>
+__global__ __launch_bounds__(256) void k_grads_teacher(const float *__restrict__ pred, float *__restrict__ grad, int64_t N, int K, float inv_t, uint32_t *absmax,
+                                                      int unit_w) {
+    const int NK = 2 * K + 1;
+    float mx[2 * EVT_MAX_K];
+#pragma unroll
+    for (int k = 0; k < 2 * EVT_MAX_K; k++) mx[k] = 0.0f;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < N; i += (int64_t)gridDim.x * 256) {
+        const float *pr = pred + (size_t)K * i;
+        float *g = grad + (size_t)NK * i;
+        const float w = unit_w ? 1.0f : g[NK - 1];
+        float e[KM], gg[KM], m = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < KM; k++) e[k] = pr[k < K ? k : K - 1];
+#pragma unroll
+        for (int k = 0; k < KM; k++) gg[k] = g[k < K ? k : K - 1];
+#pragma unroll
+        for (int k = 0; k < KM; k++) m = fmaxf(m, e[k]);
+#pragma unroll
+        for (int k = 0; k < KM; k++) {
+            if (k < K) {
+                e[k] = expf((e[k] - m) * inv_t);
+                sum += e[k];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KM; k++) {
+            if (k < K) {
+                const float q = e[k] / sum, hh = (q * (1.0f - q)) * w;
+                g[K + k] = hh;
+                mx[k] = fmaxf(mx[k], fabsf(gg[k]));
+                mx[EVT_MAX_K + k] = fmaxf(mx[EVT_MAX_K + k], hh);
+            }
+        }
+    }
+    raise_maxima(mx, K, absmax);
+}
+static int launch_grads_teacher(evt_ctx *c, uint32_t *am, dim3 grid) {
+    int r = launch_apply_pending(c);
+    if (r != EVT_OK) return r;
+    ScoreArgs a = {};
+    score_scale(a, c->teach_temperature);
+    a.x = c->pred;
+    a.xs = c->K;
+    a.g = c->grad;
+    a.gs = c->NK;
+    a.N = c->N;
+    a.V = c->K;
+    a.weights = c->unit_w ? nullptr : c->grad + c->NK - 1;
+    a.ws = c->NK;
+    a.ids = c->teach_ids;
+    a.top = c->teach_scores;
+    a.top_type = EVT_F32;
+    a.n_top = c->teach_n;
+    r = launch_distill_f32(c->stream, a);
+    if (r != EVT_OK) return r;
+    const float inv_t = (float)a.inv_t;
+    const int unit = c->unit_w ? 1 : 0;
+    if (c->K <= 4) hipLaunchKernelGGL(k_grads_teacher<4>, grid, dim3(256), 0, c->stream, c->pred, c->grad, c->N, c->K, inv_t, am, unit);
+    else if (c->K <= 8) hipLaunchKernelGGL(k_grads_teacher<8>, grid, dim3(256), 0, c->stream, c->pred, c->grad, c->N, c->K, inv_t, am, unit);
+    else hipLaunchKernelGGL(k_grads_teacher<16>, grid, dim3(256), 0, c->stream, c->pred, c->grad, c->N, c->K, inv_t, am, unit);
+    HIPCHK(hipGetLastError());
+    return EVT_OK;
+}
+
 // The quantile losses (src/loss.jl:85-91, :144-171): row k = (alpha or alpha - 1, a Float64) * w, row K + k = the raw
 // residual (not weighted: the leaf pass takes its quantile).  multi: one target column and a level per output
 // (multiquantile); otherwise one level and a target column per output (quantile).
@@ -254,6 +322,7 @@ int launch_grads(evt_ctx *c) {
     int64_t nb = (c->N + 255) / 256;
     if (nb > 2048) nb = 2048;
     dim3 grid((unsigned)nb);
+    if (c->teach_n) return launch_grads_teacher(c, am, grid);
     const uint32_t *pn = c->pend_pred ? c->nidx : nullptr; // the last tree's leaf values are added on the way
     c->pend_pred = false;
     if (EVT_IS_QUANTILE(c->loss)) {

@@ -219,7 +219,7 @@ __device__ __forceinline__ float labelled_row(const ScoreArgs &a, int64_t row, b
     float slope = 0.0f;
     if (OP == SC_POLICY) {
         float loss;
-        policy_row(a, row, a.weights ? a.weights[row] : 1.0f, logp, loss, slope);
+        policy_row(a, row, a.weights ? a.weights[row * a.ws] : 1.0f, logp, loss, slope);
         slope = (float)(slope * a.inv_t);
         if (writes) a.loss[row] = loss;
     }
@@ -235,7 +235,7 @@ __device__ __forceinline__ float labelled_row(const ScoreArgs &a, int64_t row, b
 }
 template <int OP>
 __device__ __forceinline__ void left_out(const ScoreArgs &a, int64_t row) {
-    if (OP == SC_DISTILL || OP == SC_POLICY) a.loss[row] = 0.0f;
+    if ((OP == SC_DISTILL && a.loss) || OP == SC_POLICY) a.loss[row] = 0.0f;
     if (OP == SC_LOGP || OP == SC_POLICY) a.logp[row] = 0.0f;
     if (OP == SC_LOGP && a.stats) a.stats[2 * row] = a.stats[2 * row + 1] = 0.0f;
     if (OP == SC_LOGP && a.slope) a.slope[row] = 0.0f;
@@ -300,7 +300,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     };
     if (a.early) load_row(); // whether the row counts or not
     if (OP == SC_DISTILL) {
-        w = a.weights ? a.weights[row] : 1.0f;
+        w = a.weights ? a.weights[row * a.ws] : 1.0f;
         live = w != 0.0f;
     } else {
         label = load_id(a.labels, a.label64, row);
@@ -404,7 +404,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
                 if (e.x >= 0 && pj != 0.0f) sum += pj * ((load_score(a.top, a.top_type, row * a.n_top + j) - teacher.m) - (s_x[j] - r.m));
             }
             sum = lanes_sum<64>(sum);
-            if (t == 0) a.loss[row] = state == 2 ? NAN : w * a.t2_mul * (float)((double)sum * a.inv_t + logs);
+            if (t == 0 && a.loss) a.loss[row] = state == 2 ? NAN : w * a.t2_mul * (float)((double)sum * a.inv_t + logs);
         }
         factor = state == 2 ? NAN : w * a.t_mul;
     } else {
@@ -522,7 +522,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
     T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
     const float mul = a.exp_mul;
     const bool past = a.past;
-    const float w = !in_range ? 0.0f : a.weights ? a.weights[row] : 1.0f;
+    const float w = !in_range ? 0.0f : a.weights ? a.weights[row * a.ws] : 1.0f;
     Piece<T> p[FEW ? 1 : NV];
     float few[FEW ? E : 1];
     if constexpr (FEW) {
@@ -674,7 +674,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
         }
         cross = lanes_sum<G::SIZE>(cross);
     }
-    if (t == 0) {
+    if (t == 0 && a.loss) {
         const double logs = r.s == 0.0f ? 0.0 : log_sum(r.s * one);
         a.loss[row] = none ? NAN : w * a.t2_mul * (float)((double)((sum - cross) * one) * a.inv_t + logs);
     }
@@ -739,35 +739,57 @@ __global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, int pairs, c
     __shared__ int s_cnt[2][16];
     const int t = threadIdx.x, p = blockIdx.x;
     int64_t from[2], to[2];
-    double lp[2], len[2];
+    double lp[2] = {0.0, 0.0}, len[2];
+    int cnt[2] = {0, 0};
     bool bad = false;
+#pragma unroll
     for (int k = 0; k < 2; k++) {
         from[k] = a.bounds[p + k * pairs];
         to[k] = a.bounds[p + k * pairs + 1];
+    }
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
         if (from[k] < 0 || to[k] > a.N || to[k] < from[k]) { // not ascending, or out of the rows
             bad = true;
             from[k] = to[k] = 0;
         }
-        double sum = 0.0;
-        int cnt = 0;
-        for (int64_t i = from[k] + t; i < to[k]; i += 1024) {
-            sum += (double)a.logp[i];
-            cnt += load_id(a.labels, a.label64, i) >= 0;
+    }
+    const int64_t longer = to[0] - from[0] > to[1] - from[1] ? to[0] - from[0] : to[1] - from[1];
+    for (int64_t i = t; i < longer; i += 1024) {
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            if (from[k] + i < to[k]) {
+                lp[k] += (double)a.logp[from[k] + i];
+                cnt[k] += load_id(a.labels, a.label64, from[k] + i) >= 0;
+            }
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            lp[k] += __shfl_xor(lp[k], o);
+            cnt[k] += __shfl_xor(cnt[k], o);
+        }
+    if ((t & 63) == 0)
+        for (int k = 0; k < 2; k++) s_sum[k][t >> 6] = lp[k], s_cnt[k][t >> 6] = cnt[k];
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        lp[k] = s_sum[k][t & 15];
+        cnt[k] = s_cnt[k][t & 15];
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            lp[k] += __shfl_xor(lp[k], o);
+            cnt[k] += __shfl_xor(cnt[k], o);
         }
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-            sum += __shfl_xor(sum, o);
-            cnt += __shfl_xor(cnt, o);
-        }
-        if ((t & 63) == 0) s_sum[k][t >> 6] = sum, s_cnt[k][t >> 6] = cnt;
-    }
-    __syncthreads();
     for (int k = 0; k < 2; k++) {
-        double sum = 0.0;
-        int cnt = 0;
-        for (int w = 0; w < 16; w++) sum += s_sum[k][w], cnt += s_cnt[k][w];
-        len[k] = average && cnt ? cnt : 1;
-        lp[k] = sum / len[k];
+        len[k] = average && cnt[k] ? cnt[k] : 1;
+        lp[k] /= len[k];
     }
     const double w = a.weights ? a.weights[p] : 1.0;
     const double h = beta * ((lp[0] - lp[1]) - ((double)ref_logp[p] - (double)ref_logp[p + pairs])) - margin;
@@ -862,6 +884,14 @@ static int launch_scores(hipStream_t s, const ScoreArgs &a, int dtype) {
     return r;
 }
 
+void score_scale(ScoreArgs &a, double temperature) {
+    a.inv_t = 1.0 / temperature;
+    a.exp_mul = (float)(1.4426950408889634 / temperature);
+    a.t_mul = (float)temperature;
+    a.t2_mul = (float)(temperature * temperature);
+}
+int launch_distill_f32(hipStream_t s, const ScoreArgs &a) { return launch_scores<SC_DISTILL>(s, a, EVT_F32); }
+
 // ---- entry points ---------------------------------------------------------------------------
 static bool on_device(const void *p) {
     hipPointerAttribute_t attr;
@@ -905,10 +935,8 @@ static int take_scores(const evt_scores *s, bool grad_needed, int32_t flags, Sco
     a.g = s->grad;
     a.xs = s->row_stride;
     a.gs = s->grad_stride;
-    a.inv_t = 1.0 / s->temperature;
-    a.exp_mul = (float)(1.4426950408889634 / s->temperature);
-    a.t_mul = (float)s->temperature;
-    a.t2_mul = (float)(s->temperature * s->temperature);
+    a.ws = 1;
+    score_scale(a, s->temperature);
     a.past = (double)a.N * a.V * size > 256e6;
     return check_device(flags, s->x, s->grad);
 }
@@ -925,8 +953,9 @@ static int take_labels(const void *labels, int32_t dtype, ScoreArgs &a) {
         if (_r != EVT_OK) return _r;     \
     } while (0)
 
-extern "C" int evt_class_logp(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, float *logp, float *stats, int32_t flags) {
+extern "C" int evt_class_logp(void *stream, const void *scores, const void *labels, int32_t label_dtype, float *logp, float *stats, int32_t flags) {
     return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
     ScoreArgs a = {};
     TRY(take_scores(s, false, flags, a));
     TRY(take_labels(labels, label_dtype, a));
@@ -939,9 +968,10 @@ extern "C" int evt_class_logp(void *stream, const evt_scores *s, const void *lab
     });
 }
 
-extern "C" int evt_class_logp_grad(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const float *stats, const float *dlogp,
+extern "C" int evt_class_logp_grad(void *stream, const void *scores, const void *labels, int32_t label_dtype, const float *stats, const float *dlogp,
                                    int32_t flags) {
     return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
     ScoreArgs a = {};
     TRY(take_scores(s, true, flags, a));
     TRY(take_labels(labels, label_dtype, a));
@@ -954,9 +984,10 @@ extern "C" int evt_class_logp_grad(void *stream, const evt_scores *s, const void
     });
 }
 
-extern "C" int evt_distill_loss(void *stream, const evt_scores *s, const void *top_ids, int32_t id_dtype, const void *top_scores, int32_t top_dtype,
+extern "C" int evt_distill_loss(void *stream, const void *scores, const void *top_ids, int32_t id_dtype, const void *top_scores, int32_t top_dtype,
                                 int32_t n_top, const float *weights, float *loss, int32_t flags) {
     return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
     ScoreArgs a = {};
     TRY(take_scores(s, false, flags, a));
     ARGCHK(id_dtype == EVT_I32 || id_dtype == EVT_I64, "top_ids must be EVT_I32 or EVT_I64");
@@ -976,10 +1007,11 @@ extern "C" int evt_distill_loss(void *stream, const evt_scores *s, const void *t
     });
 }
 
-extern "C" int evt_policy_loss(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const float *old_logp, const float *advantages,
+extern "C" int evt_policy_loss(void *stream, const void *scores, const void *labels, int32_t label_dtype, const float *old_logp, const float *advantages,
                                const float *ref_logp, const float *weights, double clip_low, double clip_high, double kl_coef, float *loss, float *logp,
                                int32_t flags) {
     return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
     ScoreArgs a = {};
     TRY(take_scores(s, false, flags, a));
     TRY(take_labels(labels, label_dtype, a));
@@ -1004,10 +1036,11 @@ extern "C" int evt_policy_loss(void *stream, const evt_scores *s, const void *la
     });
 }
 
-extern "C" int evt_preference_loss(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
+extern "C" int evt_preference_loss(void *stream, const void *scores, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
                                    const float *ref_logp, const float *weights, double beta, double label_smoothing, double margin, int32_t average,
                                    float *loss, float *seq_logp, float *work, int32_t flags) {
     return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
     ScoreArgs a = {};
     TRY(take_scores(s, false, flags, a));
     TRY(take_labels(labels, label_dtype, a));

@@ -22,7 +22,8 @@ struct ScoreArgs {
     // rows outside [bounds[0], bounds[n_bounds - 1]) are left out (nullptr: none is)
     const int32_t *bounds;
     int32_t n_bounds;
-    const float *weights; // a row's, nullptr: ones
+    const float *weights; // a row's, ws elements apart, nullptr: ones
+    int64_t ws;
     float *loss, *logp, *stats;
     float *slope; // SC_GRAD reads a row's dloss / dlogp here; SC_LOGP clears it for the kernel that fills it in (nullptr: does not)
     // SC_DISTILL
@@ -34,3 +35,6 @@ struct ScoreArgs {
     double log_lo, log_hi; // the bounds of logp - old_logp
     double lo, hi, kl;
 };
+
+void score_scale(ScoreArgs &a, double temperature);
+int launch_distill_f32(hipStream_t s, const ScoreArgs &a); // loss nullptr: none

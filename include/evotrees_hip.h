@@ -193,6 +193,13 @@ int evt_set_feature_meta(evt_handle h, const uint8_t *feattypes, const int32_t *
  * use the Float64 values (src/loss.jl:85-91), the metrics T(alpha) (src/callback.jl:62-66). */
 int evt_set_alphas(evt_handle h, const double *alphas, int32_t n);
 
+/* No counterpart in the reference: an mlogloss handle that is fitted to a teacher - a larger model, or a language model that scored the rows - in place of
+ * its target's labels.  ids and scores are nobs x n_top (a row's entries side by side): the classes the teacher kept of each row, counted from 0 (level code - 1;
+ * below 0: no entry), and their scores.  evt_update_grads then computes the gradients of evt_distill_loss at this temperature,
+ * T (q - p) w with q = softmax(pred / T) and p = softmax(scores / T) over the row's entries, and the second-order rows q (1 - q) w.  A row without entries has no
+ * gradient.  n_top 0 (ids and scores may be NULL) goes back to the labels, which the metric is computed from in either case. */
+int evt_set_teacher(evt_handle h, const int32_t *ids, const float *scores, int32_t n_top, double temperature);
+
 /* update_grads!(cache.∇, cache.pred, cache.y, L, params): src/loss.jl:100-111, :219-236;
  * device twin ext/.../loss.jl:183-191. */
 int evt_update_grads(evt_handle h);
@@ -416,15 +423,15 @@ typedef struct {
 
 /* logp[i] = log q[i, labels[i]], and stats[2 i], stats[2 i + 1] = the row's maximum of x and sum of exp((x - maximum) / temperature) (both 0
  * for a row left out), which the gradient takes: grad[i, :] = dlogp[i] (onehot(labels[i]) - q[i, :]) / temperature.  A row with dlogp 0 is not read. */
-int evt_class_logp(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, float *logp, float *stats, int32_t flags);
-int evt_class_logp_grad(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const float *stats, const float *dlogp,
+int evt_class_logp(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, float *logp, float *stats, int32_t flags);
+int evt_class_logp_grad(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, const float *stats, const float *dlogp,
                         int32_t flags);
 
 /* Distillation from a teacher that kept its n_top best classes of each row (1 .. 1024): top_ids and top_scores are nrows x n_top, an id below 0 is no
  * entry, and an id may come twice.  With p = softmax(top_scores / temperature) over a row's entries and w = weights[i] (NULL: 1):
  *   loss[i] = w temperature^2 sum_j p_j (log p_j - log q[id_j]),   grad[i, c] = w temperature (q_c - sum of p_j with id_j == c).
  * A row without entries, or with none above -inf, is left out. */
-int evt_distill_loss(void *stream, const evt_scores *s, const void *top_ids, int32_t id_dtype, const void *top_scores, int32_t top_dtype,
+int evt_distill_loss(void *stream, const void *scores /* evt_scores */, const void *top_ids, int32_t id_dtype, const void *top_scores, int32_t top_dtype,
                      int32_t n_top, const float *weights, float *loss, int32_t flags);
 
 /* The clipped policy loss of every token: with r = exp(logp - old_logp), A = advantages[i], b = ref_logp - logp and w = weights[i] (NULL: 1),
@@ -432,7 +439,7 @@ int evt_distill_loss(void *stream, const evt_scores *s, const void *top_ids, int
  *   grad[i, :] = dloss/dlogp (onehot(label) - q) / temperature,  dloss/dlogp = w (-r A where the first term is the smaller or both are equal, else 0;
  *   + kl_coef (1 - exp(b))).
  * An advantage of 0 has no share in the first term whatever r is.  ref_logp may be NULL with kl_coef 0, and is not read then. */
-int evt_policy_loss(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const float *old_logp, const float *advantages,
+int evt_policy_loss(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, const float *old_logp, const float *advantages,
                     const float *ref_logp, const float *weights, double clip_low, double clip_high, double kl_coef, float *loss, float *logp,
                     int32_t flags);
 
@@ -443,7 +450,7 @@ int evt_policy_loss(void *stream, const evt_scores *s, const void *labels, int32
  *   loss[p] = w (-(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)).
  * The gradient of sum_p loss[p] is written for every row: 0 for those in front of the first and behind the last sequence.  A pair whose
  * offsets do not ascend or leave the rows gets NaN.  work: 4 nrows floats that the call may write.  label_smoothing in [0, 0.5]. */
-int evt_preference_loss(void *stream, const evt_scores *s, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
+int evt_preference_loss(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
                         const float *ref_logp, const float *weights, double beta, double label_smoothing, double margin, int32_t average,
                         float *loss, float *seq_logp, float *work, int32_t flags);
 

@@ -139,3 +139,10 @@ def test_c_entry_points_refuse(evt):
         assert policy(scores(), **more) == E.EVT_ERR_ARG
     for more in (dict(n=0), dict(n=1 << 30), dict(beta=0.0), dict(beta=float("inf")), dict(soft=0.7), dict(margin=float("inf")), dict(avg=2)):
         assert pref(scores(), **more) == E.EVT_ERR_ARG
+
+
+def test_a_teacher_needs_a_classifier(evt):
+    import numpy as np
+    with pytest.raises(ValueError, match="mlogloss"):
+        evt.init(evt.EvoTreeRegressor(), np.zeros((4, 1)), np.zeros(4), teacher=evt.Teacher(np.zeros((4, 1), int), np.zeros((4, 1))))
+    assert evt._lib.load().evt_set_teacher(None, None, None, 0, 1.0) == evt._lib.EVT_ERR_ARG

@@ -7,7 +7,7 @@ classes, a language model's vocabulary as well as a classifier's levels, and hav
 
 Scores are a (rows, classes) tensor of float32, bfloat16 or float16 whose classes lie side by side (`scores.stride(1) == 1`); rows may be
 any distance apart.  Labels and class ids count from 0 and are int32 or int64; a negative one stands for none.  Values that
-belong to a row, an entry or a pair are contiguous float32.  All tensors of a call are on one GPU; the work is queued on that GPU's current
+belong to a row, an entry or a pair are contiguous float32.  Temperatures are from 1e-4 to 1e4.  All tensors of a call are on one GPU; the work is queued on that GPU's current
 stream and nothing waits for it.  As the gradients of this package's other losses, these are returned, not recorded: there is no autograd
 graph, and a loss's weights stand in for what a chain rule would multiply it by.  `out` takes the gradient: a tensor like the scores, or the scores
 themselves, which the gradient then replaces.
@@ -81,7 +81,7 @@ class _Call:
         if x.stride(1) != 1 and classes > 1:
             raise ValueError("the scores of a row must lie side by side, got strides %s" % (x.stride(),))
         self.x, self.kind, self.rows, self.device = x, kind, rows, x.get_device()
-        self.temperature = _number("temperature", temperature, 0.0, _INF, True)
+        self.temperature = _number("temperature", temperature, 1e-4, 1e4)
 
     def check(self, name, v, shape, kinds):
         """v's address, and its type's code by way of `kinds`."""

@@ -725,7 +725,7 @@ extern "C" int evt_set_teacher(evt_handle c, const int32_t *ids, const float *sc
     ARGCHK(c->loss == EVT_LOSS_MLOGLOSS, "a teacher needs the mlogloss loss");
     ARGCHK(n_top >= 0 && n_top <= EVT_SCORES_MAX_TOP, "n_top must be in [0, 1024]");
     ARGCHK(n_top == 0 || (ids && scores), "ids and scores must not be NULL");
-    ARGCHK(n_top == 0 || (temperature > 0.0 && temperature < INFINITY), "temperature must be positive and finite");
+    ARGCHK(n_top == 0 || (temperature >= 1e-4 && temperature <= 1e4), "temperature must be in [1e-4, 1e4]");
     int32_t *ti = nullptr;
     float *ts = nullptr;
     if (n_top) {

@@ -170,8 +170,8 @@ __device__ __forceinline__ float load_score(const void *p, int type, int64_t i) 
     return type == EVT_F32 ? ((const float *)p)[i] : type == EVT_BF16 ? (float)((const bf16_t *)p)[i] : (float)((const half_t *)p)[i];
 }
 
-// log(s) to 3e-8: the exponent's share in 64 bits, the mantissa's, of at most 0.35, in 32.  (In 32 bits altogether a sum over a large vocabulary costs
-// 5e-7, in 64 a block of sixteen wavefronts about 4 us a row.)
+// log(s) to 3e-8: the exponent's share in 64 bits, the mantissa's, of at most 0.35, in 32.  (In 32 bits altogether the logarithm of a sum over a large
+// vocabulary is off by 5e-7; in 64 it is some hundred instructions of every wavefront.)
 __device__ __forceinline__ double log_sum(float s) {
     int k;
     float f = frexpf(s, &k);
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     static_assert(OP != SC_DISTILL || G::ROWS == 1, "k_distill_short has the others");
     extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs, then the scores of these classes
     __shared__ int s_state;                  // SC_DISTILL: 1 a teacher, 2 with an id of no class
-    const int64_t row = (int64_t)blockIdx.x * G::ROWS + G::slot();
+    const int64_t row = a.row0 + (int64_t)blockIdx.x * G::ROWS + G::slot();
     if (G::ROWS > 1 && row >= a.N) return;
     const int t = G::rank(), V = a.V;
     const T *x = (const T *)a.x + row * a.xs;
@@ -465,7 +465,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
 template <typename T, int OP>
 __global__ __launch_bounds__(256) void k_few_classes(ScoreArgs a) {
     constexpr int KM = Piece<T>::E;
-    const int64_t row = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t row = a.row0 + (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (row >= a.N) return;
     const int V = a.V;
     const T *x = (const T *)a.x + row * a.xs;
@@ -515,7 +515,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
     const int V = a.V, k1 = a.n_top, ks = k1 | 1, vs = (V + 2) | 1; // odd distances: rows that lanes read side by side start in different banks
     int2 *const s_all = (int2 *)s_dyn; // (class, V for no entry, V + 1 for no class; score)
     float *const s_share = (float *)(s_all + G::ROWS * ks);
-    const int64_t row0 = (int64_t)blockIdx.x * G::ROWS, row = row0 + G::slot();
+    const int64_t row0 = a.row0 + (int64_t)blockIdx.x * G::ROWS, row = row0 + G::slot();
     const int t = G::rank();
     const bool in_range = row < a.N;
     const T *x = (const T *)a.x + (in_range ? row : a.N - 1) * a.xs;
@@ -585,7 +585,7 @@ __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top
         r = lanes_join<G::SIZE>(r, mul);
     }
     // The teacher's entries, four at a time, for each is a trip to shared memory or two: their maximum while each leaves its number at its class, then
-    // exp of each in the number's place - another number there is an entry of the same class.  (Added up there by float atomics, 165 cycles a
+    // exp of each in the number's place - another number there is an entry of the same class.  (Added up there by float atomics, some 165 cycles a
     // wavefront each, 8M rows of 7 classes and entries take 347 us for 237.)
     float most = LOWEST, total = 0.0f, sum = 0.0f;
     bool none = false, twice = false;
@@ -812,11 +812,20 @@ __global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, int pairs, c
     }
 }
 
+// A launch has fewer than 2^32 threads: more rows go in several.  f(args, blocks) for each
+template <typename F>
+static void slices(ScoreArgs a, int rows, int threads, F &&f) {
+    const int64_t most = (int64_t)(1 << 22) * 1024 / threads - 1; // blocks
+    for (a.row0 = 0; a.row0 < a.N; a.row0 += most * rows) {
+        const int64_t left = (a.N - a.row0 + rows - 1) / rows;
+        f(a, dim3((unsigned)(left < most ? left : most)));
+    }
+}
 template <typename T, int OP, int NV, class G>
 static int launch_rows(hipStream_t s, ScoreArgs a) {
     a.early = a.N <= 512;
     const size_t lds = OP == SC_DISTILL ? (size_t)a.n_top * 12 : 0;
-    hipLaunchKernelGGL((k_rows<T, OP, NV, G>), dim3((unsigned)((a.N + G::ROWS - 1) / G::ROWS)), dim3(G::THREADS), lds, s, a);
+    slices(a, G::ROWS, G::THREADS, [&](const ScoreArgs &b, dim3 grid) { hipLaunchKernelGGL((k_rows<T, OP, NV, G>), grid, dim3(G::THREADS), lds, s, b); });
     return EVT_OK;
 }
 // Distillation of short rows: true where the lanes hold a row of n pieces and a block's memory its teachers, 52 KB so that a unit has three blocks
@@ -825,18 +834,21 @@ static bool launch_distill(hipStream_t s, const ScoreArgs &a, int64_t n) {
     const size_t lds = G::ROWS * ((size_t)(a.n_top | 1) * 8 + (size_t)((a.V + 2) | 1) * 4);
     if ((NV ? a.V < Piece<T>::E || n > (int64_t)G::SIZE * NV : a.V >= Piece<T>::E) || (lds > 53248 && G::SIZE < 64) || lds > 65536) return false;
     const uint32_t magic = a.n_top > 1 ? (uint32_t)(((1ull << 32) + a.n_top - 1) / a.n_top) : 0u; // exact for e / n_top, e * n_top < 2^32
-    hipLaunchKernelGGL((k_distill_short<T, NV, G>), dim3((unsigned)((a.N + G::ROWS - 1) / G::ROWS)), dim3(256), lds, s, a, magic);
+    slices(a, G::ROWS, 256, [&](const ScoreArgs &b, dim3 grid) { hipLaunchKernelGGL((k_distill_short<T, NV, G>), grid, dim3(256), lds, s, b, magic); });
     return true;
 }
 template <typename T, int OP>
 static int launch_typed(hipStream_t s, const ScoreArgs &a) {
     constexpr int E = Piece<T>::E;
     const int64_t n = ((int64_t)a.V + E - 1) / E;
+    const bool few = a.N <= 256; // no more than a unit each
     if constexpr (OP == SC_DISTILL) {
-        if (launch_distill<T, 0, Lanes<1>>(s, a, n) || launch_distill<T, 0, Lanes<8>>(s, a, n) || launch_distill<T, 0, Lanes<64>>(s, a, n) ||
-            launch_distill<T, 4, Lanes<1>>(s, a, n) || launch_distill<T, 4, Lanes<2>>(s, a, n) || launch_distill<T, 4, Lanes<4>>(s, a, n) ||
-            launch_distill<T, 4, Lanes<8>>(s, a, n) || launch_distill<T, 4, Lanes<16>>(s, a, n) || launch_distill<T, 4, Lanes<32>>(s, a, n) ||
-            launch_distill<T, 4, Lanes<64>>(s, a, n))
+        if (launch_distill<T, 0, Lanes<1>>(s, a, n) || launch_distill<T, 0, Lanes<8>>(s, a, n) || launch_distill<T, 0, Lanes<64>>(s, a, n)) return EVT_OK;
+        // few rows of more than a few classes: a block to each is done sooner (4 rows of 2048 bf16: 9.5 us by lanes, 6.1 so)
+        if ((!few || n <= 32) &&
+            (launch_distill<T, 4, Lanes<1>>(s, a, n) || launch_distill<T, 4, Lanes<2>>(s, a, n) || launch_distill<T, 4, Lanes<4>>(s, a, n) ||
+             launch_distill<T, 4, Lanes<8>>(s, a, n) || launch_distill<T, 4, Lanes<16>>(s, a, n) || launch_distill<T, 4, Lanes<32>>(s, a, n) ||
+             launch_distill<T, 4, Lanes<64>>(s, a, n)))
             return EVT_OK;
         if (a.V < E) {
             evt_set_error("no form for %d classes and %d entries", a.V, a.n_top); // k_rows' last piece would start in front of the row
@@ -844,7 +856,7 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
         }
     } else {
         if (a.V < E) {
-            hipLaunchKernelGGL((k_few_classes<T, OP>), dim3((unsigned)((a.N + 255) / 256)), dim3(256), 0, s, a);
+            slices(a, 256, 256, [&](const ScoreArgs &b, dim3 grid) { hipLaunchKernelGGL((k_few_classes<T, OP>), grid, dim3(256), 0, s, b); });
             return EVT_OK;
         }
         // lanes to a row: four pieces each
@@ -858,10 +870,9 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
     }
     if constexpr (OP == SC_GRAD) {
         const int64_t parts = (n + 1023) / 1024, blocks = a.N * parts;
-        hipLaunchKernelGGL(k_slope_rows<T>, dim3((unsigned)(blocks < (1 << 30) ? blocks : (1 << 30))), dim3(256), 0, s, a, (int)parts);
+        hipLaunchKernelGGL(k_slope_rows<T>, dim3((unsigned)(blocks < (1 << 23) ? blocks : (1 << 23))), dim3(256), 0, s, a, (int)parts);
         return EVT_OK;
     } else {
-        const bool few = a.N <= 256;
         if constexpr (OP != SC_DISTILL) {
             if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
         }
@@ -914,7 +925,7 @@ static int take_scores(const evt_scores *s, bool grad_needed, int32_t flags, Sco
     ARGCHK(flags == 0 || flags == EVT_STATIC_TRUSTED, "flags takes 0 or EVT_STATIC_TRUSTED");
     ARGCHK(s->dtype == EVT_F32 || s->dtype == EVT_BF16 || s->dtype == EVT_F16, "scores must be EVT_F32, EVT_BF16 or EVT_F16");
     ARGCHK(s->nrows >= 0 && s->nrows <= INT32_MAX && s->nclass >= 1, "nrows must be in [0, 2^31 - 1], nclass >= 1");
-    ARGCHK(s->temperature > 0.0 && s->temperature < INFINITY, "temperature must be positive and finite");
+    ARGCHK(s->temperature >= 1e-4 && s->temperature <= 1e4, "temperature must be in [1e-4, 1e4]"); // factors and their squares stay far from float's ends
     a.N = s->nrows;
     a.V = s->nclass;
     if (a.N == 0) return EVT_OK;
@@ -1044,7 +1055,7 @@ extern "C" int evt_preference_loss(void *stream, const void *scores, const void 
     ScoreArgs a = {};
     TRY(take_scores(s, false, flags, a));
     TRY(take_labels(labels, label_dtype, a));
-    ARGCHK(n_pairs >= 1 && n_pairs < (1 << 30), "n_pairs must be in [1, 2^30 - 1]");
+    ARGCHK(n_pairs >= 1 && n_pairs < (1 << 22), "n_pairs must be in [1, 2^22 - 1]");
     ARGCHK(beta > 0.0 && beta < INFINITY && label_smoothing >= 0.0 && label_smoothing <= 0.5 && margin > -INFINITY && margin < INFINITY,
            "beta must be positive, label_smoothing in [0, 0.5], margin finite");
     ARGCHK(average == 0 || average == 1, "average takes 0 or 1");

@@ -12,6 +12,7 @@ struct ScoreArgs {
     void *g; // nullptr: no gradient; x itself: in place
     int64_t xs, gs; // elements from row to row
     int64_t N;
+    int64_t row0; // the launch's first row
     int32_t V;
     int32_t past;   // the gradient is stored past the caches
     int32_t early;  // few rows: a row's scores are requested before it is known whether it counts

@@ -418,7 +418,7 @@ typedef struct {
     int64_t nrows;       /* 0 .. 2^31 - 1; 0: the call does nothing */
     int32_t nclass;      /* >= 1 */
     int32_t dtype;
-    double temperature;  /* > 0 */
+    double temperature;  /* 1e-4 .. 1e4 */
 } evt_scores;
 
 /* logp[i] = log q[i, labels[i]], and stats[2 i], stats[2 i + 1] = the row's maximum of x and sum of exp((x - maximum) / temperature) (both 0
@@ -443,7 +443,7 @@ int evt_policy_loss(void *stream, const void *scores /* evt_scores */, const voi
                     const float *ref_logp, const float *weights, double clip_low, double clip_high, double kl_coef, float *loss, float *logp,
                     int32_t flags);
 
-/* The preference loss of n_pairs pairs of sequences packed one behind the other: sequence k has the rows offsets[k] .. offsets[k + 1] - 1
+/* The preference loss of n_pairs pairs (below 2^22) of sequences packed one behind the other: sequence k has the rows offsets[k] .. offsets[k + 1] - 1
  * (2 n_pairs + 1 ascending row numbers), the chosen one of pair p is sequence p and the rejected one n_pairs + p.  seq_logp[k] is the sum of its rows' log
  * q[label] - of those with a label - or with average their mean (0 of none), ref_logp[k] the reference model's, and with w = weights[p] (NULL: 1)
  *   h = beta ((seq_logp[p] - seq_logp[n_pairs + p]) - (ref_logp[p] - ref_logp[n_pairs + p])) - margin,

@@ -34,7 +34,7 @@ def test_scores_are_checked(evt):
     for call in _all(evt, x):  # nothing else is wrong with these: the scores are on no GPU
         with pytest.raises(ValueError, match="on a GPU"):
             call()
-    for T in (0.0, -1.0, float("inf"), float("nan")):
+    for T in (0.0, -1.0, 0.9e-4, 1.1e4, float("inf"), float("nan")):
         for call in _all(evt, x, temperature=T):
             with pytest.raises(ValueError, match="temperature"):
                 call()
@@ -118,7 +118,7 @@ def test_c_entry_points_refuse(evt):
 
     every = (logp, grad, distill, policy, pref)
     wrong = [None, scores(x=None), scores(xs=-1), scores(gs=9), scores(n=-1), scores(n=1 << 31), scores(v=0), scores(v=-5), scores(dtype=1), scores(dtype=9),
-             scores(t=0.0), scores(t=float("nan")), scores(t=float("inf")), scores(x=p + 1), scores(g=q + 2), scores(g=p + 4), scores(g=p, gs=12), scores(g=p + 40),
+             scores(t=0.0), scores(t=9e-5), scores(t=11000.0), scores(t=float("nan")), scores(t=float("inf")), scores(x=p + 1), scores(g=q + 2), scores(g=p + 4), scores(g=p, gs=12), scores(g=p + 40),
              scores(g=p - 4)]
     for call in every:
         for s in wrong:
@@ -137,7 +137,7 @@ def test_c_entry_points_refuse(evt):
         assert distill(scores(), **more) == E.EVT_ERR_ARG
     for more in (dict(lo=-0.1), dict(lo=1.5), dict(hi=-1.0), dict(hi=float("nan")), dict(kl=-1.0), dict(kl=float("inf")), dict(kl=0.1)):
         assert policy(scores(), **more) == E.EVT_ERR_ARG
-    for more in (dict(n=0), dict(n=1 << 30), dict(beta=0.0), dict(beta=float("inf")), dict(soft=0.7), dict(margin=float("inf")), dict(avg=2)):
+    for more in (dict(n=0), dict(n=1 << 22), dict(beta=0.0), dict(beta=float("inf")), dict(soft=0.7), dict(margin=float("inf")), dict(avg=2)):
         assert pref(scores(), **more) == E.EVT_ERR_ARG
 
 

@@ -257,6 +257,40 @@ def test_one_row_for_all(evt):
             assert torch.equal(u, v)
 
 
+@pytest.mark.parametrize("N,V,dtype", [(17_000_100, 4200, torch.bfloat16), (68_000_000, 1100, torch.float16), (34_000_000, 700, torch.float32)])
+def test_rows_of_several_launches(evt, N, V, dtype):
+    """More rows than one launch has threads for; all of them one row in memory."""
+    x, gen = _scores(V, dtype, 8, 1, special=False)
+    lab = torch.full((N,), 3, dtype=torch.int32)
+    lab[-1], lab[N // 2], lab[-2] = V - 1, -1, 0
+    lp, stats = evt.class_logp(x.cuda().expand(N, V), lab.cuda())
+    # other numbers of rows may take other forms, whose sums are in another order: held against 64 bits, and all the rows alike against each other
+    want, tol, _ = plain.logp(x.expand(4, V), torch.tensor([3, V - 1, -1, 0]), 1.0)
+    plain.close("logp", torch.stack([lp[0], lp[-1], lp[N // 2], lp[-2]]), want, tol)
+    lp[-1] = lp[N // 2] = lp[-2] = lp[0].clone()
+    assert (lp == lp[0]).all() and (stats[:, 1] == stats[0, 1]).sum() == N - 1
+
+
+def test_extreme_scores_and_temperatures(evt):
+    """Scores at the ends of their type - masks of its lowest value - and the least and greatest temperature."""
+    for dtype in plain.TYPES.values():
+        top = torch.finfo(dtype).max
+        for T in (1e-4, 1.0, 1e4):
+            for V in (5, 20, 600, 9000):
+                x = torch.zeros(6, V, dtype=dtype)
+                x[0] = -top  # every class as likely as the next
+                x[1, 1:] = -top
+                x[2] = top
+                x[3, : V // 2] = -top
+                x[4, 0], x[4, 1] = top, -top
+                lab = torch.tensor([1, 0, V - 1, V - 1, 0, 2])
+                want, tol, rows = plain.logp(x, lab, T)
+                lp, stats = evt.class_logp(x.cuda(), lab.cuda(), T)
+                plain.close("logp", lp, want, tol)
+                d = torch.ones(6)
+                plain.close("grad", evt.class_logp_grad(x.cuda(), lab.cuda(), stats, d.cuda(), T), *plain.label_grad(rows, lab, d.double(), T, dtype))
+
+
 def test_no_rows_and_no_gradient(evt):
     x = torch.zeros(0, 50, device="cuda")
     lab = torch.zeros(0, dtype=torch.int64, device="cuda")

@@ -24,6 +24,7 @@ _TRUSTED = 2  # EVT_STATIC_TRUSTED: the tensors say where they are
 _INF = float("inf")
 _torch = None
 _makers = {}  # by device
+_entries = {}  # by name
 
 
 def _load():
@@ -54,16 +55,9 @@ def _bad(name, v, x, shape, kinds):
     raise ValueError("%s must be contiguous" % name)
 
 
-def _number(name, v, low, high, open_low=False):
-    v = float(v)
-    if not (low < v if open_low else low <= v) or not v <= high or v == _INF:
-        raise ValueError("%s must be finite and in %s%s, %s], got %s" % (name, "(" if open_low else "[", low, high, v))
-    return v
-
-
 class _Call:
     """A call on some scores: the checks of what belongs to them, and the launch on their device's current stream."""
-    __slots__ = ("x", "kind", "rows", "device", "temperature")
+    __slots__ = ("x", "kind", "rows", "classes", "device", "temperature")
 
     def __init__(self, x, temperature):
         if _torch is None:
@@ -80,8 +74,9 @@ class _Call:
             raise ValueError("the scores must have 1 to 2^31 - 1 classes and at most 2^31 - 1 rows, got shape %s" % (tuple(x.shape),))
         if x.stride(1) != 1 and classes > 1:
             raise ValueError("the scores of a row must lie side by side, got strides %s" % (x.stride(),))
-        self.x, self.kind, self.rows, self.device = x, kind, rows, x.get_device()
-        self.temperature = _number("temperature", temperature, 1e-4, 1e4)
+        self.x, self.kind, self.rows, self.classes, self.device, self.temperature = x, kind, rows, classes, x.get_device(), float(temperature)
+        if not 1e-4 <= self.temperature <= 1e4:
+            raise ValueError("temperature must be in [1e-4, 1e4], got %s" % temperature)
 
     def check(self, name, v, shape, kinds):
         """v's address, and its type's code by way of `kinds`."""
@@ -123,13 +118,14 @@ class _Call:
         return make(shape)
 
     def run(self, name, grad, *args):
-        x, dev = self.x, self.device
+        x, dev, rows, classes = self.x, self.device, self.rows, self.classes
         if dev < 0:
             raise ValueError("the scores must be on a GPU, got %s" % x.device)
-        rows, classes = x.shape
         s = _lib.EvtScores(x.data_ptr(), x.stride(0) if rows > 1 else classes, None if grad is None else grad.data_ptr(),
                            0 if grad is None else grad.stride(0) if rows > 1 else classes, rows, classes, self.kind, self.temperature)
-        call = getattr(_lib.load(), name)
+        call = _entries.get(name)
+        if call is None:
+            call = _entries[name] = getattr(_lib.load(), name)
         if dev == _device():
             rc = call(_stream(dev), C.byref(s), *args, _TRUSTED)
         else:
@@ -189,8 +185,9 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, clip_low=0
     call = _Call(logits, temperature)
     at = call.check("actions", actions, (call.rows,), _INTS)
     old_at, advantages_at = call.floats("old_logp", old_logp), call.floats("advantages", advantages)
-    clip_low, clip_high = _number("clip_low", clip_low, 0.0, 1.0), _number("clip_high", clip_high, 0.0, _INF)
-    kl_coef = _number("kl_coef", kl_coef, 0.0, _INF)
+    clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
+    if not (0.0 <= clip_low <= 1.0 and 0.0 <= clip_high < _INF and 0.0 <= kl_coef < _INF):
+        raise ValueError("clip_low must be in [0, 1], clip_high and kl_coef finite and at least 0, got %s, %s and %s" % (clip_low, clip_high, kl_coef))
     ref_at, weights_at = call.optional("ref_logp", ref_logp, call.rows), call.optional("weights", weights, call.rows)
     if ref_at is None and kl_coef:
         raise ValueError("kl_coef needs ref_logp")
@@ -217,9 +214,9 @@ def preference_loss(logits, labels, offsets, ref_logp, beta=0.1, label_smoothing
         raise ValueError("offsets must be a vector of an odd number of row numbers, at least 3: one more than there are sequences")
     seqs = offsets.shape[0] - 1
     offsets_at, ref_at = call.check("offsets", offsets, (seqs + 1,), _I32S), call.check("ref_logp", ref_logp, (seqs,), _F32S)
-    beta = _number("beta", beta, 0.0, _INF, True)
-    label_smoothing = _number("label_smoothing", label_smoothing, 0.0, 0.5)
-    margin = _number("margin", margin, -_INF, _INF)
+    beta, label_smoothing, margin = float(beta), float(label_smoothing), float(margin)
+    if not (0.0 < beta < _INF and 0.0 <= label_smoothing <= 0.5 and -_INF < margin < _INF):
+        raise ValueError("beta must be positive and finite, label_smoothing in [0, 0.5], margin finite, got %s, %s and %s" % (beta, label_smoothing, margin))
     weights_at = call.optional("weights", weights, seqs // 2)
     g = call.gradient(grad, out)
     loss, seq_logp, work = call.values(seqs // 2), _like(ref_logp), call.values(4 * call.rows)

@@ -137,6 +137,23 @@ def test_preference_loss(evt, V, dtype, average):
     assert not grad[:2].any() and not grad[38:].any()
 
 
+@pytest.mark.parametrize("V,N,dtype", [(5, 2600, "f32"), (7, 2500, "bf16"), (130, 2400, "f16"), (1300, 2300, "f32"), (4100, 2200, "bf16")])
+def test_preference_many_rows(evt, V, N, dtype):
+    """More rows than one launch finds the pairs of: the slopes come from a kernel of their own.  An odd number of pairs, sequences of no rows among them."""
+    x, gen = _scores(V, plain.TYPES[dtype], V, N, special=False)
+    lab = torch.randint(-1, V, (N,), generator=gen)
+    cuts = torch.randint(3, N - 5, (9,), generator=gen).sort().values
+    off = torch.cat([torch.tensor([3]), cuts[:4], cuts[3:4], cuts[4:], torch.tensor([N - 5])])[:11].to(torch.int32)
+    lp = torch.cat([torch.zeros(1, dtype=torch.float64), plain.logp(x, lab, 1.0)[0].cumsum(0)])
+    ref = (lp[off[1:].long()] - lp[off[:-1].long()] + torch.randn(10, generator=gen) * 3).float()
+    w = torch.tensor([1.0, 0.0, 0.5, 2.0, 1.0])
+    loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), off.cuda(), ref.cuda(), beta=0.2, weights=w.cuda())
+    want = plain.preference(x, lab, off, ref, 0.2, 0.0, 0.0, False, 1.0, w)
+    plain.close("loss", loss, *want[0])
+    plain.close("seq_logp", seq, *want[1])
+    plain.close("grad", grad, *want[2])
+
+
 def test_preference_bad_rows_and_offsets(evt):
     """A NaN score or a label past the classes spoils its own pair, offsets that do not ascend theirs; the others are as they are alone."""
     V, N = 130, 24

@@ -25,7 +25,8 @@ struct Piece {
     Raw r;
     __device__ __forceinline__ void load(const T *p) { r = *(const Raw *)p; }
     // past: by the caches.  A gradient that the last of them (256 MB) cannot hold only drives out what the next pass reads (8 pairs, 5003 x 32 768 bf16, loss and
-    // gradient again and again: the first pass over the scores 67 us, 39 so); a smaller one stays for its reader
+    // gradient again and again: the first pass over the scores 67 us, 39 so); a smaller one stays for its reader.  Not of short rows, where a store has parts of
+    // lines that the second cache would put together (4.2M x 64 bf16: 290 us, 530 so; from 256 pieces on 0 to 5 % less)
     __device__ __forceinline__ void store(T *p, bool past) const {
         typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
         const u4 v = {r.w[0], r.w[1], r.w[2], r.w[3]};
@@ -98,7 +99,7 @@ __device__ __forceinline__ MaxSum take(MaxSum a, const float *f, float mul) {
     return {m, a.s * exp_of(a.m, m, mul) + s[0]};
 }
 // Reductions over G neighbouring lanes whose result every one of them has: by moves within rows of sixteen lanes and gfx950's swaps of rows between two
-// registers, a few cycles a step where a trip through the LDS crossbar is a hundred (with the scores requested early, 8 rows of 32 768 classes take 4.8 us for 6.3).
+// registers, a few cycles a step where a trip through the LDS crossbar is a hundred (8 rows of 32 768 classes: 6.3 us, 4.8 so).
 template <int CTRL>
 __device__ __forceinline__ float moved(float v) {
     return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false));
@@ -127,6 +128,15 @@ template <int G>
 __device__ __forceinline__ MaxSum lanes_join(MaxSum a, float mul) {
     const float m = over_lanes<G>(a.m, [](float x, float y) { return fmaxf(x, y); });
     return {m, lanes_sum<G>(a.s * exp_of(a.m, m, mul))};
+}
+// What every lane of a wavefront has alike, in scalar registers: a block that holds 16 pieces a thread has no vector register to spare
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(v))); }
+__device__ __forceinline__ MaxSum uniform(MaxSum a) { return {uniform(a.m), uniform(a.s)}; }
+// v, of which the compiler does not know that it is v: what is computed from it is computed where it is used, and does not stay in registers from the
+// loads to the stores (16 offsets did, in pairs: 128 registers and spills in the largest blocks, 111 and none so)
+__device__ __forceinline__ int again(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
 }
 template <int G>
 __device__ __forceinline__ bool lanes_any(bool v) {
@@ -161,7 +171,7 @@ struct Waves {
         a = lanes_join<64>(a, mul);
         if ((threadIdx.x & 63) == 0) s_a[threadIdx.x >> 6] = a;
         __syncthreads();
-        return lanes_join<W>(s_a[threadIdx.x & (W - 1)], mul);
+        return uniform(lanes_join<W>(s_a[threadIdx.x & (W - 1)], mul));
     }
 };
 
@@ -280,7 +290,9 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     const T *x = (const T *)a.x + row * a.xs;
     T *g = a.g ? (T *)a.g + row * a.gs : nullptr;
     const float mul = a.exp_mul;
-    const bool past = a.past;
+    // a teacher's classes are stored a second time: behind the caches that is a line read and written for each (89 448 x 3001 f32 of 32 entries: 520 us past the
+    // caches, 462 not; 2048 x 131072 of 64 454 | 494)
+    const bool past = a.past && (OP != SC_DISTILL || V > 4096 * E);
     float w = 1.0f, x_label = 0.0f, given = 0.0f;
     bool live = true, bad = false;
     int64_t label = -1;
@@ -289,16 +301,6 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     // them at the row's start all the same.  first: where the thread's piece would start; at: where it is
     const int base = sizeof(T) == 2 && ((uintptr_t)x & 2) ? -1 : 0;
     const auto at = [&](int first) { return first < 0 ? 0 : first + E <= V ? first : V - E; };
-    const auto load_row = [&]() {
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int o = base + (t + i * G::SIZE) * E;
-            // past the row's end: the last piece, which counts once.  Lanes leave out what no lane has; between the loads of a block the branches cost
-            // more than the loads (8192 x 131072 bf16: 1020 for 790 us)
-            if (G::ROWS == 1 || base + i * G::SIZE * E < V) p[i].load(x, at(o));
-        }
-    };
-    if (a.early) load_row(); // whether the row counts or not
     if (OP == SC_DISTILL) {
         w = a.weights ? a.weights[row * a.ws] : 1.0f;
         live = w != 0.0f;
@@ -318,7 +320,13 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         if (OP != SC_LOGP && g) clear_row(g, V, t, G::SIZE, past);
         return;
     }
-    if (!a.early) load_row();
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int o = base + (t + i * G::SIZE) * E;
+        // past the row's end: the last piece, which counts once.  Lanes leave out what no lane has; between the loads of a block the branches cost
+        // more than the loads (8192 x 131072 bf16: 1020 for 790 us)
+        if (G::ROWS == 1 || base + i * G::SIZE * E < V) p[i].load(x, at(o));
+    }
     int2 *const s_top = (int2 *)s_dyn;
     float *const s_x = (float *)(s_top + a.n_top);
     MaxSum teacher = {LOWEST, 0.0f};
@@ -334,7 +342,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
             s_x[j] = in ? (float)x[id] : 0.0f;
             teacher = take<1>(teacher, &s, mul);
         }
-        teacher = lanes_join<64>(teacher, mul);
+        teacher = uniform(lanes_join<64>(teacher, mul));
         none = __any(none);
         if (t == 0) s_state = teacher.s == 0.0f ? 0 : none ? 2 : 1; // a sum that is no number is a teacher
 #pragma unroll 1
@@ -344,9 +352,10 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     if (OP == SC_GRAD) {
         r = {fmaxf(a.stats[2 * row], LOWEST), a.stats[2 * row + 1]};
     } else {
+        const int tt = again(t);
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int o = base + (t + i * G::SIZE) * E;
+            const int o = base + (tt + i * G::SIZE) * E;
             if (o < V) {
                 float f[E];
                 p[i].get(f);
@@ -417,9 +426,10 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     }
     if (OP == SC_LOGP || !g) return;
     fq = factor * inv;
+    const int tt = again(t);
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        int o = base + (t + i * G::SIZE) * E;
+        int o = base + (tt + i * G::SIZE) * E;
         if (o < V) {
             o = at(o);
             float f[E];
@@ -787,7 +797,9 @@ __global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, PairArgs q) 
 // 8192 bf16: 6.6 us for 5.0 + 4.8); the last blocks write the losses.
 template <typename T, bool PAIRS>
 __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, PairArgs q, int parts) {
-    constexpr int E = Piece<T>::E, PART = 256 * 4 * E;
+    constexpr int E = Piece<T>::E;
+    // classes, at most 1024 pieces; the parts alike (32 764 x 8193 bf16, 1025 pieces a row: 308 us by 1024 and 1, 224 so)
+    const int part = ((a.V + E - 1) / E + parts - 1) / parts * E;
     const int64_t blocks = a.N * parts;
     const bool past = a.past;
     if (PAIRS && blockIdx.x >= blocks) {
@@ -798,10 +810,10 @@ __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, PairArgs q, int
     }
     for (int64_t b = blockIdx.x; b < blocks; b += gridDim.x) {
         const int64_t row = b / parts;
-        const int64_t c0 = (b - row * parts) * PART;
+        const int64_t c0 = (b - row * parts) * part;
         const T *x = (const T *)a.x + row * a.xs + c0;
         T *g = (T *)a.g + row * a.gs + c0;
-        const int V = (int)(a.V - c0 < PART ? a.V - c0 : PART), t = threadIdx.x;
+        const int V = (int)(a.V - c0 < part ? a.V - c0 : part), t = threadIdx.x;
         const int64_t label = load_id(a.labels, a.label64, row);
         float given = 0.0f;
         bool live = label >= 0;
@@ -864,16 +876,16 @@ static void slices(ScoreArgs a, int rows, int threads, F &&f) {
 }
 template <typename T, int OP, int NV, class G>
 static int launch_rows(hipStream_t s, ScoreArgs a) {
-    a.early = a.N <= 512;
     const size_t lds = OP == SC_DISTILL ? (size_t)a.n_top * 12 : 0;
     slices(a, G::ROWS, G::THREADS, [&](const ScoreArgs &b, dim3 grid) { hipLaunchKernelGGL((k_rows<T, OP, NV, G>), grid, dim3(G::THREADS), lds, s, b); });
     return EVT_OK;
 }
-// Distillation of short rows: true where the lanes hold a row of n pieces and a block's memory its teachers, 52 KB so that a unit has three blocks
+// Distillation of short rows: true where the lanes hold a row of n pieces and a block's memory its teachers: 25 KB, six blocks to a unit, or more lanes to a row
+// (bf16, 32 entries, at 52 | 25 | 20 KB: 2.7M x 100 670 | 429 | 590 us, 8M x 33 1461 | 921 | 901)
 template <typename T, int NV, class G>
 static bool launch_distill(hipStream_t s, const ScoreArgs &a, int64_t n) {
     const size_t lds = G::ROWS * ((size_t)(a.n_top | 1) * 8 + (size_t)((a.V + 2) | 1) * 4);
-    if ((NV ? a.V < Piece<T>::E || n > (int64_t)G::SIZE * NV : a.V >= Piece<T>::E) || (lds > 53248 && G::SIZE < 64) || lds > 65536) return false;
+    if ((NV ? a.V < Piece<T>::E || n > (int64_t)G::SIZE * NV : a.V >= Piece<T>::E) || (lds > 26000 && G::SIZE < 64) || lds > 65536) return false;
     const uint32_t magic = a.n_top > 1 ? (uint32_t)(((1ull << 32) + a.n_top - 1) / a.n_top) : 0u; // exact for e / n_top, e * n_top < 2^32
     slices(a, G::ROWS, 256, [&](const ScoreArgs &b, dim3 grid) { hipLaunchKernelGGL((k_distill_short<T, NV, G>), grid, dim3(256), lds, s, b, magic); });
     return true;
@@ -889,7 +901,7 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
         if ((!few || n <= 32) &&
             (launch_distill<T, 4, Lanes<1>>(s, a, n) || launch_distill<T, 4, Lanes<2>>(s, a, n) || launch_distill<T, 4, Lanes<4>>(s, a, n) ||
              launch_distill<T, 4, Lanes<8>>(s, a, n) || launch_distill<T, 4, Lanes<16>>(s, a, n) || launch_distill<T, 4, Lanes<32>>(s, a, n) ||
-             launch_distill<T, 4, Lanes<64>>(s, a, n)))
+             launch_distill<T, 4, Lanes<64>>(s, a, n) || (E == 4 && launch_distill<T, 8, Lanes<64>>(s, a, n))))
             return EVT_OK;
         if (a.V < E) {
             evt_set_error("no form for %d classes and %d entries", a.V, a.n_top); // k_rows' last piece would start in front of the row
@@ -900,7 +912,8 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
             slices(a, 256, 256, [&](const ScoreArgs &b, dim3 grid) { hipLaunchKernelGGL((k_few_classes<T, OP>), grid, dim3(256), 0, s, b); });
             return EVT_OK;
         }
-        // lanes to a row: four pieces each
+        // Lanes to a row: four pieces each (one each pays a row's own work and its reductions four times as often: 4.2M x 64 bf16, log-probabilities | policy,
+        // 170 | 330 us for 135 | 270)
         if (n <= 4) return launch_rows<T, OP, 4, Lanes<1>>(s, a);
         if (n <= 8) return launch_rows<T, OP, 4, Lanes<2>>(s, a);
         if (n <= 16) return launch_rows<T, OP, 4, Lanes<4>>(s, a);
@@ -909,16 +922,21 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
         if (n <= 128) return launch_rows<T, OP, 4, Lanes<32>>(s, a);
         if (n <= 256) return launch_rows<T, OP, 4, Lanes<64>>(s, a);
     }
+    if constexpr (OP != SC_DISTILL) {
+        // a wavefront to a row, eight pieces a lane (89 478 x 3000 bf16, log-probabilities: 140 us by blocks of 256, 88 so); few rows are done sooner by blocks
+        if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
+    }
     if constexpr (OP == SC_GRAD) {
         const int64_t parts = (n + 1023) / 1024, blocks = a.N * parts;
         hipLaunchKernelGGL((k_slope_rows<T, false>), dim3((unsigned)(blocks < (1 << 23) ? blocks : (1 << 23))), dim3(256), 0, s, a, PairArgs{}, (int)parts);
         return EVT_OK;
     } else {
-        if constexpr (OP != SC_DISTILL) {
-            if (!few && n <= 512) return launch_rows<T, OP, 8, Lanes<64>>(s, a);
-        }
+        // No gradient: the row streams by.  Blocks of 1024 for few rows (16 x 32 768 bf16: 5.5 us by 256, 5.1) and long ones (4096 x 65 536: 95 | 86 us),
+        // of 256 for the others (16 384 x 16 384: 127 us by 1024, 88)
         if (OP == SC_LOGP || !a.g) return few || n >= 8192 ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 4, Waves<4>>(s, a);
-        // the row stays in registers
+        // The row stays in registers, 1024 pieces a unit, in the smallest blocks that hold it: while one waits for its row another computes and a third stores
+        // (policy, bf16, 1024 threads | so: 16 384 x 16 384 224 | 195 us, 8192 x 32 768 225 | 213, 4096 x 65 536 243 | 203).  No more rows than
+        // units: 1024 threads each (16 x 32 768: 9.7 us by 256, 7.4; 256 rows 12.3 | 10.5, but 384 14.2 | 15.3)
         if constexpr (OP != SC_LOGP) {
             if (few) return n <= 4096 ? launch_rows<T, OP, 4, Waves<16>>(s, a) : launch_rows<T, OP, 16, Waves<16>>(s, a);
             if (n <= 1024) return launch_rows<T, OP, 4, Waves<4>>(s, a);
@@ -998,7 +1016,7 @@ static int take_scores(const evt_scores *s, bool grad_needed, int32_t flags, Sco
     a.gs = s->grad_stride;
     a.ws = 1;
     score_scale(a, s->temperature);
-    a.past = (double)a.N * a.V * size > 256e6;
+    a.past = (double)a.N * a.V * size > 256e6 && a.V > 256 * 16 / size;
     return check_device(flags, s->x, s->grad);
 }
 static int take_labels(const void *labels, int32_t dtype, ScoreArgs &a) {

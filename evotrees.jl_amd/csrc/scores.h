@@ -15,7 +15,6 @@ struct ScoreArgs {
     int64_t row0; // the launch's first row
     int32_t V;
     int32_t past;   // the gradient is stored past the caches
-    int32_t early;  // few rows: a row's scores are requested before it is known whether it counts
     double inv_t;   // 1 / temperature
     float exp_mul;  // log2(e) / temperature: exp(d / T) = exp2(d * exp_mul)
     const void *labels;

@@ -70,8 +70,8 @@ class _Call:
         if x.dim() != 2:
             raise ValueError("the scores must be a (rows, classes) matrix, got shape %s" % (tuple(x.shape),))
         rows, classes = x.shape
-        if not 1 <= classes <= 0x7FFFFFFF or rows > 0x7FFFFFFF:
-            raise ValueError("the scores must have 1 to 2^31 - 1 classes and at most 2^31 - 1 rows, got shape %s" % (tuple(x.shape),))
+        if not 1 <= classes <= 1 << 30 or rows > 0x7FFFFFFF:
+            raise ValueError("the scores must have 1 to 2^30 classes and at most 2^31 - 1 rows, got shape %s" % (tuple(x.shape),))
         if x.stride(1) != 1 and classes > 1:
             raise ValueError("the scores of a row must lie side by side, got strides %s" % (x.stride(),))
         self.x, self.kind, self.rows, self.classes, self.device, self.temperature = x, kind, rows, classes, x.get_device(), float(temperature)

@@ -992,7 +992,7 @@ static int take_scores(const evt_scores *s, bool grad_needed, int32_t flags, Sco
     ARGCHK(s, "scores must not be NULL");
     ARGCHK(flags == 0 || flags == EVT_STATIC_TRUSTED, "flags takes 0 or EVT_STATIC_TRUSTED");
     ARGCHK(s->dtype == EVT_F32 || s->dtype == EVT_BF16 || s->dtype == EVT_F16, "scores must be EVT_F32, EVT_BF16 or EVT_F16");
-    ARGCHK(s->nrows >= 0 && s->nrows <= INT32_MAX && s->nclass >= 1, "nrows must be in [0, 2^31 - 1], nclass >= 1");
+    ARGCHK(s->nrows >= 0 && s->nrows <= INT32_MAX && s->nclass >= 1 && s->nclass <= (1 << 30), "nrows must be in [0, 2^31 - 1], nclass in [1, 2^30]");
     ARGCHK(s->temperature >= 1e-4 && s->temperature <= 1e4, "temperature must be in [1e-4, 1e4]"); // factors and their squares stay far from float's ends
     a.N = s->nrows;
     a.V = s->nclass;

@@ -416,7 +416,7 @@ typedef struct {
     void *grad;          /* of x's type, or NULL */
     int64_t grad_stride; /* >= nclass */
     int64_t nrows;       /* 0 .. 2^31 - 1; 0: the call does nothing */
-    int32_t nclass;      /* >= 1 */
+    int32_t nclass;      /* 1 .. 2^30 */
     int32_t dtype;
     double temperature;  /* 1e-4 .. 1e4 */
 } evt_scores;

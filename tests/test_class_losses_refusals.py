@@ -27,7 +27,7 @@ def _all(evt, x, **more):
 def test_scores_are_checked(evt):
     x, lab, v, ids, off = _good()
     for bad, error in ((x.double(), TypeError), (x.long(), TypeError), (x.numpy(), TypeError), (x[0], ValueError), (x[None], ValueError),
-                       (torch.zeros(4, 0), ValueError), (torch.zeros(10, 4).t(), ValueError), (torch.zeros(4, 20)[:, ::2], ValueError)):
+                       (torch.zeros(4, 0), ValueError), (torch.zeros(4, 1).expand(4, (1 << 30) + 1), ValueError), (torch.zeros(10, 4).t(), ValueError), (torch.zeros(4, 20)[:, ::2], ValueError)):
         for call in _all(evt, bad):
             with pytest.raises(error):
                 call()
@@ -117,7 +117,7 @@ def test_c_entry_points_refuse(evt):
         return L.evt_preference_loss(None, s, lab, kind, off, n, ref, w, beta, soft, margin, avg, loss, seq, work, flags)
 
     every = (logp, grad, distill, policy, pref)
-    wrong = [None, scores(x=None), scores(xs=-1), scores(gs=9), scores(n=-1), scores(n=1 << 31), scores(v=0), scores(v=-5), scores(dtype=1), scores(dtype=9),
+    wrong = [None, scores(x=None), scores(xs=-1), scores(gs=9), scores(n=-1), scores(n=1 << 31), scores(v=0), scores(v=(1 << 30) + 1, gs=1 << 31), scores(v=-5), scores(dtype=1), scores(dtype=9),
              scores(t=0.0), scores(t=9e-5), scores(t=11000.0), scores(t=float("nan")), scores(t=float("inf")), scores(x=p + 1), scores(g=q + 2), scores(g=p + 4), scores(g=p, gs=12), scores(g=p + 40),
              scores(g=p - 4)]
     for call in every:

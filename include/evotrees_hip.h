@@ -415,7 +415,7 @@ typedef struct {
     int64_t row_stride;
     void *grad;          /* of x's type, or NULL */
     int64_t grad_stride; /* >= nclass */
-    int64_t nrows;       /* 0 .. 2^31 - 1; 0: the call does nothing */
+    int64_t nrows;       /* 0 .. 2^31 - 1; of 0 rows nothing is written but the losses of empty pairs */
     int32_t nclass;      /* 1 .. 2^30 */
     int32_t dtype;
     double temperature;  /* 1e-4 .. 1e4 */

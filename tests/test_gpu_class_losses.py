@@ -455,3 +455,93 @@ def test_preference_training_step(evt):
     assert (grad - same).abs().max() < 0.0025 * 2.0 ** -15 + 8 * plain.U * 0.05
     _, lp2, pg = evt.policy_loss(xg, labg, lp, -slope)
     assert torch.equal(lp, lp2) and (pg - same).abs().max() < 40 * plain.U * 0.05  # r = 1 but for the rounding of lp, of at most 32
+
+
+@pytest.mark.parametrize("V,dtype", [(1100, "f32"), (2050, "bf16"), (2100, "f32"), (3001, "f16"), (4099, "bf16"), (4097, "f32"), (8193, "bf16"), (9000, "f32"), (16390, "f16"),
+                                     (16385, "bf16"), (20000, "f32"), (32770, "bf16"), (33000, "f32"), (65537, "f16"), (66001, "f32"), (131075, "bf16"), (140001, "f16")])
+def test_more_rows_than_units(evt, V, dtype):
+    """The forms that many rows take, in blocks of every size, rows at odd addresses, some left out."""
+    N = 263
+    x, gen = _scores(V, plain.TYPES[dtype], V + 9, N)
+    lab = _labels(N, V, gen)
+    xg = _placed(x, V % 3, V % 2)
+    want, tol, rows = plain.logp(x, lab, 1.0)
+    lp, stats = evt.class_logp(xg, lab.cuda())
+    plain.close("logp", lp, want, tol)
+    adv = torch.randn(N, generator=gen)
+    adv[20] = 0.0
+    old = want.nan_to_num(0, 0, -3).float()  # r = 1 but for the roundings: between the bounds
+    w = torch.rand(N, generator=gen) + 0.5
+    w[30] = 0.0
+    case = plain.policy(x, lab, old, adv, None, 0.2, 0.2, 0.0, 1.0, w)
+    loss, lp2, grad = evt.policy_loss(xg, lab.cuda(), old.cuda(), adv.cuda(), weights=w.cuda())
+    plain.close("policy loss", loss, *case[0])
+    plain.close("policy grad", grad, *case[2])
+    plain.close("logp grad", evt.class_logp_grad(xg, lab.cuda(), stats, adv.cuda()), *plain.label_grad(rows, lab, adv.double(), 1.0, x.dtype))
+    ids = torch.randint(-1, V, (N, 7), generator=gen, dtype=torch.int32)
+    ids[40, 2] = ids[40, 5] = 3
+    top = torch.randn(N, 7, generator=gen) * 2
+    case = plain.distill(x, ids, top, 1.0, w)
+    loss, grad = evt.distill_loss(xg, ids.cuda(), top.cuda(), weights=w.cuda())
+    plain.close("distill loss", loss, *case[0])
+    plain.close("distill grad", grad, *case[1])
+    plain.close("distill loss alone", evt.distill_loss(xg, ids.cuda(), top.cuda(), weights=w.cuda(), grad=False)[0], *case[0])
+    target = _placed(x, V % 3, V % 2)  # in place
+    assert torch.equal(evt.distill_loss(target, ids.cuda(), top.cuda(), weights=w.cuda(), out=target)[1].nan_to_num(9.0), grad.nan_to_num(9.0))
+
+
+def test_rows_left_out_hold_anything(evt):
+    """NaN and infinities in the rows, entries and values of what is left out reach nothing."""
+    for V in (3, 40, 700, 9001):
+        N = 12
+        x, gen = _scores(V, torch.bfloat16, V, N, special=False)
+        clean = x.clone()
+        lab = torch.randint(0, V, (N,), generator=gen)
+        lab[2:5] = -1
+        x[2], x[3], x[4, 0] = math.nan, math.inf, math.nan
+        v = torch.randn(N, generator=gen)
+        bad = v.clone()
+        bad[2:5] = math.nan
+        calls = []
+        for z, u in ((x, bad), (clean, v)):
+            z, u, l = z.cuda(), u.cuda(), lab.cuda()
+            lp, st = evt.class_logp(z, l)
+            ids = torch.zeros(N, 3, dtype=torch.int64)
+            ids[:, 1] = V - 1
+            ids[:, 2] = -1
+            ids[2:5] = -5
+            top = torch.ones(N, 3)
+            if u[2] != u[2]:
+                top[:, 2], top[2:5] = math.nan, math.inf
+            off = torch.tensor([0, 6, N], dtype=torch.int32)
+            calls.append([lp, st, evt.class_logp_grad(z, l, st, u), *evt.policy_loss(z, l, u, u, u, kl_coef=0.1, weights=u.abs()),
+                          *evt.distill_loss(z, ids.cuda(), top.cuda(), weights=v.abs().cuda()), *evt.preference_loss(z, l, off.cuda(), v[:2].cuda())])
+        for a, b in zip(*calls):
+            assert torch.equal(a, b) and not torch.isnan(a).any()
+
+
+def test_threads_on_streams_of_their_own(evt):
+    """Calls of several threads at once, each on its own stream."""
+    import threading
+    x, gen = _scores(6007, torch.float16, 44, 50, special=False)
+    calls = _calls(evt, x.cuda(), gen)
+    want = [[t.clone() for t in f()] for f in calls]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = [f() for f in calls]
+                stream.synchronize()
+                for a, b in zip(got, want):
+                    for u, v in zip(a, b):
+                        if not torch.equal(u, v):
+                            wrong.append(1)
+    threads = [threading.Thread(target=work) for _ in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -206,8 +206,8 @@ def preference_loss(logits, labels, offsets, ref_logp, beta=0.1, label_smoothing
     offsets: int32, sequence k has the rows offsets[k] to offsets[k + 1] - 1; the first half of the sequences are the chosen ones, the second half,
     in the same order, the rejected.  ref_logp: the reference model's log-probability of every sequence.  weights: one for each pair.
     With h = beta ((chosen - rejected) - (ref chosen - ref rejected)) - margin a pair's loss is weights * (-(1 - label_smoothing) log sigmoid(h)
-    - label_smoothing log sigmoid(-h)).  Rows of no sequence get a gradient of 0; offsets that do not ascend or leave the rows
-    make their pair's results NaN."""
+    - label_smoothing log sigmoid(-h)).  Rows of no sequence get a gradient of 0; offsets that do not ascend, leave the rows or
+    lie outside the first and the last make their pair's results NaN."""
     call = _Call(logits, temperature)
     at = call.check("labels", labels, (call.rows,), _INTS)
     if not isinstance(offsets, _torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:

@@ -714,6 +714,7 @@ __device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q,
     Pair r;
     double len[2];
     int cnt[2] = {0, 0};
+    const int64_t first = a.bounds[0], last = a.bounds[a.n_bounds - 1]; // rows outside have no logp
     r.bad = false;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
@@ -723,7 +724,7 @@ __device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q,
     }
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        if (r.from[k] < 0 || r.to[k] > a.N || r.to[k] < r.from[k]) { // not ascending, or out of the rows
+        if (r.from[k] < 0 || r.to[k] > a.N || r.to[k] < r.from[k] || r.from[k] < first || r.to[k] > last) { // not ascending, or out of the rows
             r.bad = true;
             r.from[k] = r.to[k] = 0;
         }

@@ -197,7 +197,7 @@ int evt_set_alphas(evt_handle h, const double *alphas, int32_t n);
  * its target's labels.  ids and scores are nobs x n_top (a row's entries side by side): the classes the teacher kept of each row, counted from 0 (level code - 1;
  * below 0: no entry), and their scores.  evt_update_grads then computes the gradients of evt_distill_loss at this temperature,
  * T (q - p) w with q = softmax(pred / T) and p = softmax(scores / T) over the row's entries, and the second-order rows q (1 - q) w.  A row without entries has no
- * gradient.  n_top 0 (ids and scores may be NULL) goes back to the labels, which the metric is computed from in either case. */
+ * gradient; its second-order rows and its weight count all the same (a weight of 0 leaves it out altogether).  n_top 0 (ids and scores may be NULL) goes back to the labels, which the metric is computed from in either case. */
 int evt_set_teacher(evt_handle h, const int32_t *ids, const float *scores, int32_t n_top, double temperature);
 
 /* update_grads!(cache.∇, cache.pred, cache.y, L, params): src/loss.jl:100-111, :219-236;
@@ -403,7 +403,7 @@ int evt_predict_static(void *stream, int64_t nobs, int32_t nfeats, const uint8_t
  * With z = x / temperature, q = softmax(z) over a row's nclass scores and log q its logarithm:
  *  - Scores are EVT_F32, EVT_BF16 or EVT_F16, a row's side by side, rows row_stride elements apart (any alignment; 0: one row for all).
  *    Differences, exponentials and sums are 32-bit, losses 64-bit until they are written; a gradient is rounded once, to the scores' type.
- *  - A score of -inf is a class that cannot be: q = 0, no gradient through it.  A row of nothing else has log q = -inf and q = 0 everywhere.
+ *  - A score of -inf is a class that cannot be: q = 0, also in its gradient.  A row of nothing else has log q = -inf and q = 0 everywhere.
  *    A NaN or +inf makes its row's results NaN, and no other's.
  *  - Labels and ids count from 0 (EVT_I32 or EVT_I64).  A negative label leaves its row out: loss, logp and gradient are 0 and the row is not read.
  *    One of nclass or more makes the row's results NaN.  A row of weight 0 has no loss and no gradient, whatever its scores.
@@ -449,7 +449,8 @@ int evt_policy_loss(void *stream, const void *scores /* evt_scores */, const voi
  *   h = beta ((seq_logp[p] - seq_logp[n_pairs + p]) - (ref_logp[p] - ref_logp[n_pairs + p])) - margin,
  *   loss[p] = w (-(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)).
  * The gradient of sum_p loss[p] is written for every row: 0 for those in front of the first and behind the last sequence.  A pair whose
- * offsets do not ascend or leave the rows gets NaN.  work: 4 nrows floats that the call may write.  label_smoothing in [0, 0.5]. */
+ * offsets do not ascend, leave the rows or lie outside offsets[0] .. offsets[2 n_pairs] gets NaN; where offsets descend, rows that two sequences then
+ * have take the gradient of either.  work: 4 nrows floats that the call may write.  label_smoothing in [0, 0.5]. */
 int evt_preference_loss(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
                         const float *ref_logp, const float *weights, double beta, double label_smoothing, double margin, int32_t average,
                         float *loss, float *seq_logp, float *work, int32_t flags);

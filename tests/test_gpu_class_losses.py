@@ -545,3 +545,21 @@ def test_threads_on_streams_of_their_own(evt):
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("V,N", [(130, 24), (33_000, 600)])  # one launch for slopes and losses, and two
+def test_preference_offsets_past_the_last(evt, V, N):
+    """A sequence behind the last offset has rows that no loss counts: its pair is NaN, not the loss of no rows."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(N, V, generator=gen)
+    lab = torch.randint(0, V, (N,), generator=gen)
+    ref = torch.randn(6, generator=gen) - 20
+    off = torch.tensor([0, 3, 18, 6, 6, 9, 12], dtype=torch.int32)  # sequence 1 ends behind row 11, 2 descends; pairs are (0, 3), (1, 4), (2, 5)
+    loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), off.cuda(), ref.cuda())
+    assert torch.isnan(loss).tolist() == [False, True, True]
+    assert torch.isnan(seq).tolist() == [False, True, True, False, True, True]
+    alone, tol = plain.preference(x, lab, torch.tensor([0, 3, 3]), ref[[0, 3]], 0.1, 0.0, 0.0, False, 1.0, None)[0]
+    plain.close("loss", loss[:1], alone, tol)
+    off = torch.tensor([6, 9, 0, 3, 12], dtype=torch.int32)  # sequence 1 descends, 2 begins in front of the first: pairs (0, 2), (1, 3)
+    loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), off.cuda(), ref[:4].cuda())
+    assert torch.isnan(loss).all() and torch.isnan(seq).all()

@@ -693,8 +693,13 @@ def okay_to_continue(config, m, cache):
 
 def update(config, m, cache, x_train=None, y_train=None, w_train=None, teacher=None):
     """MMI.update, src/MLJ.jl:38-57: warm restart on the handle the first fit kept (`fit(..., return_cache=True)`);
-    any change other than a larger nrounds refits from scratch."""
+    any change other than a larger nrounds refits from scratch.  A refit takes teacher as it takes x_train, y_train and w_train; rounds added to the
+    handle go on with its teacher, or with the one given."""
+    if teacher is not None and config.loss != "mlogloss":
+        raise ValueError("a teacher needs the mlogloss loss, got %s" % config.loss)
     if okay_to_continue(config, m, cache):
+        if teacher is not None:
+            cache.handle.set_teacher(teacher.ids, teacher.logits, teacher.temperature)
         while m.info["nrounds"] < config.nrounds:
             grow_evotree(m, cache, config, more=m.info["nrounds"] + 1 < config.nrounds)
         cache.config = config

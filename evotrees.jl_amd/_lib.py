@@ -376,7 +376,7 @@ class Handle:
             raise ValueError("a teacher's ids and scores must both be %d x n_top" % self.N)
         if ids.size and (ids.max() >= self.K):
             raise ValueError("a teacher's ids must be below the number of classes (%d)" % self.K)
-        ids, scores = np.ascontiguousarray(np.maximum(ids, -1), np.int32), np.ascontiguousarray(scores, np.float32)
+        ids, scores = np.ascontiguousarray(np.maximum(ids, -1) if ids.dtype.kind == "i" else ids, np.int32), np.ascontiguousarray(scores, np.float32)
         check(load().evt_set_teacher(self._h, ptr(ids), ptr(scores), ids.shape[1], float(temperature)))
 
     def update_grads(self):

@@ -148,3 +148,43 @@ def test_refusals(evt):
             mse.set_teacher(np.zeros((10, 1), int), np.zeros((10, 1)))
     finally:
         mse.close()
+
+
+def test_unsigned_ids(evt):
+    rng = np.random.default_rng(5)
+    N, K = 60, 4
+    h = _handle(evt, N, K, None, rng)
+    try:
+        ids, scores = rng.integers(0, K, (N, 2)), rng.standard_normal((N, 2)).astype(np.float32)
+        grads = []
+        for kind in (np.int64, np.uint8, np.uint32, np.uint64):
+            h.set_teacher(ids.astype(kind), scores)
+            h.update_grads()
+            grads.append(h.get_grads())
+        assert all(np.array_equal(g, grads[0]) for g in grads[1:])
+    finally:
+        h.close()
+
+
+def test_update_with_another_teacher(evt):
+    rng = np.random.default_rng(11)
+    N, K = 3000, 3
+    x, y = rng.standard_normal((N, 4)), rng.integers(0, K, N)
+    first, second = evt.Teacher(*_teacher(rng, N, K, 2)), evt.Teacher(*_teacher(rng, N, K, 2), 2.0)
+    kw = dict(max_depth=3, eta=0.3)
+
+    def grown(*teachers):
+        m, cache = evt.fit(evt.EvoTreeClassifier(nrounds=2, **kw), x_train=x, y_train=y, teacher=first, return_cache=True, verbosity=0)
+        m, cache = evt.update(evt.EvoTreeClassifier(nrounds=4, **kw), m, cache, *teachers)
+        p = m(x)
+        cache.handle.close()
+        return p
+
+    kept = grown()
+    assert np.array_equal(kept, evt.fit(evt.EvoTreeClassifier(nrounds=4, **kw), x_train=x, y_train=y, teacher=first, verbosity=0)(x))
+    assert np.array_equal(kept, grown(None, None, None, first))
+    assert not np.array_equal(kept, grown(None, None, None, second))
+    m, cache = evt.fit(evt.EvoTreeRegressor(nrounds=1), x_train=x, y_train=x[:, 0], return_cache=True, verbosity=0)
+    with pytest.raises(ValueError, match="mlogloss"):
+        evt.update(evt.EvoTreeRegressor(nrounds=2), m, cache, teacher=first)
+    cache.handle.close()

@@ -768,10 +768,12 @@ __device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q,
     }
     const double w = q.weights ? q.weights[p] : 1.0;
     const double h = q.beta * ((r.lp[0] - r.lp[1]) - ((double)q.ref_logp[p] - (double)q.ref_logp[p + q.pairs])) - q.margin;
-    const double e = exp(-fabs(h)), up = log1p(e) + (h < 0.0 ? -h : 0.0); // -log sigma(h)
+    const double e = exp(-fabs(h)), one = log1p(e), up = one + (h < 0.0 ? -h : 0.0), down = one + (h > 0.0 ? h : 0.0); // -log sigma(h), -log sigma(-h)
     // the smaller of the two probabilities exactly: 1 - sigma(h) where h is large is sigma(-h)
     const double sig = (h < 0.0 ? e : 1.0) / (1.0 + e), lose = (h < 0.0 ? 1.0 : e) / (1.0 + e);
-    double dh = w * (q.soft * sig - (1.0 - q.soft) * lose), loss = w * (up + (q.soft != 0.0 ? q.soft * h : 0.0));
+    double dh = w * (q.soft * sig - (1.0 - q.soft) * lose), loss = w * up;
+    // an answer that cannot be has an infinite h: the two terms apart, neither of which is a difference
+    if (q.soft != 0.0) loss = w * ((1.0 - q.soft) * up + q.soft * down);
     if (w == 0.0) dh = loss = 0.0;
     if (r.bad) dh = loss = NAN;
     r.loss = (float)loss;

@@ -206,8 +206,9 @@ def preference_loss(logits, labels, offsets, ref_logp, beta=0.1, label_smoothing
     offsets: int32, sequence k has the rows offsets[k] to offsets[k + 1] - 1; the first half of the sequences are the chosen ones, the second half,
     in the same order, the rejected.  ref_logp: the reference model's log-probability of every sequence.  weights: one for each pair.
     With h = beta ((chosen - rejected) - (ref chosen - ref rejected)) - margin a pair's loss is weights * (-(1 - label_smoothing) log sigmoid(h)
-    - label_smoothing log sigmoid(-h)).  Rows of no sequence get a gradient of 0; offsets that do not ascend, leave the rows or
-    lie outside the first and the last make their pair's results NaN."""
+    - label_smoothing log sigmoid(-h)).  Rows of no sequence get a gradient of 0.  Offsets that do not ascend, leave the rows or
+    lie outside the first and the last are no sequence: its pair's loss and the gradient of its partner's rows are NaN.  A row that two sequences
+    have, where offsets descend, takes the gradient of one of them, the same one in every call."""
     call = _Call(logits, temperature)
     at = call.check("labels", labels, (call.rows,), _INTS)
     if not isinstance(offsets, _torch.Tensor) or offsets.dim() != 1 or offsets.shape[0] < 3 or offsets.shape[0] % 2 == 0:

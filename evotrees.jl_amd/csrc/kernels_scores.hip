@@ -699,22 +699,27 @@ struct PairArgs {
 };
 // A pair's loss by a block of 64 W threads: the sequences' sums of logp (means with `average`), h = beta ((lp_c - lp_r) - (ref_c - ref_r)) - margin,
 // loss = w (-(1 - e) log sigma(h) - e log sigma(-h)), and the slope dloss / dlogp of a row of either.  Sequences 0 .. pairs - 1 are the chosen
-// ones, the rest the rejected.  Sums of 64 bits in an order that the lengths alone decide.
+// ones, the rest the rejected.  Sums of 64 bits in an order that the lengths and W decide.
 struct Pair {
     int64_t from[2], to[2];
     double lp[2];
     float loss, slope[2];
     bool bad;
 };
+// Rows from .. to - 1 ascend, are rows of the scores and lie between the first offset and the last: rows outside have no logp
+__device__ __forceinline__ bool is_sequence(const ScoreArgs &a, int64_t from, int64_t to, int64_t first, int64_t last) {
+    return from >= 0 && to <= a.N && from <= to && from >= first && to <= last;
+}
+// flag: one thread's, and then any thread's
 template <int W>
-__device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q, int p) {
+__device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q, int p, bool &flag) {
     __shared__ double s_sum[2][W];
-    __shared__ int s_cnt[2][W];
+    __shared__ int s_cnt[2][W], s_flag[W];
     const int t = threadIdx.x;
     Pair r;
     double len[2];
     int cnt[2] = {0, 0};
-    const int64_t first = a.bounds[0], last = a.bounds[a.n_bounds - 1]; // rows outside have no logp
+    const int64_t first = a.bounds[0], last = a.bounds[a.n_bounds - 1];
     r.bad = false;
 #pragma unroll
     for (int k = 0; k < 2; k++) {
@@ -724,7 +729,7 @@ __device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q,
     }
 #pragma unroll
     for (int k = 0; k < 2; k++) {
-        if (r.from[k] < 0 || r.to[k] > a.N || r.to[k] < r.from[k] || r.from[k] < first || r.to[k] > last) { // not ascending, or out of the rows
+        if (!is_sequence(a, r.from[k], r.to[k], first, last)) {
             r.bad = true;
             r.from[k] = r.to[k] = 0;
         }
@@ -746,9 +751,13 @@ __device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q,
             r.lp[k] += __shfl_xor(r.lp[k], o);
             cnt[k] += __shfl_xor(cnt[k], o);
         }
-    if ((t & 63) == 0)
+    flag = __any(flag);
+    if ((t & 63) == 0) {
         for (int k = 0; k < 2; k++) s_sum[k][t >> 6] = r.lp[k], s_cnt[k][t >> 6] = cnt[k];
+        s_flag[t >> 6] = flag;
+    }
     __syncthreads();
+    flag = __any(s_flag[t & (W - 1)]);
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         r.lp[k] = s_sum[k][t & (W - 1)];
@@ -786,13 +795,27 @@ __device__ __forceinline__ void write_pair(const ScoreArgs &a, const PairArgs &q
 #pragma unroll
     for (int k = 0; k < 2; k++) q.seq_logp[p + k * q.pairs] = r.bad ? NAN : (float)r.lp[k];
 }
-// One block to a pair, which leaves its slope at every row of the two
-__global__ __launch_bounds__(1024) void k_scores_pairs(ScoreArgs a, PairArgs q) {
-    const Pair r = pair_loss<16>(a, q, blockIdx.x);
+// Sequences share rows only where offsets descend somewhere between them.  Such a row has the slope of the most bits, an order that depends neither on which
+// block comes first nor on the form; SC_LOGP left 0, which has none.
+__device__ __forceinline__ uint32_t most_bits(uint32_t a, float slope) { return a > __float_as_uint(slope) ? a : __float_as_uint(slope); }
+// One block to a pair, which leaves its slope at every row of the two: by atomics where the offsets descend, or are so many that looking costs more (one block's
+// 500 000 rows: 370 us by atomics, 328 without)
+#define LOOK_FOR_SHARED 4096 // offsets
+template <int W>
+__global__ __launch_bounds__(64 * W) void k_scores_pairs(ScoreArgs a, PairArgs q) {
+    const int n = 2 * q.pairs;
+    bool shared = n > LOOK_FOR_SHARED;
+    if (!shared)
+        for (int k = threadIdx.x; k < n; k += 64 * W) shared |= a.bounds[k + 1] < a.bounds[k];
+    const Pair r = pair_loss<W>(a, q, blockIdx.x, shared);
     if (threadIdx.x == 0) write_pair(a, q, blockIdx.x, r);
 #pragma unroll
-    for (int k = 0; k < 2; k++)
-        for (int64_t i = r.from[k] + threadIdx.x; i < r.to[k]; i += 1024) a.slope[i] = r.slope[k];
+    for (int k = 0; k < 2; k++) {
+        if (shared)
+            for (int64_t i = r.from[k] + threadIdx.x; i < r.to[k]; i += 64 * W) atomicMax((uint32_t *)&a.slope[i], most_bits(0, r.slope[k]));
+        else
+            for (int64_t i = r.from[k] + threadIdx.x; i < r.to[k]; i += 64 * W) a.slope[i] = r.slope[k];
+    }
 }
 
 // The gradient of given slopes, where rows are long: nothing is joined, a block has a part of a row.
@@ -803,11 +826,13 @@ __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, PairArgs q, int
     constexpr int E = Piece<T>::E;
     // classes, at most 1024 pieces; the parts alike (32 764 x 8193 bf16, 1025 pieces a row: 308 us by 1024 and 1, 224 so)
     const int part = ((a.V + E - 1) / E + parts - 1) / parts * E;
+    __shared__ int2 s_two[4];
     const int64_t blocks = a.N * parts;
     const bool past = a.past;
     if (PAIRS && blockIdx.x >= blocks) {
         const int p = (int)(blockIdx.x - blocks);
-        const Pair r = pair_loss<4>(a, q, p);
+        bool none = false;
+        const Pair r = pair_loss<4>(a, q, p, none);
         if (threadIdx.x == 0) write_pair(a, q, p, r);
         return;
     }
@@ -821,17 +846,43 @@ __global__ __launch_bounds__(256) void k_slope_rows(ScoreArgs a, PairArgs q, int
         float given = 0.0f;
         bool live = label >= 0;
         if (!PAIRS && a.bounds) live = live && row >= a.bounds[0] && row < a.bounds[a.n_bounds - 1];
-        if (PAIRS && live) { // the first sequence that has the row
-            int seq = -1;
-            for (int k0 = 0; k0 < 2 * q.pairs && seq < 0; k0 += 64) {
-                const int k = k0 + (t & 63);
-                const uint64_t has = __ballot(k < 2 * q.pairs && row >= a.bounds[k < 2 * q.pairs ? k : 0] && row < a.bounds[k < 2 * q.pairs ? k + 1 : 0]);
-                if (has) seq = k0 + __builtin_ctzll(has);
+        if (PAIRS && live) { // the sequences that have the row: none, one, or more where offsets descend
+            const int n = 2 * q.pairs, first = a.bounds[0] < 0 ? 0 : a.bounds[0], last = a.bounds[n] < a.N ? a.bounds[n] : (int)a.N, at = (int)row;
+            uint32_t best = 0;
+            for (int from = 0; from < n;) {
+                int seq = -1, next = n; // the first of them from `from` on, and the one behind it
+                // up to 64 by every wavefront, more by a wavefront each and handed round (1000 pairs, 1000 rows of 2048 bf16: 19.1 us by every one)
+                const bool each = n - from <= 64;
+                for (int k0 = each ? from : from + (t & ~63); k0 < n && next == n; k0 += 256) {
+                    const int k = k0 + (t & 63), c = k < n ? k : n - 1, b0 = a.bounds[c], b1 = a.bounds[c + 1];
+                    uint64_t has = __ballot(k < n && at >= b0 && at < b1 && b0 >= first && b1 <= last); // is_sequence
+                    if (has && seq < 0) {
+                        seq = k0 + __builtin_ctzll(has);
+                        has &= has - 1;
+                    }
+                    if (has) next = k0 + __builtin_ctzll(has);
+                }
+                if (!each) {
+                    if ((t & 63) == 0) s_two[t >> 6] = {seq, next};
+                    __syncthreads();
+                    seq = -1, next = n;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int2 two = s_two[i];
+                        if (two.x < 0) continue;
+                        const int later = seq < 0 ? n : seq < two.x ? two.x : seq; // the second of the two firsts
+                        seq = seq < 0 || two.x < seq ? two.x : seq;
+                        next = min(next, min(later, two.y));
+                    }
+                }
+                if (seq < 0) break;
+                if (from) __syncthreads(); // everyone has read the sums of the pair before
+                bool none = false;
+                const Pair r = pair_loss<4>(a, q, seq < q.pairs ? seq : seq - q.pairs, none);
+                best = most_bits(best, r.slope[seq >= q.pairs]);
+                from = next;
             }
-            if (seq >= 0) {
-                const Pair r = pair_loss<4>(a, q, seq < q.pairs ? seq : seq - q.pairs);
-                given = r.from[seq >= q.pairs] < r.to[seq >= q.pairs] ? r.slope[seq >= q.pairs] : 0.0f; // no row of a sequence that is none
-            }
+            given = __uint_as_float(best);
         } else if (live) {
             given = a.slope[row];
         }
@@ -1146,7 +1197,9 @@ extern "C" int evt_preference_loss(void *stream, const void *scores, const void 
         HIPCHK(hipGetLastError());
         return EVT_OK;
     }
-    hipLaunchKernelGGL(k_scores_pairs, dim3((unsigned)n_pairs), dim3(1024), 0, st, a, q);
+    // many pairs are short ones (1M rows of 7 classes in 100 000 pairs, the whole call: 1076 us by 1024 threads, 251 by 256)
+    if (q.pairs * 2 > LOOK_FOR_SHARED) hipLaunchKernelGGL(k_scores_pairs<4>, dim3((unsigned)n_pairs), dim3(256), 0, st, a, q);
+    else hipLaunchKernelGGL(k_scores_pairs<16>, dim3((unsigned)n_pairs), dim3(1024), 0, st, a, q);
     HIPCHK(hipGetLastError());
     if (!a.N || !a.g) return EVT_OK;
     return launch_scores<SC_GRAD>(st, a, s->dtype);

@@ -448,9 +448,10 @@ int evt_policy_loss(void *stream, const void *scores /* evt_scores */, const voi
  * q[label] - of those with a label - or with average their mean (0 of none), ref_logp[k] the reference model's, and with w = weights[p] (NULL: 1)
  *   h = beta ((seq_logp[p] - seq_logp[n_pairs + p]) - (ref_logp[p] - ref_logp[n_pairs + p])) - margin,
  *   loss[p] = w (-(1 - label_smoothing) log sigmoid(h) - label_smoothing log sigmoid(-h)).
- * The gradient of sum_p loss[p] is written for every row: 0 for those in front of the first and behind the last sequence.  A pair whose
- * offsets do not ascend, leave the rows or lie outside offsets[0] .. offsets[2 n_pairs] gets NaN; where offsets descend, rows that two sequences then
- * have take the gradient of either.  work: 4 nrows floats that the call may write.  label_smoothing in [0, 0.5]. */
+ * The gradient of sum_p loss[p] is written for every row: 0 for those in front of the first and behind the last sequence.  A sequence
+ * whose offsets descend, leave the rows or lie outside offsets[0] .. offsets[2 n_pairs] is none: its seq_logp, its pair's loss and the gradient of its
+ * partner's rows are NaN, its own rows have no gradient from it.  Where offsets descend two sequences may both have a row, which takes the gradient of one of them, the same
+ * one in every call.  work: 4 nrows floats that the call may write.  label_smoothing in [0, 0.5]. */
 int evt_preference_loss(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, const int32_t *offsets, int32_t n_pairs,
                         const float *ref_logp, const float *weights, double beta, double label_smoothing, double margin, int32_t average,
                         float *loss, float *seq_logp, float *work, int32_t flags);

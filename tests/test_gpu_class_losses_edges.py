@@ -48,3 +48,92 @@ def test_preference_of_impossible_answers(evt, V, N, soft):
     plain.close("loss", loss, want, tol + plain.U * want.abs().nan_to_num(0, 0, 0) + 2.0 ** -149)
     assert seq[0] == -math.inf and seq[5] == -math.inf and seq[2] == -math.inf
     plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))
+
+
+def _pair_slopes(x, lab, off, ref, beta):
+    """(slope, what it may be off by) that each sequence's pair gives its rows: NaN for both of a pair one of which is no sequence."""
+    lp, lp_off, rows = plain.logp(x, lab, 1.0)
+    half = (len(off) - 1) // 2
+    ok = [0 <= a <= b <= len(lab) and a >= off[0] and b <= off[-1] for a, b in zip(off, off[1:])]
+    slopes, offs, seen = [0.0] * (2 * half), [0.0] * (2 * half), ok
+    for p in range(half):
+        c, r = slice(off[p], off[p + 1]), slice(off[half + p], off[half + p + 1])
+        if not (ok[p] and ok[half + p]):
+            slopes[p] = slopes[half + p] = math.nan
+            continue
+        h = beta * (float(lp[c].sum() - lp[r].sum()) - (float(ref[p]) - float(ref[half + p])))
+        win, lose = 1 / (1 + math.exp(-h)), 1 / (1 + math.exp(h))
+        slopes[p], slopes[half + p] = -beta * lose, beta * lose
+        offs[p] = offs[half + p] = beta * 2 * win * lose * beta * float(lp_off[c].sum() + lp_off[r].sum()) + 2 * plain.U * beta * lose
+    return slopes, offs, seen, rows
+
+
+@pytest.mark.parametrize("V,N", [(130, 24), (130, 3000), (33_000, 600)])  # slopes and losses in one launch, and in two
+def test_preference_gradient_where_offsets_descend(evt, V, N):
+    """Rows of a sequence that is none take the gradient of another that has them, whatever the form; rows of no other take none."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(N, V, generator=gen)
+    lab = torch.randint(0, V, (N,), generator=gen)
+    for off in ([0, 20, 2, 4, 6, 8, 10],  # sequence 0 ends behind the last, 1 descends; pairs (0, 3), (1, 4), (2, 5)
+                [6, 9, 0, 3, 12],  # sequence 1 descends, 2 begins in front of the first
+                [4, 7, 3, 12, 9, 12, 20]):  # 1 descends, 2 begins in front, 3 descends
+        ref = torch.randn(len(off) - 1, generator=gen) - 20
+        slopes, offs, ok, rows = _pair_slopes(x, lab, off, ref, 0.1)
+        slope, slope_off = torch.zeros(N, dtype=torch.float64), torch.zeros(N, dtype=torch.float64)
+        owned = torch.zeros(N, dtype=torch.int32)
+        for k, (a, b) in enumerate(zip(off, off[1:])):
+            if ok[k]:
+                slope[a:b], slope_off[a:b] = slopes[k], offs[k]
+                owned[a:b] += 1
+        assert owned.max() == 1
+        loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), torch.tensor(off, dtype=torch.int32).cuda(), ref.cuda())
+        plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))
+
+
+@pytest.mark.parametrize("V,N", [(130, 24), (130, 3000), (33_000, 600)])
+def test_preference_rows_of_two_sequences(evt, V, N):
+    """Two sequences that both have a row (the offsets descend between them): one of their gradients, the same one in every call and in every form."""
+    gen = torch.Generator().manual_seed(V + 1)
+    x = torch.randn(N, V, generator=gen)
+    lab = torch.randint(0, V, (N,), generator=gen)
+    off = [0, 5, 3, 8, 10, 12, 14, 16, 18]  # 1 descends; 0 and 2 share rows 3 and 4; pairs (0, 4), (1, 5), (2, 6), (3, 7)
+    ref = torch.randn(8, generator=gen) - 20
+    ref[0] -= 40  # the slope of pair 2 is the larger by far
+    slopes, offs, ok, rows = _pair_slopes(x, lab, off, ref, 0.1)
+    assert abs(slopes[2]) > 1.2 * abs(slopes[0])
+    args = x.cuda(), lab.cuda(), torch.tensor(off, dtype=torch.int32).cuda(), ref.cuda()
+    loss, seq, grad = evt.preference_loss(*args)
+    slope, slope_off = torch.zeros(N, dtype=torch.float64), torch.zeros(N, dtype=torch.float64)
+    for k in (0, 3, 4, 5, 6, 7, 2):  # the larger slope's last
+        slope[off[k]:off[k + 1]], slope_off[off[k]:off[k + 1]] = slopes[k], offs[k]
+    plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))
+    for _ in range(20):
+        for a, b in zip(evt.preference_loss(*args), (loss, seq, grad)):
+            assert torch.equal(a.nan_to_num(9.0), b.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("V,N,pairs,dtype", [(2100, 500, 300, "f32"), (2100, 1000, 1000, "bf16"), (16, 9000, 5000, "f32")])  # one launch; one launch; two, many pairs
+def test_preference_many_pairs(evt, V, N, pairs, dtype):
+    """More sequences than a wavefront looks at: each row's gradient is its own pair's; of two sequences that descending offsets give a row one's, whichever place they have."""
+    gen = torch.Generator().manual_seed(pairs)
+    x = torch.randn(N, V, generator=gen).to(plain.TYPES[dtype])
+    lab = torch.randint(0, V, (N,), generator=gen)
+    ref = torch.randn(2 * pairs, generator=gen)
+    off = torch.randint(0, N + 1, (2 * pairs + 1,), generator=gen).sort().values.to(torch.int32)
+    want = plain.preference(x, lab, off, ref, 0.1, 0.0, 0.0, False, 1.0, None)
+    loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), off.cuda(), ref.cuda())
+    plain.close("loss", loss, *want[0])
+    plain.close("grad", grad, *want[2])
+    # sequences k and m > k + 1 (the one between descends) both have rows 40 to 59, and no other has
+    for k, m in ((3, 70), (10, 12), (100, pairs + 200), (pairs - 1, 2 * pairs - 2)):
+        bounds = [0] * (k + 1) + [60] * (m - k - 1) + [40] + [100] * (2 * pairs - m)
+        lab[40:60] = 1
+        slopes, offs, ok, rows = _pair_slopes(x, lab, bounds, ref, 0.1)
+        assert len(bounds) == 2 * pairs + 1 and ok[k] and ok[m] and not ok[m - 1]
+        slope, slope_off = torch.zeros(N, dtype=torch.float64), torch.zeros(N, dtype=torch.float64)
+        def bits(s):  # of a slope's float, as an unsigned number
+            return int(torch.tensor([s], dtype=torch.float32).view(torch.int32)) & 0xFFFFFFFF
+        for j in sorted((k, m), key=lambda j: bits(slopes[j])):
+            slope[bounds[j]:bounds[j + 1]], slope_off[bounds[j]:bounds[j + 1]] = slopes[j], offs[j]
+        loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), torch.tensor(bounds, dtype=torch.int32).cuda(), ref.cuda())
+        plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))

@@ -283,7 +283,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     constexpr int E = Piece<T>::E;
     static_assert(OP != SC_DISTILL || G::ROWS == 1, "k_distill_short has the others");
     extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs, then the scores of these classes
-    __shared__ int s_state;                  // SC_DISTILL: 1 a teacher, 2 with an id of no class
+    __shared__ int s_state;                  // SC_DISTILL: 1 a teacher, 2 with an id of no class or a score that is no number or +inf
     const int64_t row = a.row0 + (int64_t)blockIdx.x * G::ROWS + G::slot();
     if (G::ROWS > 1 && row >= a.N) return;
     const int t = G::rank(), V = a.V;
@@ -344,7 +344,7 @@ __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
         }
         teacher = uniform(lanes_join<64>(teacher, mul));
         none = __any(none);
-        if (t == 0) s_state = teacher.s == 0.0f ? 0 : none ? 2 : 1; // a sum that is no number is a teacher
+        if (t == 0) s_state = teacher.s == 0.0f ? 0 : none || teacher.s != teacher.s ? 2 : 1;
 #pragma unroll 1
         for (int j = t; j < a.n_top; j += 64) s_top[j].y = __float_as_int(exp_of(__int_as_float(s_top[j].y), teacher.m, mul) * (1.0f / teacher.s));
     }

@@ -430,7 +430,8 @@ int evt_class_logp_grad(void *stream, const void *scores /* evt_scores */, const
 /* Distillation from a teacher that kept its n_top best classes of each row (1 .. 1024): top_ids and top_scores are nrows x n_top, an id below 0 is no
  * entry, and an id may come twice.  With p = softmax(top_scores / temperature) over a row's entries and w = weights[i] (NULL: 1):
  *   loss[i] = w temperature^2 sum_j p_j (log p_j - log q[id_j]),   grad[i, c] = w temperature (q_c - sum of p_j with id_j == c).
- * A row without entries, or with none above -inf, is left out. */
+ * A row without entries, or with none above -inf, is left out.  A NaN or +inf among an entry's scores, or an id of nclass or more, makes the row's loss and all of
+ * its gradient NaN. */
 int evt_distill_loss(void *stream, const void *scores /* evt_scores */, const void *top_ids, int32_t id_dtype, const void *top_scores, int32_t top_dtype,
                      int32_t n_top, const float *weights, float *loss, int32_t flags);
 

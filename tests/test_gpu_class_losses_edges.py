@@ -137,3 +137,20 @@ def test_preference_many_pairs(evt, V, N, pairs, dtype):
             slope[bounds[j]:bounds[j + 1]], slope_off[bounds[j]:bounds[j + 1]] = slopes[j], offs[j]
         loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), torch.tensor(bounds, dtype=torch.int32).cuda(), ref.cuda())
         plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))
+
+
+@pytest.mark.parametrize("V,N", [(3, 9), (7, 9), (100, 9), (1500, 300), (3001, 300), (50_021, 9)])  # every form
+@pytest.mark.parametrize("dtype", list(plain.TYPES))
+def test_teacher_scores_that_are_no_numbers(evt, V, N, dtype):
+    """A NaN or +inf among the teacher's scores of a row that counts: its loss is NaN and all of its gradient; the other rows are as they were."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(N, V, generator=gen).to(plain.TYPES[dtype])
+    ids = torch.stack([torch.randperm(V, generator=gen)[:3] for _ in range(N)])
+    top = torch.randn(N, 3, generator=gen)
+    want = plain.distill(x, ids, top, 1.0, None)
+    top[2, 1], top[5, 0] = math.nan, math.inf
+    for k in (2, 5):
+        want[0][0][k] = want[1][0][k] = math.nan
+    loss, grad = evt.distill_loss(x.cuda(), ids.cuda(), top.cuda())
+    plain.close("loss", loss, *want[0])
+    plain.close("grad", grad, *want[1])

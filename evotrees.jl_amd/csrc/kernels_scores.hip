@@ -196,6 +196,12 @@ __device__ __forceinline__ double row_logp(const ScoreArgs &a, MaxSum r, float x
 }
 __device__ __forceinline__ float inverse_sum(MaxSum r) { return r.s == 0.0f ? 0.0f : 1.0f / r.s; }
 
+// exp(x) with 32 bits of digits and the exponents of 64
+__device__ __forceinline__ double exp_wide(double x) {
+    x = x > 1500.0 ? 1500.0 : x < -1500.0 ? -1500.0 : x; // infinite or 0 either way; a NaN stays
+    const double k = rint(x * 1.4426950408889634);
+    return ldexp((double)expf((float)(x - k * 0.6931471805599453)), (int)k);
+}
 // The policy loss of a token and its derivative by logp: -min(r A, clip(r) A) + kl (exp(b) - b - 1), r = exp(logp - old), b = ref - logp.
 // The differences are 64-bit, and the side of the bounds that r is on is found from them: a ratio next to a bound has a whole row's gradient or none.
 // An advantage of zero has no share in it, however far apart the two policies are, a weight of zero no loss.
@@ -204,15 +210,22 @@ __device__ __forceinline__ void policy_row(const ScoreArgs &a, int64_t row, floa
     const float adv = a.adv[row];
     if (adv != 0.0f) {
         const double gap = logp - (double)a.old_logp[row];
-        const double free = -(double)expf((float)gap) * adv;
+        // beyond float's range an advantage or a weight may bring the product back into it
+        const double free = -(fabs(gap) <= 80.0 ? (double)expf((float)gap) : exp_wide(gap)) * adv;
         if (adv > 0.0f ? gap > a.log_hi : gap < a.log_lo) l = -(adv > 0.0f ? a.hi : a.lo) * adv;
         else l = d = free; // a NaN too
     }
     if (a.kl != 0.0) {
         const double back = (double)a.ref_logp[row] - logp;
-        const float b = (float)back, e = expm1f(b);
+        const float b = (float)back;
+        double e = expm1f(b), rest;
         // e - b cancels where the policies are close: there the series up to b^7 / 7!, the rest of which is under 2^-26 of it
-        const float rest = fabsf(b) < 0.25f ? b * b * (0.5f + b * (1.0f / 6 + b * (1.0f / 24 + b * (1.0f / 120 + b * (1.0f / 720 + b * (1.0f / 5040)))))) : e - b;
+        if (fabsf(b) < 0.25f) {
+            rest = b * b * (0.5f + b * (1.0f / 6 + b * (1.0f / 24 + b * (1.0f / 120 + b * (1.0f / 720 + b * (1.0f / 5040))))));
+        } else {
+            if (b > 80.0f) e = exp_wide(back);
+            rest = e - back;
+        }
         l += a.kl * rest;
         d -= a.kl * e;
     }

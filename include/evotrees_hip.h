@@ -402,7 +402,9 @@ int evt_predict_static(void *stream, int64_t nobs, int32_t nfeats, const uint8_t
  *
  * With z = x / temperature, q = softmax(z) over a row's nclass scores and log q its logarithm:
  *  - Scores are EVT_F32, EVT_BF16 or EVT_F16, a row's side by side, rows row_stride elements apart (any alignment; 0: one row for all).
- *    Differences, exponentials and sums are 32-bit, losses 64-bit until they are written; a gradient is rounded once, to the scores' type.
+ *    Differences, exponentials and sums over classes and entries have 32 bits; logarithms, ratios, sums over a sequence and the policy's and the pairs' losses
+ *    have the range and the sums of 64 until they are written, distillation's loss its logarithms only.  A gradient is rounded once, to the
+ *    scores' type; where dloss/dlogp itself is beyond float's range its row's gradient is infinite or NaN.
  *  - A score of -inf is a class that cannot be: q = 0, also in its gradient.  A row of nothing else has log q = -inf and q = 0 everywhere.
  *    A NaN or +inf makes its row's results NaN, and no other's.
  *  - Labels and ids count from 0 (EVT_I32 or EVT_I64).  A negative label leaves its row out: loss, logp and gradient are 0 and the row is not read.

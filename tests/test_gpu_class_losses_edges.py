@@ -154,3 +154,36 @@ def test_teacher_scores_that_are_no_numbers(evt, V, N, dtype):
     loss, grad = evt.distill_loss(x.cuda(), ids.cuda(), top.cuda())
     plain.close("loss", loss, *want[0])
     plain.close("grad", grad, *want[1])
+
+
+@pytest.mark.parametrize("V", [3, 7, 40, 700, 9001, 140_001])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_policies_far_apart(evt, V, dtype):
+    """exp(logp - old) and exp(ref - logp) beyond float's range, with advantages, weights and a kl_coef that bring the loss back into it: the loss
+    and the gradient are finite, and 0 at a class that cannot be."""
+    gen = torch.Generator().manual_seed(V)
+    gaps = torch.tensor([90.0, 120.0, 170.0, -95.0, -120.0, 0.1, 80.5, 88.9])
+    adv = torch.tensor([-1e-3, -1e-10, -1e-25, 1e20, 1e30, 1.0, -1e-4, -0.1])
+    w = torch.tensor([1.0, 1e-7, 1e-30, 1.0, 0.5, 1.0, 1.0, 1.0])
+    N = len(gaps)
+    x = torch.randn(N, V, generator=gen)
+    x[:, 1] = -math.inf
+    x = x.to(plain.TYPES[dtype])
+    lab = torch.randint(0, V, (N,), generator=gen)
+    lab[lab == 1] = 2
+    lp = plain.logp(x, lab, 1.0)[0]
+    old = (lp - gaps).float()
+    loss, logp, grad = evt.policy_loss(x.cuda(), lab.cuda(), old.cuda(), adv.cuda(), weights=w.cuda())
+    want = plain.policy(x, lab, old, adv, None, 0.2, 0.2, 0.0, 1.0, w)
+    assert torch.isfinite(want[0][0]).all() and (want[0][0] != 0).all() and not want[2][0][:, 1].any()
+    plain.close("loss", loss, *want[0])
+    plain.close("grad", grad, *want[2])
+    # the KL term alone: 0.05 exp(90) is 6e37
+    ref = (lp + torch.tensor([90.0, 88.8, 100.0, 150.0, -90.0, -300.0, 81.0, 0.2])).float()
+    w = torch.tensor([1.0, 1.0, 1e-6, 1e-30, 1.0, 1.0, 1.0, 1.0])
+    none = torch.zeros(N)
+    loss, logp, grad = evt.policy_loss(x.cuda(), lab.cuda(), old.cuda(), none.cuda(), ref.cuda(), kl_coef=0.05, weights=w.cuda())
+    want = plain.policy(x, lab, old, none, ref, 0.2, 0.2, 0.05, 1.0, w)
+    assert torch.isfinite(want[0][0]).all() and torch.isfinite(want[2][0]).all()
+    plain.close("kl loss", loss, *want[0])
+    plain.close("kl grad", grad, *want[2])

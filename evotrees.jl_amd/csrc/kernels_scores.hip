@@ -212,8 +212,8 @@ __device__ __forceinline__ void policy_row(const ScoreArgs &a, int64_t row, floa
         const double gap = logp - (double)a.old_logp[row];
         // beyond float's range an advantage or a weight may bring the product back into it
         const double free = -(fabs(gap) <= 80.0 ? (double)expf((float)gap) : exp_wide(gap)) * adv;
-        if (adv > 0.0f ? gap > a.log_hi : gap < a.log_lo) l = -(adv > 0.0f ? a.hi : a.lo) * adv;
-        else l = d = free; // a NaN too
+        if (adv > 0.0f ? gap > a.log_hi : adv < 0.0f && gap < a.log_lo) l = -(adv > 0.0f ? a.hi : a.lo) * adv;
+        else l = d = free; // a NaN too, of the ratio or the advantage
     }
     if (a.kl != 0.0) {
         const double back = (double)a.ref_logp[row] - logp;

@@ -187,3 +187,16 @@ def test_policies_far_apart(evt, V, dtype):
     assert torch.isfinite(want[0][0]).all() and torch.isfinite(want[2][0]).all()
     plain.close("kl loss", loss, *want[0])
     plain.close("kl grad", grad, *want[2])
+
+
+@pytest.mark.parametrize("V", [3, 40, 9001])
+def test_advantage_that_is_no_number(evt, V):
+    """Its row's loss and gradient are NaN on either side of the bounds and between them; no other row's are."""
+    gen = torch.Generator().manual_seed(V)
+    x = torch.randn(6, V, generator=gen)
+    lab = torch.randint(0, V, (6,), generator=gen)
+    old = (plain.logp(x, lab, 1.0)[0] - torch.tensor([-1.0, 0.0, 1.0, -1.0, 0.0, 1.0])).float()
+    adv = torch.tensor([math.nan, math.nan, math.nan, 1.0, 1.0, 1.0])
+    loss, logp, grad = evt.policy_loss(x.cuda(), lab.cuda(), old.cuda(), adv.cuda())
+    assert torch.isnan(loss).tolist() == [True] * 3 + [False] * 3 and not torch.isnan(logp).any()
+    assert torch.isnan(grad[:3]).all() and torch.isfinite(grad[3:]).all()

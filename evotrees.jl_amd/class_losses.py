@@ -8,9 +8,10 @@ classes, a language model's vocabulary as well as a classifier's levels, and hav
 Scores are a (rows, classes) tensor of float32, bfloat16 or float16 whose classes lie side by side (`scores.stride(1) == 1`); rows may be
 any distance apart.  Labels and class ids count from 0 and are int32 or int64; a negative one stands for none.  Values that
 belong to a row, an entry or a pair are contiguous float32.  Temperatures are from 1e-4 to 1e4.  All tensors of a call are on one GPU; the work is queued on that GPU's current
-stream and nothing waits for it.  As the gradients of this package's other losses, these are returned, not recorded: there is no autograd
-graph, and a loss's weights stand in for what a chain rule would multiply it by.  `out` takes the gradient: a tensor like the scores, or the scores
-themselves, which the gradient then replaces.
+stream and nothing waits for it.  As the gradients of this package's other losses, these are returned, not recorded: results never require a
+gradient, also where the scores do, so that a loss added to a recorded one has no part in its backward pass.  The returned gradient goes on from there
+(`logits.backward(grad)`), and a loss's weights stand in for what a chain rule would multiply it by.  `out` takes the gradient: a tensor like the scores, or the scores
+themselves, which the gradient then replaces - a change of that tensor as any operation in place is, which a recorded operation that kept it reports.
 
 Wrong arguments raise ValueError or TypeError before anything is queued; what a call refuses in the library raises EvtError."""
 import ctypes as C
@@ -29,7 +30,7 @@ _entries = {}  # by name
 
 def _load():
     """torch, the codes of its types and what a call needs of it; imported with the first call, a fit needs none."""
-    global _torch, _FLOATS, _INTS, _F32S, _I32S, _like, _device, _stream
+    global _torch, _FLOATS, _INTS, _F32S, _I32S, _like, _device, _stream, _changed
     import torch
     _F32S = {torch.float32: _F32}
     _FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
@@ -37,6 +38,7 @@ def _load():
     _INTS = {torch.int32: _I32, torch.int64: _I64}
     _like = torch.empty_like
     _device = torch.cuda.current_device
+    _changed = torch.autograd.graph.increment_version
     # the current stream's handle without a Stream object around it, 1.1 us less a call
     _stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
     _torch = torch
@@ -57,7 +59,7 @@ def _bad(name, v, x, shape, kinds):
 
 class _Call:
     """A call on some scores: the checks of what belongs to them, and the launch on their device's current stream."""
-    __slots__ = ("x", "kind", "rows", "classes", "device", "temperature")
+    __slots__ = ("x", "kind", "rows", "classes", "device", "temperature", "out")
 
     def __init__(self, x, temperature):
         if _torch is None:
@@ -96,6 +98,7 @@ class _Call:
     def gradient(self, want, out):
         """The tensor the gradient goes to, None for none."""
         x = self.x
+        self.out = out
         if out is None:
             if not want:
                 return None
@@ -133,11 +136,14 @@ class _Call:
                 rc = call(_stream(dev), C.byref(s), *args, _TRUSTED)
         if rc:
             _lib.check(rc)
+        if grad is not None and self.out is not None and not grad.is_inference():
+            _changed(grad)
 
 
 def class_logp(logits, labels, temperature=1.0):
     """Log-probability of every row's label under softmax(logits / temperature), and each row's maximum and sum of exponentials, which
-    class_logp_grad takes: tensors (rows,) and (rows, 2), both float32.  Both are 0 for a row whose label is negative."""
+    class_logp_grad takes: tensors (rows,) and (rows, 2), both float32.  Both are 0 for a row whose label is negative.  Nothing is recorded for a backward
+    pass: class_logp_grad is it."""
     call = _Call(logits, temperature)
     rows = call.rows
     at = call.check("labels", labels, (rows,), _INTS)
@@ -159,7 +165,7 @@ def class_logp_grad(logits, labels, stats, dlogp, temperature=1.0, out=None):
 
 def distill_loss(logits, top_ids, top_logits, temperature=1.0, weights=None, grad=True, out=None):
     """Distillation from a teacher's best classes: for every row weights * temperature^2 * KL(softmax(top_logits / temperature) over the row's entries ||
-    softmax(logits / temperature)), and the gradient of the sum of all rows' losses by the logits (None with grad=False).
+    softmax(logits / temperature)), and the gradient of the sum of all rows' losses by the logits (None with grad=False), which is returned, not recorded.
 
     top_ids, top_logits: (rows, n_top), at most 1024 entries; a negative id is no entry.  top_logits may be float32, bfloat16 or float16."""
     call = _Call(logits, temperature)
@@ -177,7 +183,8 @@ def distill_loss(logits, top_ids, top_logits, temperature=1.0, weights=None, gra
 
 def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, clip_low=0.2, clip_high=0.2, kl_coef=0.0, temperature=1.0, weights=None, grad=True,
                 out=None):
-    """The clipped policy loss of every token, its log-probability, and the gradient of the sum of all losses by the logits (None with grad=False).
+    """The clipped policy loss of every token, its log-probability, and the gradient of the sum of all losses by the logits (None with grad=False), which is
+    returned, not recorded.
 
     With r = exp(logp - old_logp) the loss is weights * (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(b) - b - 1)), A the
     advantage and b = ref_logp - logp.  A negative action marks a padded row: its loss, log-probability and gradient are 0.  A weight of 0 leaves
@@ -201,7 +208,7 @@ def policy_loss(logits, actions, old_logp, advantages, ref_logp=None, clip_low=0
 def preference_loss(logits, labels, offsets, ref_logp, beta=0.1, label_smoothing=0.0, margin=0.0, average=False, temperature=1.0, weights=None,
                     grad=True, out=None):
     """The preference loss of pairs of sequences packed one behind the other, the log-probability of every sequence (summed over its labelled
-    rows, their mean with `average`), and the gradient of the sum of all losses by the logits (None with grad=False).
+    rows, their mean with `average`), and the gradient of the sum of all losses by the logits (None with grad=False), which is returned, not recorded.
 
     offsets: int32, sequence k has the rows offsets[k] to offsets[k + 1] - 1; the first half of the sequences are the chosen ones, the second half,
     in the same order, the rejected.  ref_logp: the reference model's log-probability of every sequence.  weights: one for each pair.

@@ -200,3 +200,44 @@ def test_advantage_that_is_no_number(evt, V):
     loss, logp, grad = evt.policy_loss(x.cuda(), lab.cuda(), old.cuda(), adv.cuda())
     assert torch.isnan(loss).tolist() == [True] * 3 + [False] * 3 and not torch.isnan(logp).any()
     assert torch.isnan(grad[:3]).all() and torch.isfinite(grad[3:]).all()
+
+
+def test_out_counts_as_a_change(evt):
+    """A gradient written over a tensor that a recorded operation kept: its backward pass says so and does not compute with the gradient."""
+    N, V = 12, 50
+    lab = torch.randint(0, V, (N,)).cuda()
+    v = torch.randn(N).cuda()
+    off = torch.tensor([0, 5, 12], dtype=torch.int32).cuda()
+    stats = torch.ones(N, 2).cuda()
+    leaf = torch.randn(N, V).cuda().requires_grad_()
+    for call in (lambda y: evt.class_logp_grad(y, lab, stats, v, out=y), lambda y: evt.distill_loss(y, lab[:, None], v[:, None], out=y),
+                 lambda y: evt.policy_loss(y, lab, v, v, out=y), lambda y: evt.preference_loss(y, lab, off, v[:2].contiguous(), out=y)):
+        y = leaf.exp()
+        before = y._version
+        call(y)
+        assert y._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        box = torch.zeros(N, V + 3).cuda()
+        before = box._version
+        call_out = box[:, 1:V + 1]
+        call_out.copy_(leaf.detach())
+        assert box._version == before + 1
+        call(call_out)
+        assert box._version == before + 2
+    with torch.inference_mode():  # tensors made here have no such count
+        z = leaf.detach() * 2.0
+        assert evt.policy_loss(z, lab, v, v, out=z)[2] is z
+    z = evt.policy_loss(z, lab, v, v, out=z)[2]
+
+
+def test_results_are_not_recorded(evt):
+    """Scores that require a gradient: no result does, and the returned gradient goes on by hand."""
+    N, V = 12, 50
+    leaf = torch.randn(N, V).cuda().requires_grad_()
+    lab, v = torch.randint(0, V, (N,)).cuda(), torch.randn(N).cuda()
+    logits = leaf * 2.0
+    loss, logp, grad = evt.policy_loss(logits, lab, v - 4, v)
+    logits.backward(grad)
+    assert not loss.requires_grad and not logp.requires_grad and not grad.requires_grad and torch.equal(leaf.grad, grad * 2.0)
+    assert not any(t.requires_grad for t in evt.class_logp(logits, lab))

@@ -1041,8 +1041,7 @@ int launch_distill_f32(hipStream_t s, const ScoreArgs &a) { return launch_scores
 // ---- entry points ---------------------------------------------------------------------------
 static bool on_device(const void *p) {
     hipPointerAttribute_t attr;
-    const bool ok = hipPointerGetAttributes(&attr, p) == hipSuccess && attr.devicePointer != nullptr &&
-                    (attr.type == hipMemoryTypeDevice || attr.type == hipMemoryTypeHost || attr.type == hipMemoryTypeManaged);
+    const bool ok = hipPointerGetAttributes(&attr, p) == hipSuccess && attr.type == hipMemoryTypeDevice; // pinned host memory has no atomics
     (void)hipGetLastError();
     return ok;
 }

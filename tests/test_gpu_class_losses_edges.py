@@ -1,5 +1,6 @@
 """The losses over rows of class scores where a value is at the end of its range, is none, or stands in more than one sequence: against their formulas in
 64 bits."""
+import ctypes as C
 import math
 
 import pytest
@@ -241,3 +242,23 @@ def test_results_are_not_recorded(evt):
     logits.backward(grad)
     assert not loss.requires_grad and not logp.requires_grad and not grad.requires_grad and torch.equal(leaf.grad, grad * 2.0)
     assert not any(t.requires_grad for t in evt.class_logp(logits, lab))
+
+
+def test_host_memory_is_refused(evt):
+    """The C entry points ask where a pointer lies unless the caller vouches for it: pinned host memory is not device memory."""
+    L, E = evt._lib.load(), evt._lib
+    x, lab = torch.zeros(4, 10).cuda(), torch.zeros(4, dtype=torch.int64).cuda()
+    out = torch.zeros(4, 2).cuda()
+    host = [torch.zeros(4, 10).pin_memory(), torch.zeros(4, dtype=torch.int64).pin_memory(), torch.zeros(4, 2).pin_memory()]
+
+    def call(x, lab, out):
+        s = E.EvtScores(x.data_ptr(), 10, None, 0, 4, 10, 0, 1.0)
+        return L.evt_class_logp(None, C.byref(s), lab.data_ptr(), 5, out.data_ptr(), stats.data_ptr(), 0)
+
+    stats = torch.zeros(4, 2).cuda()
+    torch.cuda.synchronize()
+    assert call(x, lab, out) == E.EVT_OK
+    torch.cuda.synchronize()
+    for args in ((host[0], lab, out), (x, host[1], out), (x, lab, host[2])):
+        assert call(*args) == E.EVT_ERR_ARG and b"device memory" in L.evt_last_error()
+    torch.cuda.synchronize()

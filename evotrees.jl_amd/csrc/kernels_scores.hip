@@ -295,7 +295,7 @@ template <typename T, int OP, int NV, class G>
 __global__ __launch_bounds__(G::THREADS) void k_rows(ScoreArgs a) {
     constexpr int E = Piece<T>::E;
     static_assert(OP != SC_DISTILL || G::ROWS == 1, "k_distill_short has the others");
-    extern __shared__ unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs, then the scores of these classes
+    extern __shared__ __align__(16) unsigned char s_dyn[]; // SC_DISTILL: n_top (id, probability) pairs, then the scores of these classes
     __shared__ int s_state;                  // SC_DISTILL: 1 a teacher, 2 with an id of no class or a score that is no number or +inf
     const int64_t row = a.row0 + (int64_t)blockIdx.x * G::ROWS + G::slot();
     if (G::ROWS > 1 && row >= a.N) return;
@@ -534,7 +534,7 @@ template <typename T, int NV, class G>
 __global__ __launch_bounds__(256) void k_distill_short(ScoreArgs a, uint32_t top_magic) {
     constexpr int E = Piece<T>::E;
     constexpr bool FEW = NV == 0; // V < E: every lane has the whole row, and shares the teacher's entries
-    extern __shared__ unsigned char s_dyn[];
+    extern __shared__ __align__(16) unsigned char s_dyn[];
     const int V = a.V, k1 = a.n_top, ks = k1 | 1, vs = (V + 2) | 1; // odd distances: rows that lanes read side by side start in different banks
     int2 *const s_all = (int2 *)s_dyn; // (class, V for no entry, V + 1 for no class; score)
     float *const s_share = (float *)(s_all + G::ROWS * ks);

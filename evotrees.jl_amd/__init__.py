@@ -130,8 +130,8 @@ class EvoTreeMLE(_Learner):
 
 class Teacher:
     """What a classifier is fitted to in place of its target's labels (`fit(..., teacher=)`): the classes another model thinks best of every row and their
-    scores (logits), as distill_loss takes them.  ids, logits: (rows, n_top); an id is a position among the target's sorted levels, from 0,
-    and one below 0 is no entry.  The labels still give the levels, the bias and the metric."""
+    scores (logits), as distill_loss takes them.  ids, logits: (rows, n_top) arrays or torch tensors, 1 to 1024 entries a row; an id is a position among the
+    target's sorted levels, from 0, and one below 0 is no entry.  The labels still give the levels, the bias and the metric."""
 
     def __init__(self, ids, logits, temperature=1.0):
         self.ids, self.logits, self.temperature = ids, logits, float(temperature)

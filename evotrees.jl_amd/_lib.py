@@ -303,6 +303,14 @@ class TreeArrays:
         return EvtTreeOut(address(self.feat), address(self.cond_bin), address(self.w), address(self.gain), address(self.pred), address(self.split))
 
 
+def host_array(v):
+    """v as a numpy array: a torch tensor of any device and type too."""
+    if hasattr(v, "detach"):
+        v = v.detach()
+        v = (v.float() if v.is_floating_point() else v).cpu()
+    return np.asarray(v)
+
+
 class Handle:
     """One training cache on the device (the reference's CacheGPU)."""
 
@@ -364,16 +372,16 @@ class Handle:
         check(load().evt_set_feature_meta(self._h, ptr(ft), ptr(mo)))
 
     def set_teacher(self, ids, scores, temperature=1.0):
-        """ids, scores: (N, n_top) classes from 0 (below 0: none) and their scores, which the gradients of mlogloss are computed from then; None
+        """ids, scores: (N, n_top) arrays, or torch tensors on any device, of classes from 0 (below 0: none) and their scores, which the gradients of mlogloss are computed from then; None
         for both: from the labels again."""
         if ids is None and scores is None:
             check(load().evt_set_teacher(self._h, None, None, 0, 1.0))
             return
-        ids = np.asarray(ids)
+        ids, scores = host_array(ids), host_array(scores)
         if ids.dtype.kind not in "iu":
             raise ValueError("a teacher's ids must be whole numbers")
-        if ids.ndim != 2 or ids.shape[0] != self.N or np.shape(scores) != ids.shape:
-            raise ValueError("a teacher's ids and scores must both be %d x n_top" % self.N)
+        if ids.ndim != 2 or ids.shape[0] != self.N or ids.shape[1] < 1 or np.shape(scores) != ids.shape:
+            raise ValueError("a teacher's ids and scores must both be %d x n_top, of one entry a row at least" % self.N)
         if ids.size and (ids.max() >= self.K):
             raise ValueError("a teacher's ids must be below the number of classes (%d)" % self.K)
         ids, scores = np.ascontiguousarray(np.maximum(ids, -1) if ids.dtype.kind == "i" else ids, np.int32), np.ascontiguousarray(scores, np.float32)

@@ -197,7 +197,8 @@ int evt_set_alphas(evt_handle h, const double *alphas, int32_t n);
  * its target's labels.  ids and scores are nobs x n_top (a row's entries side by side): the classes the teacher kept of each row, counted from 0 (level code - 1;
  * below 0: no entry), and their scores.  evt_update_grads then computes the gradients of evt_distill_loss at this temperature,
  * T (q - p) w with q = softmax(pred / T) and p = softmax(scores / T) over the row's entries, and the second-order rows q (1 - q) w.  A row without entries has no
- * gradient; its second-order rows and its weight count all the same (a weight of 0 leaves it out altogether).  n_top 0 (ids and scores may be NULL) goes back to the labels, which the metric is computed from in either case. */
+ * gradient; its second-order rows and its weight count all the same (a weight of 0 leaves it out altogether).  A teacher stays until another, also through evt_set_target; n_top 0 (ids and scores may be NULL) goes back
+ * to the labels, which the metric is computed from in either case. */
 int evt_set_teacher(evt_handle h, const int32_t *ids, const float *scores, int32_t n_top, double temperature);
 
 /* update_grads!(cache.∇, cache.pred, cache.y, L, params): src/loss.jl:100-111, :219-236;

@@ -964,7 +964,7 @@ static int launch_typed(hipStream_t s, const ScoreArgs &a) {
     const bool few = a.N <= 256; // no more than a unit each
     if constexpr (OP == SC_DISTILL) {
         if (launch_distill<T, 0, Lanes<1>>(s, a, n) || launch_distill<T, 0, Lanes<8>>(s, a, n) || launch_distill<T, 0, Lanes<64>>(s, a, n)) return EVT_OK;
-        // few rows of more than a few classes: a block to each is done sooner (4 rows of 2048 bf16: 9.5 us by lanes, 6.1 so)
+        // few rows of more than a few classes: a block to each (4 rows of 2048 bf16, on the device: 6.9 us by lanes, 5.9 so; 256 rows of 512: 5.8 | 6.4)
         if ((!few || n <= 32) &&
             (launch_distill<T, 4, Lanes<1>>(s, a, n) || launch_distill<T, 4, Lanes<2>>(s, a, n) || launch_distill<T, 4, Lanes<4>>(s, a, n) ||
              launch_distill<T, 4, Lanes<8>>(s, a, n) || launch_distill<T, 4, Lanes<16>>(s, a, n) || launch_distill<T, 4, Lanes<32>>(s, a, n) ||

@@ -442,7 +442,7 @@ int evt_distill_loss(void *stream, const void *scores /* evt_scores */, const vo
  *   loss[i] = w (-min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_coef (exp(b) - b - 1)),
  *   grad[i, :] = dloss/dlogp (onehot(label) - q) / temperature,  dloss/dlogp = w (-r A where the first term is the smaller or both are equal, else 0;
  *   + kl_coef (1 - exp(b))).
- * An advantage of 0 has no share in the first term whatever r is.  ref_logp may be NULL with kl_coef 0, and is not read then. */
+ * An advantage of 0 has no share in the first term whatever r is.  Where logp is -inf the KL term is infinity less infinity, a NaN.  ref_logp may be NULL with kl_coef 0, and is not read then. */
 int evt_policy_loss(void *stream, const void *scores /* evt_scores */, const void *labels, int32_t label_dtype, const float *old_logp, const float *advantages,
                     const float *ref_logp, const float *weights, double clip_low, double clip_high, double kl_coef, float *loss, float *logp,
                     int32_t flags);

@@ -199,8 +199,8 @@ __device__ __forceinline__ float inverse_sum(MaxSum r) { return r.s == 0.0f ? 0.
 // exp(x) with 32 bits of digits and the exponents of 64
 __device__ __forceinline__ double exp_wide(double x) {
     x = x > 1500.0 ? 1500.0 : x < -1500.0 ? -1500.0 : x; // infinite or 0 either way; a NaN stays
-    const double k = rint(x * 1.4426950408889634);
-    return ldexp((double)expf((float)(x - k * 0.6931471805599453)), (int)k);
+    const int k = x == x ? (int)rint(x * 1.4426950408889634) : 0;
+    return ldexp((double)expf((float)(x - k * 0.6931471805599453)), k);
 }
 // The policy loss of a token and its derivative by logp: -min(r A, clip(r) A) + kl (exp(b) - b - 1), r = exp(logp - old), b = ref - logp.
 // The differences are 64-bit, and the side of the bounds that r is on is found from them: a ratio next to a bound has a whole row's gradient or none.

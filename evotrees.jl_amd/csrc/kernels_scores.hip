@@ -800,7 +800,7 @@ __device__ __forceinline__ Pair pair_loss(const ScoreArgs &a, const PairArgs &q,
     if (r.bad) dh = loss = NAN;
     r.loss = (float)loss;
 #pragma unroll
-    for (int k = 0; k < 2; k++) r.slope[k] = (float)((k ? -dh : dh) * q.beta / len[k]);
+    for (int k = 0; k < 2; k++) r.slope[k] = (float)((k ? -dh : dh) * q.beta / len[k]) + 0.0f; // no -0: most_bits
     return r;
 }
 __device__ __forceinline__ void write_pair(const ScoreArgs &a, const PairArgs &q, int p, const Pair &r) {
@@ -809,7 +809,7 @@ __device__ __forceinline__ void write_pair(const ScoreArgs &a, const PairArgs &q
     for (int k = 0; k < 2; k++) q.seq_logp[p + k * q.pairs] = r.bad ? NAN : (float)r.lp[k];
 }
 // Sequences share rows only where offsets descend somewhere between them.  Such a row has the slope of the most bits, an order that depends neither on which
-// block comes first nor on the form; SC_LOGP left 0, which has none.
+// block comes first nor on the form; a slope of 0, which SC_LOGP left as well, has none.
 __device__ __forceinline__ uint32_t most_bits(uint32_t a, float slope) { return a > __float_as_uint(slope) ? a : __float_as_uint(slope); }
 // One block to a pair, which leaves its slope at every row of the two: by atomics where the offsets descend, or are so many that looking costs more (one block's
 // 500 000 rows: 370 us by atomics, 328 without)

@@ -140,6 +140,26 @@ def test_preference_many_pairs(evt, V, N, pairs, dtype):
         plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))
 
 
+@pytest.mark.parametrize("V,N", [(130, 24), (130, 3000)])
+def test_preference_rows_shared_with_a_pair_without_slope(evt, V, N):
+    """A row takes the gradient of the sequence whose pair has one, not that of a pair of weight 0, on whichever side."""
+    gen = torch.Generator().manual_seed(V + 2)
+    x = torch.randn(N, V, generator=gen)
+    lab = torch.randint(0, V, (N,), generator=gen)
+    off = [0, 2, 4, 6, 8, 14, 11, 18, 20]  # pairs (0, 4), (1, 5), (2, 6), (3, 7); 5 descends, 4 and 6 share rows 11 to 13
+    ref = torch.randn(8, generator=gen) - 20
+    for without in (0, 2):
+        w = torch.ones(4)
+        w[without] = 0.0
+        loss, seq, grad = evt.preference_loss(x.cuda(), lab.cuda(), torch.tensor(off, dtype=torch.int32).cuda(), ref.cuda(), weights=w.cuda())
+        slopes, offs, ok, rows = _pair_slopes(x, lab, off, ref, 0.1)
+        slope, slope_off = torch.zeros(N, dtype=torch.float64), torch.zeros(N, dtype=torch.float64)
+        for k in range(8):
+            if ok[k] and k % 4 != without:
+                slope[off[k]:off[k + 1]], slope_off[off[k]:off[k + 1]] = slopes[k], offs[k]
+        plain.close("grad", grad, *plain.label_grad(rows, lab, slope, 1.0, x.dtype, slope_off))
+
+
 @pytest.mark.parametrize("V,N", [(3, 9), (7, 9), (100, 9), (1500, 300), (3001, 300), (50_021, 9)])  # every form
 @pytest.mark.parametrize("dtype", list(plain.TYPES))
 def test_teacher_scores_that_are_no_numbers(evt, V, N, dtype):

@@ -211,19 +211,20 @@ __device__ __forceinline__ void policy_row(const ScoreArgs &a, int64_t row, floa
     if (adv != 0.0f) {
         const double gap = logp - (double)a.old_logp[row];
         // beyond float's range an advantage or a weight may bring the product back into it
-        const double free = -(fabs(gap) <= 80.0 ? (double)expf((float)gap) : exp_wide(gap)) * adv;
+        double ratio = expf((float)gap);
+        if (__builtin_expect(fabsf((float)gap) > 80.0f, 0)) ratio = exp_wide(gap);
+        const double free = -ratio * adv;
         if (adv > 0.0f ? gap > a.log_hi : adv < 0.0f && gap < a.log_lo) l = -(adv > 0.0f ? a.hi : a.lo) * adv;
         else l = d = free; // a NaN too, of the ratio or the advantage
     }
     if (a.kl != 0.0) {
         const double back = (double)a.ref_logp[row] - logp;
-        const float b = (float)back;
-        double e = expm1f(b), rest;
+        const float b = (float)back, e32 = expm1f(b);
         // e - b cancels where the policies are close: there the series up to b^7 / 7!, the rest of which is under 2^-26 of it
-        if (fabsf(b) < 0.25f) {
-            rest = b * b * (0.5f + b * (1.0f / 6 + b * (1.0f / 24 + b * (1.0f / 120 + b * (1.0f / 720 + b * (1.0f / 5040))))));
-        } else {
-            if (b > 80.0f) e = exp_wide(back);
+        const float r32 = fabsf(b) < 0.25f ? b * b * (0.5f + b * (1.0f / 6 + b * (1.0f / 24 + b * (1.0f / 120 + b * (1.0f / 720 + b * (1.0f / 5040)))))) : e32 - b;
+        double e = e32, rest = r32;
+        if (__builtin_expect(b > 80.0f, 0)) {
+            e = exp_wide(back);
             rest = e - back;
         }
         l += a.kl * rest;

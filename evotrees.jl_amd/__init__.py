@@ -20,10 +20,12 @@ import numpy as np
 from . import _lib
 from ._lib import EvtError, Handle, TreeArrays, make_params, splitmix_mask  # noqa: F401
 from .class_losses import class_logp, class_logp_grad, distill_loss, policy_loss, preference_loss
+from .expert_rows import RowPlan, combine_rows, combine_rows_grad, drop_rows, plan_rows, route_rows, route_rows_grad, sort_rows
 
 __all__ = ["EvoTreeRegressor", "EvoTreeCount", "EvoTreeClassifier", "EvoTreeMLE", "EvoTree", "Tree", "Teacher", "fit", "predict", "predict_leaf_idx", "init",
            "grow_evotree", "update", "okay_to_continue", "get_edges", "get_edges_table", "binarize_table", "check_args", "CallBack", "init_logger", "update_logger", "EvtError",
-           "class_logp", "class_logp_grad", "distill_loss", "policy_loss", "preference_loss"]
+           "class_logp", "class_logp_grad", "distill_loss", "policy_loss", "preference_loss",
+           "RowPlan", "route_rows", "route_rows_grad", "plan_rows", "sort_rows", "combine_rows", "combine_rows_grad", "drop_rows"]
 
 _GPU_DEVICES = ("gpu", "rocm", "amd", "hip")
 _EXP_LINK = ("poisson", "gamma", "tweedie")

@@ -32,6 +32,7 @@ EXPORTS = [
     "evt_lds_atomic_rate", "evt_global_atomic_rate", "evt_trim", "evt_binarize", "evt_bin_columns", "evt_order_stats",
     "evt_model_create", "evt_model_destroy", "evt_model_predict",
     "evt_set_teacher", "evt_class_logp", "evt_class_logp_grad", "evt_distill_loss", "evt_policy_loss", "evt_preference_loss",
+    "evt_route_rows", "evt_route_rows_grad", "evt_plan_rows", "evt_sort_rows", "evt_combine_rows", "evt_combine_rows_grad", "evt_drop_rows",
 ]
 
 
@@ -54,6 +55,12 @@ class EvtTreeOut(C.Structure):
 class EvtScores(C.Structure):
     _fields_ = [("x", C.c_void_p), ("row_stride", C.c_int64), ("grad", C.c_void_p), ("grad_stride", C.c_int64), ("nrows", C.c_int64),
                 ("nclass", C.c_int32), ("dtype", C.c_int32), ("temperature", C.c_double)]
+
+
+class EvtRows(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64), ("residual", C.c_void_p),
+                ("residual_stride", C.c_int64), ("nrows", C.c_int64), ("nfeats", C.c_int32), ("dtype", C.c_int32), ("p", C.c_double), ("seed", C.c_uint64),
+                ("seed_dev", C.c_void_p), ("layer", C.c_uint32)]
 
 
 _lib = None
@@ -129,6 +136,13 @@ def load():
         "evt_distill_loss": [vp, vp, vp, i32, vp, i32, i32, vp, vp, i32],
         "evt_policy_loss": [vp, vp, vp, i32, vp, vp, vp, vp, C.c_double, C.c_double, C.c_double, vp, vp, i32],
         "evt_preference_loss": [vp, vp, vp, i32, vp, i32, vp, vp, C.c_double, C.c_double, C.c_double, i32, vp, vp, vp, i32],
+        "evt_route_rows": [vp, vp, i32, i32, vp, vp, i32],
+        "evt_route_rows_grad": [vp, vp, i32, i32, vp, i32, vp, vp, i32],
+        "evt_plan_rows": [vp, vp, i32, i64, i32, i32, vp, vp, vp, vp, i32],
+        "evt_sort_rows": [vp, vp, vp, vp, i32, i32, i32],
+        "evt_combine_rows": [vp, vp, vp, vp, i32, i32],
+        "evt_combine_rows_grad": [vp, vp, vp, i64, vp, vp, vp, vp, i32, i32, i32],
+        "evt_drop_rows": [vp, vp, i32],
         "evt_predict_static": [vp, i64, i32, vp, vp, i32, i32, i32, i64, vp, vp, vp, vp, vp, i32, vp, vp],
     }
     for name, args in sigs.items():

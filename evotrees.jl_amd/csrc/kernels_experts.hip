@@ -1,0 +1,993 @@
+// Rows through experts: the choice of each row's experts from its class scores, the tables that order rows by expert, rows sorted by them and combined
+// again, dropout, and the gradients of these (formulas: include/evotrees_hip.h).
+//
+// All of it moves bytes: a score, a feature or a table entry is read once and written once, in pieces of sixteen bytes, by groups of lanes that share a row.
+// Products, sums and exponentials are 32-bit, and a value is rounded once, when it is written.
+#include "evt_internal.h"
+#include "pieces.h"
+#include <math.h>
+
+#define MAX_EXPERTS 4096
+#define MAX_TOP 64
+
+// ---- the choice of experts ------------------------------------------------------------------
+
+struct RouteArgs {
+    const void *x;
+    void *g;
+    int64_t xs, gs, N;
+    int32_t V, top, renormalize, id64;
+    float inv_t, exp_mul; // 1 / temperature, log2(e) / temperature
+    int32_t *ids;
+    float *w;
+    const void *ids_in;
+    const float *w_in, *dw;
+};
+
+__device__ __forceinline__ float exp_gap(float x, float m, float mul) { return __builtin_amdgcn_exp2f((x - m) * mul); }
+
+// A score and its class as one number that is the greater the better: the score's bits in an order that is theirs (zeros alike, every NaN above +inf), and
+// below them the class, complemented, so that no two are alike and the lower class is the better of two equal scores.  0: no class, or one that cannot be (-inf).
+// 16-bit scores and a class of 16 bits fit one word, which compares at twice the rate.
+template <typename T>
+struct Key {
+    typedef std::conditional_t<sizeof(T) == 2, uint32_t, uint64_t> type;
+    static __device__ __forceinline__ type of(float x, uint32_t c) {
+        uint32_t b = __float_as_uint(x + 0.0f); // -0 becomes 0
+        b = b & 0x80000000u ? ~b : b | 0x80000000u;
+        b = x != x ? 0xFFFFFFFFu : b;
+        if constexpr (std::is_same<T, half_t>::value) {
+            // the half's own bits
+            uint32_t h = __builtin_bit_cast(uint16_t, (half_t)(x + 0.0f));
+            h = h & 0x8000u ? ~h & 0xFFFFu : h | 0x8000u;
+            b = x != x ? 0xFFFFFFFFu : h << 16;
+        }
+        if constexpr (sizeof(T) == 2) return x == -INFINITY ? 0 : (b & 0xFFFF0000u) | (0xFFFFu - c);
+        else return x == -INFINITY ? 0 : (uint64_t)b << 32 | (0xFFFFu - c);
+    }
+    static __device__ __forceinline__ int chosen(type k) { return k ? (int)(0xFFFFu - (uint32_t)(k & 0xFFFFu)) : -1; }
+    static __device__ __forceinline__ float score(type k) {
+        if constexpr (std::is_same<T, half_t>::value) {
+            uint32_t h = (uint32_t)k >> 16;
+            h = h & 0x8000u ? h & 0x7FFFu : ~h & 0xFFFFu;
+            return k ? (float)__builtin_bit_cast(half_t, (uint16_t)h) : -INFINITY;
+        } else {
+            uint32_t b = sizeof(T) == 2 ? (uint32_t)k & 0xFFFF0000u : (uint32_t)((uint64_t)k >> 32);
+            b = b & 0x80000000u ? b & 0x7FFFFFFFu : sizeof(T) == 2 ? ~b & 0xFFFF0000u : ~b;
+            return k ? __uint_as_float(b) : -INFINITY;
+        }
+    }
+};
+
+template <int G>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
+    return __float_as_uint(over_lanes<G>(__uint_as_float(v), [](float a, float b) {
+        const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+        return __uint_as_float(x > y ? x : y);
+    }));
+}
+template <int G>
+__device__ __forceinline__ uint64_t lanes_max(uint64_t v) {
+    const uint32_t hi = (uint32_t)(v >> 32), most = lanes_max<G>(hi);
+    return (uint64_t)most << 32 | lanes_max<G>(hi == most ? (uint32_t)v : 0u);
+}
+
+// The greater one first
+template <typename K>
+__device__ __forceinline__ void order(K &a, K &b) {
+    const bool less = a < b;
+    const K x = less ? b : a, y = less ? a : b;
+    a = x;
+    b = y;
+}
+// Batcher's odd-even merge sort of n values, descending
+template <int N, typename K>
+__device__ __forceinline__ void sort_values(K *v) {
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; i++)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(v[i + j], v[i + j + k]);
+}
+
+// A row to G lanes of a wavefront, NV pieces a lane.  A lane sorts what it has; the best of a row is then the best of its lanes' first ones, and the lane that had it moves up.
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(256) void k_route(RouteArgs a) {
+    constexpr int E = Piece<T>::E, N = E * NV, ROWS = 256 / G;
+    typedef typename Key<T>::type K;
+    extern __shared__ __align__(16) unsigned char s_dyn[]; // [ROWS][top] keys
+    const int rank = threadIdx.x & (G - 1), slot = threadIdx.x / G, V = a.V;
+    K *const s_best = (K *)s_dyn + slot * a.top;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + slot; row < a.N; row += (int64_t)gridDim.x * ROWS) {
+        const T *x = (const T *)a.x + row * a.xs;
+        Piece<T> p[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (rank + i * G) * E;
+            p[i].r = {};
+            if (c + E <= V) p[i].load(x + c);
+            else if (c < V) p[i].load_some(x + c, V - c);
+        }
+        K v[N];
+        float f[N];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            p[i].get(f + i * E);
+#pragma unroll
+            for (int k = 0; k < E; k++) {
+                const int c = (rank + i * G) * E + k;
+                if (c >= V) f[i * E + k] = -INFINITY;
+                v[i * E + k] = Key<T>::of(f[i * E + k], c);
+            }
+        }
+        sort_values<N>(v);
+        float most = 0.0f, total = 0.0f;
+        for (int j = 0; j < a.top; j++) {
+            const K best = lanes_max<G>(v[0]);
+            const float score = Key<T>::score(best);
+            if (j == 0) most = score;
+            total += best ? exp_gap(score, most, a.exp_mul) : 0.0f;
+            if (rank == 0) s_best[j] = best;
+            if (v[0] == best) {
+#pragma unroll
+                for (int i = 0; i + 1 < N; i++) v[i] = v[i + 1];
+                v[N - 1] = 0;
+            }
+        }
+        if (!a.renormalize) {
+            total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < N; i++) total += f[i] == -INFINITY ? 0.0f : exp_gap(f[i], most, a.exp_mul);
+            total = lanes_sum<G>(total);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const float inv = 1.0f / total;
+        for (int j = rank; j < a.top; j += G) {
+            const K best = s_best[j];
+            a.ids[row * a.top + j] = Key<T>::chosen(best);
+            a.w[row * a.top + j] = best ? exp_gap(Key<T>::score(best), most, a.exp_mul) * inv : 0.0f;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The gradient of the weights: a row to G lanes.  What the chosen classes have is put together in shared memory.
+template <typename T, int G, int NV>
+__global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
+    constexpr int E = Piece<T>::E, ROWS = 256 / G, ROW = G * NV * E;
+    extern __shared__ __align__(16) float s_rows[]; // [ROWS][ROW]
+    const int rank = threadIdx.x & (G - 1), slot = threadIdx.x / G, V = a.V;
+    float *const s = s_rows + slot * ROW;
+    for (int64_t row = (int64_t)blockIdx.x * ROWS + slot; row < a.N; row += (int64_t)gridDim.x * ROWS) {
+        Piece<T> p[NV];
+        if (!a.renormalize) {
+            const T *x = (const T *)a.x + row * a.xs;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int c = (rank + i * G) * E;
+                p[i].r = {};
+                if (c + E <= V) p[i].load(x + c);
+                else if (c < V) p[i].load_some(x + c, V - c);
+            }
+        }
+        float mean = 0.0f;
+        bool none = false; // an id of no class
+        for (int j = rank; j < a.top; j += G) {
+            const int64_t at = row * a.top + j, id = a.id64 ? ((const int64_t *)a.ids_in)[at] : ((const int32_t *)a.ids_in)[at];
+            none |= id >= V;
+            if (id >= 0) mean += a.w_in[at] * a.dw[at];
+        }
+        mean = lanes_sum<G>(none ? NAN : mean);
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int k = 0; k < E; k += 4) *(float4 *)(s + (rank + i * G) * E + k) = {0.0f, 0.0f, 0.0f, 0.0f};
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        for (int j = rank; j < a.top; j += G) {
+            const int64_t at = row * a.top + j, id = a.id64 ? ((const int64_t *)a.ids_in)[at] : ((const int32_t *)a.ids_in)[at];
+            if (id >= 0 && id < V) atomicAdd(s + id, a.renormalize ? a.w_in[at] * (a.dw[at] - mean) : a.w_in[at] * a.dw[at]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float f[NV * E], m = -INFINITY, total = 0.0f;
+        if (!a.renormalize) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                p[i].get(f + i * E);
+#pragma unroll
+                for (int k = 0; k < E; k++) {
+                    if ((rank + i * G) * E + k >= V) f[i * E + k] = -INFINITY;
+                    m = fmaxf(m, f[i * E + k]);
+                }
+            }
+            m = over_lanes<G>(m, [](float u, float v) { return fmaxf(u, v); });
+#pragma unroll
+            for (int i = 0; i < NV * E; i++) {
+                f[i] = f[i] == -INFINITY ? 0.0f : exp_gap(f[i], m, a.exp_mul);
+                total += f[i];
+            }
+            total = lanes_sum<G>(total);
+        }
+        const float factor = total == 0.0f ? 0.0f : -mean / total;
+        T *g = (T *)a.g + row * a.gs;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (rank + i * G) * E;
+            if (c < V) {
+                float o[E];
+#pragma unroll
+                for (int k = 0; k < E; k++) {
+                    o[k] = s[c + k];
+                    if (!a.renormalize) o[k] += f[i * E + k] * factor;
+                    o[k] *= a.inv_t;
+                    if (mean != mean) o[k] = NAN;
+                }
+                Piece<T> q;
+                q.set(o);
+                if (c + E <= V) q.store(g + c, false);
+                else q.store_some(g + c, V - c);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- the tables of rows by expert ------------------------------------------------------------
+
+struct PlanArgs {
+    const void *ids;
+    int64_t n; // rows x top
+    int32_t id64, E, bits, nb;
+    int32_t *place, *source, *offsets, *table;
+};
+#define PLAN_ITEMS 16
+#define PLAN_CHUNK (256 * PLAN_ITEMS) // entries of a block
+
+__device__ __forceinline__ int expert_of(const PlanArgs &a, int64_t i) {
+    if (i >= a.n) return -1;
+    const int64_t id = a.id64 ? ((const int64_t *)a.ids)[i] : ((const int32_t *)a.ids)[i];
+    return id >= 0 && id < a.E ? (int)id : -1;
+}
+
+// How many entries of each block's an expert has: table[block][expert], or [expert][block] for many blocks
+__global__ __launch_bounds__(256) void k_plan_count(PlanArgs a, int by_expert) {
+    __shared__ int s_n[MAX_EXPERTS];
+    for (int e = threadIdx.x; e < a.E; e += 256) s_n[e] = 0;
+    __syncthreads();
+    const int64_t first = (int64_t)blockIdx.x * PLAN_CHUNK + threadIdx.x;
+    int id[PLAN_ITEMS];
+#pragma unroll
+    for (int i = 0; i < PLAN_ITEMS; i++) id[i] = expert_of(a, first + i * 256);
+#pragma unroll
+    for (int i = 0; i < PLAN_ITEMS; i++)
+        if (id[i] >= 0) atomicAdd(s_n + id[i], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += 256) a.table[by_expert ? (int64_t)e * a.nb + blockIdx.x : (int64_t)blockIdx.x * a.E + e] = s_n[e];
+}
+
+// The block's exclusive sum over its threads' values, and all of it
+template <int W>
+__device__ __forceinline__ int block_exclusive(int v, int &all) {
+    __shared__ int s_w[W];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int sum = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int u = __shfl_up(sum, d);
+        if (lane >= d) sum += u;
+    }
+    if (lane == 63) s_w[wave] = sum;
+    __syncthreads();
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        if (w < wave) before += s_w[w];
+        all += s_w[w];
+    }
+    __syncthreads();
+    return before + sum - v;
+}
+
+// Each expert's counts become what the blocks before have, the expert's total goes behind the table: a block to an expert
+__global__ __launch_bounds__(256) void k_plan_sums(PlanArgs a) {
+    int32_t *t = a.table + (int64_t)blockIdx.x * a.nb;
+    int carry = 0;
+    for (int b0 = 0; b0 < a.nb; b0 += 256 * 8) {
+        int v[8], sum = 0, all;
+        const int b = b0 + (int)threadIdx.x * 8;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[i] = b + i < a.nb ? t[b + i] : 0;
+            sum += v[i];
+        }
+        int at = carry + block_exclusive<4>(sum, all);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (b + i < a.nb) t[b + i] = at;
+            at += v[i];
+        }
+        carry += all;
+    }
+    if (threadIdx.x == 0) a.table[(int64_t)a.E * a.nb + blockIdx.x] = carry;
+}
+
+// Where the counts before a block come from
+enum { PLAN_ALONE, PLAN_BLOCKS, PLAN_SUMS };
+
+// Every entry's place: the experts before its own, its expert's entries of the blocks before, of the wavefronts before, and of the lanes before, found by
+// comparing the experts' bits over the wavefront.  Each wavefront has consecutive entries, so that an expert's keep their order.
+template <int W, int ITEMS, int FROM>
+__global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
+    constexpr int THREADS = 64 * W;
+    extern __shared__ __align__(16) int s_plan[]; // [E] where the block's entries of an expert start, then [W / 2][E] pairs of wavefronts' counts
+    int *const s_base = s_plan;
+    uint16_t *const s_wave = (uint16_t *)(s_plan + a.E);
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), E = a.E;
+    for (int e = threadIdx.x; e < E * (W / 2); e += THREADS) s_plan[E + e] = 0;
+    const int64_t first = ((int64_t)blockIdx.x * W + wave) * (64 * ITEMS) + lane;
+    int id[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) id[i] = expert_of(a, first + i * 64);
+    __syncthreads();
+    const auto half = [&](int e) { return ((wave >> 1) * E + e) * 2 + (wave & 1); };
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++)
+        if (id[i] >= 0) atomicAdd(s_plan + E + (wave >> 1) * E + id[i], 1 << (16 * (wave & 1)));
+    __syncthreads();
+    // an expert's start: the threads have consecutive experts
+    const int per = (E + THREADS - 1) / THREADS, e0 = threadIdx.x * per, e1 = e0 + per < E ? e0 + per : E;
+    int sum = 0, all;
+    for (int e = e0; e < e1; e++) {
+        int total = 0, before = 0, mine = 0;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            uint16_t &c = s_wave[((w >> 1) * E + e) * 2 + (w & 1)];
+            const int n = c;
+            c = (uint16_t)mine;
+            mine += n;
+        }
+        if (FROM == PLAN_ALONE) total = mine;
+        else if (FROM == PLAN_SUMS) {
+            total = a.table[(int64_t)E * a.nb + e];
+            before = a.table[(int64_t)e * a.nb + blockIdx.x];
+        } else {
+            for (int b = 0; b < a.nb; b++) {
+                const int n = a.table[(int64_t)b * E + e];
+                if (b < (int)blockIdx.x) before += n;
+                total += n;
+            }
+        }
+        s_base[e] = sum + before;
+        if (blockIdx.x == 0) a.offsets[e] = sum;
+        sum += total;
+    }
+    const int start = block_exclusive<W>(sum, all);
+    for (int e = e0; e < e1; e++) {
+        s_base[e] += start;
+        if (blockIdx.x == 0) a.offsets[e] += start;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[E] = all;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const int e = id[i];
+        uint64_t same = __ballot(e >= 0);
+        for (int b = 0; b < a.bits; b++) {
+            const bool set = (e >> b) & 1;
+            const uint64_t with = __ballot(set);
+            same &= set ? with : ~with;
+        }
+        const int64_t at = first + i * 64;
+        int pos = -1;
+        if (e >= 0) {
+            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
+            volatile uint16_t *c = s_wave + half(e);
+            const int n = *c + before;
+            pos = s_base[e] + n;
+            __builtin_amdgcn_wave_barrier();
+            if ((same >> lane) == 1) *c = (uint16_t)(n + 1); // the last of them
+            if (pos < a.n) a.source[pos] = (int)at; // always, unless somebody writes the ids meanwhile
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (at < a.n) a.place[at] = pos;
+    }
+    // behind the last
+    for (int64_t p = all + (int64_t)blockIdx.x * THREADS + threadIdx.x; p < a.n; p += (int64_t)gridDim.x * THREADS) a.source[p] = -1;
+}
+
+// ---- rows ------------------------------------------------------------------------------------
+
+struct RowArgs {
+    const void *x, *res, *y;
+    void *out;
+    int64_t xs, rs, ys, os; // elements from row to row
+    int64_t N, n;           // rows; sorted rows, rows x top
+    int32_t H, top, pieces, chunk; // pieces of a row, and of a block's part of it
+    int32_t parts;
+    const int32_t *place, *count;
+    const float *w;
+    float *dw;
+    // dropout: an element is dropped whose 32 bits are below this
+    uint32_t drop, layer;
+    float scale;
+    const uint64_t *seed_at; // nullptr: seed
+    uint64_t seed;
+};
+
+#define TAIL_BLOCKS 64
+#define GAMMA 0x9E3779B97F4A7C15ull
+__device__ __forceinline__ uint64_t mixed(uint64_t z) {
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+// Dropout of a row's pieces, whose bits come from SplitMix64 (Steele, Lea, Flood 2014), as a row sample's do: nothing is stored, the gradient draws them again.
+// Four values have the sixteen-bit quarters of one output, which decide unless one of them is just the threshold's upper half: one in 65 536, whose lower
+// half is drawn then.
+struct Drop {
+    uint64_t key, base;
+    uint32_t words;
+    __device__ __forceinline__ Drop(const RowArgs &a) {
+        key = mixed((a.seed_at ? *a.seed_at : a.seed) + (uint64_t)(a.layer + 1ull) * GAMMA);
+        words = ((uint32_t)a.H + 3) / 4;
+    }
+    __device__ __forceinline__ void row(int64_t r) { base = ((uint64_t)r * words + 1) * GAMMA; }
+    template <int E>
+    __device__ __forceinline__ void apply(const RowArgs &a, int v, float *f) const {
+        const uint32_t hi = a.drop >> 16, lo = a.drop & 0xFFFFu;
+#pragma unroll
+        for (int q = 0; q < E / 4; q++) {
+            const uint64_t at = base + (uint64_t)(uint32_t)(v * (E / 4) + q) * GAMMA;
+            const uint64_t word = mixed(key + at);
+            const uint32_t half[2] = {(uint32_t)word, (uint32_t)(word >> 32)};
+            bool tie = false;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t bits = (half[k / 2] >> (16 * (k & 1))) & 0xFFFFu;
+                tie |= bits == hi;
+                f[4 * q + k] = bits < hi ? 0.0f : f[4 * q + k] * a.scale;
+            }
+            if (__builtin_expect(lo != 0 && tie, 0)) {
+                const uint64_t second = mixed(~key + at);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    if (((word >> (16 * k)) & 0xFFFF) == hi && ((second >> (16 * k)) & 0xFFFF) < lo) f[4 * q + k] = 0.0f;
+            }
+        }
+    }
+};
+
+// The row and part of it that a group of G threads has
+template <int G>
+struct Share {
+    static constexpr int ROWS = 256 / G;
+    int64_t row;
+    int part, rank;
+    __device__ __forceinline__ Share(const RowArgs &a, int64_t block) {
+        const int64_t group = a.parts == 1 ? block : block / a.parts;
+        part = a.parts == 1 ? 0 : (int)(block - group * a.parts);
+        rank = threadIdx.x & (G - 1);
+        row = group * ROWS + (G >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, int v, int H) {
+    constexpr int E = Piece<T>::E;
+    if ((v + 1) * E <= H) p.load(x + (size_t)v * E);
+    else p.load_some(x + (size_t)v * E, H - v * E);
+}
+template <typename T>
+__device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, int v, int H) {
+    constexpr int E = Piece<T>::E;
+    if ((v + 1) * E <= H) p.store(x + (size_t)v * E, false);
+    else p.store_some(x + (size_t)v * E, H - v * E);
+}
+
+// Rows to their places: each row is read once and written `top` times, times a weight if there are weights.  DOT: and the sums of its products with the rows that
+// lie at these places in y.
+template <typename T, int G, bool DROP, bool DOT>
+__global__ __launch_bounds__(256) void k_spread(RowArgs a, int64_t blocks) {
+    constexpr int E = Piece<T>::E, TOP = 8;
+    __shared__ float s_dot[4][TOP];
+    const Drop drop_of(a);
+    // behind the last of the sorted rows: the grid's last blocks
+    if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
+        const int count = *a.count;
+        for (int64_t p = (int64_t)(count < 0 ? 0 : count) + (blockIdx.x - (gridDim.x - TAIL_BLOCKS)); p < a.n; p += TAIL_BLOCKS)
+            for (int v = threadIdx.x; v < a.pieces; v += 256) {
+                Piece<T> z;
+                z.r = {};
+                store_piece(z, (T *)a.out + p * a.os, v, a.H);
+            }
+        return;
+    }
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x - TAIL_BLOCKS) {
+        const Share<G> me(a, block);
+        const bool in = me.row < a.N;
+        Drop drop = drop_of;
+        if (DROP) drop.row(me.row);
+        const T *x = (const T *)a.x + me.row * a.xs;
+        const int v1 = me.part * a.chunk + a.chunk < a.pieces ? me.part * a.chunk + a.chunk : a.pieces;
+        for (int j0 = 0; j0 < a.top; j0 += TOP) {
+            int at[TOP];
+            float w[TOP], dot[TOP];
+#pragma unroll
+            for (int j = 0; j < TOP; j++) {
+                at[j] = in && j0 + j < a.top ? a.place[me.row * a.top + j0 + j] : -1;
+                w[j] = a.w && in && j0 + j < a.top ? a.w[me.row * a.top + j0 + j] : 1.0f;
+                dot[j] = 0.0f;
+                if ((uint32_t)at[j] >= (uint64_t)a.n) at[j] = -1;
+            }
+            if (in)
+                for (int v = me.part * a.chunk + me.rank; v < v1; v += G) {
+                    Piece<T> p, q[TOP];
+                    float f[E];
+                    load_piece(p, x, v, a.H);
+                    if (DOT) {
+#pragma unroll
+                        for (int j = 0; j < TOP; j++)
+                            if (at[j] >= 0) load_piece(q[j], (const T *)a.y + at[j] * a.ys, v, a.H);
+                    }
+                    p.get(f);
+                    if (DROP) drop.template apply<E>(a, v, f);
+#pragma unroll
+                    for (int j = 0; j < TOP; j++)
+                        if (at[j] >= 0) {
+                            if (DROP || a.w) {
+                                float g[E];
+#pragma unroll
+                                for (int k = 0; k < E; k++) g[k] = f[k] * w[j];
+                                p.set(g);
+                            }
+                            store_piece(p, (T *)a.out + at[j] * a.os, v, a.H);
+                            if (DOT) {
+                                float g[E];
+                                q[j].get(g);
+                                float sum = 0.0f;
+#pragma unroll
+                                for (int k = 0; k < E; k++) sum += f[k] * g[k];
+                                dot[j] += sum;
+                            }
+                        }
+                }
+            if (DOT) {
+#pragma unroll
+                for (int j = 0; j < TOP; j++) dot[j] = lanes_sum<(G < 64 ? G : 64)>(dot[j]);
+                if (G > 64) {
+                    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+                        for (int j = 0; j < TOP; j++) s_dot[threadIdx.x >> 6][j] = dot[j];
+                    __syncthreads();
+#pragma unroll
+                    for (int j = 0; j < TOP; j++) dot[j] = (s_dot[0][j] + s_dot[1][j]) + (s_dot[2][j] + s_dot[3][j]);
+                    __syncthreads();
+                }
+                if (in && me.rank == 0)
+#pragma unroll
+                    for (int j = 0; j < TOP; j++)
+                        if (j0 + j < a.top) a.dw[me.row * a.top + j0 + j] = at[j] >= 0 ? dot[j] : 0.0f;
+            }
+        }
+    }
+}
+
+// Every row's sum over its places, times the weights if there are any, with dropout and a residual
+template <typename T, int G, bool DROP>
+__global__ __launch_bounds__(256) void k_combine(RowArgs a, int64_t blocks) {
+    constexpr int E = Piece<T>::E, TOP = 8;
+    const Drop drop_of(a);
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const Share<G> me(a, block);
+        if (me.row >= a.N) continue;
+        Drop drop = drop_of;
+        if (DROP) drop.row(me.row);
+        const int v1 = me.part * a.chunk + a.chunk < a.pieces ? me.part * a.chunk + a.chunk : a.pieces;
+        for (int v = me.part * a.chunk + me.rank; v < v1; v += G) {
+            Piece<T> res;
+            float sum[E] = {};
+            if (a.res) load_piece(res, (const T *)a.res + me.row * a.rs, v, a.H);
+            for (int j0 = 0; j0 < a.top; j0 += TOP) {
+                int at[TOP];
+                Piece<T> p[TOP];
+#pragma unroll
+                for (int j = 0; j < TOP; j++) {
+                    at[j] = j0 + j < a.top ? a.place[me.row * a.top + j0 + j] : -1;
+                    if ((uint32_t)at[j] >= (uint64_t)a.n) at[j] = -1;
+                    if (at[j] >= 0) load_piece(p[j], (const T *)a.y + at[j] * a.ys, v, a.H);
+                }
+#pragma unroll
+                for (int j = 0; j < TOP; j++)
+                    if (at[j] >= 0) {
+                        const float w = a.w ? a.w[me.row * a.top + j0 + j] : 1.0f;
+                        float f[E];
+                        p[j].get(f);
+#pragma unroll
+                        for (int k = 0; k < E; k++) sum[k] += w * f[k];
+                    }
+            }
+            if (DROP) drop.template apply<E>(a, v, sum);
+            if (a.res) {
+                float f[E];
+                res.get(f);
+#pragma unroll
+                for (int k = 0; k < E; k++) sum[k] += f[k];
+            }
+            Piece<T> o;
+            o.set(sum);
+            store_piece(o, (T *)a.out + me.row * a.os, v, a.H);
+        }
+    }
+}
+
+template <typename T, int G>
+__global__ __launch_bounds__(256) void k_drop(RowArgs a, int64_t blocks) {
+    constexpr int E = Piece<T>::E;
+    const Drop drop_of(a);
+    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
+        const Share<G> me(a, block);
+        if (me.row >= a.N) continue;
+        Drop drop = drop_of;
+        drop.row(me.row);
+        const int v1 = me.part * a.chunk + a.chunk < a.pieces ? me.part * a.chunk + a.chunk : a.pieces;
+        for (int v = me.part * a.chunk + me.rank; v < v1; v += G) {
+            Piece<T> p, res;
+            float f[E];
+            load_piece(p, (const T *)a.x + me.row * a.xs, v, a.H);
+            if (a.res) load_piece(res, (const T *)a.res + me.row * a.rs, v, a.H);
+            p.get(f);
+            if (a.drop) drop.template apply<E>(a, v, f);
+            if (a.res) {
+                float g[E];
+                res.get(g);
+#pragma unroll
+                for (int k = 0; k < E; k++) f[k] += g[k];
+            }
+            p.set(f);
+            store_piece(p, (T *)a.out + me.row * a.os, v, a.H);
+        }
+    }
+}
+
+// ---- launches --------------------------------------------------------------------------------
+
+// Lanes that share a row: enough for sixteen scores each, all of a wavefront from 1024 scores on
+template <typename T, int G, int NV, bool GRAD>
+static void launch_route_as(hipStream_t s, const RouteArgs &a) {
+    constexpr int ROWS = 256 / G;
+    const int64_t blocks = (a.N + ROWS - 1) / ROWS;
+    const dim3 grid((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22));
+    if constexpr (GRAD) hipLaunchKernelGGL((k_route_grad<T, G, NV>), grid, dim3(256), ROWS * G * NV * Piece<T>::E * 4, s, a);
+    else hipLaunchKernelGGL((k_route<T, G, NV>), grid, dim3(256), ROWS * a.top * sizeof(typename Key<T>::type), s, a);
+}
+template <typename T, bool GRAD>
+static void launch_route_typed(hipStream_t s, const RouteArgs &a) {
+    constexpr int U = 16 / Piece<T>::E;
+    const int n = (a.V + 15) / 16; // lanes
+    if (n <= 1) launch_route_as<T, 1, U, GRAD>(s, a);
+    else if (n <= 2) launch_route_as<T, 2, U, GRAD>(s, a);
+    else if (n <= 4) launch_route_as<T, 4, U, GRAD>(s, a);
+    else if (n <= 8) launch_route_as<T, 8, U, GRAD>(s, a);
+    else if (n <= 16) launch_route_as<T, 16, U, GRAD>(s, a);
+    else if (n <= 32) launch_route_as<T, 32, U, GRAD>(s, a);
+    else if (n <= 64) launch_route_as<T, 64, U, GRAD>(s, a);
+    else if (n <= 128) launch_route_as<T, 64, 2 * U, GRAD>(s, a);
+    else launch_route_as<T, 64, 4 * U, GRAD>(s, a);
+}
+template <bool GRAD>
+static int launch_route(hipStream_t s, const RouteArgs &a, int dtype) {
+    if (dtype == EVT_F32) launch_route_typed<float, GRAD>(s, a);
+    else if (dtype == EVT_BF16) launch_route_typed<bf16_t, GRAD>(s, a);
+    else launch_route_typed<half_t, GRAD>(s, a);
+    HIPCHK(hipGetLastError());
+    return EVT_OK;
+}
+
+enum { ROWS_SPREAD, ROWS_COMBINE, ROWS_DROP };
+template <typename T, int G, int OP>
+static void launch_rows_as(hipStream_t s, const RowArgs &a) {
+    const int64_t blocks = (a.N + 256 / G - 1) / (256 / G) * a.parts;
+    const int64_t most = 1 << 22;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, G>), dim3(grid), dim3(256), 0, s, a, blocks);
+    else if constexpr (OP == ROWS_COMBINE) {
+        if (a.drop) hipLaunchKernelGGL((k_combine<T, G, true>), dim3(grid), dim3(256), 0, s, a, blocks);
+        else hipLaunchKernelGGL((k_combine<T, G, false>), dim3(grid), dim3(256), 0, s, a, blocks);
+    } else {
+        if (a.dw) {
+            if (a.drop) hipLaunchKernelGGL((k_spread<T, G, true, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
+            else hipLaunchKernelGGL((k_spread<T, G, false, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
+        } else {
+            if (a.drop) hipLaunchKernelGGL((k_spread<T, G, true, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
+            else hipLaunchKernelGGL((k_spread<T, G, false, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
+        }
+    }
+}
+template <typename T, int OP>
+static void launch_rows_typed(hipStream_t s, RowArgs &a) {
+    a.pieces = (a.H + Piece<T>::E - 1) / Piece<T>::E;
+    a.chunk = OP == ROWS_SPREAD && a.dw ? a.pieces : 256;
+    a.parts = (a.pieces + a.chunk - 1) / a.chunk;
+    if (a.pieces <= 1) launch_rows_as<T, 1, OP>(s, a);
+    else if (a.pieces <= 2) launch_rows_as<T, 2, OP>(s, a);
+    else if (a.pieces <= 4) launch_rows_as<T, 4, OP>(s, a);
+    else if (a.pieces <= 8) launch_rows_as<T, 8, OP>(s, a);
+    else if (a.pieces <= 16) launch_rows_as<T, 16, OP>(s, a);
+    else if (a.pieces <= 32) launch_rows_as<T, 32, OP>(s, a);
+    else if (a.pieces <= 128) launch_rows_as<T, 64, OP>(s, a);
+    else launch_rows_as<T, 256, OP>(s, a);
+}
+template <int OP>
+static int launch_rows(hipStream_t s, RowArgs &a, int dtype) {
+    if (dtype == EVT_F32) launch_rows_typed<float, OP>(s, a);
+    else if (dtype == EVT_BF16) launch_rows_typed<bf16_t, OP>(s, a);
+    else launch_rows_typed<half_t, OP>(s, a);
+    HIPCHK(hipGetLastError());
+    return EVT_OK;
+}
+
+static void launch_plan(hipStream_t s, PlanArgs &a) {
+    a.bits = 0;
+    while ((1 << a.bits) < a.E) a.bits++;
+    if (a.n <= 8192 && a.E <= 1024) {
+        a.nb = 1;
+        hipLaunchKernelGGL((k_plan_place<16, 8, PLAN_ALONE>), dim3(1), dim3(1024), a.E * 4 * 9, s, a);
+        return;
+    }
+    a.nb = (int)((a.n + PLAN_CHUNK - 1) / PLAN_CHUNK);
+    if (a.nb <= 1) {
+        hipLaunchKernelGGL((k_plan_place<4, PLAN_ITEMS, PLAN_ALONE>), dim3(1), dim3(256), a.E * 4 * 3, s, a);
+        return;
+    }
+    const bool few = a.nb <= 32;
+    hipLaunchKernelGGL(k_plan_count, dim3(a.nb), dim3(256), 0, s, a, few ? 0 : 1);
+    if (few) {
+        hipLaunchKernelGGL((k_plan_place<4, PLAN_ITEMS, PLAN_BLOCKS>), dim3(a.nb), dim3(256), a.E * 4 * 3, s, a);
+        return;
+    }
+    hipLaunchKernelGGL(k_plan_sums, dim3(a.E), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_plan_place<4, PLAN_ITEMS, PLAN_SUMS>), dim3(a.nb), dim3(256), a.E * 4 * 3, s, a);
+}
+
+// ---- entry points ------------------------------------------------------------------------------
+static bool on_device(const void *p) {
+    hipPointerAttribute_t attr;
+    const bool ok = hipPointerGetAttributes(&attr, p) == hipSuccess && attr.type == hipMemoryTypeDevice;
+    (void)hipGetLastError();
+    return ok;
+}
+template <typename... P>
+static int check_device(int32_t flags, P... ptrs) {
+    if (flags & EVT_STATIC_TRUSTED) return EVT_OK;
+    const void *all[] = {(const void *)ptrs...};
+    for (const void *p : all) ARGCHK(!p || on_device(p), "rows through experts take device memory only");
+    return EVT_OK;
+}
+#define TRY(call)                        \
+    do {                                 \
+        const int _r = (call);           \
+        if (_r != EVT_OK) return _r;     \
+    } while (0)
+
+static int check_flags(int32_t flags) {
+    ARGCHK(flags == 0 || flags == EVT_STATIC_TRUSTED, "flags takes 0 or EVT_STATIC_TRUSTED");
+    return EVT_OK;
+}
+static int size_of(int32_t dtype) { return dtype == EVT_F32 ? 4 : 2; }
+struct Extent {
+    const void *p;
+    int64_t stride, rows;
+};
+// A matrix's memory and another's have no byte in common
+static bool apart(Extent a, Extent b, int64_t width, int size) {
+    if (!a.p || !b.p || !a.rows || !b.rows) return true;
+    const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
+    const uintptr_t a1 = a0 + ((a.rows - 1) * a.stride + width) * size, b1 = b0 + ((b.rows - 1) * b.stride + width) * size;
+    return a1 <= b0 || b1 <= a0;
+}
+static bool same(Extent a, Extent b) { return a.p == b.p && (a.rows <= 1 || a.stride == b.stride); }
+
+static int take_route(const evt_scores *s, int32_t top, int32_t renormalize, int32_t flags, RouteArgs &a) {
+    ARGCHK(s, "scores must not be NULL");
+    TRY(check_flags(flags));
+    ARGCHK(s->dtype == EVT_F32 || s->dtype == EVT_BF16 || s->dtype == EVT_F16, "scores must be EVT_F32, EVT_BF16 or EVT_F16");
+    ARGCHK(s->nrows >= 0 && s->nrows <= INT32_MAX && s->nclass >= 1 && s->nclass <= MAX_EXPERTS, "nrows must be in [0, 2^31 - 1], nclass in [1, 4096]");
+    ARGCHK(top >= 1 && top <= MAX_TOP && top <= s->nclass, "top must be in [1, 64] and at most nclass");
+    ARGCHK(renormalize == 0 || renormalize == 1, "renormalize takes 0 or 1");
+    ARGCHK(s->temperature >= 1e-4 && s->temperature <= 1e4, "temperature must be in [1e-4, 1e4]");
+    ARGCHK(s->row_stride >= 0, "row_stride must not be negative");
+    a.N = s->nrows;
+    a.V = s->nclass;
+    a.top = top;
+    a.renormalize = renormalize;
+    a.x = s->x;
+    a.xs = s->row_stride;
+    a.inv_t = (float)(1.0 / s->temperature);
+    a.exp_mul = (float)(1.4426950408889634 / s->temperature);
+    if (a.N) ARGCHK(s->x && (uintptr_t)s->x % size_of(s->dtype) == 0, "scores must not be NULL and be aligned to their type");
+    return EVT_OK;
+}
+
+extern "C" int evt_route_rows(void *stream, const void *scores, int32_t top, int32_t renormalize, int32_t *experts, float *weights, int32_t flags) {
+    return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
+    RouteArgs a = {};
+    TRY(take_route(s, top, renormalize, flags, a));
+    if (a.N == 0) return EVT_OK;
+    ARGCHK(experts && weights, "experts and weights must not be NULL");
+    TRY(check_device(flags, s->x, experts, weights));
+    a.ids = experts;
+    a.w = weights;
+    return launch_route<false>((hipStream_t)stream, a, s->dtype);
+    });
+}
+
+extern "C" int evt_route_rows_grad(void *stream, const void *scores, int32_t top, int32_t renormalize, const void *experts, int32_t id_dtype,
+                                   const float *weights, const float *dweights, int32_t flags) {
+    return guarded([&]() -> int {
+    const evt_scores *const s = static_cast<const evt_scores *>(scores);
+    RouteArgs a = {};
+    TRY(take_route(s, top, renormalize, flags, a));
+    ARGCHK(id_dtype == EVT_I32 || id_dtype == EVT_I64, "experts must be EVT_I32 or EVT_I64");
+    if (a.N == 0) return EVT_OK;
+    const int size = size_of(s->dtype);
+    ARGCHK(experts && weights && dweights && s->grad, "experts, weights, dweights and grad must not be NULL");
+    ARGCHK((uintptr_t)s->grad % size == 0, "gradients must be aligned to their type");
+    ARGCHK(a.N == 1 || s->grad_stride >= s->nclass, "grad_stride must be at least nclass");
+    const Extent x = {s->x, s->row_stride, a.N}, g = {s->grad, s->grad_stride, a.N};
+    ARGCHK(same(x, g) || apart(x, g, a.V, size), "grad must be the scores' own memory, row for row, or lie apart from them");
+    TRY(check_device(flags, s->x, s->grad, experts, weights, dweights));
+    a.g = s->grad;
+    a.gs = s->grad_stride;
+    a.ids_in = experts;
+    a.id64 = id_dtype == EVT_I64;
+    a.w_in = weights;
+    a.dw = dweights;
+    return launch_route<true>((hipStream_t)stream, a, s->dtype);
+    });
+}
+
+extern "C" int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype, int64_t nrows, int32_t top, int32_t nexperts, int32_t *place, int32_t *source,
+                             int32_t *offsets, int32_t *work, int32_t flags) {
+    return guarded([&]() -> int {
+    TRY(check_flags(flags));
+    ARGCHK(id_dtype == EVT_I32 || id_dtype == EVT_I64, "experts must be EVT_I32 or EVT_I64");
+    ARGCHK(nexperts >= 1 && nexperts <= MAX_EXPERTS, "nexperts must be in [1, 4096]");
+    ARGCHK(top >= 1 && nrows >= 0 && nrows <= INT32_MAX / top, "top must be at least 1, nrows * top in [0, 2^31 - 1]");
+    ARGCHK(offsets, "offsets must not be NULL");
+    PlanArgs a = {};
+    a.n = nrows * top;
+    ARGCHK(a.n == 0 || (experts && place && source && work), "experts, place, source and work must not be NULL");
+    TRY(check_device(flags, experts, place, source, offsets, work));
+    a.ids = experts;
+    a.id64 = id_dtype == EVT_I64;
+    a.E = nexperts;
+    a.place = place;
+    a.source = source;
+    a.offsets = offsets;
+    a.table = work;
+    launch_plan((hipStream_t)stream, a);
+    HIPCHK(hipGetLastError());
+    return EVT_OK;
+    });
+}
+
+// What every entry point checks of its rows: x has nx of them, out and residual no
+static int take_rows(const evt_rows *r, int64_t nx, int64_t no, int32_t flags, RowArgs &a) {
+    TRY(check_flags(flags));
+    ARGCHK(r->dtype == EVT_F32 || r->dtype == EVT_BF16 || r->dtype == EVT_F16, "rows must be EVT_F32, EVT_BF16 or EVT_F16");
+    ARGCHK(r->nfeats >= 1 && r->nfeats <= (1 << 24), "nfeats must be in [1, 2^24]");
+    ARGCHK(r->p >= 0.0 && r->p < 1.0, "p must be in [0, 1)");
+    const int size = size_of(r->dtype);
+    ARGCHK(r->x_stride >= 0 && r->residual_stride >= 0, "strides must not be negative");
+    ARGCHK(nx <= 0 || no <= 0 || (r->x && r->out), "rows and out must not be NULL");
+    ARGCHK((uintptr_t)r->x % size == 0 && (uintptr_t)r->out % size == 0 && (uintptr_t)r->residual % size == 0, "rows must be aligned to their type");
+    ARGCHK(no <= 1 || r->out_stride >= r->nfeats, "out_stride must be at least nfeats");
+    a.x = r->x;
+    a.xs = r->x_stride;
+    a.out = r->out;
+    a.os = r->out_stride;
+    a.res = r->residual;
+    a.rs = r->residual_stride;
+    a.N = r->nrows;
+    a.H = r->nfeats;
+    const double drop = rint(r->p * 4294967296.0);
+    a.drop = drop < 4294967295.0 ? (uint32_t)drop : 4294967295u;
+    a.scale = (float)(4294967296.0 / (4294967296.0 - a.drop));
+    a.seed = r->seed;
+    a.seed_at = r->seed_dev;
+    a.layer = r->layer;
+    const Extent x = {r->x, r->x_stride, nx}, out = {r->out, r->out_stride, no}, res = {r->residual, r->residual_stride, no};
+    ARGCHK((nx == no && same(x, out)) || apart(x, out, a.H, size), "out must lie apart from the rows, or of drop_rows be their own memory, row for row");
+    ARGCHK(same(res, out) || apart(res, out, a.H, size), "out must be the residual's own memory, row for row, or lie apart from it");
+    return check_device(flags, r->x, r->out, r->residual, r->seed_dev);
+}
+static int take_places(int64_t nrows, int32_t top, int32_t nexperts, const int32_t *place, RowArgs &a) {
+    ARGCHK(nexperts >= 1 && nexperts <= MAX_EXPERTS, "nexperts must be in [1, 4096]");
+    ARGCHK(top >= 1 && nrows >= 0 && nrows <= INT32_MAX / top, "top must be at least 1, nrows * top in [0, 2^31 - 1]");
+    ARGCHK(place || nrows == 0, "place must not be NULL");
+    a.place = place;
+    a.top = top;
+    a.n = nrows * top;
+    return EVT_OK;
+}
+
+extern "C" int evt_sort_rows(void *stream, const void *rows, const int32_t *place, const int32_t *offsets, int32_t top, int32_t nexperts, int32_t flags) {
+    return guarded([&]() -> int {
+    const evt_rows *const r = static_cast<const evt_rows *>(rows);
+    ARGCHK(r, "rows must not be NULL");
+    RowArgs a = {};
+    TRY(take_places(r->nrows, top, nexperts, place, a));
+    TRY(take_rows(r, r->nrows, a.n, flags, a));
+    ARGCHK(!r->residual && r->p == 0.0, "sorted rows have no residual and no dropout");
+    ARGCHK(top > 1 || r->x != r->out, "sorted rows must lie apart from the rows");
+    if (a.N == 0) return EVT_OK;
+    ARGCHK(offsets, "offsets must not be NULL");
+    TRY(check_device(flags, place, offsets));
+    a.count = offsets + nexperts;
+    return launch_rows<ROWS_SPREAD>((hipStream_t)stream, a, r->dtype);
+    });
+}
+
+extern "C" int evt_combine_rows(void *stream, const void *rows, const int32_t *place, const float *weights, int32_t top, int32_t flags) {
+    return guarded([&]() -> int {
+    const evt_rows *const r = static_cast<const evt_rows *>(rows);
+    ARGCHK(r, "rows must not be NULL");
+    RowArgs a = {};
+    TRY(take_places(r->nrows, top, 1, place, a));
+    TRY(take_rows(r, a.n, r->nrows, flags, a));
+    ARGCHK(top > 1 || r->x != r->out, "combined rows must lie apart from the experts' rows");
+    if (a.N == 0) return EVT_OK;
+    TRY(check_device(flags, place, weights));
+    a.y = a.x;
+    a.ys = a.xs;
+    a.w = weights;
+    return launch_rows<ROWS_COMBINE>((hipStream_t)stream, a, r->dtype);
+    });
+}
+
+extern "C" int evt_combine_rows_grad(void *stream, const void *rows, const void *y, int64_t y_stride, const int32_t *place, const int32_t *offsets,
+                                     const float *weights, float *dweights, int32_t top, int32_t nexperts, int32_t flags) {
+    return guarded([&]() -> int {
+    const evt_rows *const r = static_cast<const evt_rows *>(rows);
+    ARGCHK(r, "rows must not be NULL");
+    RowArgs a = {};
+    TRY(take_places(r->nrows, top, nexperts, place, a));
+    TRY(take_rows(r, r->nrows, a.n, flags, a));
+    ARGCHK(!r->residual, "the gradient takes no residual");
+    ARGCHK((y != nullptr) == (dweights != nullptr) && (!y || weights), "y and dweights come together, and with weights");
+    ARGCHK(y_stride >= 0 && (uintptr_t)y % size_of(r->dtype) == 0, "y must be aligned to its type, its stride not negative");
+    ARGCHK(top > 1 || r->x != r->out, "the experts' gradients must lie apart from the rows'");
+    ARGCHK(apart({y, y_stride, a.n}, {r->out, r->out_stride, a.n}, a.H, size_of(r->dtype)), "the experts' gradients must lie apart from y");
+    if (a.N == 0) return EVT_OK;
+    ARGCHK(offsets, "offsets must not be NULL");
+    TRY(check_device(flags, y, place, offsets, weights, dweights));
+    a.count = offsets + nexperts;
+    a.y = y;
+    a.ys = y_stride;
+    a.w = weights;
+    a.dw = dweights;
+    return launch_rows<ROWS_SPREAD>((hipStream_t)stream, a, r->dtype);
+    });
+}
+
+extern "C" int evt_drop_rows(void *stream, const void *rows, int32_t flags) {
+    return guarded([&]() -> int {
+    const evt_rows *const r = static_cast<const evt_rows *>(rows);
+    ARGCHK(r, "rows must not be NULL");
+    ARGCHK(r->nrows >= 0 && r->nrows <= INT32_MAX, "nrows must be in [0, 2^31 - 1]");
+    RowArgs a = {};
+    TRY(take_rows(r, r->nrows, r->nrows, flags, a));
+    if (a.N == 0) return EVT_OK;
+    return launch_rows<ROWS_DROP>((hipStream_t)stream, a, r->dtype);
+    });
+}

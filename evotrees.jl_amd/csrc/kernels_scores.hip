@@ -9,72 +9,8 @@
 //
 // Scores are 16 or 32 bits wide; differences, exponentials, sums and losses are 32-bit, a gradient is rounded once, when it is written.
 #include "scores.h"
+#include "pieces.h"
 #include <math.h>
-#include <type_traits>
-
-typedef _Float16 half_t;
-typedef __bf16 bf16_t;
-
-// Sixteen bytes of scores as they lie in memory, at any address their type allows.
-template <typename T>
-struct Piece {
-    static constexpr int E = 16 / sizeof(T);
-    struct __attribute__((packed, aligned(sizeof(T)))) Raw {
-        uint32_t w[4];
-    };
-    Raw r;
-    __device__ __forceinline__ void load(const T *p) { r = *(const Raw *)p; }
-    // past: by the caches.  A gradient that the last of them (256 MB) cannot hold only drives out what the next pass reads (8 pairs, 5003 x 32 768 bf16, loss and
-    // gradient again and again: the first pass over the scores 67 us, 39 so); a smaller one stays for its reader.  Not of short rows, where a store has parts of
-    // lines that the second cache would put together (4.2M x 64 bf16: 290 us, 530 so; from 256 pieces on 0 to 5 % less)
-    __device__ __forceinline__ void store(T *p, bool past) const {
-        typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
-        const u4 v = {r.w[0], r.w[1], r.w[2], r.w[3]};
-        if (past) {
-            asm volatile(""); // in front and behind, so that the two stores stay apart: joined, the hint is lost
-            __builtin_nontemporal_store(v, (u4 *)p);
-            asm volatile("");
-        } else {
-            *(u4 *)p = v;
-        }
-    }
-    // o elements behind a base: a 32-bit offset is an operand of the access where a pointer is two registers for every piece
-    __device__ __forceinline__ void load(const T *p, uint32_t o) { r = *(const Raw *)((const char *)p + o * (uint32_t)sizeof(T)); }
-    __device__ __forceinline__ void store(T *p, uint32_t o, bool past) const { store((T *)((char *)p + o * (uint32_t)sizeof(T)), past); }
-    __device__ __forceinline__ void get(float *f) const {
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) f[k] = __uint_as_float(r.w[k]);
-        } else if constexpr (std::is_same<T, bf16_t>::value) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                f[2 * k] = __uint_as_float(r.w[k] << 16);
-                f[2 * k + 1] = __uint_as_float(r.w[k] & 0xffff0000u);
-            }
-        } else {
-            typedef half_t h2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const h2 v = __builtin_bit_cast(h2, r.w[k]);
-                f[2 * k] = (float)v[0];
-                f[2 * k + 1] = (float)v[1];
-            }
-        }
-    }
-    __device__ __forceinline__ void set(const float *f) { // rounds to nearest
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) r.w[k] = __float_as_uint(f[k]);
-        } else {
-            typedef T t2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const t2 v = {(T)f[2 * k], (T)f[2 * k + 1]};
-                r.w[k] = __builtin_bit_cast(uint32_t, v);
-            }
-        }
-    }
-};
 
 // (m, s): the maximum of some scores, at least the lowest finite number, and the sum of their exp((x - m) / T).  Scores of -inf count nothing, a
 // NaN or +inf makes s a NaN, and s is 0 where every score is -inf.
@@ -97,32 +33,6 @@ __device__ __forceinline__ MaxSum take(MaxSum a, const float *f, float mul) {
 #pragma unroll
         for (int k = 0; k < w; k++) s[k] += s[k + w];
     return {m, a.s * exp_of(a.m, m, mul) + s[0]};
-}
-// Reductions over G neighbouring lanes whose result every one of them has: by moves within rows of sixteen lanes and gfx950's swaps of rows between two
-// registers, a few cycles a step where a trip through the LDS crossbar is a hundred (8 rows of 32 768 classes: 6.3 us, 4.8 so).
-template <int CTRL>
-__device__ __forceinline__ float moved(float v) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, 0xf, 0xf, false));
-}
-template <int G, typename F>
-__device__ __forceinline__ float over_lanes(float v, F &&f) {
-    if (G >= 2) v = f(v, moved<0xB1>(v));   // quad_perm: lane ^ 1
-    if (G >= 4) v = f(v, moved<0x4E>(v));   // quad_perm: lane ^ 2
-    if (G >= 8) v = f(v, moved<0x141>(v));  // row_half_mirror: the other four of eight
-    if (G >= 16) v = f(v, moved<0x140>(v)); // row_mirror: the other eight of sixteen
-    if (G >= 32) {
-        const auto h = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(h[0]), __uint_as_float(h[1]));
-    }
-    if (G >= 64) {
-        const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(h[0]), __uint_as_float(h[1]));
-    }
-    return v;
-}
-template <int G>
-__device__ __forceinline__ float lanes_sum(float v) {
-    return over_lanes<G>(v, [](float x, float y) { return x + y; });
 }
 template <int G>
 __device__ __forceinline__ MaxSum lanes_join(MaxSum a, float mul) {

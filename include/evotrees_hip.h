@@ -460,6 +460,73 @@ int evt_preference_loss(void *stream, const void *scores /* evt_scores */, const
                         const float *ref_logp, const float *weights, double beta, double label_smoothing, double margin, int32_t average,
                         float *loss, float *seq_logp, float *work, int32_t flags);
 
+/* ---- rows through experts ------------------------------------------------------------------
+ * No counterpart in the reference: what a model of several experts does with its rows - a language model's tokens between two layers, or a table's rows at the
+ * leaves of a tree (evt_predict_leaf_idx) - around the experts' own products.  Stateless and device-only, in the manner of the losses above: device pointers of the
+ * current device, the caller's stream, nothing allocated, copied, waited for or kept; calls may overlap and be captured.  Results do not depend on the
+ * grid or the order of blocks: equal calls give equal bits.
+ *
+ * The choice of experts: the `top` best scores of each of nrows rows of nclass experts' scores (1 .. 4096; top 1 .. 64, at most nclass), the best first; of equal
+ * scores the lower expert's comes first.  With z = x / temperature and e_j the chosen
+ *   weights[i, j] = exp(z_ej) / sum of exp(z) over the row's chosen (renormalize 1) or over all of its experts (0).
+ * A score of -inf is an expert that cannot be chosen: a row with fewer others has the id -1 and the weight 0 in what is left.  A NaN (the best of all scores)
+ * or +inf makes its row's weights NaN.  experts, weights: nrows x top.  grad is not used.
+ * The gradient, from what the choice returned and the weights' gradient dweights, written to grad (which may be the scores' own memory, as above):
+ *   renormalize 1: grad[i, c] = sum over j with e_j == c of w_j (dw_j - m) / temperature,  m = sum_j w_j dw_j;
+ *   renormalize 0: grad[i, c] = (sum over j with e_j == c of w_j dw_j - q_c m) / temperature,  q = softmax(z).
+ * A negative id has no part in it, whatever stands at its weight and slope.  A NaN among the others, an id of nclass or more, or with renormalize 0 a NaN or +inf
+ * among the scores makes the row's gradient NaN.  With renormalize 1 the scores are not read. */
+int evt_route_rows(void *stream, const void *scores /* evt_scores */, int32_t top, int32_t renormalize, int32_t *experts, float *weights, int32_t flags);
+int evt_route_rows_grad(void *stream, const void *scores /* evt_scores */, int32_t top, int32_t renormalize, const void *experts, int32_t id_dtype,
+                        const float *weights, const float *dweights, int32_t flags);
+
+/* The tables that order rows by expert.  experts: nrows x top ids (EVT_I32 or EVT_I64; nrows * top < 2^31, nexperts 1 .. 4096); an id outside
+ * 0 .. nexperts - 1 is none, and one may come twice in a row.  Entry i = row * top + j of an expert stands behind its expert's entries of lower i:
+ *   place[i] = its place in that order (-1: none),  source[place[i]] = i (-1 behind the last),  expert e has the places offsets[e] .. offsets[e + 1] - 1
+ * (nexperts + 1 numbers).  work: EVT_PLAN_WORK(nrows * top, nexperts) int32 that the call may write. */
+#define EVT_PLAN_WORK(n, nexperts) ((((int64_t)(n) + 4095) / 4096 + 1) * (int64_t)(nexperts))
+int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype, int64_t nrows, int32_t top, int32_t nexperts, int32_t *place, int32_t *source,
+                  int32_t *offsets, int32_t *work, int32_t flags);
+
+/* Rows of nfeats values (EVT_F32, EVT_BF16 or EVT_F16, alike in a call), a row's side by side, rows a stride of elements apart (any alignment; 0: one row
+ * for all, where it is only read).  Products and sums have 32 bits, a value is rounded once.  Elements between nfeats and out_stride stay as they are.
+ *
+ * Dropout: an element of row r and column c has 32 random bits; drop(v) is 0 - whatever v is - where they are below t = p 2^32 (rounded) and
+ * v 2^32 / (2^32 - t) elsewhere.  The bits come from SplitMix64 as a row sample's do (evt_draw_mask): with key = output number `layer` (from 0) of the generator started at the seed,
+ * their upper half is bits 16 (c % 4) .. of output number r ceil(nfeats / 4) + c / 4 of the generator started at key, their lower half the same bits of the same
+ * output of the one started at ~key.  No mask is stored: the same seed, layer, r and c give the same bits, in the gradient as well. */
+typedef struct {
+    const void *x;
+    int64_t x_stride;
+    void *out;
+    int64_t out_stride;
+    const void *residual; /* NULL: none */
+    int64_t residual_stride;
+    int64_t nrows;  /* 0 .. 2^31 - 1 */
+    int32_t nfeats; /* 1 .. 2^24 */
+    int32_t dtype;
+    double p;       /* of dropout, [0, 1); 0: none, the seed is not read */
+    uint64_t seed;
+    const uint64_t *seed_dev; /* device memory that holds the seed when the work runs, as a captured call's replays need it; NULL: `seed` */
+    uint32_t layer;
+} evt_rows;
+
+/* out[place[i, j]] = x[i] for each of nrows rows, 0 for sorted rows that no entry has.  out: nrows * top rows, apart from x.  The gradient is evt_combine_rows
+ * without weights. */
+int evt_sort_rows(void *stream, const void *rows /* evt_rows */, const int32_t *place, const int32_t *offsets, int32_t top, int32_t nexperts, int32_t flags);
+
+/* out[i] = residual[i] + drop(sum_j weights[i, j] x[place[i, j]]), x the nrows * top sorted rows and j over the row's entries that have a place; weights nrows x top,
+ * NULL: ones.  out may be the residual's own memory. */
+int evt_combine_rows(void *stream, const void *rows /* evt_rows */, const int32_t *place, const float *weights, int32_t top, int32_t flags);
+/* Its gradients: with x the nrows rows of out's gradient and d = drop(x[i])
+ *   out[place[i, j]] = weights[i, j] d,  dweights[i, j] = sum over the features of d y[place[i, j]];
+ * rows of out that no entry has, and dweights of entries without a place, are 0.  y: what was combined; y and dweights NULL: out alone.  The residual's gradient is x. */
+int evt_combine_rows_grad(void *stream, const void *rows /* evt_rows */, const void *y, int64_t y_stride, const int32_t *place, const int32_t *offsets,
+                          const float *weights, float *dweights, int32_t top, int32_t nexperts, int32_t flags);
+
+/* out[i] = residual[i] + drop(x[i]).  out may be x's or the residual's own memory.  The gradient by x is the same call on out's gradient, without a residual. */
+int evt_drop_rows(void *stream, const void *rows /* evt_rows */, int32_t flags);
+
 /* ---- measurement ---------------------------------------------------------------------
  * Kernel classes timed with HIP events on the handle's stream when profiling is on.  Kernels that do the work of several classes
  * count as one: a tree of one launch is one PARTITION launch, and none of HIST or SCAN; of one kernel per level, the root's is a

@@ -407,15 +407,17 @@ __global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
 // ---- rows ------------------------------------------------------------------------------------
 
 struct RowArgs {
-    const void *x, *res, *y;
+    const void *x, *res;
     void *out;
-    int64_t xs, rs, ys, os; // elements from row to row
-    int64_t N, n;           // rows; sorted rows, rows x top
-    int32_t H, top, pieces, chunk; // pieces of a row, and of a block's part of it
-    int32_t parts;
+    int64_t xs, rs, os; // elements from row to row
     const int32_t *place, *count;
     const float *w;
+    const void *y;
+    int64_t ys;
     float *dw;
+    uint32_t N, n;                     // rows; sorted rows, rows x top
+    uint32_t row0;                     // the launch's first row
+    uint32_t H, top, pieces, parts;    // pieces of a row; parts: of 64 pieces
     // dropout: an element is dropped whose 32 bits are below this
     uint32_t drop, layer;
     float scale;
@@ -423,239 +425,280 @@ struct RowArgs {
     uint64_t seed;
 };
 
-#define TAIL_BLOCKS 64
 #define GAMMA 0x9E3779B97F4A7C15ull
 __device__ __forceinline__ uint64_t mixed(uint64_t z) {
     z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
     z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
     return z ^ (z >> 31);
 }
-// Dropout of a row's pieces, whose bits come from SplitMix64 (Steele, Lea, Flood 2014), as a row sample's do: nothing is stored, the gradient draws them again.
-// Four values have the sixteen-bit quarters of one output, which decide unless one of them is just the threshold's upper half: one in 65 536, whose lower
+// Dropout of E values of a row from piece v on, whose bits come from SplitMix64 (Steele, Lea, Flood 2014), as a row sample's do: nothing is stored, the gradient draws
+// them again.  Four values have the sixteen-bit quarters of one output, which decide unless one of them is just the threshold's upper half: one in 65 536, whose lower
 // half is drawn then.
-struct Drop {
-    uint64_t key, base;
-    uint32_t words;
-    __device__ __forceinline__ Drop(const RowArgs &a) {
-        key = mixed((a.seed_at ? *a.seed_at : a.seed) + (uint64_t)(a.layer + 1ull) * GAMMA);
-        words = ((uint32_t)a.H + 3) / 4;
+template <int E>
+__device__ __forceinline__ void drop_values(const RowArgs &a, uint64_t key, uint32_t row, uint32_t v, float *f) {
+    const uint32_t hi = a.drop >> 16, lo = a.drop & 0xFFFFu, words = (a.H + 3) / 4;
+    const uint64_t first = (uint64_t)row * words + 1;
+#pragma unroll
+    for (int q = 0; q < E / 4; q++) {
+        const uint64_t at = (first + (v * (E / 4) + q)) * GAMMA, word = mixed(key + at);
+        const uint32_t half[2] = {(uint32_t)word, (uint32_t)(word >> 32)};
+        bool tie = false;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const uint32_t bits = (half[k / 2] >> (16 * (k & 1))) & 0xFFFFu;
+            tie |= bits == hi;
+            f[4 * q + k] = bits < hi ? 0.0f : f[4 * q + k] * a.scale;
+        }
+        if (__builtin_expect(lo != 0 && tie, 0)) {
+            const uint64_t second = mixed(~key + at);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (((word >> (16 * k)) & 0xFFFF) == hi && ((second >> (16 * k)) & 0xFFFF) < lo) f[4 * q + k] = 0.0f;
+        }
     }
-    __device__ __forceinline__ void row(int64_t r) { base = ((uint64_t)r * words + 1) * GAMMA; }
-    template <int E>
-    __device__ __forceinline__ void apply(const RowArgs &a, int v, float *f) const {
-        const uint32_t hi = a.drop >> 16, lo = a.drop & 0xFFFFu;
+}
+__device__ __forceinline__ uint64_t drop_key(const RowArgs &a) { return mixed((a.seed_at ? *a.seed_at : a.seed) + ((uint64_t)a.layer + 1) * GAMMA); }
+
+typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+// Piece v of a row of H values.  The last one, where it is not whole, is read from where it ends and moved down, without a branch.  TINY: rows
+// of less than a piece
+template <bool TINY, typename T>
+__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H) {
+    constexpr uint32_t E = Piece<T>::E;
+    if (TINY) {
+        p.load_some(x, H);
+        return;
+    }
+    const uint32_t at = v * E, last = H - E;
+    const u4 r = *(const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
+    const uint32_t n = H % E;
+    if (n == 0) { // of all lanes alike
 #pragma unroll
-        for (int q = 0; q < E / 4; q++) {
-            const uint64_t at = base + (uint64_t)(uint32_t)(v * (E / 4) + q) * GAMMA;
-            const uint64_t word = mixed(key + at);
-            const uint32_t half[2] = {(uint32_t)word, (uint32_t)(word >> 32)};
-            bool tie = false;
+        for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
+    } else {
+        const uint32_t up = E - n, words = up * sizeof(T) / 4;
+        uint32_t w[5];
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                const uint32_t bits = (half[k / 2] >> (16 * (k & 1))) & 0xFFFFu;
-                tie |= bits == hi;
-                f[4 * q + k] = bits < hi ? 0.0f : f[4 * q + k] * a.scale;
-            }
-            if (__builtin_expect(lo != 0 && tie, 0)) {
-                const uint64_t second = mixed(~key + at);
+        for (uint32_t k = 0; k < 4; k++) {
+            w[k] = r[k];
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                    if (((word >> (16 * k)) & 0xFFFF) == hi && ((second >> (16 * k)) & 0xFFFF) < lo) f[4 * q + k] = 0.0f;
-            }
+            for (uint32_t d = 1; d < 4; d++) w[k] = words == d ? (d + k < 4 ? r[(d + k) & 3] : 0u) : w[k];
+        }
+        w[4] = 0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (sizeof(T) == 2) w[k] = up & 1 ? __builtin_amdgcn_alignbit(w[k + 1], w[k], 16) : w[k];
+            p.r.w[k] = at > last ? w[k] : r[k];
+        }
+    }
+}
+template <bool TINY, typename T>
+__device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v, uint32_t H) {
+    constexpr uint32_t E = Piece<T>::E;
+    T *const o = x + (size_t)v * E;
+    if (!TINY && v * E + E <= H) p.store(o, false);
+    else p.store_some(o, H % E);
+}
+
+// The row and piece that a thread has.  ROW: a wavefront's are of one row, which the compiler knows; otherwise the pieces of all rows follow each other, and
+// no lane is idle.
+template <bool ROW>
+struct Share {
+    uint32_t row, v;
+    bool in;
+    __device__ __forceinline__ Share(const RowArgs &a) {
+        if (ROW) {
+            const uint32_t i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64), r = i / a.parts;
+            v = (i - r * a.parts) * 64 + (threadIdx.x & 63);
+            row = a.row0 + r;
+            in = row < a.N && v < a.pieces;
+        } else {
+            const uint32_t i = blockIdx.x * 256 + threadIdx.x, r = i / a.pieces;
+            v = i - r * a.pieces;
+            row = a.row0 + r;
+            in = row < a.N;
         }
     }
 };
 
-// The row and part of it that a group of G threads has
-template <int G>
-struct Share {
-    static constexpr int ROWS = 256 / G;
-    int64_t row;
-    int part, rank;
-    __device__ __forceinline__ Share(const RowArgs &a, int64_t block) {
-        const int64_t group = a.parts == 1 ? block : block / a.parts;
-        part = a.parts == 1 ? 0 : (int)(block - group * a.parts);
-        rank = threadIdx.x & (G - 1);
-        row = group * ROWS + (G >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G);
-    }
-};
-
-template <typename T>
-__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, int v, int H) {
-    constexpr int E = Piece<T>::E;
-    if ((v + 1) * E <= H) p.load(x + (size_t)v * E);
-    else p.load_some(x + (size_t)v * E, H - v * E);
-}
-template <typename T>
-__device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, int v, int H) {
-    constexpr int E = Piece<T>::E;
-    if ((v + 1) * E <= H) p.store(x + (size_t)v * E, false);
-    else p.store_some(x + (size_t)v * E, H - v * E);
+// Sorted rows that no entry has: 0, by the launch's last blocks
+#define TAIL_BLOCKS 64
+template <bool TINY, typename T>
+__device__ void clear_behind(const RowArgs &a, uint32_t block) {
+    Piece<T> z;
+    z.r = {};
+    const int count = *a.count;
+    for (uint32_t p = (count < 0 ? 0u : (uint32_t)count) + block; p < a.n; p += TAIL_BLOCKS)
+        for (uint32_t v = threadIdx.x; v < a.pieces; v += 256) store_piece<TINY>(z, (T *)a.out + p * a.os, v, a.H);
 }
 
-// Rows to their places: each row is read once and written `top` times, times a weight if there are weights.  DOT: and the sums of its products with the rows that
-// lie at these places in y.
-template <typename T, int G, bool DROP, bool DOT>
-__global__ __launch_bounds__(256) void k_spread(RowArgs a, int64_t blocks) {
+// Rows to their places: each row is read once and written `top` times, times a weight if there are weights
+template <typename T, bool ROW, bool TINY, bool DROP>
+__global__ __launch_bounds__(256) void k_spread(RowArgs a) {
     constexpr int E = Piece<T>::E, TOP = 8;
-    __shared__ float s_dot[4][TOP];
-    const Drop drop_of(a);
-    // behind the last of the sorted rows: the grid's last blocks
     if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
-        const int count = *a.count;
-        for (int64_t p = (int64_t)(count < 0 ? 0 : count) + (blockIdx.x - (gridDim.x - TAIL_BLOCKS)); p < a.n; p += TAIL_BLOCKS)
-            for (int v = threadIdx.x; v < a.pieces; v += 256) {
-                Piece<T> z;
-                z.r = {};
-                store_piece(z, (T *)a.out + p * a.os, v, a.H);
-            }
+        if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
         return;
     }
-    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x - TAIL_BLOCKS) {
-        const Share<G> me(a, block);
-        const bool in = me.row < a.N;
-        Drop drop = drop_of;
-        if (DROP) drop.row(me.row);
-        const T *x = (const T *)a.x + me.row * a.xs;
-        const int v1 = me.part * a.chunk + a.chunk < a.pieces ? me.part * a.chunk + a.chunk : a.pieces;
-        for (int j0 = 0; j0 < a.top; j0 += TOP) {
-            int at[TOP];
-            float w[TOP], dot[TOP];
+    const Share<ROW> me(a);
+    if (!me.in) return;
+    Piece<T> p;
+    load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
+    float f[E];
+    if (DROP || a.w) p.get(f);
+    if (DROP) drop_values<E>(a, drop_key(a), me.row, me.v, f);
+    const size_t e0 = (size_t)me.row * a.top;
+    for (uint32_t j0 = 0; j0 < a.top; j0 += TOP) {
+        uint32_t at[TOP];
 #pragma unroll
-            for (int j = 0; j < TOP; j++) {
-                at[j] = in && j0 + j < a.top ? a.place[me.row * a.top + j0 + j] : -1;
-                w[j] = a.w && in && j0 + j < a.top ? a.w[me.row * a.top + j0 + j] : 1.0f;
-                dot[j] = 0.0f;
-                if ((uint32_t)at[j] >= (uint64_t)a.n) at[j] = -1;
-            }
-            if (in)
-                for (int v = me.part * a.chunk + me.rank; v < v1; v += G) {
-                    Piece<T> p, q[TOP];
-                    float f[E];
-                    load_piece(p, x, v, a.H);
-                    if (DOT) {
+        for (int j = 0; j < TOP; j++) at[j] = j0 + j < a.top ? (uint32_t)a.place[e0 + j0 + j] : ~0u;
 #pragma unroll
-                        for (int j = 0; j < TOP; j++)
-                            if (at[j] >= 0) load_piece(q[j], (const T *)a.y + at[j] * a.ys, v, a.H);
-                    }
-                    p.get(f);
-                    if (DROP) drop.template apply<E>(a, v, f);
+        for (int j = 0; j < TOP; j++)
+            if (at[j] < a.n) {
+                if (DROP || a.w) {
+                    const float w = a.w ? a.w[e0 + j0 + j] : 1.0f;
+                    float g[E];
 #pragma unroll
-                    for (int j = 0; j < TOP; j++)
-                        if (at[j] >= 0) {
-                            if (DROP || a.w) {
-                                float g[E];
-#pragma unroll
-                                for (int k = 0; k < E; k++) g[k] = f[k] * w[j];
-                                p.set(g);
-                            }
-                            store_piece(p, (T *)a.out + at[j] * a.os, v, a.H);
-                            if (DOT) {
-                                float g[E];
-                                q[j].get(g);
-                                float sum = 0.0f;
-#pragma unroll
-                                for (int k = 0; k < E; k++) sum += f[k] * g[k];
-                                dot[j] += sum;
-                            }
-                        }
+                    for (int k = 0; k < E; k++) g[k] = f[k] * w;
+                    p.set(g);
                 }
-            if (DOT) {
-#pragma unroll
-                for (int j = 0; j < TOP; j++) dot[j] = lanes_sum<(G < 64 ? G : 64)>(dot[j]);
-                if (G > 64) {
-                    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-                        for (int j = 0; j < TOP; j++) s_dot[threadIdx.x >> 6][j] = dot[j];
-                    __syncthreads();
-#pragma unroll
-                    for (int j = 0; j < TOP; j++) dot[j] = (s_dot[0][j] + s_dot[1][j]) + (s_dot[2][j] + s_dot[3][j]);
-                    __syncthreads();
-                }
-                if (in && me.rank == 0)
-#pragma unroll
-                    for (int j = 0; j < TOP; j++)
-                        if (j0 + j < a.top) a.dw[me.row * a.top + j0 + j] = at[j] >= 0 ? dot[j] : 0.0f;
+                store_piece<TINY>(p, (T *)a.out + at[j] * a.os, me.v, a.H);
             }
+    }
+}
+
+// ... and the sums of its products with the rows that lie at these places in y: a row to G threads.
+template <typename T, int G, int TOP, bool TINY, bool DROP>
+__global__ __launch_bounds__(G < 256 ? 256 : G) void k_spread_dot(RowArgs a) {
+    constexpr int E = Piece<T>::E, THREADS = G < 256 ? 256 : G, ROWS = THREADS / G, W = G / 64;
+    __shared__ float s_dot[W > 1 ? W : 1][TOP];
+    if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
+        if (a.row0 == 0 && threadIdx.x < 256) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
+        return;
+    }
+    const uint32_t rank = threadIdx.x & (G - 1), slot = G >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G;
+    const uint32_t row = a.row0 + blockIdx.x * ROWS + slot;
+    if (ROWS > 1 && row >= a.N) return;
+    const T *x = (const T *)a.x + row * a.xs;
+    const uint64_t key = DROP ? drop_key(a) : 0;
+    const size_t e0 = (size_t)row * a.top;
+    for (uint32_t j0 = 0; j0 < a.top; j0 += TOP) {
+        uint32_t at[TOP];
+        float w[TOP], dot[TOP];
+#pragma unroll
+        for (int j = 0; j < TOP; j++) {
+            at[j] = j0 + j < a.top ? (uint32_t)a.place[e0 + j0 + j] : ~0u;
+            w[j] = j0 + j < a.top ? a.w[e0 + j0 + j] : 0.0f;
+            dot[j] = 0.0f;
+        }
+        for (uint32_t v = rank; v < a.pieces; v += G) {
+            Piece<T> p, q[TOP];
+            float f[E];
+            load_piece<TINY>(p, x, v, a.H);
+#pragma unroll
+            for (int j = 0; j < TOP; j++)
+                if (at[j] < a.n) load_piece<TINY>(q[j], (const T *)a.y + at[j] * a.ys, v, a.H);
+            p.get(f);
+            if (DROP) drop_values<E>(a, key, row, v, f);
+#pragma unroll
+            for (int j = 0; j < TOP; j++)
+                if (at[j] < a.n) {
+                    float g[E];
+#pragma unroll
+                    for (int k = 0; k < E; k++) g[k] = f[k] * w[j];
+                    p.set(g);
+                    store_piece<TINY>(p, (T *)a.out + at[j] * a.os, v, a.H);
+                    q[j].get(g);
+                    float sum = f[0] * g[0];
+#pragma unroll
+                    for (int k = 1; k < E; k++) sum = __builtin_fmaf(f[k], g[k], sum);
+                    dot[j] += sum;
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < TOP; j++) dot[j] = lanes_sum<(G < 64 ? G : 64)>(dot[j]);
+        if (W > 1) {
+            if (j0) __syncthreads();
+            if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+                for (int j = 0; j < TOP; j++) s_dot[threadIdx.x >> 6][j] = dot[j];
+            }
+            __syncthreads();
+            if (threadIdx.x < TOP && j0 + threadIdx.x < a.top) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < W; k++) sum += s_dot[k][threadIdx.x];
+                a.dw[e0 + j0 + threadIdx.x] = sum;
+            }
+        } else if (rank == 0) {
+#pragma unroll
+            for (int j = 0; j < TOP; j++)
+                if (j0 + j < a.top) a.dw[e0 + j0 + j] = dot[j];
         }
     }
 }
 
 // Every row's sum over its places, times the weights if there are any, with dropout and a residual
-template <typename T, int G, bool DROP>
-__global__ __launch_bounds__(256) void k_combine(RowArgs a, int64_t blocks) {
-    constexpr int E = Piece<T>::E, TOP = 8;
-    const Drop drop_of(a);
-    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-        const Share<G> me(a, block);
-        if (me.row >= a.N) continue;
-        Drop drop = drop_of;
-        if (DROP) drop.row(me.row);
-        const int v1 = me.part * a.chunk + a.chunk < a.pieces ? me.part * a.chunk + a.chunk : a.pieces;
-        for (int v = me.part * a.chunk + me.rank; v < v1; v += G) {
-            Piece<T> res;
-            float sum[E] = {};
-            if (a.res) load_piece(res, (const T *)a.res + me.row * a.rs, v, a.H);
-            for (int j0 = 0; j0 < a.top; j0 += TOP) {
-                int at[TOP];
-                Piece<T> p[TOP];
+template <typename T, bool ROW, bool TINY, int TOP, bool DROP>
+__global__ __launch_bounds__(256) void k_combine(RowArgs a) {
+    constexpr int E = Piece<T>::E;
+    const Share<ROW> me(a);
+    if (!me.in) return;
+    Piece<T> res;
+    float sum[E] = {};
+    if (a.res) load_piece<TINY>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    const size_t e0 = (size_t)me.row * a.top;
+    for (uint32_t j0 = 0; j0 < a.top; j0 += TOP) {
+        uint32_t at[TOP];
+        float w[TOP];
+        Piece<T> p[TOP];
 #pragma unroll
-                for (int j = 0; j < TOP; j++) {
-                    at[j] = j0 + j < a.top ? a.place[me.row * a.top + j0 + j] : -1;
-                    if ((uint32_t)at[j] >= (uint64_t)a.n) at[j] = -1;
-                    if (at[j] >= 0) load_piece(p[j], (const T *)a.y + at[j] * a.ys, v, a.H);
-                }
+        for (int j = 0; j < TOP; j++) at[j] = j0 + j < a.top ? (uint32_t)a.place[e0 + j0 + j] : ~0u;
 #pragma unroll
-                for (int j = 0; j < TOP; j++)
-                    if (at[j] >= 0) {
-                        const float w = a.w ? a.w[me.row * a.top + j0 + j] : 1.0f;
-                        float f[E];
-                        p[j].get(f);
+        for (int j = 0; j < TOP; j++) w[j] = a.w && j0 + j < a.top ? a.w[e0 + j0 + j] : 1.0f;
 #pragma unroll
-                        for (int k = 0; k < E; k++) sum[k] += w * f[k];
-                    }
-            }
-            if (DROP) drop.template apply<E>(a, v, sum);
-            if (a.res) {
+        for (int j = 0; j < TOP; j++)
+            if (at[j] < a.n) load_piece<TINY>(p[j], (const T *)a.x + at[j] * a.xs, me.v, a.H);
+#pragma unroll
+        for (int j = 0; j < TOP; j++)
+            if (at[j] < a.n) {
                 float f[E];
-                res.get(f);
+                p[j].get(f);
 #pragma unroll
-                for (int k = 0; k < E; k++) sum[k] += f[k];
+                for (int k = 0; k < E; k++) sum[k] = __builtin_fmaf(w[j], f[k], sum[k]);
             }
-            Piece<T> o;
-            o.set(sum);
-            store_piece(o, (T *)a.out + me.row * a.os, v, a.H);
-        }
     }
+    if (DROP) drop_values<E>(a, drop_key(a), me.row, me.v, sum);
+    if (a.res) {
+        float f[E];
+        res.get(f);
+#pragma unroll
+        for (int k = 0; k < E; k++) sum[k] += f[k];
+    }
+    Piece<T> o;
+    o.set(sum);
+    store_piece<TINY>(o, (T *)a.out + me.row * a.os, me.v, a.H);
 }
 
-template <typename T, int G>
-__global__ __launch_bounds__(256) void k_drop(RowArgs a, int64_t blocks) {
+template <typename T, bool ROW, bool TINY>
+__global__ __launch_bounds__(256) void k_drop(RowArgs a) {
     constexpr int E = Piece<T>::E;
-    const Drop drop_of(a);
-    for (int64_t block = blockIdx.x; block < blocks; block += gridDim.x) {
-        const Share<G> me(a, block);
-        if (me.row >= a.N) continue;
-        Drop drop = drop_of;
-        drop.row(me.row);
-        const int v1 = me.part * a.chunk + a.chunk < a.pieces ? me.part * a.chunk + a.chunk : a.pieces;
-        for (int v = me.part * a.chunk + me.rank; v < v1; v += G) {
-            Piece<T> p, res;
-            float f[E];
-            load_piece(p, (const T *)a.x + me.row * a.xs, v, a.H);
-            if (a.res) load_piece(res, (const T *)a.res + me.row * a.rs, v, a.H);
-            p.get(f);
-            if (a.drop) drop.template apply<E>(a, v, f);
-            if (a.res) {
-                float g[E];
-                res.get(g);
+    const Share<ROW> me(a);
+    if (!me.in) return;
+    Piece<T> p, res;
+    float f[E];
+    load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
+    if (a.res) load_piece<TINY>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    p.get(f);
+    if (a.drop) drop_values<E>(a, drop_key(a), me.row, me.v, f);
+    if (a.res) {
+        float g[E];
+        res.get(g);
 #pragma unroll
-                for (int k = 0; k < E; k++) f[k] += g[k];
-            }
-            p.set(f);
-            store_piece(p, (T *)a.out + me.row * a.os, v, a.H);
-        }
+        for (int k = 0; k < E; k++) f[k] += g[k];
     }
+    p.set(f);
+    store_piece<TINY>(p, (T *)a.out + me.row * a.os, me.v, a.H);
 }
 
 // ---- launches --------------------------------------------------------------------------------
@@ -693,38 +736,56 @@ static int launch_route(hipStream_t s, const RouteArgs &a, int dtype) {
 }
 
 enum { ROWS_SPREAD, ROWS_COMBINE, ROWS_DROP };
-template <typename T, int G, int OP>
-static void launch_rows_as(hipStream_t s, const RowArgs &a) {
-    const int64_t blocks = (a.N + 256 / G - 1) / (256 / G) * a.parts;
-    const int64_t most = 1 << 22;
-    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
-    if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, G>), dim3(grid), dim3(256), 0, s, a, blocks);
-    else if constexpr (OP == ROWS_COMBINE) {
-        if (a.drop) hipLaunchKernelGGL((k_combine<T, G, true>), dim3(grid), dim3(256), 0, s, a, blocks);
-        else hipLaunchKernelGGL((k_combine<T, G, false>), dim3(grid), dim3(256), 0, s, a, blocks);
+template <typename T, bool ROW, bool TINY, int OP>
+static void launch_rows_as(hipStream_t s, const RowArgs &a, unsigned grid) {
+    if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, ROW, TINY>), dim3(grid), dim3(256), 0, s, a);
+    else if constexpr (OP == ROWS_SPREAD) {
+        if (a.drop) hipLaunchKernelGGL((k_spread<T, ROW, TINY, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_spread<T, ROW, TINY, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
     } else {
-        if (a.dw) {
-            if (a.drop) hipLaunchKernelGGL((k_spread<T, G, true, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
-            else hipLaunchKernelGGL((k_spread<T, G, false, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
-        } else {
-            if (a.drop) hipLaunchKernelGGL((k_spread<T, G, true, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
-            else hipLaunchKernelGGL((k_spread<T, G, false, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a, blocks);
-        }
+        const auto go = [&](auto top) {
+            if (a.drop) hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, true>), dim3(grid), dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, false>), dim3(grid), dim3(256), 0, s, a);
+        };
+        if (a.top <= 2) go(std::integral_constant<int, 2>());
+        else if (a.top <= 4) go(std::integral_constant<int, 4>());
+        else go(std::integral_constant<int, 8>());
     }
+}
+template <typename T, int G, bool TINY>
+static void launch_dot_as(hipStream_t s, const RowArgs &a, unsigned groups) {
+    constexpr int THREADS = G < 256 ? 256 : G, ROWS = THREADS / G;
+    const unsigned grid = (groups + ROWS - 1) / ROWS + TAIL_BLOCKS;
+    const auto go = [&](auto top) {
+        if (a.drop) hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, true>), dim3(grid), dim3(THREADS), 0, s, a);
+        else hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, false>), dim3(grid), dim3(THREADS), 0, s, a);
+    };
+    if (a.top <= 2) go(std::integral_constant<int, 2>());
+    else if (a.top <= 4) go(std::integral_constant<int, 4>());
+    else go(std::integral_constant<int, 8>());
 }
 template <typename T, int OP>
 static void launch_rows_typed(hipStream_t s, RowArgs &a) {
-    a.pieces = (a.H + Piece<T>::E - 1) / Piece<T>::E;
-    a.chunk = OP == ROWS_SPREAD && a.dw ? a.pieces : 256;
-    a.parts = (a.pieces + a.chunk - 1) / a.chunk;
-    if (a.pieces <= 1) launch_rows_as<T, 1, OP>(s, a);
-    else if (a.pieces <= 2) launch_rows_as<T, 2, OP>(s, a);
-    else if (a.pieces <= 4) launch_rows_as<T, 4, OP>(s, a);
-    else if (a.pieces <= 8) launch_rows_as<T, 8, OP>(s, a);
-    else if (a.pieces <= 16) launch_rows_as<T, 16, OP>(s, a);
-    else if (a.pieces <= 32) launch_rows_as<T, 32, OP>(s, a);
-    else if (a.pieces <= 128) launch_rows_as<T, 64, OP>(s, a);
-    else launch_rows_as<T, 256, OP>(s, a);
+    constexpr int E = Piece<T>::E;
+    a.pieces = (a.H + E - 1) / E;
+    a.parts = (a.pieces + 63) / 64;
+    const bool tiny = a.H < E, by_row = a.pieces >= 64;
+    const uint32_t each = a.pieces < 64 ? 64 : a.parts * 64; // threads a row, at most
+    const uint32_t most = (1u << 30) / each > 0 ? (1u << 30) / each : 1; // rows of a launch
+    for (uint64_t row0 = 0; row0 < a.N; row0 += most) {
+        a.row0 = (uint32_t)row0;
+        const uint32_t rows = a.N - a.row0 < most ? a.N - a.row0 : most;
+        if (OP == ROWS_SPREAD && a.dw) {
+            if (tiny) launch_dot_as<T, 8, true>(s, a, rows);
+            else if (a.pieces <= 8) launch_dot_as<T, 8, false>(s, a, rows);
+            else if (a.pieces <= 16) launch_dot_as<T, 16, false>(s, a, rows);
+            else if (a.pieces <= 32) launch_dot_as<T, 32, false>(s, a, rows);
+            else if (a.pieces <= 128) launch_dot_as<T, 64, false>(s, a, rows);
+            else launch_dot_as<T, 256, false>(s, a, rows);
+        } else if (tiny) launch_rows_as<T, false, true, OP>(s, a, (rows + 255) / 256);
+        else if (by_row) launch_rows_as<T, true, false, OP>(s, a, (unsigned)(((uint64_t)rows * a.parts + 3) / 4));
+        else launch_rows_as<T, false, false, OP>(s, a, (unsigned)(((uint64_t)rows * a.pieces + 255) / 256));
+    }
 }
 template <int OP>
 static int launch_rows(hipStream_t s, RowArgs &a, int dtype) {
@@ -898,8 +959,8 @@ static int take_rows(const evt_rows *r, int64_t nx, int64_t no, int32_t flags, R
     a.os = r->out_stride;
     a.res = r->residual;
     a.rs = r->residual_stride;
-    a.N = r->nrows;
-    a.H = r->nfeats;
+    a.N = (uint32_t)r->nrows;
+    a.H = (uint32_t)r->nfeats;
     const double drop = rint(r->p * 4294967296.0);
     a.drop = drop < 4294967295.0 ? (uint32_t)drop : 4294967295u;
     a.scale = (float)(4294967296.0 / (4294967296.0 - a.drop));
@@ -917,7 +978,7 @@ static int take_places(int64_t nrows, int32_t top, int32_t nexperts, const int32
     ARGCHK(place || nrows == 0, "place must not be NULL");
     a.place = place;
     a.top = top;
-    a.n = nrows * top;
+    a.n = (uint32_t)(nrows * top);
     return EVT_OK;
 }
 
@@ -948,8 +1009,6 @@ extern "C" int evt_combine_rows(void *stream, const void *rows, const int32_t *p
     ARGCHK(top > 1 || r->x != r->out, "combined rows must lie apart from the experts' rows");
     if (a.N == 0) return EVT_OK;
     TRY(check_device(flags, place, weights));
-    a.y = a.x;
-    a.ys = a.xs;
     a.w = weights;
     return launch_rows<ROWS_COMBINE>((hipStream_t)stream, a, r->dtype);
     });

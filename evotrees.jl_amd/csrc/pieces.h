@@ -60,14 +60,16 @@ struct Piece {
     __device__ __forceinline__ void store_some(T *p, int n) const {
         typedef uint32_t u2 __attribute__((ext_vector_type(2), aligned(2)));
         typedef uint32_t u1 __attribute__((aligned(2)));
-        const u2 a = {r.w[0], r.w[1]};
+        const uint32_t w0 = r.w[0], w1 = r.w[1], w2 = r.w[2], w3 = r.w[3]; // values: a choice between places would keep the piece in memory
+        const u2 a = {w0, w1};
         if constexpr (sizeof(T) == 4) {
             if (n & 2) *(u2 *)p = a;
-            if (n & 1) *(u1 *)(p + (n & 2)) = n & 2 ? r.w[2] : r.w[0];
+            if (n & 1) *(u1 *)(p + (n & 2)) = n & 2 ? w2 : w0;
         } else {
+            const uint32_t low = n & 2 ? w1 : w0, high = n & 2 ? w3 : w2;
             if (n & 4) *(u2 *)p = a;
-            if (n & 2) *(u1 *)(p + (n & 4)) = n & 4 ? r.w[2] : r.w[0];
-            if (n & 1) *(uint16_t *)(p + (n & 6)) = (uint16_t)(n & 4 ? (n & 2 ? r.w[3] : r.w[2]) : n & 2 ? r.w[1] : r.w[0]);
+            if (n & 2) *(u1 *)(p + (n & 4)) = n & 4 ? w2 : w0;
+            if (n & 1) *(uint16_t *)(p + (n & 6)) = (uint16_t)(n & 4 ? high : low);
         }
     }
     __device__ __forceinline__ void get(float *f) const {

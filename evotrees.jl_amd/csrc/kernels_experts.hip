@@ -26,63 +26,152 @@ struct RouteArgs {
 
 __device__ __forceinline__ float exp_gap(float x, float m, float mul) { return __builtin_amdgcn_exp2f((x - m) * mul); }
 
-// A score and its class as one number that is the greater the better: the score's bits in an order that is theirs (zeros alike, every NaN above +inf), and
-// below them the class, complemented, so that no two are alike and the lower class is the better of two equal scores.  0: no class, or one that cannot be (-inf).
-// 16-bit scores and a class of 16 bits fit one word, which compares at twice the rate.
-template <typename T>
-struct Key {
-    typedef std::conditional_t<sizeof(T) == 2, uint32_t, uint64_t> type;
-    static __device__ __forceinline__ type of(float x, uint32_t c) {
-        uint32_t b = __float_as_uint(x + 0.0f); // -0 becomes 0
-        b = b & 0x80000000u ? ~b : b | 0x80000000u;
-        b = x != x ? 0xFFFFFFFFu : b;
-        if constexpr (std::is_same<T, half_t>::value) {
-            // the half's own bits
-            uint32_t h = __builtin_bit_cast(uint16_t, (half_t)(x + 0.0f));
-            h = h & 0x8000u ? ~h & 0xFFFFu : h | 0x8000u;
-            b = x != x ? 0xFFFFFFFFu : h << 16;
-        }
-        if constexpr (sizeof(T) == 2) return x == -INFINITY ? 0 : (b & 0xFFFF0000u) | (0xFFFFu - c);
-        else return x == -INFINITY ? 0 : (uint64_t)b << 32 | (0xFFFFu - c);
+typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+// Piece v of a row of H values.  The last one, where it is not whole, is read from where it ends and moved down, without a branch; what is behind the row is
+// `fill`, two or one values of a word.  TINY: rows of less than a piece
+template <bool TINY, typename T>
+__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H, uint32_t fill = 0) {
+    constexpr uint32_t E = Piece<T>::E;
+    if (TINY) {
+        p.load_some(x, H);
+        return;
     }
-    static __device__ __forceinline__ int chosen(type k) { return k ? (int)(0xFFFFu - (uint32_t)(k & 0xFFFFu)) : -1; }
-    static __device__ __forceinline__ float score(type k) {
-        if constexpr (std::is_same<T, half_t>::value) {
-            uint32_t h = (uint32_t)k >> 16;
-            h = h & 0x8000u ? h & 0x7FFFu : ~h & 0xFFFFu;
-            return k ? (float)__builtin_bit_cast(half_t, (uint16_t)h) : -INFINITY;
-        } else {
-            uint32_t b = sizeof(T) == 2 ? (uint32_t)k & 0xFFFF0000u : (uint32_t)((uint64_t)k >> 32);
-            b = b & 0x80000000u ? b & 0x7FFFFFFFu : sizeof(T) == 2 ? ~b & 0xFFFF0000u : ~b;
-            return k ? __uint_as_float(b) : -INFINITY;
+    const uint32_t at = v * E, last = H - E;
+    const u4 r = *(const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
+    const uint32_t n = H % E;
+    if (n == 0) { // of all lanes alike
+#pragma unroll
+        for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
+    } else {
+        const uint32_t up = E - n, words = up * sizeof(T) / 4;
+        uint32_t w[5];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; k++) {
+            w[k] = r[k];
+#pragma unroll
+            for (uint32_t d = 1; d < 4; d++) w[k] = words == d ? (d + k < 4 ? r[(d + k) & 3] : fill) : w[k];
         }
+        w[4] = fill;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            if (sizeof(T) == 2) w[k] = up & 1 ? __builtin_amdgcn_alignbit(w[k + 1], w[k], 16) : w[k];
+            p.r.w[k] = at > last ? w[k] : r[k];
+        }
+    }
+}
+
+// A score and its class as one number that is the greater the better, and no two are alike: the score in an order that numbers have (zeros alike), and below it the
+// class such that of two equal scores the lower one's is the greater.  Scores of -inf, and what is behind a row, are below every other.
+template <typename T>
+struct Best {
+    // 16-bit scores: a whole number of 32 bits, the score's sign and magnitude as its upper half
+    typedef int32_t type;
+    static constexpr int32_t INF = std::is_same<T, bf16_t>::value ? 0x7F80 : 0x7C00;
+    static constexpr uint32_t NONE = (0x8000u | INF) << 16 | 0x8000u | INF; // -inf, twice
+    static __device__ __forceinline__ int32_t lowest() { return INT32_MIN; }
+    static __device__ __forceinline__ void of(const Piece<T> &p, uint32_t c0, int32_t *v, bool &odd) {
+        typedef short s2 __attribute__((ext_vector_type(2)));
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 most = {0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint32_t x = p.r.w[j], size = x & 0x7FFF7FFFu;
+            const s2 m = __builtin_bit_cast(s2, x) >> (short)15;
+            const uint32_t s = __builtin_bit_cast(uint32_t, __builtin_bit_cast(s2, size ^ __builtin_bit_cast(uint32_t, m)) - m);
+            most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, size));
+            v[2 * j] = (int32_t)(s << 16 | (0xFFFFu - (c0 + 2 * j)));
+            v[2 * j + 1] = (int32_t)((s & 0xFFFF0000u) | (0xFFFFu - (c0 + 2 * j + 1)));
+        }
+        odd |= most[0] > INF || most[1] > INF;
+    }
+    // scores that are no numbers are the best there are
+    static __device__ void nan_first(const Piece<T> &p, int32_t *v) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (((p.r.w[j / 2] >> (16 * (j & 1))) & 0x7FFFu) > INF) v[j] = (int32_t)(0x7FFF0000u | ((uint32_t)v[j] & 0xFFFFu));
+    }
+    static __device__ __forceinline__ bool is_class(int32_t k) { return (k >> 16) > -INF; }
+    static __device__ __forceinline__ int of_class(int32_t k) { return 0xFFFF - (k & 0xFFFF); }
+    static __device__ __forceinline__ float score(int32_t k) {
+        const int32_t s = k >> 16;
+        const uint32_t bits = (uint32_t)(s < 0 ? 0x8000 - s : s);
+        return (float)__builtin_bit_cast(T, (uint16_t)bits);
+    }
+    static __device__ __forceinline__ int32_t greater(int32_t a, int32_t b) { return a > b ? a : b; }
+    static __device__ __forceinline__ int32_t lesser(int32_t a, int32_t b) { return a < b ? a : b; }
+    template <int CTRL>
+    static __device__ __forceinline__ int32_t moved(int32_t v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+    // the two that lanes D apart have, in both of them
+    template <int D>
+    static __device__ __forceinline__ void both(int32_t v, int32_t &x, int32_t &y) {
+        const auto h = D == 16 ? __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false) : __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+        x = (int32_t)h[0];
+        y = (int32_t)h[1];
+    }
+};
+template <>
+struct Best<float> {
+    // 32-bit scores: a double of the score, exact, with the class in the lowest 12 of the 29 bits that the score leaves 0.  Doubles have a maximum and a minimum of one
+    // instruction each where a pair of words takes a comparison and four choices.
+    typedef double type;
+    static constexpr uint32_t NONE = 0xFF800000u;
+    static __device__ __forceinline__ double lowest() { return -0x1p129; }
+    static __device__ __forceinline__ double tagged(double d, uint32_t c) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, d);
+        const uint32_t sign = (uint32_t)((int32_t)(b >> 32) >> 31);
+        return __builtin_bit_cast(double, b | ((c ^ ~sign) & 0xFFFu));
+    }
+    static __device__ __forceinline__ void of(const Piece<float> &p, uint32_t c0, double *v, bool &odd) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float x = __uint_as_float(p.r.w[j]) + 0.0f; // -0 becomes 0
+            odd |= !(x < INFINITY);
+            v[j] = tagged(fmax((double)x, -0x1p129), c0 + j);
+        }
+    }
+    static __device__ void nan_first(const Piece<float> &p, double *v) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float x = __uint_as_float(p.r.w[j]);
+            // +inf with a tag would be no number
+            if (!(x < INFINITY)) v[j] = tagged(x != x ? 0x1p130 : 0x1p129, of_class(v[j]));
+        }
+    }
+    static __device__ __forceinline__ bool is_class(double k) { return k > -0x1p128; }
+    static __device__ __forceinline__ int of_class(double k) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, k);
+        return (int)(((uint32_t)b ^ ~(uint32_t)((int32_t)(b >> 32) >> 31)) & 0xFFFu);
+    }
+    static __device__ __forceinline__ float score(double k) { // infinite for no number, too
+        return (float)__builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~0xFFFull);
+    }
+    static __device__ __forceinline__ double greater(double a, double b) { return fmax(a, b); }
+    static __device__ __forceinline__ double lesser(double a, double b) { return fmin(a, b); }
+    template <int CTRL>
+    static __device__ __forceinline__ double moved(double v) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        return __builtin_bit_cast(double, (uint64_t)(uint32_t)Best<bf16_t>::moved<CTRL>((int32_t)(b >> 32)) << 32 | (uint32_t)Best<bf16_t>::moved<CTRL>((int32_t)b));
+    }
+    template <int D>
+    static __device__ __forceinline__ void both(double v, double &x, double &y) {
+        const uint64_t b = __builtin_bit_cast(uint64_t, v);
+        int32_t x1, y1, x0, y0;
+        Best<bf16_t>::both<D>((int32_t)(b >> 32), x1, y1);
+        Best<bf16_t>::both<D>((int32_t)b, x0, y0);
+        x = __builtin_bit_cast(double, (uint64_t)(uint32_t)x1 << 32 | (uint32_t)x0);
+        y = __builtin_bit_cast(double, (uint64_t)(uint32_t)y1 << 32 | (uint32_t)y0);
     }
 };
 
-template <int G>
-__device__ __forceinline__ uint32_t lanes_max(uint32_t v) {
-    return __float_as_uint(over_lanes<G>(__uint_as_float(v), [](float a, float b) {
-        const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-        return __uint_as_float(x > y ? x : y);
-    }));
-}
-template <int G>
-__device__ __forceinline__ uint64_t lanes_max(uint64_t v) {
-    const uint32_t hi = (uint32_t)(v >> 32), most = lanes_max<G>(hi);
-    return (uint64_t)most << 32 | lanes_max<G>(hi == most ? (uint32_t)v : 0u);
-}
-
-// The greater one first
-template <typename K>
-__device__ __forceinline__ void order(K &a, K &b) {
-    const bool less = a < b;
-    const K x = less ? b : a, y = less ? a : b;
+template <typename T, typename V>
+__device__ __forceinline__ void order(V &a, V &b) { // the greater one first
+    const V x = Best<T>::greater(a, b), y = Best<T>::lesser(a, b);
     a = x;
     b = y;
 }
-// Batcher's odd-even merge sort of n values, descending
-template <int N, typename K>
-__device__ __forceinline__ void sort_values(K *v) {
+// Batcher's odd-even merge sort of N values, descending
+template <typename T, int N, typename V>
+__device__ __forceinline__ void sort_values(V *v) {
 #pragma unroll
     for (int p = 1; p < N; p *= 2)
 #pragma unroll
@@ -91,69 +180,159 @@ __device__ __forceinline__ void sort_values(K *v) {
             for (int j = k % p; j + k < N; j += 2 * k)
 #pragma unroll
                 for (int i = 0; i < k; i++)
-                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order(v[i + j], v[i + j + k]);
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) order<T>(v[i + j], v[i + j + k]);
+}
+// The K best of two descending lists of K, into the first: the greater ones of the first and the second turned round are they, in an order that rises and falls, which
+// the halves' exchanges (Batcher's bitonic ones) make descend.
+template <typename T, int K, typename V, typename F>
+__device__ __forceinline__ void join(V *a, F &&other) {
+    V c[K];
+#pragma unroll
+    for (int i = 0; i < K; i++) c[i] = Best<T>::greater(a[i], other(K - 1 - i));
+#pragma unroll
+    for (int i = 0; i < K; i++) a[i] = c[i];
+#pragma unroll
+    for (int k = K / 2; k >= 1; k /= 2)
+#pragma unroll
+        for (int i = 0; i < K; i++)
+            if ((i & k) == 0) order<T>(a[i], a[i + k]);
+}
+// ... of the G lanes that share a row, in every one of them
+template <typename T, int K, int G, typename V>
+__device__ __forceinline__ void join_lanes(V *a) {
+    typedef Best<T> B;
+    if (G >= 2) join<T, K>(a, [&](int i) { return B::template moved<0xB1>(a[i]); });
+    if (G >= 4) join<T, K>(a, [&](int i) { return B::template moved<0x4E>(a[i]); });
+    if (G >= 8) join<T, K>(a, [&](int i) { return B::template moved<0x141>(a[i]); });
+    if (G >= 16) join<T, K>(a, [&](int i) { return B::template moved<0x140>(a[i]); });
+    V b[K];
+    if (G >= 32) {
+#pragma unroll
+        for (int i = 0; i < K; i++) B::template both<16>(a[i], a[i], b[i]);
+        join<T, K>(a, [&](int i) { return b[i]; });
+    }
+    if (G >= 64) {
+#pragma unroll
+        for (int i = 0; i < K; i++) B::template both<32>(a[i], a[i], b[i]);
+        join<T, K>(a, [&](int i) { return b[i]; });
+    }
 }
 
-// A row to G lanes of a wavefront, NV pieces a lane.  A lane sorts what it has; the best of a row is then the best of its lanes' first ones, and the lane that had it moves up.
-template <typename T, int G, int NV>
+template <typename T, int NV, int G>
+__device__ __forceinline__ void load_scores(Piece<T> *p, const T *x, int rank, int V) {
+    constexpr int E = Piece<T>::E;
+    constexpr uint32_t NONE = Best<T>::NONE;
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        const int c = (rank + i * G) * E;
+#pragma unroll
+        for (int k = 0; k < 4; k++) p[i].r.w[k] = NONE;
+        if (V >= E) {
+            if (c < V) load_piece<false>(p[i], x, rank + i * G, V, NONE);
+        } else if (c < V) {
+            p[i].load_some(x, V);
+#pragma unroll
+            for (int k = 0; k < E; k++)
+                if (k >= V) {
+                    if (sizeof(T) == 4) p[i].r.w[k & 3] = NONE;
+                    else p[i].r.w[k / 2] = k & 1 ? (p[i].r.w[k / 2] & 0xFFFFu) | (NONE & 0xFFFF0000u) : (p[i].r.w[k / 2] & 0xFFFF0000u) | (NONE & 0xFFFFu);
+                }
+        }
+    }
+}
+
+// A row to G lanes of a wavefront, NV pieces a lane: each lane finds the K best of its scores by sorting K at a time and joining, then the lanes join theirs.  MORE: any
+// number, from as many lists of K as there are: the lists' first ones are compared and the lane that has the best moves up.
+template <typename T, int G, int NV, int K, bool MORE>
 __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
-    constexpr int E = Piece<T>::E, N = E * NV, ROWS = 256 / G;
-    typedef typename Key<T>::type K;
-    extern __shared__ __align__(16) unsigned char s_dyn[]; // [ROWS][top] keys
+    constexpr int E = Piece<T>::E, N = E * NV, ROWS = 256 / G, KEPT = MORE ? N : K;
+    typedef Best<T> B;
+    typedef typename B::type Value;
+    extern __shared__ __align__(16) unsigned char s_dyn[]; // MORE: [ROWS][top] of the best
     const int rank = threadIdx.x & (G - 1), slot = threadIdx.x / G, V = a.V;
-    K *const s_best = (K *)s_dyn + slot * a.top;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + slot; row < a.N; row += (int64_t)gridDim.x * ROWS) {
-        const T *x = (const T *)a.x + row * a.xs;
         Piece<T> p[NV];
+        load_scores<T, NV, G>(p, (const T *)a.x + row * a.xs, rank, V);
+        Value v[N];
+        bool odd = false;
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (rank + i * G) * E;
-            p[i].r = {};
-            if (c + E <= V) p[i].load(x + c);
-            else if (c < V) p[i].load_some(x + c, V - c);
+        for (int i = 0; i < NV; i++) B::of(p[i], (rank + i * G) * E, v + i * E, odd);
+        if (__builtin_expect(__any(odd), 0)) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) B::nan_first(p[i], v + i * E);
         }
-        K v[N];
-        float f[N];
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            p[i].get(f + i * E);
+        for (int i = 0; i < N; i += KEPT) sort_values<T, KEPT>(v + i);
+        float most, total = 0.0f;
+        Value *const s_best = (Value *)s_dyn + slot * a.top;
+        if constexpr (MORE) {
+            for (int j = 0; j < a.top; j++) {
+                Value best[1] = {v[0]};
+                join_lanes<T, 1, G>(best);
+                if (j == 0) most = B::score(best[0]);
+                if (B::is_class(best[0])) total += exp_gap(B::score(best[0]), most, a.exp_mul);
+                if (rank == 0) s_best[j] = best[0];
+                if (v[0] == best[0]) {
 #pragma unroll
-            for (int k = 0; k < E; k++) {
-                const int c = (rank + i * G) * E + k;
-                if (c >= V) f[i * E + k] = -INFINITY;
-                v[i * E + k] = Key<T>::of(f[i * E + k], c);
+                    for (int i = 0; i + 1 < N; i++) v[i] = v[i + 1];
+                    v[N - 1] = B::lowest();
+                }
             }
-        }
-        sort_values<N>(v);
-        float most = 0.0f, total = 0.0f;
-        for (int j = 0; j < a.top; j++) {
-            const K best = lanes_max<G>(v[0]);
-            const float score = Key<T>::score(best);
-            if (j == 0) most = score;
-            total += best ? exp_gap(score, most, a.exp_mul) : 0.0f;
-            if (rank == 0) s_best[j] = best;
-            if (v[0] == best) {
+        } else {
 #pragma unroll
-                for (int i = 0; i + 1 < N; i++) v[i] = v[i + 1];
-                v[N - 1] = 0;
-            }
+            for (int s = K; s < N; s *= 2)
+#pragma unroll
+                for (int i = 0; i + s < N; i += 2 * s) join<T, K>(v + i, [&](int k) { return v[i + s + k]; });
+            join_lanes<T, K, G>(v);
+            most = B::score(v[0]);
         }
         if (!a.renormalize) {
             total = 0.0f;
 #pragma unroll
-            for (int i = 0; i < N; i++) total += f[i] == -INFINITY ? 0.0f : exp_gap(f[i], most, a.exp_mul);
+            for (int i = 0; i < NV; i++) {
+                float f[E];
+                p[i].get(f);
+#pragma unroll
+                for (int k = 0; k < E; k++) total += f[k] == -INFINITY ? 0.0f : exp_gap(f[k], most, a.exp_mul);
+            }
             total = lanes_sum<G>(total);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const float inv = 1.0f / total;
-        for (int j = rank; j < a.top; j += G) {
-            const K best = s_best[j];
-            a.ids[row * a.top + j] = Key<T>::chosen(best);
-            a.w[row * a.top + j] = best ? exp_gap(Key<T>::score(best), most, a.exp_mul) * inv : 0.0f;
+        if constexpr (MORE) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const float inv = 1.0f / total;
+            for (int j = rank; j < a.top; j += G) {
+                const Value best = s_best[j];
+                const bool is = B::is_class(best);
+                a.ids[row * a.top + j] = is ? B::of_class(best) : -1;
+                a.w[row * a.top + j] = is ? exp_gap(B::score(best), most, a.exp_mul) * inv : 0.0f;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        } else { // lane j has the j-th best, or each lane every G-th
+            constexpr int MINE = K > G ? K / G : 1;
+            float e[MINE];
+            int id[MINE];
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < MINE; i++) {
+                Value best = v[0];
+#pragma unroll
+                for (int k = 1; k < K; k++) best = rank + i * G == k ? v[k] : best;
+                const bool is = rank + i * G < a.top && B::is_class(best);
+                id[i] = is ? B::of_class(best) : -1;
+                e[i] = is ? exp_gap(B::score(best), most, a.exp_mul) : 0.0f;
+                sum += e[i];
+            }
+            if (a.renormalize) total = lanes_sum<G>(sum);
+            const float inv = 1.0f / total;
+#pragma unroll
+            for (int i = 0; i < MINE; i++)
+                if (rank + i * G < a.top) {
+                    a.ids[row * a.top + rank + i * G] = id[i];
+                    a.w[row * a.top + rank + i * G] = id[i] >= 0 ? e[i] * inv : 0.0f;
+                }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
     }
 }
 
@@ -168,13 +347,7 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
         Piece<T> p[NV];
         if (!a.renormalize) {
             const T *x = (const T *)a.x + row * a.xs;
-#pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const int c = (rank + i * G) * E;
-                p[i].r = {};
-                if (c + E <= V) p[i].load(x + c);
-                else if (c < V) p[i].load_some(x + c, V - c);
-            }
+            load_scores<T, NV, G>(p, x, rank, V);
         }
         float mean = 0.0f;
         bool none = false; // an id of no class
@@ -203,7 +376,6 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
                 p[i].get(f + i * E);
 #pragma unroll
                 for (int k = 0; k < E; k++) {
-                    if ((rank + i * G) * E + k >= V) f[i * E + k] = -INFINITY;
                     m = fmaxf(m, f[i * E + k]);
                 }
             }
@@ -459,39 +631,6 @@ __device__ __forceinline__ void drop_values(const RowArgs &a, uint64_t key, uint
 }
 __device__ __forceinline__ uint64_t drop_key(const RowArgs &a) { return mixed((a.seed_at ? *a.seed_at : a.seed) + ((uint64_t)a.layer + 1) * GAMMA); }
 
-typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
-// Piece v of a row of H values.  The last one, where it is not whole, is read from where it ends and moved down, without a branch.  TINY: rows
-// of less than a piece
-template <bool TINY, typename T>
-__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H) {
-    constexpr uint32_t E = Piece<T>::E;
-    if (TINY) {
-        p.load_some(x, H);
-        return;
-    }
-    const uint32_t at = v * E, last = H - E;
-    const u4 r = *(const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
-    const uint32_t n = H % E;
-    if (n == 0) { // of all lanes alike
-#pragma unroll
-        for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
-    } else {
-        const uint32_t up = E - n, words = up * sizeof(T) / 4;
-        uint32_t w[5];
-#pragma unroll
-        for (uint32_t k = 0; k < 4; k++) {
-            w[k] = r[k];
-#pragma unroll
-            for (uint32_t d = 1; d < 4; d++) w[k] = words == d ? (d + k < 4 ? r[(d + k) & 3] : 0u) : w[k];
-        }
-        w[4] = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (sizeof(T) == 2) w[k] = up & 1 ? __builtin_amdgcn_alignbit(w[k + 1], w[k], 16) : w[k];
-            p.r.w[k] = at > last ? w[k] : r[k];
-        }
-    }
-}
 template <bool TINY, typename T>
 __device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v, uint32_t H) {
     constexpr uint32_t E = Piece<T>::E;
@@ -703,18 +842,26 @@ __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
 
 // ---- launches --------------------------------------------------------------------------------
 
-// Lanes that share a row: enough for sixteen scores each, all of a wavefront from 1024 scores on
+// Lanes that share a row: enough for sixteen scores each; from 129 16-bit scores on for 32
 template <typename T, int G, int NV, bool GRAD>
 static void launch_route_as(hipStream_t s, const RouteArgs &a) {
     constexpr int ROWS = 256 / G;
     const int64_t blocks = (a.N + ROWS - 1) / ROWS;
     const dim3 grid((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22));
     if constexpr (GRAD) hipLaunchKernelGGL((k_route_grad<T, G, NV>), grid, dim3(256), ROWS * G * NV * Piece<T>::E * 4, s, a);
-    else hipLaunchKernelGGL((k_route<T, G, NV>), grid, dim3(256), ROWS * a.top * sizeof(typename Key<T>::type), s, a);
+    else if (a.top <= 2) hipLaunchKernelGGL((k_route<T, G, NV, 2, false>), grid, dim3(256), 0, s, a);
+    else if (a.top <= 4) hipLaunchKernelGGL((k_route<T, G, NV, 4, false>), grid, dim3(256), 0, s, a);
+    else if (a.top <= 8) hipLaunchKernelGGL((k_route<T, G, NV, 8, false>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_route<T, G, NV, 0, true>), grid, dim3(256), ROWS * a.top * sizeof(typename Best<T>::type), s, a);
 }
 template <typename T, bool GRAD>
 static void launch_route_typed(hipStream_t s, const RouteArgs &a) {
     constexpr int U = 16 / Piece<T>::E;
+    if constexpr (sizeof(T) == 2 && !GRAD) {
+        if (a.V > 128 && a.V <= 256) return launch_route_as<T, 8, 2 * U, GRAD>(s, a);
+        if (a.V > 256 && a.V <= 512) return launch_route_as<T, 16, 2 * U, GRAD>(s, a);
+        if (a.V > 512 && a.V <= 1024) return launch_route_as<T, 32, 2 * U, GRAD>(s, a);
+    }
     const int n = (a.V + 15) / 16; // lanes
     if (n <= 1) launch_route_as<T, 1, U, GRAD>(s, a);
     else if (n <= 2) launch_route_as<T, 2, U, GRAD>(s, a);

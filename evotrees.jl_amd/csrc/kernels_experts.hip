@@ -639,20 +639,26 @@ __device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v,
     else p.store_some(o, H % E);
 }
 
+// The block of rows that a block has, of as many as the 8 dies divide.  Blocks go round the dies, and each of them has the next of its own eighth of the rows: neighbours among an
+// expert's sorted rows come from neighbouring rows, so that the line where one ends and the next begins is put together in one die's cache (32 768 x 8 rows of 4099
+// bf16 sorted: 597 us with the blocks as they come, 546 so; of 4096 values, whole lines, 479 | 491)
+__device__ __forceinline__ uint32_t own_block(uint32_t blocks) {
+    return (blockIdx.x & 7) * (blocks / 8) + blockIdx.x / 8;
+}
 // The row and piece that a thread has.  ROW: a wavefront's are of one row, which the compiler knows; otherwise the pieces of all rows follow each other, and
 // no lane is idle.
 template <bool ROW>
 struct Share {
     uint32_t row, v;
     bool in;
-    __device__ __forceinline__ Share(const RowArgs &a) {
+    __device__ __forceinline__ Share(const RowArgs &a, uint32_t block) {
         if (ROW) {
-            const uint32_t i = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + threadIdx.x / 64), r = i / a.parts;
+            const uint32_t i = __builtin_amdgcn_readfirstlane(block * 4 + threadIdx.x / 64), r = i / a.parts;
             v = (i - r * a.parts) * 64 + (threadIdx.x & 63);
             row = a.row0 + r;
             in = row < a.N && v < a.pieces;
         } else {
-            const uint32_t i = blockIdx.x * 256 + threadIdx.x, r = i / a.pieces;
+            const uint32_t i = block * 256 + threadIdx.x, r = i / a.pieces;
             v = i - r * a.pieces;
             row = a.row0 + r;
             in = row < a.N;
@@ -668,7 +674,7 @@ __device__ void clear_behind(const RowArgs &a, uint32_t block) {
     z.r = {};
     const int count = *a.count;
     for (uint32_t p = (count < 0 ? 0u : (uint32_t)count) + block; p < a.n; p += TAIL_BLOCKS)
-        for (uint32_t v = threadIdx.x; v < a.pieces; v += 256) store_piece<TINY>(z, (T *)a.out + p * a.os, v, a.H);
+        for (uint32_t v = threadIdx.x; v < a.pieces; v += blockDim.x) store_piece<TINY>(z, (T *)a.out + p * a.os, v, a.H);
 }
 
 // Rows to their places: each row is read once and written `top` times, times a weight if there are weights
@@ -679,7 +685,7 @@ __global__ __launch_bounds__(256) void k_spread(RowArgs a) {
         if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
         return;
     }
-    const Share<ROW> me(a);
+    const Share<ROW> me(a, own_block(gridDim.x - TAIL_BLOCKS));
     if (!me.in) return;
     Piece<T> p;
     load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
@@ -706,18 +712,19 @@ __global__ __launch_bounds__(256) void k_spread(RowArgs a) {
     }
 }
 
-// ... and the sums of its products with the rows that lie at these places in y: a row to G threads.
+// ... and the sums of its products with the rows that lie at these places in y: a row to G lanes, or (G = 0) to a block of as many wavefronts as it has.
 template <typename T, int G, int TOP, bool TINY, bool DROP>
-__global__ __launch_bounds__(G < 256 ? 256 : G) void k_spread_dot(RowArgs a) {
-    constexpr int E = Piece<T>::E, THREADS = G < 256 ? 256 : G, ROWS = THREADS / G, W = G / 64;
-    __shared__ float s_dot[W > 1 ? W : 1][TOP];
+__global__ __launch_bounds__(G ? 256 : 1024) void k_spread_dot(RowArgs a) {
+    constexpr int E = Piece<T>::E, ROWS = G ? 256 / G : 1;
+    __shared__ float s_dot[G ? 1 : 16][TOP];
+    const uint32_t size = G ? G : blockDim.x;
     if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
-        if (a.row0 == 0 && threadIdx.x < 256) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
+        if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
         return;
     }
-    const uint32_t rank = threadIdx.x & (G - 1), slot = G >= 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / G) : threadIdx.x / G;
-    const uint32_t row = a.row0 + blockIdx.x * ROWS + slot;
-    if (ROWS > 1 && row >= a.N) return;
+    const uint32_t rank = G ? threadIdx.x & (G - 1) : threadIdx.x, slot = G == 0 ? 0 : G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / (G ? G : 1);
+    const uint32_t row = a.row0 + own_block(gridDim.x - TAIL_BLOCKS) * ROWS + slot;
+    if (row >= a.N) return;
     const T *x = (const T *)a.x + row * a.xs;
     const uint64_t key = DROP ? drop_key(a) : 0;
     const size_t e0 = (size_t)row * a.top;
@@ -730,7 +737,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_spread_dot(RowArgs a) {
             w[j] = j0 + j < a.top ? a.w[e0 + j0 + j] : 0.0f;
             dot[j] = 0.0f;
         }
-        for (uint32_t v = rank; v < a.pieces; v += G) {
+        for (uint32_t v = rank; v < a.pieces; v += size) {
             Piece<T> p, q[TOP];
             float f[E];
             load_piece<TINY>(p, x, v, a.H);
@@ -755,8 +762,8 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_spread_dot(RowArgs a) {
                 }
         }
 #pragma unroll
-        for (int j = 0; j < TOP; j++) dot[j] = lanes_sum<(G < 64 ? G : 64)>(dot[j]);
-        if (W > 1) {
+        for (int j = 0; j < TOP; j++) dot[j] = lanes_sum<(G ? G : 64)>(dot[j]);
+        if constexpr (G == 0) {
             if (j0) __syncthreads();
             if ((threadIdx.x & 63) == 0) {
 #pragma unroll
@@ -765,8 +772,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_spread_dot(RowArgs a) {
             __syncthreads();
             if (threadIdx.x < TOP && j0 + threadIdx.x < a.top) {
                 float sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < W; k++) sum += s_dot[k][threadIdx.x];
+                for (uint32_t k = 0; k < blockDim.x / 64; k++) sum += s_dot[k][threadIdx.x];
                 a.dw[e0 + j0 + threadIdx.x] = sum;
             }
         } else if (rank == 0) {
@@ -781,7 +787,7 @@ __global__ __launch_bounds__(G < 256 ? 256 : G) void k_spread_dot(RowArgs a) {
 template <typename T, bool ROW, bool TINY, int TOP, bool DROP>
 __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     constexpr int E = Piece<T>::E;
-    const Share<ROW> me(a);
+    const Share<ROW> me(a, own_block(gridDim.x));
     if (!me.in) return;
     Piece<T> res;
     float sum[E] = {};
@@ -822,7 +828,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
 template <typename T, bool ROW, bool TINY>
 __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
     constexpr int E = Piece<T>::E;
-    const Share<ROW> me(a);
+    const Share<ROW> me(a, blockIdx.x);
     if (!me.in) return;
     Piece<T> p, res;
     float f[E];
@@ -882,9 +888,11 @@ static int launch_route(hipStream_t s, const RouteArgs &a, int dtype) {
     return EVT_OK;
 }
 
+static unsigned round_up(unsigned blocks) { return (blocks + 7) / 8 * 8; }
 enum { ROWS_SPREAD, ROWS_COMBINE, ROWS_DROP };
 template <typename T, bool ROW, bool TINY, int OP>
 static void launch_rows_as(hipStream_t s, const RowArgs &a, unsigned grid) {
+    grid = round_up(grid);
     if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, ROW, TINY>), dim3(grid), dim3(256), 0, s, a);
     else if constexpr (OP == ROWS_SPREAD) {
         if (a.drop) hipLaunchKernelGGL((k_spread<T, ROW, TINY, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
@@ -900,12 +908,12 @@ static void launch_rows_as(hipStream_t s, const RowArgs &a, unsigned grid) {
     }
 }
 template <typename T, int G, bool TINY>
-static void launch_dot_as(hipStream_t s, const RowArgs &a, unsigned groups) {
-    constexpr int THREADS = G < 256 ? 256 : G, ROWS = THREADS / G;
-    const unsigned grid = (groups + ROWS - 1) / ROWS + TAIL_BLOCKS;
+static void launch_dot_as(hipStream_t s, const RowArgs &a, unsigned groups, int threads = 256) {
+    constexpr int ROWS = G ? 256 / G : 1;
+    const unsigned grid = round_up((groups + ROWS - 1) / ROWS) + TAIL_BLOCKS;
     const auto go = [&](auto top) {
-        if (a.drop) hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, true>), dim3(grid), dim3(THREADS), 0, s, a);
-        else hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, false>), dim3(grid), dim3(THREADS), 0, s, a);
+        if (a.drop) hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, true>), dim3(grid), dim3(threads), 0, s, a);
+        else hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, false>), dim3(grid), dim3(threads), 0, s, a);
     };
     if (a.top <= 2) go(std::integral_constant<int, 2>());
     else if (a.top <= 4) go(std::integral_constant<int, 4>());
@@ -927,8 +935,13 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
             else if (a.pieces <= 8) launch_dot_as<T, 8, false>(s, a, rows);
             else if (a.pieces <= 16) launch_dot_as<T, 16, false>(s, a, rows);
             else if (a.pieces <= 32) launch_dot_as<T, 32, false>(s, a, rows);
-            else if (a.pieces <= 128) launch_dot_as<T, 64, false>(s, a, rows);
-            else launch_dot_as<T, 256, false>(s, a, rows);
+            else if (a.pieces <= 64) launch_dot_as<T, 64, false>(s, a, rows);
+            else {
+                // blocks of up to 4 wavefronts in as many turns as it takes (32 768 rows of 8 x 4096 bf16: 1022 us by 8 or 16 wavefronts, 913 so; of 4099 1352 and
+                // 1664 | 1083), of up to 16 where rows are few (16 rows of 8 x 16 384: 20.4 us by 4, 11.1 by 16; 512 of 4096 16.3 | 14.9)
+                const int most = rows <= 512 ? 16 : 4, turns = (a.parts + most - 1) / most;
+                launch_dot_as<T, 0, false>(s, a, rows, 64 * ((a.parts + turns - 1) / turns));
+            }
         } else if (tiny) launch_rows_as<T, false, true, OP>(s, a, (rows + 255) / 256);
         else if (by_row) launch_rows_as<T, true, false, OP>(s, a, (unsigned)(((uint64_t)rows * a.parts + 3) / 4));
         else launch_rows_as<T, false, false, OP>(s, a, (unsigned)(((uint64_t)rows * a.pieces + 255) / 256));

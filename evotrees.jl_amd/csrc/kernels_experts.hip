@@ -420,8 +420,6 @@ struct PlanArgs {
     int32_t id64, E, bits, nb;
     int32_t *place, *source, *offsets, *table;
 };
-#define PLAN_ITEMS 16
-#define PLAN_CHUNK (256 * PLAN_ITEMS) // entries of a block
 
 __device__ __forceinline__ int expert_of(const PlanArgs &a, int64_t i) {
     if (i >= a.n) return -1;
@@ -430,40 +428,47 @@ __device__ __forceinline__ int expert_of(const PlanArgs &a, int64_t i) {
 }
 
 // How many entries of each block's an expert has: table[block][expert], or [expert][block] for many blocks
+template <int ITEMS>
 __global__ __launch_bounds__(256) void k_plan_count(PlanArgs a, int by_expert) {
-    __shared__ int s_n[MAX_EXPERTS];
-    for (int e = threadIdx.x; e < a.E; e += 256) s_n[e] = 0;
-    __syncthreads();
-    const int64_t first = (int64_t)blockIdx.x * PLAN_CHUNK + threadIdx.x;
-    int id[PLAN_ITEMS];
+    extern __shared__ __align__(16) int s_plan[]; // [E]
+    for (int e = threadIdx.x; e < a.E; e += 256) s_plan[e] = 0;
+    const int64_t first = (int64_t)blockIdx.x * (256 * ITEMS) + threadIdx.x;
+    int id[ITEMS];
 #pragma unroll
-    for (int i = 0; i < PLAN_ITEMS; i++) id[i] = expert_of(a, first + i * 256);
-#pragma unroll
-    for (int i = 0; i < PLAN_ITEMS; i++)
-        if (id[i] >= 0) atomicAdd(s_n + id[i], 1);
+    for (int i = 0; i < ITEMS; i++) id[i] = expert_of(a, first + i * 256);
     __syncthreads();
-    for (int e = threadIdx.x; e < a.E; e += 256) a.table[by_expert ? (int64_t)e * a.nb + blockIdx.x : (int64_t)blockIdx.x * a.E + e] = s_n[e];
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++)
+        if (id[i] >= 0) atomicAdd(s_plan + id[i], 1);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += 256) a.table[by_expert ? (int64_t)e * a.nb + blockIdx.x : (int64_t)blockIdx.x * a.E + e] = s_plan[e];
 }
 
+// Inclusive sum over the wavefront's lanes: within rows of sixteen by shifts, then the rows' last ones go to the rows behind
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int sum_from(int v) { return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int lanes_inclusive(int v) {
+    v = sum_from<0x111, 0xf>(v); // row_shr 1, 2, 4, 8
+    v = sum_from<0x112, 0xf>(v);
+    v = sum_from<0x114, 0xf>(v);
+    v = sum_from<0x118, 0xf>(v);
+    v = sum_from<0x142, 0xa>(v); // row_bcast 15
+    return sum_from<0x143, 0xc>(v); // row_bcast 31
+}
 // The block's exclusive sum over its threads' values, and all of it
 template <int W>
 __device__ __forceinline__ int block_exclusive(int v, int &all) {
     __shared__ int s_w[W];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int sum = v;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int u = __shfl_up(sum, d);
-        if (lane >= d) sum += u;
-    }
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sum = lanes_inclusive(v);
     if (lane == 63) s_w[wave] = sum;
     __syncthreads();
     int before = 0;
     all = 0;
 #pragma unroll
     for (int w = 0; w < W; w++) {
-        if (w < wave) before += s_w[w];
-        all += s_w[w];
+        const int n = s_w[w];
+        if (w < wave) before += n;
+        all += n;
     }
     __syncthreads();
     return before + sum - v;
@@ -500,26 +505,40 @@ enum { PLAN_ALONE, PLAN_BLOCKS, PLAN_SUMS };
 template <int W, int ITEMS, int FROM>
 __global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
     constexpr int THREADS = 64 * W;
-    extern __shared__ __align__(16) int s_plan[]; // [E] where the block's entries of an expert start, then [W / 2][E] pairs of wavefronts' counts
-    int *const s_base = s_plan;
-    uint16_t *const s_wave = (uint16_t *)(s_plan + a.E);
+    // [E] where the block's entries of an expert start, [W / 2][E] pairs of wavefronts' counts, and of PLAN_BLOCKS [2][E] the blocks' sums
+    extern __shared__ __align__(16) int s_plan[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), E = a.E;
-    for (int e = threadIdx.x; e < E * (W / 2); e += THREADS) s_plan[E + e] = 0;
-    const int64_t first = ((int64_t)blockIdx.x * W + wave) * (64 * ITEMS) + lane;
+    int *const s_base = s_plan, *const s_all = s_plan + E * (1 + W / 2), *const s_before = s_all + E;
+    uint16_t *const s_wave = (uint16_t *)(s_plan + E);
+    for (int e = threadIdx.x; e < E * (W / 2 + (FROM == PLAN_BLOCKS ? 2 : 0)); e += THREADS) s_plan[E + e] = 0;
+    const int64_t wave0 = ((int64_t)blockIdx.x * W + wave) * (64 * ITEMS), first = wave0 + lane;
     int id[ITEMS];
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) id[i] = expert_of(a, first + i * 64);
     __syncthreads();
-    const auto half = [&](int e) { return ((wave >> 1) * E + e) * 2 + (wave & 1); };
 #pragma unroll
     for (int i = 0; i < ITEMS; i++)
         if (id[i] >= 0) atomicAdd(s_plan + E + (wave >> 1) * E + id[i], 1 << (16 * (wave & 1)));
+    if (FROM == PLAN_BLOCKS) { // all of the blocks' counts, which are few
+        const int cells = a.nb * E, mine = blockIdx.x * E, step = THREADS % E;
+        int e = threadIdx.x % E;
+#pragma unroll 8
+        for (int c = threadIdx.x; c < cells; c += THREADS) {
+            const int n = a.table[c];
+            if (n) {
+                atomicAdd(s_all + e, n);
+                if (c < mine) atomicAdd(s_before + e, n);
+            }
+            e += step;
+            e -= e >= E ? E : 0;
+        }
+    }
     __syncthreads();
     // an expert's start: the threads have consecutive experts
     const int per = (E + THREADS - 1) / THREADS, e0 = threadIdx.x * per, e1 = e0 + per < E ? e0 + per : E;
     int sum = 0, all;
     for (int e = e0; e < e1; e++) {
-        int total = 0, before = 0, mine = 0;
+        int total, before = 0, mine = 0;
 #pragma unroll
         for (int w = 0; w < W; w++) {
             uint16_t &c = s_wave[((w >> 1) * E + e) * 2 + (w & 1)];
@@ -532,11 +551,8 @@ __global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
             total = a.table[(int64_t)E * a.nb + e];
             before = a.table[(int64_t)e * a.nb + blockIdx.x];
         } else {
-            for (int b = 0; b < a.nb; b++) {
-                const int n = a.table[(int64_t)b * E + e];
-                if (b < (int)blockIdx.x) before += n;
-                total += n;
-            }
+            total = s_all[e];
+            before = s_before[e];
         }
         s_base[e] = sum + before;
         if (blockIdx.x == 0) a.offsets[e] = sum;
@@ -551,18 +567,22 @@ __global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < ITEMS; i++) {
+        if (wave0 + i * 64 >= a.n) break;
         const int e = id[i];
-        uint64_t same = __ballot(e >= 0);
+        uint64_t same = __ballot(e >= 0); // the lanes with the same expert
+        uint32_t lo = (uint32_t)same, hi = (uint32_t)(same >> 32);
         for (int b = 0; b < a.bits; b++) {
-            const bool set = (e >> b) & 1;
-            const uint64_t with = __ballot(set);
-            same &= set ? with : ~with;
+            const uint32_t set = (uint32_t)__builtin_amdgcn_sbfe(e, b, 1); // all ones or none
+            const uint64_t with = __ballot(set != 0);
+            lo &= ~((uint32_t)with ^ set);
+            hi &= ~((uint32_t)(with >> 32) ^ set);
         }
+        same = (uint64_t)hi << 32 | lo;
         const int64_t at = first + i * 64;
         int pos = -1;
         if (e >= 0) {
-            const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(same >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)same, 0));
-            volatile uint16_t *c = s_wave + half(e);
+            const int before = __builtin_amdgcn_mbcnt_hi(hi, __builtin_amdgcn_mbcnt_lo(lo, 0));
+            volatile uint16_t *c = s_wave + ((wave >> 1) * E + e) * 2 + (wave & 1);
             const int n = *c + before;
             pos = s_base[e] + n;
             __builtin_amdgcn_wave_barrier();
@@ -959,24 +979,30 @@ static int launch_rows(hipStream_t s, RowArgs &a, int dtype) {
 static void launch_plan(hipStream_t s, PlanArgs &a) {
     a.bits = 0;
     while ((1 << a.bits) < a.E) a.bits++;
+    a.nb = 1;
+    if (a.n <= 1024) {
+        hipLaunchKernelGGL((k_plan_place<4, 4, PLAN_ALONE>), dim3(1), dim3(256), a.E * 12, s, a);
+        return;
+    }
     if (a.n <= 8192 && a.E <= 1024) {
-        a.nb = 1;
-        hipLaunchKernelGGL((k_plan_place<16, 8, PLAN_ALONE>), dim3(1), dim3(1024), a.E * 4 * 9, s, a);
+        hipLaunchKernelGGL((k_plan_place<16, 8, PLAN_ALONE>), dim3(1), dim3(1024), a.E * 36, s, a);
         return;
     }
-    a.nb = (int)((a.n + PLAN_CHUNK - 1) / PLAN_CHUNK);
-    if (a.nb <= 1) {
-        hipLaunchKernelGGL((k_plan_place<4, PLAN_ITEMS, PLAN_ALONE>), dim3(1), dim3(256), a.E * 4 * 3, s, a);
+    const bool small = a.n <= (int64_t)1024 * 1024;
+    const int chunk = small ? 1024 : 4096;
+    a.nb = (int)((a.n + chunk - 1) / chunk);
+    const dim3 grid(a.nb), block(256);
+    const bool few = (int64_t)a.nb * a.E <= 4096;
+    const size_t count_lds = a.E * 4, place_lds = a.E * 12;
+    if (small) hipLaunchKernelGGL(k_plan_count<4>, grid, block, count_lds, s, a, few ? 0 : 1);
+    else hipLaunchKernelGGL(k_plan_count<16>, grid, block, count_lds, s, a, 1);
+    if (small && few) {
+        hipLaunchKernelGGL((k_plan_place<4, 4, PLAN_BLOCKS>), grid, block, a.E * 20, s, a);
         return;
     }
-    const bool few = a.nb <= 32;
-    hipLaunchKernelGGL(k_plan_count, dim3(a.nb), dim3(256), 0, s, a, few ? 0 : 1);
-    if (few) {
-        hipLaunchKernelGGL((k_plan_place<4, PLAN_ITEMS, PLAN_BLOCKS>), dim3(a.nb), dim3(256), a.E * 4 * 3, s, a);
-        return;
-    }
-    hipLaunchKernelGGL(k_plan_sums, dim3(a.E), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((k_plan_place<4, PLAN_ITEMS, PLAN_SUMS>), dim3(a.nb), dim3(256), a.E * 4 * 3, s, a);
+    hipLaunchKernelGGL(k_plan_sums, dim3(a.E), block, 0, s, a);
+    if (small) hipLaunchKernelGGL((k_plan_place<4, 4, PLAN_SUMS>), grid, block, place_lds, s, a);
+    else hipLaunchKernelGGL((k_plan_place<4, 16, PLAN_SUMS>), grid, block, place_lds, s, a);
 }
 
 // ---- entry points ------------------------------------------------------------------------------

@@ -274,7 +274,7 @@ def plan_rows(experts, n_experts):
     if device < 0:
         raise ValueError("experts must be on a GPU, got %s" % on)
     tables = _make(device, torch.int32, (2 * n + n_experts + 1,), on)
-    work = _make(device, torch.int32, (((n + 4095) // 4096 + 1) * n_experts,), on)
+    work = _make(device, torch.int32, (((n + 1023) // 1024 + 1) * n_experts,), on)
     plan = RowPlan(rows, top, n_experts, device, on, tables)
     _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, work.data_ptr())
     return plan

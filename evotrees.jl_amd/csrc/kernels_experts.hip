@@ -27,10 +27,10 @@ struct RouteArgs {
 __device__ __forceinline__ float exp_gap(float x, float m, float mul) { return __builtin_amdgcn_exp2f((x - m) * mul); }
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
-// Piece v of a row of H values.  The last one, where it is not whole, is read from where it ends and moved down, without a branch; what is behind the row is
-// `fill`, two or one values of a word.  TINY: rows of less than a piece
+// Piece v of a row of H values, in two steps, so that several are on their way before the first is waited for.  The last one, where it is not whole, is read from where
+// the row ends...  TINY: rows of less than a piece
 template <bool TINY, typename T>
-__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H, uint32_t fill = 0) {
+__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H) {
     constexpr uint32_t E = Piece<T>::E;
     if (TINY) {
         p.load_some(x, H);
@@ -38,30 +38,34 @@ __device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, 
     }
     const uint32_t at = v * E, last = H - E;
     const u4 r = *(const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
+#pragma unroll
+    for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
+}
+// ... and moved down here; what is behind the row becomes `fill`, two or one values of a word.
+template <bool TINY, typename T>
+__device__ __forceinline__ void settle_piece(Piece<T> &p, uint32_t v, uint32_t H, uint32_t fill = 0) {
+    constexpr uint32_t E = Piece<T>::E;
     const uint32_t n = H % E;
-    if (n == 0) { // of all lanes alike
+    if (TINY || n == 0) return; // of all lanes alike
+    const uint32_t up = E - n, words = up * sizeof(T) / 4;
+    const bool moves = v * E > H - E;
+    uint32_t w[5];
 #pragma unroll
-        for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
-    } else {
-        const uint32_t up = E - n, words = up * sizeof(T) / 4;
-        uint32_t w[5];
+    for (uint32_t k = 0; k < 4; k++) {
+        w[k] = p.r.w[k];
 #pragma unroll
-        for (uint32_t k = 0; k < 4; k++) {
-            w[k] = r[k];
+        for (uint32_t d = 1; d < 4; d++) w[k] = words == d ? (d + k < 4 ? p.r.w[(d + k) & 3] : fill) : w[k];
+    }
+    w[4] = fill;
 #pragma unroll
-            for (uint32_t d = 1; d < 4; d++) w[k] = words == d ? (d + k < 4 ? r[(d + k) & 3] : fill) : w[k];
-        }
-        w[4] = fill;
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            if (sizeof(T) == 2) w[k] = up & 1 ? __builtin_amdgcn_alignbit(w[k + 1], w[k], 16) : w[k];
-            p.r.w[k] = at > last ? w[k] : r[k];
-        }
+    for (int k = 0; k < 4; k++) {
+        if (sizeof(T) == 2) w[k] = up & 1 ? __builtin_amdgcn_alignbit(w[k + 1], w[k], 16) : w[k];
+        p.r.w[k] = moves ? w[k] : p.r.w[k];
     }
 }
 
 // A score and its class as one number that is the greater the better, and no two are alike: the score in an order that numbers have (zeros alike), and below it the
-// class such that of two equal scores the lower one's is the greater.  Scores of -inf, and what is behind a row, are below every other.
+// class as a tag, counted from the last one down, so that of two equal scores the lower class's is the greater.  Scores of -inf, and what is behind a row, are below every other.
 template <typename T>
 struct Best {
     // 16-bit scores: a whole number of 32 bits, the score's sign and magnitude as its upper half
@@ -69,7 +73,8 @@ struct Best {
     static constexpr int32_t INF = std::is_same<T, bf16_t>::value ? 0x7F80 : 0x7C00;
     static constexpr uint32_t NONE = (0x8000u | INF) << 16 | 0x8000u | INF; // -inf, twice
     static __device__ __forceinline__ int32_t lowest() { return INT32_MIN; }
-    static __device__ __forceinline__ void of(const Piece<T> &p, uint32_t c0, int32_t *v, bool &odd) {
+    // the scores of a piece, with the tags that count down from `tag`
+    static __device__ __forceinline__ void of(const Piece<T> &p, uint32_t tag, int32_t *v, bool &odd) {
         typedef short s2 __attribute__((ext_vector_type(2)));
         typedef unsigned short us2 __attribute__((ext_vector_type(2)));
         us2 most = {0, 0};
@@ -79,8 +84,8 @@ struct Best {
             const s2 m = __builtin_bit_cast(s2, x) >> (short)15;
             const uint32_t s = __builtin_bit_cast(uint32_t, __builtin_bit_cast(s2, size ^ __builtin_bit_cast(uint32_t, m)) - m);
             most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, size));
-            v[2 * j] = (int32_t)(s << 16 | (0xFFFFu - (c0 + 2 * j)));
-            v[2 * j + 1] = (int32_t)((s & 0xFFFF0000u) | (0xFFFFu - (c0 + 2 * j + 1)));
+            v[2 * j] = (int32_t)(s << 16 | (tag - 2 * j));
+            v[2 * j + 1] = (int32_t)((s & 0xFFFF0000u) | (tag - 2 * j - 1));
         }
         odd |= most[0] > INF || most[1] > INF;
     }
@@ -90,8 +95,9 @@ struct Best {
         for (int j = 0; j < 8; j++)
             if (((p.r.w[j / 2] >> (16 * (j & 1))) & 0x7FFFu) > INF) v[j] = (int32_t)(0x7FFF0000u | ((uint32_t)v[j] & 0xFFFFu));
     }
+    static __device__ __forceinline__ void add_tag(int32_t &k, uint32_t tag) { k ^= (int32_t)tag; }
     static __device__ __forceinline__ bool is_class(int32_t k) { return (k >> 16) > -INF; }
-    static __device__ __forceinline__ int of_class(int32_t k) { return 0xFFFF - (k & 0xFFFF); }
+    static __device__ __forceinline__ int tag_of(int32_t k) { return k & 0xFFFF; }
     static __device__ __forceinline__ float score(int32_t k) {
         const int32_t s = k >> 16;
         const uint32_t bits = (uint32_t)(s < 0 ? 0x8000 - s : s);
@@ -100,7 +106,7 @@ struct Best {
     static __device__ __forceinline__ int32_t greater(int32_t a, int32_t b) { return a > b ? a : b; }
     static __device__ __forceinline__ int32_t lesser(int32_t a, int32_t b) { return a < b ? a : b; }
     template <int CTRL>
-    static __device__ __forceinline__ int32_t moved(int32_t v) { return __builtin_amdgcn_update_dpp(v, v, CTRL, 0xf, 0xf, false); }
+    static __device__ __forceinline__ int32_t moved(int32_t v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
     // the two that lanes D apart have, in both of them
     template <int D>
     static __device__ __forceinline__ void both(int32_t v, int32_t &x, int32_t &y) {
@@ -116,31 +122,30 @@ struct Best<float> {
     typedef double type;
     static constexpr uint32_t NONE = 0xFF800000u;
     static __device__ __forceinline__ double lowest() { return -0x1p129; }
-    static __device__ __forceinline__ double tagged(double d, uint32_t c) {
-        const uint64_t b = __builtin_bit_cast(uint64_t, d);
-        const uint32_t sign = (uint32_t)((int32_t)(b >> 32) >> 31);
-        return __builtin_bit_cast(double, b | ((c ^ ~sign) & 0xFFFu));
-    }
-    static __device__ __forceinline__ void of(const Piece<float> &p, uint32_t c0, double *v, bool &odd) {
+    // the lesser bits make a negative number the greater one: its tag is turned round
+    static __device__ __forceinline__ uint64_t turned(uint64_t b) { return b | ((uint32_t)((int32_t)(b >> 32) >> 31) & 0xFFFu); }
+    static __device__ __forceinline__ double tagged(double d, uint32_t tag) { return __builtin_bit_cast(double, turned(__builtin_bit_cast(uint64_t, d)) ^ tag); }
+    static __device__ __forceinline__ void of(const Piece<float> &p, uint32_t tag, double *v, bool &odd) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const float x = __uint_as_float(p.r.w[j]) + 0.0f; // -0 becomes 0
             odd |= !(x < INFINITY);
-            v[j] = tagged(fmax((double)x, -0x1p129), c0 + j);
+            v[j] = tagged(x == -INFINITY ? -0x1p129 : (double)x, tag - j);
         }
     }
+    static __device__ __forceinline__ void add_tag(double &k, uint32_t tag) { k = __builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) ^ tag); }
     static __device__ void nan_first(const Piece<float> &p, double *v) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const float x = __uint_as_float(p.r.w[j]);
             // +inf with a tag would be no number
-            if (!(x < INFINITY)) v[j] = tagged(x != x ? 0x1p130 : 0x1p129, of_class(v[j]));
+            if (!(x < INFINITY)) v[j] = tagged(x != x ? 0x1p130 : 0x1p129, tag_of(v[j]));
         }
     }
     static __device__ __forceinline__ bool is_class(double k) { return k > -0x1p128; }
-    static __device__ __forceinline__ int of_class(double k) {
+    static __device__ __forceinline__ int tag_of(double k) {
         const uint64_t b = __builtin_bit_cast(uint64_t, k);
-        return (int)(((uint32_t)b ^ ~(uint32_t)((int32_t)(b >> 32) >> 31)) & 0xFFFu);
+        return (int)(((uint32_t)b ^ (uint32_t)((int32_t)(b >> 32) >> 31)) & 0xFFFu);
     }
     static __device__ __forceinline__ float score(double k) { // infinite for no number, too
         return (float)__builtin_bit_cast(double, __builtin_bit_cast(uint64_t, k) & ~0xFFFull);
@@ -222,22 +227,31 @@ template <typename T, int NV, int G>
 __device__ __forceinline__ void load_scores(Piece<T> *p, const T *x, int rank, int V) {
     constexpr int E = Piece<T>::E;
     constexpr uint32_t NONE = Best<T>::NONE;
+    if (V >= E) {
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int c = (rank + i * G) * E;
+        for (int i = 0; i < NV; i++) load_piece<false>(p[i], x, rank + i * G, V); // behind the row: its last piece again
+        if (V < NV * G * E) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                settle_piece<false>(p[i], rank + i * G, V, NONE);
+#pragma unroll
+                for (int k = 0; k < 4; k++) p[i].r.w[k] = (rank + i * G) * E < V ? p[i].r.w[k] : NONE;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int k = 0; k < 4; k++) p[i].r.w[k] = NONE;
-        if (V >= E) {
-            if (c < V) load_piece<false>(p[i], x, rank + i * G, V, NONE);
-        } else if (c < V) {
-            p[i].load_some(x, V);
+    if (rank == 0) {
+        p[0].load_some(x, V);
 #pragma unroll
-            for (int k = 0; k < E; k++)
-                if (k >= V) {
-                    if (sizeof(T) == 4) p[i].r.w[k & 3] = NONE;
-                    else p[i].r.w[k / 2] = k & 1 ? (p[i].r.w[k / 2] & 0xFFFFu) | (NONE & 0xFFFF0000u) : (p[i].r.w[k / 2] & 0xFFFF0000u) | (NONE & 0xFFFFu);
-                }
-        }
+        for (int k = 0; k < E; k++)
+            if (k >= V) {
+                if (sizeof(T) == 4) p[0].r.w[k & 3] = NONE;
+                else p[0].r.w[k / 2] = k & 1 ? (p[0].r.w[k / 2] & 0xFFFFu) | (NONE & 0xFFFF0000u) : (p[0].r.w[k / 2] & 0xFFFF0000u) | (NONE & 0xFFFFu);
+            }
     }
 }
 
@@ -256,16 +270,20 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
         Value v[N];
         bool odd = false;
 #pragma unroll
-        for (int i = 0; i < NV; i++) B::of(p[i], (rank + i * G) * E, v + i * E, odd);
+        for (int i = 0; i < NV; i++) B::of(p[i], (NV - 1 - i) * G * E + E - 1, v + i * E, odd);
         if (__builtin_expect(__any(odd), 0)) {
 #pragma unroll
             for (int i = 0; i < NV; i++) B::nan_first(p[i], v + i * E);
         }
 #pragma unroll
         for (int i = 0; i < N; i += KEPT) sort_values<T, KEPT>(v + i);
+        // a lane's share of the tag comes when few are left
+        const uint32_t lane_tag = (G - 1 - rank) * E;
         float most, total = 0.0f;
         Value *const s_best = (Value *)s_dyn + slot * a.top;
         if constexpr (MORE) {
+#pragma unroll
+            for (int i = 0; i < N; i++) B::add_tag(v[i], lane_tag);
             for (int j = 0; j < a.top; j++) {
                 Value best[1] = {v[0]};
                 join_lanes<T, 1, G>(best);
@@ -283,6 +301,8 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
             for (int s = K; s < N; s *= 2)
 #pragma unroll
                 for (int i = 0; i + s < N; i += 2 * s) join<T, K>(v + i, [&](int k) { return v[i + s + k]; });
+#pragma unroll
+            for (int i = 0; i < K; i++) B::add_tag(v[i], lane_tag);
             join_lanes<T, K, G>(v);
             most = B::score(v[0]);
         }
@@ -304,7 +324,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
             for (int j = rank; j < a.top; j += G) {
                 const Value best = s_best[j];
                 const bool is = B::is_class(best);
-                a.ids[row * a.top + j] = is ? B::of_class(best) : -1;
+                a.ids[row * a.top + j] = is ? G * N - 1 - B::tag_of(best) : -1;
                 a.w[row * a.top + j] = is ? exp_gap(B::score(best), most, a.exp_mul) * inv : 0.0f;
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -320,7 +340,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
 #pragma unroll
                 for (int k = 1; k < K; k++) best = rank + i * G == k ? v[k] : best;
                 const bool is = rank + i * G < a.top && B::is_class(best);
-                id[i] = is ? B::of_class(best) : -1;
+                id[i] = is ? G * N - 1 - B::tag_of(best) : -1;
                 e[i] = is ? exp_gap(B::score(best), most, a.exp_mul) : 0.0f;
                 sum += e[i];
             }
@@ -709,6 +729,7 @@ __global__ __launch_bounds__(256) void k_spread(RowArgs a) {
     if (!me.in) return;
     Piece<T> p;
     load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
+    settle_piece<TINY>(p, me.v, a.H);
     float f[E];
     if (DROP || a.w) p.get(f);
     if (DROP) drop_values<E>(a, drop_key(a), me.row, me.v, f);
@@ -764,6 +785,7 @@ __global__ __launch_bounds__(G ? 256 : 1024) void k_spread_dot(RowArgs a) {
 #pragma unroll
             for (int j = 0; j < TOP; j++)
                 if (at[j] < a.n) load_piece<TINY>(q[j], (const T *)a.y + at[j] * a.ys, v, a.H);
+            settle_piece<TINY>(p, v, a.H);
             p.get(f);
             if (DROP) drop_values<E>(a, key, row, v, f);
 #pragma unroll
@@ -774,6 +796,7 @@ __global__ __launch_bounds__(G ? 256 : 1024) void k_spread_dot(RowArgs a) {
                     for (int k = 0; k < E; k++) g[k] = f[k] * w[j];
                     p.set(g);
                     store_piece<TINY>(p, (T *)a.out + at[j] * a.os, v, a.H);
+                    settle_piece<TINY>(q[j], v, a.H);
                     q[j].get(g);
                     float sum = f[0] * g[0];
 #pragma unroll
@@ -828,6 +851,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
         for (int j = 0; j < TOP; j++)
             if (at[j] < a.n) {
                 float f[E];
+                settle_piece<TINY>(p[j], me.v, a.H);
                 p[j].get(f);
 #pragma unroll
                 for (int k = 0; k < E; k++) sum[k] = __builtin_fmaf(w[j], f[k], sum[k]);
@@ -836,6 +860,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     if (DROP) drop_values<E>(a, drop_key(a), me.row, me.v, sum);
     if (a.res) {
         float f[E];
+        settle_piece<TINY>(res, me.v, a.H);
         res.get(f);
 #pragma unroll
         for (int k = 0; k < E; k++) sum[k] += f[k];
@@ -854,10 +879,12 @@ __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
     float f[E];
     load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
     if (a.res) load_piece<TINY>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    settle_piece<TINY>(p, me.v, a.H);
     p.get(f);
     if (a.drop) drop_values<E>(a, drop_key(a), me.row, me.v, f);
     if (a.res) {
         float g[E];
+        settle_piece<TINY>(res, me.v, a.H);
         res.get(g);
 #pragma unroll
         for (int k = 0; k < E; k++) f[k] += g[k];

@@ -356,7 +356,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     }
 }
 
-// The gradient of the weights: a row to G lanes.  What the chosen classes have is put together in shared memory.
+// The gradient of the weights: a row to G lanes.  What the chosen classes have is put together in shared memory, a word to a class.
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
     constexpr int E = Piece<T>::E, ROWS = 256 / G, ROW = G * NV * E;
@@ -365,49 +365,53 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
     float *const s = s_rows + slot * ROW;
     for (int64_t row = (int64_t)blockIdx.x * ROWS + slot; row < a.N; row += (int64_t)gridDim.x * ROWS) {
         Piece<T> p[NV];
-        if (!a.renormalize) {
-            const T *x = (const T *)a.x + row * a.xs;
-            load_scores<T, NV, G>(p, x, rank, V);
+        if (!a.renormalize) load_scores<T, NV, G>(p, (const T *)a.x + row * a.xs, rank, V);
+        // a lane's first entry stays in registers, the others of long choices are read twice
+        const int64_t e0 = row * a.top;
+        const auto id_at = [&](int j) { return a.id64 ? ((const int64_t *)a.ids_in)[e0 + j] : (int64_t)((const int32_t *)a.ids_in)[e0 + j]; };
+        const bool has = rank < a.top;
+        const int64_t id = has ? id_at(rank) : -1;
+        const float w = has ? a.w_in[e0 + rank] : 0.0f, dw = has ? a.dw[e0 + rank] : 0.0f;
+        float mean = id >= V ? NAN : id >= 0 ? w * dw : 0.0f; // an id of no class makes the row's gradient NaN
+        for (int j = rank + G; j < a.top; j += G) {
+            const int64_t i = id_at(j);
+            if (i >= 0) mean += i >= V ? NAN : a.w_in[e0 + j] * a.dw[e0 + j];
         }
-        float mean = 0.0f;
-        bool none = false; // an id of no class
-        for (int j = rank; j < a.top; j += G) {
-            const int64_t at = row * a.top + j, id = a.id64 ? ((const int64_t *)a.ids_in)[at] : ((const int32_t *)a.ids_in)[at];
-            none |= id >= V;
-            if (id >= 0) mean += a.w_in[at] * a.dw[at];
-        }
-        mean = lanes_sum<G>(none ? NAN : mean);
+        mean = lanes_sum<G>(mean);
+        const float less = a.renormalize ? mean : 0.0f;
 #pragma unroll
-        for (int i = 0; i < NV; i++)
-#pragma unroll
-            for (int k = 0; k < E; k += 4) *(float4 *)(s + (rank + i * G) * E + k) = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < NV * E; k += 4) *(float4 *)(s + (k / 4 * G + rank) * 4) = {0.0f, 0.0f, 0.0f, 0.0f};
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        for (int j = rank; j < a.top; j += G) {
-            const int64_t at = row * a.top + j, id = a.id64 ? ((const int64_t *)a.ids_in)[at] : ((const int32_t *)a.ids_in)[at];
-            if (id >= 0 && id < V) atomicAdd(s + id, a.renormalize ? a.w_in[at] * (a.dw[at] - mean) : a.w_in[at] * a.dw[at]);
+        if (id >= 0 && id < V) atomicAdd(s + id, w * (dw - less) * a.inv_t);
+        for (int j = rank + G; j < a.top; j += G) {
+            const int64_t i = id_at(j);
+            if (i >= 0 && i < V) atomicAdd(s + i, a.w_in[e0 + j] * (a.dw[e0 + j] - less) * a.inv_t);
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        float f[NV * E], m = -INFINITY, total = 0.0f;
+        float m = -INFINITY, factor = 0.0f;
         if (!a.renormalize) {
+            float total = 0.0f;
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                p[i].get(f + i * E);
+                float f[E];
+                p[i].get(f);
 #pragma unroll
-                for (int k = 0; k < E; k++) {
-                    m = fmaxf(m, f[i * E + k]);
-                }
+                for (int k = 0; k < E; k++) m = fmaxf(m, f[k]);
             }
             m = over_lanes<G>(m, [](float u, float v) { return fmaxf(u, v); });
+            m = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int i = 0; i < NV * E; i++) {
-                f[i] = f[i] == -INFINITY ? 0.0f : exp_gap(f[i], m, a.exp_mul);
-                total += f[i];
+            for (int i = 0; i < NV; i++) {
+                float f[E];
+                p[i].get(f);
+#pragma unroll
+                for (int k = 0; k < E; k++) total += exp_gap(f[k], m, a.exp_mul);
             }
             total = lanes_sum<G>(total);
+            factor = total == 0.0f ? 0.0f : -mean * a.inv_t / total;
         }
-        const float factor = total == 0.0f ? 0.0f : -mean / total;
         T *g = (T *)a.g + row * a.gs;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
@@ -415,11 +419,15 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
             if (c < V) {
                 float o[E];
 #pragma unroll
-                for (int k = 0; k < E; k++) {
-                    o[k] = s[c + k];
-                    if (!a.renormalize) o[k] += f[i * E + k] * factor;
-                    o[k] *= a.inv_t;
-                    if (mean != mean) o[k] = NAN;
+                for (int k = 0; k < E; k += 4) *(float4 *)(o + k) = *(const float4 *)(s + c + k);
+                if (!a.renormalize) {
+                    float f[E];
+                    p[i].get(f);
+#pragma unroll
+                    for (int k = 0; k < E; k++) o[k] = __builtin_fmaf(exp_gap(f[k], m, a.exp_mul), factor, o[k]);
+                } else if (__builtin_expect(mean != mean, 0)) {
+#pragma unroll
+                    for (int k = 0; k < E; k++) o[k] = NAN;
                 }
                 Piece<T> q;
                 q.set(o);

@@ -102,35 +102,25 @@ class RowPlan:
     """The tables that order rows by expert, from plan_rows.  place: (rows, top), where each entry of `experts` stands among the sorted rows, -1 if it is no
     expert's; source: (rows * top,), row * top + column of the entry at each place, -1 behind the last; offsets: (n_experts + 1,), expert e has the places
     offsets[e] to offsets[e + 1] - 1.  All are int32 on the device of `experts`."""
-    __slots__ = ("rows", "top", "experts", "device", "_on", "_tables", "_at", "_views")
+    __slots__ = ("rows", "top", "experts", "device", "offsets_at", "_on", "_tables", "_at")
 
     def __init__(self, rows, top, experts, device, on, tables):
         self.rows, self.top, self.experts, self.device, self._on, self._tables = rows, top, experts, device, on, tables
         self._at = tables.data_ptr()
-        self._views = None
-
-    def _view(self):
-        if self._views is None:
-            n = self.rows * self.top
-            t = self._tables
-            self._views = t[:n].view(self.rows, self.top), t[n:2 * n], t[2 * n:2 * n + self.experts + 1]
-        return self._views
+        self.offsets_at = self._at + 8 * rows * top
 
     @property
     def place(self):
-        return self._view()[0]
+        return self._tables.as_strided((self.rows, self.top), (self.top, 1), 0)
 
     @property
     def source(self):
-        return self._view()[1]
+        n = self.rows * self.top
+        return self._tables.as_strided((n,), (1,), n)
 
     @property
     def offsets(self):
-        return self._view()[2]
-
-    @property
-    def offsets_at(self):
-        return self._at + 8 * self.rows * self.top
+        return self._tables.as_strided((self.experts + 1,), (1,), 2 * self.rows * self.top)
 
 
 class _Rows:
@@ -273,10 +263,10 @@ def plan_rows(experts, n_experts):
     at = _check("experts", experts, experts.shape, _scores._INTS, device, on)
     if device < 0:
         raise ValueError("experts must be on a GPU, got %s" % on)
-    tables = _make(device, torch.int32, (2 * n + n_experts + 1,), on)
-    work = _make(device, torch.int32, (((n + 1023) // 1024 + 1) * n_experts,), on)
-    plan = RowPlan(rows, top, n_experts, device, on, tables)
-    _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, work.data_ptr())
+    # the tables, and what the call works in behind them
+    kept = 2 * n + n_experts + 1
+    plan = RowPlan(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + ((n + 1023) // 1024 + 1) * n_experts,), on))
+    _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, plan._at + 4 * kept)
     return plan
 
 

@@ -107,6 +107,44 @@ struct Piece {
     }
 };
 
+typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
+// Piece v of a row of H values, in two steps, so that several are on their way before the first is waited for.  The last one, where it is not whole, is read from where
+// the row ends...  TINY: rows of less than a piece
+template <bool TINY, typename T>
+__device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H) {
+    constexpr uint32_t E = Piece<T>::E;
+    if (TINY) {
+        p.load_some(x, H);
+        return;
+    }
+    const uint32_t at = v * E, last = H - E;
+    const u4 r = *(const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
+#pragma unroll
+    for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
+}
+// ... and moved down here; what is behind the row becomes `fill`, two or one values of a word.
+template <bool TINY, typename T>
+__device__ __forceinline__ void settle_piece(Piece<T> &p, uint32_t v, uint32_t H, uint32_t fill = 0) {
+    constexpr uint32_t E = Piece<T>::E;
+    const uint32_t n = H % E;
+    if (TINY || n == 0) return; // of all lanes alike
+    const uint32_t up = E - n, words = up * sizeof(T) / 4;
+    const bool moves = v * E > H - E;
+    uint32_t w[5];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; k++) {
+        w[k] = p.r.w[k];
+#pragma unroll
+        for (uint32_t d = 1; d < 4; d++) w[k] = words == d ? (d + k < 4 ? p.r.w[(d + k) & 3] : fill) : w[k];
+    }
+    w[4] = fill;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        if (sizeof(T) == 2) w[k] = up & 1 ? __builtin_amdgcn_alignbit(w[k + 1], w[k], 16) : w[k];
+        p.r.w[k] = moves ? w[k] : p.r.w[k];
+    }
+}
+
 // Reductions over G neighbouring lanes whose result every one of them has: by moves within rows of sixteen lanes and gfx950's swaps of rows between two
 // registers, a few cycles a step where a trip through the LDS crossbar is a hundred (8 rows of 32 768 classes: 6.3 us, 4.8 so).
 template <int CTRL>

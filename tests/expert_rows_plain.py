@@ -123,13 +123,13 @@ def threshold(p):
     return min(int(round(p * 2 ** 32)), 2 ** 32 - 1)
 
 
-def bits(rows, features, seed, layer):
-    """The 32 bits of every element."""
+def bits(rows, features, seed, layer, first=0):
+    """The 32 bits of every element of rows first to first + rows - 1."""
     key = splitmix(seed & M, layer)
     words = (features + 3) // 4
 
     def outputs(start):
-        z = np.arange(1, rows * words + 1, dtype=np.uint64)
+        z = np.arange(first * words + 1, (first + rows) * words + 1, dtype=np.uint64)
         with np.errstate(over="ignore"):
             z = np.uint64(start) + z * np.uint64(0x9E3779B97F4A7C15)
             z = (z ^ (z >> np.uint64(30))) * np.uint64(0xBF58476D1CE4E5B9)

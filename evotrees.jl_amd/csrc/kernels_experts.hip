@@ -206,6 +206,7 @@ struct RowArgs {
     // dropout: an element is dropped whose 32 bits are below this
     uint32_t drop, layer;
     float scale;
+    int32_t past; // results go past the caches
     const uint64_t *seed_at; // nullptr: seed
     uint64_t seed;
 };
@@ -245,10 +246,10 @@ __device__ __forceinline__ void drop_values(const RowArgs &a, uint64_t key, uint
 __device__ __forceinline__ uint64_t drop_key(const RowArgs &a) { return mixed((a.seed_at ? *a.seed_at : a.seed) + ((uint64_t)a.layer + 1) * GAMMA); }
 
 template <bool TINY, typename T>
-__device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v, uint32_t H) {
+__device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v, uint32_t H, bool past = false) {
     constexpr uint32_t E = Piece<T>::E;
     T *const o = x + (size_t)v * E;
-    if (!TINY && v * E + E <= H) p.store(o, false);
+    if (!TINY && v * E + E <= H) p.store(o, past);
     else p.store_some(o, H % E);
 }
 
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     if (!me.in) return;
     Piece<T> res;
     float sum[E] = {};
-    if (a.res) load_piece<TINY>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    if (a.res) load_piece<TINY, true>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
     const size_t e0 = (size_t)me.row * a.top;
     for (uint32_t j0 = 0; j0 < a.top; j0 += TOP) {
         uint32_t at[TOP];
@@ -419,7 +420,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
         for (int j = 0; j < TOP; j++) w[j] = a.w && j0 + j < a.top ? a.w[e0 + j0 + j] : 1.0f;
 #pragma unroll
         for (int j = 0; j < TOP; j++)
-            if (at[j] < a.n) load_piece<TINY>(p[j], (const T *)a.x + at[j] * a.xs, me.v, a.H);
+            if (at[j] < a.n) load_piece<TINY, true>(p[j], (const T *)a.x + at[j] * a.xs, me.v, a.H);
 #pragma unroll
         for (int j = 0; j < TOP; j++)
             if (at[j] < a.n) {
@@ -440,7 +441,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     }
     Piece<T> o;
     o.set(sum);
-    store_piece<TINY>(o, (T *)a.out + me.row * a.os, me.v, a.H);
+    store_piece<TINY>(o, (T *)a.out + me.row * a.os, me.v, a.H, a.past);
 }
 
 template <typename T, bool ROW, bool TINY>
@@ -450,8 +451,8 @@ __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
     if (!me.in) return;
     Piece<T> p, res;
     float f[E];
-    load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
-    if (a.res) load_piece<TINY>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    load_piece<TINY, true>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
+    if (a.res) load_piece<TINY, true>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
     settle_piece<TINY>(p, me.v, a.H);
     p.get(f);
     if (a.drop) drop_values<E>(a, drop_key(a), me.row, me.v, f);
@@ -463,7 +464,7 @@ __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
         for (int k = 0; k < E; k++) f[k] += g[k];
     }
     p.set(f);
-    store_piece<TINY>(p, (T *)a.out + me.row * a.os, me.v, a.H);
+    store_piece<TINY>(p, (T *)a.out + me.row * a.os, me.v, a.H, a.past);
 }
 
 // ---- launches --------------------------------------------------------------------------------
@@ -504,6 +505,11 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     constexpr int E = Piece<T>::E;
     a.pieces = (a.H + E - 1) / E;
     a.parts = (a.pieces + 63) / 64;
+    // Results that the second caches (8 x 4 MB) cannot hold go past them, and what is combined or dropped is read as something that nobody reads again soon (32 768 x 8 x 4096
+    // bf16 combined: 485 us, 470 with the loads so, 439 with both; dropout of 65 536 x 8192 with a residual 553, 542, 519; combined and read by the next kernel, the pair:
+    // 8192 x 8 x 4096 153 | 149, 1024 x 8 x 2048 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows
+    // of 4099 sorted: 535 us, 667 so), and gradients are no sooner done (908 | 911)
+    a.past = (double)a.N * a.H * sizeof(T) > 32e6;
     const bool tiny = a.H < E, by_row = a.pieces >= 64;
     const uint32_t each = a.pieces < 64 ? 64 : a.parts * 64; // threads a row, at most
     const uint32_t some = (1u << 30) / each > 0 ? (1u << 30) / each : 1, all = a.N; // rows of a launch

@@ -109,8 +109,8 @@ struct Piece {
 
 typedef uint32_t u4 __attribute__((ext_vector_type(4), aligned(2)));
 // Piece v of a row of H values, in two steps, so that several are on their way before the first is waited for.  The last one, where it is not whole, is read from where
-// the row ends...  TINY: rows of less than a piece
-template <bool TINY, typename T>
+// the row ends...  TINY: rows of less than a piece.  ONCE: nobody reads it again soon, and it need not stay in the caches
+template <bool TINY, bool ONCE = false, typename T>
 __device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, uint32_t H) {
     constexpr uint32_t E = Piece<T>::E;
     if (TINY) {
@@ -118,7 +118,8 @@ __device__ __forceinline__ void load_piece(Piece<T> &p, const T *x, uint32_t v, 
         return;
     }
     const uint32_t at = v * E, last = H - E;
-    const u4 r = *(const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
+    const u4 *const from = (const u4 *)((const char *)x + (size_t)(at < last ? at : last) * sizeof(T));
+    const u4 r = ONCE ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
     for (int k = 0; k < 4; k++) p.r.w[k] = r[k];
 }

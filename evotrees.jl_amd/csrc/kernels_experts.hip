@@ -508,8 +508,8 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     // Results that the second caches (8 x 4 MB) cannot hold go past them, and what is combined or dropped is read as something that nobody reads again soon (32 768 x 8 x 4096
     // bf16 combined: 485 us, 470 with the loads so, 439 with both; dropout of 65 536 x 8192 with a residual 553, 542, 519; combined and read by the next kernel, the pair:
     // 8192 x 8 x 4096 153 | 149, 1024 x 8 x 2048 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows
-    // of 4099 sorted: 535 us, 667 so), and gradients are no sooner done (908 | 911)
-    a.past = (double)a.N * a.H * sizeof(T) > 32e6;
+    // of 4099 sorted: 535 us, 667 so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 34.0), and gradients are no sooner done (908 | 911)
+    a.past = (double)a.N * a.H * sizeof(T) > 32e6 && (uintptr_t)a.out % 16 == 0 && a.os % E == 0 && a.H % E == 0;
     const bool tiny = a.H < E, by_row = a.pieces >= 64;
     const uint32_t each = a.pieces < 64 ? 64 : a.parts * 64; // threads a row, at most
     const uint32_t some = (1u << 30) / each > 0 ? (1u << 30) / each : 1, all = a.N; // rows of a launch

@@ -206,7 +206,6 @@ struct RowArgs {
     // dropout: an element is dropped whose 32 bits are below this
     uint32_t drop, layer;
     float scale;
-    int32_t past; // results go past the caches
     const uint64_t *seed_at; // nullptr: seed
     uint64_t seed;
 };
@@ -401,14 +400,14 @@ __global__ __launch_bounds__(G ? 256 : 1024) void k_spread_dot(RowArgs a) {
 }
 
 // Every row's sum over its places, times the weights if there are any, with dropout and a residual
-template <typename T, bool ROW, bool TINY, int TOP, bool DROP>
+template <typename T, bool ROW, bool TINY, int TOP, bool DROP, bool PAST>
 __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     constexpr int E = Piece<T>::E;
     const Share<ROW> me(a, own_block(gridDim.x));
     if (!me.in) return;
     Piece<T> res;
     float sum[E] = {};
-    if (a.res) load_piece<TINY, true>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    if (a.res) load_piece<TINY, PAST>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
     const size_t e0 = (size_t)me.row * a.top;
     for (uint32_t j0 = 0; j0 < a.top; j0 += TOP) {
         uint32_t at[TOP];
@@ -420,7 +419,7 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
         for (int j = 0; j < TOP; j++) w[j] = a.w && j0 + j < a.top ? a.w[e0 + j0 + j] : 1.0f;
 #pragma unroll
         for (int j = 0; j < TOP; j++)
-            if (at[j] < a.n) load_piece<TINY, true>(p[j], (const T *)a.x + at[j] * a.xs, me.v, a.H);
+            if (at[j] < a.n) load_piece<TINY, PAST>(p[j], (const T *)a.x + at[j] * a.xs, me.v, a.H);
 #pragma unroll
         for (int j = 0; j < TOP; j++)
             if (at[j] < a.n) {
@@ -441,18 +440,18 @@ __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     }
     Piece<T> o;
     o.set(sum);
-    store_piece<TINY>(o, (T *)a.out + me.row * a.os, me.v, a.H, a.past);
+    store_piece<TINY>(o, (T *)a.out + me.row * a.os, me.v, a.H, PAST);
 }
 
-template <typename T, bool ROW, bool TINY>
+template <typename T, bool ROW, bool TINY, bool PAST>
 __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
     constexpr int E = Piece<T>::E;
     const Share<ROW> me(a, blockIdx.x);
     if (!me.in) return;
     Piece<T> p, res;
     float f[E];
-    load_piece<TINY, true>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
-    if (a.res) load_piece<TINY, true>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
+    load_piece<TINY, PAST>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
+    if (a.res) load_piece<TINY, PAST>(res, (const T *)a.res + me.row * a.rs, me.v, a.H);
     settle_piece<TINY>(p, me.v, a.H);
     p.get(f);
     if (a.drop) drop_values<E>(a, drop_key(a), me.row, me.v, f);
@@ -464,24 +463,24 @@ __global__ __launch_bounds__(256) void k_drop(RowArgs a) {
         for (int k = 0; k < E; k++) f[k] += g[k];
     }
     p.set(f);
-    store_piece<TINY>(p, (T *)a.out + me.row * a.os, me.v, a.H, a.past);
+    store_piece<TINY>(p, (T *)a.out + me.row * a.os, me.v, a.H, PAST);
 }
 
 // ---- launches --------------------------------------------------------------------------------
 
 static unsigned round_up(unsigned blocks) { return (blocks + 7) / 8 * 8; }
 enum { ROWS_SPREAD, ROWS_COMBINE, ROWS_DROP };
-template <typename T, bool ROW, bool TINY, int OP>
+template <typename T, bool ROW, bool TINY, bool PAST, int OP>
 static void launch_rows_as(hipStream_t s, const RowArgs &a, unsigned grid) {
     grid = round_up(grid);
-    if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, ROW, TINY>), dim3(grid), dim3(256), 0, s, a);
+    if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, ROW, TINY, PAST>), dim3(grid), dim3(256), 0, s, a);
     else if constexpr (OP == ROWS_SPREAD) {
         if (a.drop) hipLaunchKernelGGL((k_spread<T, ROW, TINY, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
         else hipLaunchKernelGGL((k_spread<T, ROW, TINY, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
     } else {
         const auto go = [&](auto top) {
-            if (a.drop) hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, true>), dim3(grid), dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, false>), dim3(grid), dim3(256), 0, s, a);
+            if (a.drop) hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, true, PAST>), dim3(grid), dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, false, PAST>), dim3(grid), dim3(256), 0, s, a);
         };
         if (a.top <= 2) go(std::integral_constant<int, 2>());
         else if (a.top <= 4) go(std::integral_constant<int, 4>());
@@ -505,11 +504,11 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     constexpr int E = Piece<T>::E;
     a.pieces = (a.H + E - 1) / E;
     a.parts = (a.pieces + 63) / 64;
-    // Results that the second caches (8 x 4 MB) cannot hold go past them, and what is combined or dropped is read as something that nobody reads again soon (32 768 x 8 x 4096
+    // Results of more than half of what the second caches hold (8 x 4 MB) go past them, and what they come from is read as something that nobody reads again soon (32 768 x 8 x 4096
     // bf16 combined: 485 us, 470 with the loads so, 439 with both; dropout of 65 536 x 8192 with a residual 553, 542, 519; combined and read by the next kernel, the pair:
-    // 8192 x 8 x 4096 153 | 149, 1024 x 8 x 2048 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows
+    // 8192 x 8 x 4096 153 | 149, 4096 x 8 x 2048 38.5 | 38.6, 1024 x 8 x 2048 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows
     // of 4099 sorted: 535 us, 667 so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 34.0), and gradients are no sooner done (908 | 911)
-    a.past = (double)a.N * a.H * sizeof(T) > 32e6 && (uintptr_t)a.out % 16 == 0 && a.os % E == 0 && a.H % E == 0;
+    const bool past = OP != ROWS_SPREAD && (double)a.N * a.H * sizeof(T) > 16e6 && (uintptr_t)a.out % 16 == 0 && a.os % E == 0 && a.H % E == 0;
     const bool tiny = a.H < E, by_row = a.pieces >= 64;
     const uint32_t each = a.pieces < 64 ? 64 : a.parts * 64; // threads a row, at most
     const uint32_t some = (1u << 30) / each > 0 ? (1u << 30) / each : 1, all = a.N; // rows of a launch
@@ -529,11 +528,16 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
                 const int most = rows <= 512 ? 16 : 4, turns = (a.parts + most - 1) / most;
                 launch_dot_as<T, 0, false>(s, a, rows, 64 * ((a.parts + turns - 1) / turns));
             }
-        } else if (tiny) launch_rows_as<T, false, true, OP>(s, a, (rows + 255) / 256);
-        else if (by_row) launch_rows_as<T, true, false, OP>(s, a, (unsigned)(((uint64_t)rows * a.parts + 3) / 4));
-        else launch_rows_as<T, false, false, OP>(s, a, (unsigned)(((uint64_t)rows * a.pieces + 255) / 256));
+        } else {
+            const uint64_t threads = by_row ? (uint64_t)rows * a.parts * 64 : (uint64_t)rows * a.pieces;
+            const unsigned grid = (unsigned)((threads + 255) / 256);
+            if (tiny) launch_rows_as<T, false, true, false, OP>(s, a, grid);
+            else if (OP != ROWS_SPREAD && past) by_row ? launch_rows_as<T, true, false, OP != ROWS_SPREAD, OP>(s, a, grid) : launch_rows_as<T, false, false, OP != ROWS_SPREAD, OP>(s, a, grid);
+            else by_row ? launch_rows_as<T, true, false, false, OP>(s, a, grid) : launch_rows_as<T, false, false, false, OP>(s, a, grid);
+        }
     }
 }
+
 template <int OP>
 static int launch_rows(hipStream_t s, RowArgs &a, int dtype) {
     if (dtype == EVT_F32) launch_rows_typed<float, OP>(s, a);

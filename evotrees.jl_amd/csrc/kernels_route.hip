@@ -16,6 +16,11 @@ struct RouteArgs {
     const float *w_in, *dw;
 };
 
+// What a wavefront's lanes wrote to shared memory before can be read by its others
+__device__ __forceinline__ void lanes_wait() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 __device__ __forceinline__ float exp_gap(float x, float m, float mul) { return __builtin_amdgcn_exp2f((x - m) * mul); }
 
 // A score and its class as one number that is the greater the better, and no two are alike: the score in an order that numbers have (zeros alike), and below it the
@@ -272,8 +277,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
             total = lanes_sum<G>(total);
         }
         if constexpr (MORE) {
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            lanes_wait();
             const float inv = 1.0f / total;
             for (int j = rank; j < a.top; j += G) {
                 const Value best = s_best[j];
@@ -281,8 +285,7 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
                 a.ids[row * a.top + j] = is ? G * N - 1 - B::tag_of(best) : -1;
                 a.w[row * a.top + j] = is ? exp_gap(B::score(best), most, a.exp_mul) * inv : 0.0f;
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+            lanes_wait();
         } else { // lane j has the j-th best, or each lane every G-th
             constexpr int MINE = K > G ? K / G : 1;
             float e[MINE];
@@ -335,15 +338,36 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
         const float less = a.renormalize ? mean : 0.0f;
 #pragma unroll
         for (int k = 0; k < NV * E; k += 4) *(float4 *)(s + (k / 4 * G + rank) * 4) = {0.0f, 0.0f, 0.0f, 0.0f};
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if (id >= 0 && id < V) atomicAdd(s + id, w * (dw - less) * a.inv_t);
+        lanes_wait();
+        // Every entry writes its number at its class and looks whether it is still there: an expert that is chosen twice is none of a choice's, but may be given
+        bool twice = false;
+        if (id >= 0 && id < V) s[id] = (float)(rank + 1);
         for (int j = rank + G; j < a.top; j += G) {
             const int64_t i = id_at(j);
-            if (i >= 0 && i < V) atomicAdd(s + i, a.w_in[e0 + j] * (a.dw[e0 + j] - less) * a.inv_t);
+            if (i >= 0 && i < V) s[i] = (float)(j + 1);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        lanes_wait();
+        if (id >= 0 && id < V) twice = s[id] != (float)(rank + 1);
+        for (int j = rank + G; j < a.top; j += G) {
+            const int64_t i = id_at(j);
+            if (i >= 0 && i < V) twice |= s[i] != (float)(j + 1);
+        }
+        if (__builtin_expect(!__any(twice), 1)) {
+            if (id >= 0 && id < V) s[id] = w * (dw - less) * a.inv_t;
+            for (int j = rank + G; j < a.top; j += G) {
+                const int64_t i = id_at(j);
+                if (i >= 0 && i < V) s[i] = a.w_in[e0 + j] * (a.dw[e0 + j] - less) * a.inv_t;
+            }
+        } else { // sums, in the entries' order
+            for (int pass = 0; pass < 2; pass++)
+                for (int j = 0; j < a.top; j++) {
+                    lanes_wait();
+                    if (rank != (j & (G - 1))) continue;
+                    const int64_t i = id_at(j);
+                    if (i >= 0 && i < V) s[i] = pass ? s[i] + a.w_in[e0 + j] * (a.dw[e0 + j] - less) * a.inv_t : 0.0f;
+                }
+        }
+        lanes_wait();
         float m = -INFINITY, factor = 0.0f;
         if (!a.renormalize) {
             float total = 0.0f;
@@ -389,8 +413,7 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
                 else q.store_some(g + c, V - c);
             }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        lanes_wait();
     }
 }
 

@@ -274,3 +274,53 @@ def test_more_rows_than_a_launch_has(evt, rows, H):
     for a in range(0, rows, 1 << 20):
         part = x[a:a + (1 << 20)]
         assert bool(((part == 0) | (part == scale)).all())
+
+
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("V,top", [(5, 5), (40, 6), (256, 8), (100, 40), (3000, 64)])
+def test_one_expert_several_times_in_a_row(evt, V, top, renormalize):
+    """Its shares are added up, in the same order in every call."""
+    rows, gen = 21, torch.Generator().manual_seed(V)
+    x = torch.randn(rows, V, generator=gen)
+    ids = torch.randint(0, V, (rows, top), generator=gen)
+    ids[3] = 2
+    ids[4, ::2] = 1
+    ids[5, 1:] = -1
+    w, dw = torch.rand(rows, top, generator=gen), torch.randn(rows, top, generator=gen) * 10
+    w /= w.sum(1, keepdim=True)
+    got = evt.route_rows_grad(x.cuda(), ids.cuda(), w.cuda(), dw.cuda(), renormalize=renormalize, temperature=0.5)
+    plain.close("grad", got, *plain.route_grad(x, ids, w, dw, renormalize, 0.5))
+    for _ in range(3):
+        assert torch.equal(evt.route_rows_grad(x.cuda(), ids.cuda(), w.cuda(), dw.cuda(), renormalize=renormalize, temperature=0.5), got)
+    place, source, offsets = plain.plan(ids, V)
+    plan = evt.plan_rows(ids.cuda(), V)
+    assert plan.place.reshape(-1).tolist() == place and plan.source.tolist() == source and plan.offsets.tolist() == offsets
+
+
+@pytest.mark.parametrize("dtype", list(plain.TYPES))
+@pytest.mark.parametrize("V", [6, 64, 200, 1030])
+def test_scores_at_the_ends_of_their_type(evt, V, dtype):
+    """The lowest number is a score like others, -inf is none; several that are no numbers come first, in their order, then +inf."""
+    t = plain.TYPES[dtype]
+    info, gen = torch.finfo(t), torch.Generator().manual_seed(V)
+    x = torch.randn(8, V, generator=gen)
+    x[0] = -math.inf
+    x[0, V // 2], x[0, 1] = info.min, info.min
+    x[1] = info.min
+    x[1, V - 1] = info.max
+    x[2, ::2], x[2, 1::2] = info.max, info.min
+    x[3, 1] = x[3, V - 1] = math.nan
+    x[3, 2] = math.inf
+    x[4, 0] = x[4, V - 2] = math.inf
+    x[5] = info.smallest_normal
+    x[5, ::2] = -info.smallest_normal
+    x[6] = 0.0
+    x[6, V - 1] = info.smallest_normal * info.eps  # the least number above 0
+    x[6, 0] = -0.0
+    x = x.to(t)
+    for top in (1, 2, 4, 6):
+        for renormalize in (True, False):
+            ids, w = evt.route_rows(x.cuda(), top, renormalize=renormalize)
+            want, ww, tol = plain.route(x, top, renormalize, 1.0)
+            assert torch.equal(ids.cpu(), want), (top, ids.cpu(), want)
+            plain.close("weights", w, ww, tol.nan_to_num(0, 0, 0) + plain.U)

@@ -313,16 +313,21 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a) {
     }
 }
 
-// The gradient of the weights: a row to G lanes.  What the chosen classes have is put together in shared memory, a word to a class.
+// The gradient of weights that are probabilities among all experts: a row to G lanes.  What the chosen classes have is put together in shared memory, a word to a class.
 template <typename T, int G, int NV>
 __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
     constexpr int E = Piece<T>::E, ROWS = 256 / G, ROW = G * NV * E;
     extern __shared__ __align__(16) float s_rows[]; // [ROWS][ROW]
     const int rank = threadIdx.x & (G - 1), slot = threadIdx.x / G, V = a.V;
-    float *const s = s_rows + slot * ROW;
+    float *const s_row = s_rows + slot * ROW;
+    // a class's word: sixteen bytes of each lane side by side, so that no two lanes of a read meet in a bank
+    const auto at_class = [&](int c) -> float & {
+        const int v = c / E, i = v / G, lane = v % G;
+        return s_row[((i * (E / 4) + c % E / 4) * G + lane) * 4 + c % 4];
+    };
     for (int64_t row = (int64_t)blockIdx.x * ROWS + slot; row < a.N; row += (int64_t)gridDim.x * ROWS) {
         Piece<T> p[NV];
-        if (!a.renormalize) load_scores<T, NV, G>(p, (const T *)a.x + row * a.xs, rank, V);
+        load_scores<T, NV, G>(p, (const T *)a.x + row * a.xs, rank, V);
         // a lane's first entry stays in registers, the others of long choices are read twice
         const int64_t e0 = row * a.top;
         const auto id_at = [&](int j) { return a.id64 ? ((const int64_t *)a.ids_in)[e0 + j] : (int64_t)((const int32_t *)a.ids_in)[e0 + j]; };
@@ -335,28 +340,27 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
             if (i >= 0) mean += i >= V ? NAN : a.w_in[e0 + j] * a.dw[e0 + j];
         }
         mean = lanes_sum<G>(mean);
-        const float less = a.renormalize ? mean : 0.0f;
 #pragma unroll
-        for (int k = 0; k < NV * E; k += 4) *(float4 *)(s + (k / 4 * G + rank) * 4) = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < NV * E; k += 4) *(float4 *)(s_row + (k / 4 * G + rank) * 4) = {0.0f, 0.0f, 0.0f, 0.0f};
         lanes_wait();
         // Every entry writes its number at its class and looks whether it is still there: an expert that is chosen twice is none of a choice's, but may be given
         bool twice = false;
-        if (id >= 0 && id < V) s[id] = (float)(rank + 1);
+        if (id >= 0 && id < V) at_class((int)id) = (float)(rank + 1);
         for (int j = rank + G; j < a.top; j += G) {
             const int64_t i = id_at(j);
-            if (i >= 0 && i < V) s[i] = (float)(j + 1);
+            if (i >= 0 && i < V) at_class((int)i) = (float)(j + 1);
         }
         lanes_wait();
-        if (id >= 0 && id < V) twice = s[id] != (float)(rank + 1);
+        if (id >= 0 && id < V) twice = at_class((int)id) != (float)(rank + 1);
         for (int j = rank + G; j < a.top; j += G) {
             const int64_t i = id_at(j);
-            if (i >= 0 && i < V) twice |= s[i] != (float)(j + 1);
+            if (i >= 0 && i < V) twice |= at_class((int)i) != (float)(j + 1);
         }
         if (__builtin_expect(!__any(twice), 1)) {
-            if (id >= 0 && id < V) s[id] = w * (dw - less) * a.inv_t;
+            if (id >= 0 && id < V) at_class((int)id) = w * dw * a.inv_t;
             for (int j = rank + G; j < a.top; j += G) {
                 const int64_t i = id_at(j);
-                if (i >= 0 && i < V) s[i] = a.w_in[e0 + j] * (a.dw[e0 + j] - less) * a.inv_t;
+                if (i >= 0 && i < V) at_class((int)i) = a.w_in[e0 + j] * a.dw[e0 + j] * a.inv_t;
             }
         } else { // sums, in the entries' order
             for (int pass = 0; pass < 2; pass++)
@@ -364,32 +368,24 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
                     lanes_wait();
                     if (rank != (j & (G - 1))) continue;
                     const int64_t i = id_at(j);
-                    if (i >= 0 && i < V) s[i] = pass ? s[i] + a.w_in[e0 + j] * (a.dw[e0 + j] - less) * a.inv_t : 0.0f;
+                    if (i >= 0 && i < V) at_class((int)i) = pass ? at_class((int)i) + a.w_in[e0 + j] * a.dw[e0 + j] * a.inv_t : 0.0f;
                 }
         }
         lanes_wait();
-        float m = -INFINITY, factor = 0.0f;
-        if (!a.renormalize) {
-            float total = 0.0f;
+        float f[NV * E], m = -INFINITY, total = 0.0f;
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                float f[E];
-                p[i].get(f);
+        for (int i = 0; i < NV; i++) p[i].get(f + i * E);
 #pragma unroll
-                for (int k = 0; k < E; k++) m = fmaxf(m, f[k]);
-            }
-            m = over_lanes<G>(m, [](float u, float v) { return fmaxf(u, v); });
-            m = m == -INFINITY ? 0.0f : m;
+        for (int k = 0; k < NV * E; k++) m = fmaxf(m, f[k]);
+        m = over_lanes<G>(m, [](float u, float v) { return fmaxf(u, v); });
+        m = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                float f[E];
-                p[i].get(f);
-#pragma unroll
-                for (int k = 0; k < E; k++) total += exp_gap(f[k], m, a.exp_mul);
-            }
-            total = lanes_sum<G>(total);
-            factor = total == 0.0f ? 0.0f : -mean * a.inv_t / total;
+        for (int k = 0; k < NV * E; k++) {
+            f[k] = exp_gap(f[k], m, a.exp_mul);
+            total += f[k];
         }
+        total = lanes_sum<G>(total);
+        const float factor = total == 0.0f ? 0.0f : -mean * a.inv_t / total;
         T *g = (T *)a.g + row * a.gs;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
@@ -397,16 +393,9 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
             if (c < V) {
                 float o[E];
 #pragma unroll
-                for (int k = 0; k < E; k += 4) *(float4 *)(o + k) = *(const float4 *)(s + c + k);
-                if (!a.renormalize) {
-                    float f[E];
-                    p[i].get(f);
+                for (int k = 0; k < E; k += 4) *(float4 *)(o + k) = *(const float4 *)(s_row + ((i * (E / 4) + k / 4) * G + rank) * 4);
 #pragma unroll
-                    for (int k = 0; k < E; k++) o[k] = __builtin_fmaf(exp_gap(f[k], m, a.exp_mul), factor, o[k]);
-                } else if (__builtin_expect(mean != mean, 0)) {
-#pragma unroll
-                    for (int k = 0; k < E; k++) o[k] = NAN;
-                }
+                for (int k = 0; k < E; k++) o[k] = __builtin_fmaf(f[i * E + k], factor, o[k]);
                 Piece<T> q;
                 q.set(o);
                 if (c + E <= V) q.store(g + c, false);
@@ -414,6 +403,62 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
             }
         }
         lanes_wait();
+    }
+}
+
+// ... of weights that sum to one: the scores have no part in it, and few classes have a gradient.  A block's rows lie in shared memory as they will in the result, L lanes to a
+// row put their entries there, and all of the block's threads write the rows.
+template <typename T, int L>
+__global__ __launch_bounds__(256) void k_chosen_grad(RouteArgs a, int rows, int wide) {
+    constexpr int E = Piece<T>::E;
+    typedef std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> Bits;
+    extern __shared__ __align__(16) unsigned char s_dyn[]; // [rows][wide] of T
+    Bits *const s_rows = (Bits *)s_dyn;
+    const int rank = threadIdx.x & (L - 1), V = a.V;
+    const int64_t first = (int64_t)blockIdx.x * rows;
+    const int here = a.N - first < rows ? (int)(a.N - first) : rows;
+    for (int k = threadIdx.x * E; k < here * wide; k += 256 * E) *(uint4 *)(s_rows + k) = {0, 0, 0, 0};
+    __syncthreads();
+    const int r = threadIdx.x / L;
+    if (r < here) {
+        Bits *const s = s_rows + r * wide;
+        const int64_t at = (first + r) * a.top + rank;
+        const bool has = rank < a.top;
+        const int64_t id = has ? (a.id64 ? ((const int64_t *)a.ids_in)[at] : (int64_t)((const int32_t *)a.ids_in)[at]) : -1;
+        const float w = has ? a.w_in[at] : 0.0f, dw = has ? a.dw[at] : 0.0f;
+        const bool in = id >= 0 && id < V;
+        const float mean = lanes_sum<L>(id >= V ? NAN : id >= 0 ? w * dw : 0.0f); // an id of no class makes the row's gradient NaN
+        float value = w * (dw - mean) * a.inv_t;
+        // Every entry writes its number at its class and looks whether it is still there: an expert that is chosen twice is none of a choice's, but may be given
+        if (in) s[id] = (Bits)(rank + 1);
+        lanes_wait();
+        const bool twice = in && s[id] != (Bits)(rank + 1);
+        if (__builtin_expect(__any(twice), 0)) { // each of them has the sum, in the entries' order
+            float sum = 0.0f;
+            for (int j = 0; j < L; j++) {
+                const int other = __shfl(in ? (int)id : -1, j, L);
+                const float more = __shfl(value, j, L);
+                if (in && other == (int)id) sum += more;
+            }
+            value = sum;
+        }
+        lanes_wait();
+        if (in) s[id] = __builtin_bit_cast(Bits, (T)value);
+        if (__builtin_expect(mean != mean, 0)) {
+            lanes_wait();
+            for (int c = rank; c < V; c += L) s[c] = __builtin_bit_cast(Bits, (T)NAN);
+        }
+    }
+    __syncthreads();
+    const uint32_t pieces = (V + E - 1) / E;
+    for (uint32_t i = threadIdx.x; i < here * pieces; i += 256) {
+        const uint32_t r = i / pieces, v = i - r * pieces;
+        T *const g = (T *)a.g + (first + r) * a.gs + v * E;
+        const uint4 o = *(const uint4 *)(s_rows + r * wide + v * E);
+        Piece<T> q;
+        q.r = {{o.x, o.y, o.z, o.w}};
+        if ((int)(v * E) + E <= V) q.store(g, false);
+        else q.store_some(g, V - v * E);
     }
 }
 
@@ -469,8 +514,32 @@ static void launch_grad_as(hipStream_t s, const RouteArgs &a) {
     const int64_t blocks = (a.N + ROWS - 1) / ROWS;
     hipLaunchKernelGGL((k_route_grad<T, G, N / Piece<T>::E>), dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), ROWS * G * N * 4, s, a);
 }
+// A lane to an entry, or as many rows as 16 KB hold: ten blocks to a unit (131 072 rows of 1000, 10 of them, bf16: 57.9 us, of 8 KB rows in 32 bits 120 | 96; 64, 6 of them: 7.8
+// us, by twice and four times the rows 7.8 and 9.2; 1024 rows 3.2 | 3.7 | 4.9)
+template <typename T, int L>
+static void launch_chosen(hipStream_t s, RouteArgs a) {
+    const int wide = (a.V + 7) / 8 * 8, bytes = wide * (int)sizeof(T), rows = 16384 / bytes < 256 / L ? 16384 / bytes : 256 / L;
+    const int64_t all = a.N, some = (int64_t)rows << 22;
+    for (int64_t row0 = 0; row0 < all; row0 += some) {
+        a.N = all - row0 < some ? all - row0 : some;
+        hipLaunchKernelGGL((k_chosen_grad<T, L>), dim3((unsigned)((a.N + rows - 1) / rows)), dim3(256), (size_t)rows * bytes, s, a, rows, wide);
+        a.ids_in = (const char *)a.ids_in + a.N * a.top * (a.id64 ? 8 : 4);
+        a.w_in += a.N * a.top;
+        a.dw += a.N * a.top;
+        a.g = (T *)a.g + a.N * a.gs;
+    }
+}
 template <typename T>
 static void launch_grad_typed(hipStream_t s, const RouteArgs &a) {
+    if (a.renormalize) {
+        if (a.top <= 1) return launch_chosen<T, 1>(s, a);
+        if (a.top <= 2) return launch_chosen<T, 2>(s, a);
+        if (a.top <= 4) return launch_chosen<T, 4>(s, a);
+        if (a.top <= 8) return launch_chosen<T, 8>(s, a);
+        if (a.top <= 16) return launch_chosen<T, 16>(s, a);
+        if (a.top <= 32) return launch_chosen<T, 32>(s, a);
+        return launch_chosen<T, 64>(s, a);
+    }
     const int n = (a.V + 15) / 16;
     if (n <= 1) launch_grad_as<T, 1, 16>(s, a);
     else if (n <= 2) launch_grad_as<T, 2, 16>(s, a);

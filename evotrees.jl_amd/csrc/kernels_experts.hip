@@ -1,8 +1,8 @@
-// Rows through experts: the choice of each row's experts from its class scores, the tables that order rows by expert, rows sorted by them and combined
-// again, dropout, and the gradients of these (formulas: include/evotrees_hip.h).
+// Rows through experts: the tables that order rows by expert, rows sorted by them and combined again, dropout, and the gradients of these (formulas:
+// include/evotrees_hip.h).
 //
-// All of it moves bytes: a score, a feature or a table entry is read once and written once, in pieces of sixteen bytes, by groups of lanes that share a row.
-// Products, sums and exponentials are 32-bit, and a value is rounded once, when it is written.
+// All of it moves bytes, in pieces of sixteen: of what is read or written in order memory is the bound, of scattered rows a little less of it (262 144 rows of 4096 bf16
+// sorted: of one expert 6.06 TB/s, of 8 5.59, of 64 5.24, of 512 5.20).  Products and sums are 32-bit, and a value is rounded once, when it is written.
 #include "experts.h"
 
 // ---- the tables of rows by expert ------------------------------------------------------------
@@ -49,8 +49,8 @@ __device__ __forceinline__ int lanes_inclusive(int v) {
     return sum_from<0x143, 0xc>(v); // row_bcast 31
 }
 // The block's exclusive sum over its threads' values, and all of it
-template <int W>
 __device__ __forceinline__ int block_exclusive(int v, int &all) {
+    constexpr int W = 4;
     __shared__ int s_w[W];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sum = lanes_inclusive(v);
     if (lane == 63) s_w[wave] = sum;
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256) void k_plan_sums(PlanArgs a) {
             v[i] = b + i < a.nb ? t[b + i] : 0;
             sum += v[i];
         }
-        int at = carry + block_exclusive<4>(sum, all);
+        int at = carry + block_exclusive(sum, all);
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             if (b + i < a.nb) t[b + i] = at;
@@ -95,9 +95,9 @@ enum { PLAN_ALONE, PLAN_BLOCKS, PLAN_SUMS };
 
 // Every entry's place: the experts before its own, its expert's entries of the blocks before, of the wavefronts before, and of the lanes before, found by
 // comparing the experts' bits over the wavefront.  Each wavefront has consecutive entries, so that an expert's keep their order.
-template <int W, int ITEMS, int FROM>
-__global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
-    constexpr int THREADS = 64 * W;
+template <int ITEMS, int FROM>
+__global__ __launch_bounds__(256) void k_plan_place(PlanArgs a) {
+    constexpr int W = 4, THREADS = 64 * W; // a wavefront's count of an expert has 16 bits
     // [E] where the block's entries of an expert start, [W / 2][E] pairs of wavefronts' counts, and of PLAN_BLOCKS [2][E] the blocks' sums
     extern __shared__ __align__(16) int s_plan[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), E = a.E;
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(64 * W) void k_plan_place(PlanArgs a) {
         if (blockIdx.x == 0) a.offsets[e] = sum;
         sum += total;
     }
-    const int start = block_exclusive<W>(sum, all);
+    const int start = block_exclusive(sum, all);
     for (int e = e0; e < e1; e++) {
         s_base[e] += start;
         if (blockIdx.x == 0) a.offsets[e] += start;
@@ -509,7 +509,9 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     // 8192 x 8 x 4096 153 | 149, 4096 x 8 x 2048 38.5 | 38.6, 1024 x 8 x 2048 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows
     // of 4099 sorted: 535 us, 667 so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 34.0), and gradients are no sooner done (908 | 911)
     const bool past = OP != ROWS_SPREAD && (double)a.N * a.H * sizeof(T) > 16e6 && (uintptr_t)a.out % 16 == 0 && a.os % E == 0 && a.H % E == 0;
-    const bool tiny = a.H < E, by_row = a.pieces >= 64;
+    // Wavefronts of one row, whose places and weights are scalars, from 512 pieces on (32 768 x 8 x 4096 bf16 combined: 509 us with the rows' pieces behind each other, 502
+    // so; of 4099 sorted 568 | 536); below, lanes without a piece cost more than that gives (65 536 x 4 x 520 combined: 63 | 75, dropout with a residual 35.5 | 44.6)
+    const bool tiny = a.H < E, by_row = a.pieces >= 512;
     const uint32_t each = a.pieces < 64 ? 64 : a.parts * 64; // threads a row, at most
     const uint32_t some = (1u << 30) / each > 0 ? (1u << 30) / each : 1, all = a.N; // rows of a launch
     for (uint64_t row0 = 0; row0 < all; row0 += some) {
@@ -547,33 +549,34 @@ static int launch_rows(hipStream_t s, RowArgs &a, int dtype) {
     return EVT_OK;
 }
 
+// One block for the smallest (16 x 6 of 64 experts: 3.0 us on the device, by a block of 1024 threads 6.2; 512 x 8: 7.8 us, by two launches 7.7).  Then a launch that
+// counts, in blocks of 1024 entries (131 072 x 2: 10.1 us, of 4096 17.8; 131 072 x 8 22 | 25), from 2^20 entries on of 4096 (262 144 x 8 of 256 experts 29.9 us, of 1024 36.9, of
+// 64 experts 26.0 | 22.6; 2 000 000 x 1 of 1023 45 | 63), and one that finds the places.  Up to 2048 counts each of its blocks adds up what is before it by itself (2048 x 8 of
+// 64: 9.0 us, 10.1 with a launch for the sums; of 4096 counts, 8192 x 8 of 64: 12.2 | 10.3).
 static void launch_plan(hipStream_t s, PlanArgs &a) {
     a.bits = 0;
     while ((1 << a.bits) < a.E) a.bits++;
     a.nb = 1;
+    const dim3 block(256);
+    const size_t count_lds = a.E * 4, place_lds = a.E * 12;
     if (a.n <= 1024) {
-        hipLaunchKernelGGL((k_plan_place<4, 4, PLAN_ALONE>), dim3(1), dim3(256), a.E * 12, s, a);
+        hipLaunchKernelGGL((k_plan_place<4, PLAN_ALONE>), dim3(1), block, place_lds, s, a);
         return;
     }
-    if (a.n <= 8192 && a.E <= 1024) {
-        hipLaunchKernelGGL((k_plan_place<16, 8, PLAN_ALONE>), dim3(1), dim3(1024), a.E * 36, s, a);
-        return;
-    }
-    const bool small = a.n <= (int64_t)1024 * 1024;
+    const bool small = a.n <= 1 << 20;
     const int chunk = small ? 1024 : 4096;
     a.nb = (int)((a.n + chunk - 1) / chunk);
-    const dim3 grid(a.nb), block(256);
-    const bool few = (int64_t)a.nb * a.E <= 4096;
-    const size_t count_lds = a.E * 4, place_lds = a.E * 12;
+    const dim3 grid(a.nb);
+    const bool few = small && a.nb * a.E <= 2048;
     if (small) hipLaunchKernelGGL(k_plan_count<4>, grid, block, count_lds, s, a, few ? 0 : 1);
     else hipLaunchKernelGGL(k_plan_count<16>, grid, block, count_lds, s, a, 1);
-    if (small && few) {
-        hipLaunchKernelGGL((k_plan_place<4, 4, PLAN_BLOCKS>), grid, block, a.E * 20, s, a);
+    if (few) {
+        hipLaunchKernelGGL((k_plan_place<4, PLAN_BLOCKS>), grid, block, a.E * 20, s, a);
         return;
     }
     hipLaunchKernelGGL(k_plan_sums, dim3(a.E), block, 0, s, a);
-    if (small) hipLaunchKernelGGL((k_plan_place<4, 4, PLAN_SUMS>), grid, block, place_lds, s, a);
-    else hipLaunchKernelGGL((k_plan_place<4, 16, PLAN_SUMS>), grid, block, place_lds, s, a);
+    if (small) hipLaunchKernelGGL((k_plan_place<4, PLAN_SUMS>), grid, block, place_lds, s, a);
+    else hipLaunchKernelGGL((k_plan_place<16, PLAN_SUMS>), grid, block, place_lds, s, a);
 }
 
 // ---- entry points ------------------------------------------------------------------------------

@@ -254,7 +254,7 @@ __device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v,
 
 // The block of rows that a block has, of as many as the 8 dies divide.  Blocks go round the dies, and each of them has the next of its own eighth of the rows: neighbours among an
 // expert's sorted rows come from neighbouring rows, so that the line where one ends and the next begins is put together in one die's cache (32 768 x 8 rows of 4099
-// bf16 sorted: 597 us with the blocks as they come, 546 so; of 4096 values, whole lines, 479 | 491)
+// bf16 sorted: 571 us with the blocks as they come, 520 so; of 4096 values, whole lines, 472 | 476; gradients at the leaves of 200 003 x 100 f32 60.7 | 56.5)
 __device__ __forceinline__ uint32_t own_block(uint32_t blocks) {
     return (blockIdx.x & 7) * (blocks / 8) + blockIdx.x / 8;
 }
@@ -328,9 +328,9 @@ __global__ __launch_bounds__(256) void k_spread(RowArgs a) {
 
 // ... and the sums of its products with the rows that lie at these places in y: a row to G lanes, or (G = 0) to a block of as many wavefronts as it has.
 template <typename T, int G, int TOP, bool TINY, bool DROP>
-__global__ __launch_bounds__(G ? 256 : 1024) void k_spread_dot(RowArgs a) {
+__global__ __launch_bounds__(G ? 256 : 512) void k_spread_dot(RowArgs a) {
     constexpr int E = Piece<T>::E, ROWS = G ? 256 / G : 1;
-    __shared__ float s_dot[G ? 1 : 16][TOP];
+    __shared__ float s_dot[G ? 1 : 8][TOP];
     const uint32_t size = G ? G : blockDim.x;
     if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
         if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
@@ -505,12 +505,12 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     a.pieces = (a.H + E - 1) / E;
     a.parts = (a.pieces + 63) / 64;
     // Results of more than half of what the second caches hold (8 x 4 MB) go past them, and what they come from is read as something that nobody reads again soon (32 768 x 8 x 4096
-    // bf16 combined: 485 us, 470 with the loads so, 439 with both; dropout of 65 536 x 8192 with a residual 553, 542, 519; combined and read by the next kernel, the pair:
-    // 8192 x 8 x 4096 153 | 149, 4096 x 8 x 2048 38.5 | 38.6, 1024 x 8 x 2048 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows
-    // of 4099 sorted: 535 us, 667 so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 34.0), and gradients are no sooner done (908 | 911)
+    // bf16 combined: 486 us, 432 so; dropout of 65 536 x 8192 with a residual 537 | 499; 4096 x 8 x 2048 33.2 | 29.2, and with the kernel that reads the result 38.5 | 38.6, of
+    // 1024 rows 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows of 4099 sorted: 535 us, 667
+    // so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 33.9), and gradients are no sooner done (908 | 911)
     const bool past = OP != ROWS_SPREAD && (double)a.N * a.H * sizeof(T) > 16e6 && (uintptr_t)a.out % 16 == 0 && a.os % E == 0 && a.H % E == 0;
-    // Wavefronts of one row, whose places and weights are scalars, from 512 pieces on (32 768 x 8 x 4096 bf16 combined: 509 us with the rows' pieces behind each other, 502
-    // so; of 4099 sorted 568 | 536); below, lanes without a piece cost more than that gives (65 536 x 4 x 520 combined: 63 | 75, dropout with a residual 35.5 | 44.6)
+    // Wavefronts of one row, whose places and weights are scalars, from 512 pieces on (32 768 x 8 x 4096 bf16 combined with a residual: 467 us with the rows' pieces behind each
+    // other, 462 so; of 4099 sorted 531 | 507); below, lanes without a piece cost more than that gives (65 536 x 4 x 520 combined: 62.5 | 74.6, dropout with a residual 34.8 | 43.8)
     const bool tiny = a.H < E, by_row = a.pieces >= 512;
     const uint32_t each = a.pieces < 64 ? 64 : a.parts * 64; // threads a row, at most
     const uint32_t some = (1u << 30) / each > 0 ? (1u << 30) / each : 1, all = a.N; // rows of a launch
@@ -525,9 +525,9 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
             else if (a.pieces <= 32) launch_dot_as<T, 32, false>(s, a, rows);
             else if (a.pieces <= 64) launch_dot_as<T, 64, false>(s, a, rows);
             else {
-                // blocks of up to 4 wavefronts in as many turns as it takes (32 768 rows of 8 x 4096 bf16: 1022 us by 8 or 16 wavefronts, 913 so; of 4099 1352 and
-                // 1664 | 1083), of up to 16 where rows are few (16 rows of 8 x 16 384: 20.4 us by 4, 11.1 by 16; 512 of 4096 16.3 | 14.9)
-                const int most = rows <= 512 ? 16 : 4, turns = (a.parts + most - 1) / most;
+                // blocks of up to 8 wavefronts in as many turns as it takes (32 768 rows of 8 x 4099 bf16 with dropout: 1033 us by 4, 1004 so, 1220 by 16; 16 rows of 8 x 16 384
+                // 14.5 | 10.3 | 10.4)
+                const int turns = (a.parts + 7) / 8;
                 launch_dot_as<T, 0, false>(s, a, rows, 64 * ((a.parts + turns - 1) / turns));
             }
         } else {

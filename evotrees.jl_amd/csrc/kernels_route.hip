@@ -477,15 +477,15 @@ static void launch_route_as(hipStream_t s, const RouteArgs &a) {
     else if (a.top <= 4) launch_best<T, G, N, 4>(s, a);
     else if (a.top <= 8) launch_best<T, G, N, 8>(s, a);
     else if constexpr (N % 16 == 0) {
-        // lists of 16 doubles are too many registers (131 072 x 1000 f32, 10 of them: 306 us, 244 so; bf16 124 | 143)
+        // lists of 16 doubles are too many registers (131 072 x 10 of 1000 f32: 306 us, 244 so; bf16 124 | 148, 16 of 256 30.1 | 52.9)
         if constexpr (sizeof(T) == 2) {
             if (a.top <= 16) return launch_best<T, G, N, 16>(s, a);
         }
         launch_best<T, G, N, 0>(s, a);
     }
 }
-// Lanes that share a row, and scores of each: 24 where they are enough (lists of 16 need a multiple of that); more scores a lane are fewer lists to join
-// between lanes, but their registers leave fewer wavefronts to a unit, with 32-bit scores twice as soon.
+// Lanes that share a row, and scores of each: 24 where they are enough (131 072 x 8 of 96 bf16: 14.3 us without, 10.9 so; of 384 42.9 | 34.2, f32 88.1 | 57; lists of 16 need a
+// multiple of that); more scores a lane are fewer lists to join between lanes, but their registers leave fewer wavefronts to a unit, with 32-bit scores twice as soon.
 template <typename T>
 static void launch_route_typed(hipStream_t s, const RouteArgs &a) {
     const int V = a.V;
@@ -514,8 +514,8 @@ static void launch_grad_as(hipStream_t s, const RouteArgs &a) {
     const int64_t blocks = (a.N + ROWS - 1) / ROWS;
     hipLaunchKernelGGL((k_route_grad<T, G, N / Piece<T>::E>), dim3((unsigned)(blocks < (1 << 22) ? blocks : 1 << 22)), dim3(256), ROWS * G * N * 4, s, a);
 }
-// A lane to an entry, or as many rows as 16 KB hold: ten blocks to a unit (131 072 rows of 1000, 10 of them, bf16: 57.9 us, of 8 KB rows in 32 bits 120 | 96; 64, 6 of them: 7.8
-// us, by twice and four times the rows 7.8 and 9.2; 1024 rows 3.2 | 3.7 | 4.9)
+// As many rows as the block has lanes for their entries, or as 16 KB hold, ten blocks to a unit (131 072 rows of 8 of 256 bf16: 16.8 us with 8 KB, 15.3 so and with 32; of 10 of
+// 1000 77.3, 57.8, 55.6; of 8 of 2048 109.8 with 32, 105.5 so; four times the lanes: 6 of 64 9.3 | 7.7 us, 1024 rows of these 4.9 | 3.1)
 template <typename T, int L>
 static void launch_chosen(hipStream_t s, RouteArgs a) {
     const int wide = (a.V + 7) / 8 * 8, bytes = wide * (int)sizeof(T), rows = 16384 / bytes < 256 / L ? 16384 / bytes : 256 / L;

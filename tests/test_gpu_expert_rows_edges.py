@@ -324,3 +324,24 @@ def test_scores_at_the_ends_of_their_type(evt, V, dtype):
             want, ww, tol = plain.route(x, top, renormalize, 1.0)
             assert torch.equal(ids.cpu(), want), (top, ids.cpu(), want)
             plain.close("weights", w, ww, tol.nan_to_num(0, 0, 0) + plain.U)
+
+
+@pytest.mark.parametrize("rows", [1, 2])
+@pytest.mark.parametrize("dtype", list(plain.TYPES))
+@pytest.mark.parametrize("H", [1, 8, 100, 2048, 5003])
+def test_single_rows(evt, H, dtype, rows):
+    """A service's step: one token or two through all of it, without dropout."""
+    experts, top, t = 64, 6, plain.TYPES[dtype]
+    gen = torch.Generator().manual_seed(H + rows)
+    scores, x, res = (torch.randn(rows, n, generator=gen).to(t) for n in (experts, H, H))
+    ids, w = evt.route_rows(scores.cuda(), top)
+    want, ww, tol = plain.route(scores, top, True, 1.0)
+    assert torch.equal(ids.cpu(), want)
+    plain.close("weights", w, ww, tol)
+    plan = evt.plan_rows(ids, experts)
+    place, source, offsets = plain.plan(want, experts)
+    assert plan.place.reshape(-1).tolist() == place and plan.source.tolist() == source and plan.offsets.tolist() == offsets
+    y = evt.sort_rows(x.cuda(), plan)
+    assert torch.equal(y.cpu(), x[torch.tensor(source) // top])
+    out = evt.combine_rows(y, plan, w, residual=res.cuda())
+    plain.close("combine", out, *plain.combine(y.cpu(), plan.place.cpu(), w.cpu(), res, 0.0, 0, 0))

@@ -203,6 +203,7 @@ struct RowArgs {
     uint32_t N, n;                     // rows; sorted rows, rows x top
     uint32_t row0;                     // the launch's first row
     uint32_t H, top, pieces, parts;    // pieces of a row; parts: of 64 pieces
+    uint32_t tail;                     // blocks that clear sorted rows that no entry has
     // dropout: an element is dropped whose 32 bits are below this
     uint32_t drop, layer;
     float scale;
@@ -255,9 +256,7 @@ __device__ __forceinline__ void store_piece(const Piece<T> &p, T *x, uint32_t v,
 // The block of rows that a block has, of as many as the 8 dies divide.  Blocks go round the dies, and each of them has the next of its own eighth of the rows: neighbours among an
 // expert's sorted rows come from neighbouring rows, so that the line where one ends and the next begins is put together in one die's cache (32 768 x 8 rows of 4099
 // bf16 sorted: 571 us with the blocks as they come, 520 so; of 4096 values, whole lines, 472 | 476; gradients at the leaves of 200 003 x 100 f32 60.7 | 56.5)
-__device__ __forceinline__ uint32_t own_block(uint32_t blocks) {
-    return (blockIdx.x & 7) * (blocks / 8) + blockIdx.x / 8;
-}
+__device__ __forceinline__ uint32_t own_block(uint32_t block, uint32_t blocks) { return (block & 7) * (blocks / 8) + block / 8; }
 // The row and piece that a thread has.  ROW: a wavefront's are of one row, which the compiler knows; otherwise the pieces of all rows follow each other, and
 // no lane is idle.
 template <bool ROW>
@@ -279,26 +278,35 @@ struct Share {
     }
 };
 
-// Sorted rows that no entry has: 0, by the launch's last blocks
-#define TAIL_BLOCKS 64
+// Sorted rows that no entry has: 0, by the launch's first blocks, beside the others (65 536 x 4 x 201 bf16 with 16 000 rows of padding sorted: by 64 blocks a row
+// to a block 198 us, by 1024 46, by 1024 whose rows' pieces follow each other 37)
 template <bool TINY, typename T>
 __device__ void clear_behind(const RowArgs &a, uint32_t block) {
     Piece<T> z;
     z.r = {};
     const int count = *a.count;
-    for (uint32_t p = (count < 0 ? 0u : (uint32_t)count) + block; p < a.n; p += TAIL_BLOCKS)
-        for (uint32_t v = threadIdx.x; v < a.pieces; v += blockDim.x) store_piece<TINY>(z, (T *)a.out + p * a.os, v, a.H);
+    const uint32_t first = count < 0 ? 0u : (uint32_t)count < a.n ? (uint32_t)count : a.n;
+    const uint64_t pieces = (uint64_t)(a.n - first) * a.pieces, step = (uint64_t)a.tail * blockDim.x;
+    uint64_t i = (uint64_t)block * blockDim.x + threadIdx.x;
+    uint32_t row = first + (uint32_t)(i / a.pieces), v = (uint32_t)(i % a.pieces);
+    const uint32_t rows = (uint32_t)(step / a.pieces), more = (uint32_t)(step % a.pieces);
+    for (; i < pieces; i += step) {
+        store_piece<TINY>(z, (T *)a.out + row * a.os, v, a.H);
+        v += more;
+        row += rows + (v >= a.pieces ? 1 : 0);
+        v -= v >= a.pieces ? a.pieces : 0;
+    }
 }
 
 // Rows to their places: each row is read once and written `top` times, times a weight if there are weights
 template <typename T, bool ROW, bool TINY, bool DROP>
 __global__ __launch_bounds__(256) void k_spread(RowArgs a) {
     constexpr int E = Piece<T>::E, TOP = 8;
-    if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
-        if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
+    if (blockIdx.x < a.tail) {
+        if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x);
         return;
     }
-    const Share<ROW> me(a, own_block(gridDim.x - TAIL_BLOCKS));
+    const Share<ROW> me(a, own_block(blockIdx.x - a.tail, gridDim.x - a.tail));
     if (!me.in) return;
     Piece<T> p;
     load_piece<TINY>(p, (const T *)a.x + me.row * a.xs, me.v, a.H);
@@ -332,12 +340,12 @@ __global__ __launch_bounds__(G ? 256 : 512) void k_spread_dot(RowArgs a) {
     constexpr int E = Piece<T>::E, ROWS = G ? 256 / G : 1;
     __shared__ float s_dot[G ? 1 : 8][TOP];
     const uint32_t size = G ? G : blockDim.x;
-    if (blockIdx.x >= gridDim.x - TAIL_BLOCKS) {
-        if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x - (gridDim.x - TAIL_BLOCKS));
+    if (blockIdx.x < a.tail) {
+        if (a.row0 == 0) clear_behind<TINY, T>(a, blockIdx.x);
         return;
     }
     const uint32_t rank = G ? threadIdx.x & (G - 1) : threadIdx.x, slot = G == 0 ? 0 : G == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : threadIdx.x / (G ? G : 1);
-    const uint32_t row = a.row0 + own_block(gridDim.x - TAIL_BLOCKS) * ROWS + slot;
+    const uint32_t row = a.row0 + own_block(blockIdx.x - a.tail, gridDim.x - a.tail) * ROWS + slot;
     if (row >= a.N) return;
     const T *x = (const T *)a.x + row * a.xs;
     const uint64_t key = DROP ? drop_key(a) : 0;
@@ -403,7 +411,7 @@ __global__ __launch_bounds__(G ? 256 : 512) void k_spread_dot(RowArgs a) {
 template <typename T, bool ROW, bool TINY, int TOP, bool DROP, bool PAST>
 __global__ __launch_bounds__(256) void k_combine(RowArgs a) {
     constexpr int E = Piece<T>::E;
-    const Share<ROW> me(a, own_block(gridDim.x));
+    const Share<ROW> me(a, own_block(blockIdx.x, gridDim.x));
     if (!me.in) return;
     Piece<T> res;
     float sum[E] = {};
@@ -475,8 +483,8 @@ static void launch_rows_as(hipStream_t s, const RowArgs &a, unsigned grid) {
     grid = round_up(grid);
     if constexpr (OP == ROWS_DROP) hipLaunchKernelGGL((k_drop<T, ROW, TINY, PAST>), dim3(grid), dim3(256), 0, s, a);
     else if constexpr (OP == ROWS_SPREAD) {
-        if (a.drop) hipLaunchKernelGGL((k_spread<T, ROW, TINY, true>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((k_spread<T, ROW, TINY, false>), dim3(grid + TAIL_BLOCKS), dim3(256), 0, s, a);
+        if (a.drop) hipLaunchKernelGGL((k_spread<T, ROW, TINY, true>), dim3(grid + a.tail), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((k_spread<T, ROW, TINY, false>), dim3(grid + a.tail), dim3(256), 0, s, a);
     } else {
         const auto go = [&](auto top) {
             if (a.drop) hipLaunchKernelGGL((k_combine<T, ROW, TINY, decltype(top)::value, true, PAST>), dim3(grid), dim3(256), 0, s, a);
@@ -490,7 +498,7 @@ static void launch_rows_as(hipStream_t s, const RowArgs &a, unsigned grid) {
 template <typename T, int G, bool TINY>
 static void launch_dot_as(hipStream_t s, const RowArgs &a, unsigned groups, int threads = 256) {
     constexpr int ROWS = G ? 256 / G : 1;
-    const unsigned grid = round_up((groups + ROWS - 1) / ROWS) + TAIL_BLOCKS;
+    const unsigned grid = round_up((groups + ROWS - 1) / ROWS) + a.tail;
     const auto go = [&](auto top) {
         if (a.drop) hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, true>), dim3(grid), dim3(threads), 0, s, a);
         else hipLaunchKernelGGL((k_spread_dot<T, G, decltype(top)::value, TINY, false>), dim3(grid), dim3(threads), 0, s, a);
@@ -504,6 +512,9 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     constexpr int E = Piece<T>::E;
     a.pieces = (a.H + E - 1) / E;
     a.parts = (a.pieces + 63) / 64;
+    // One block for every 4096 pieces that may have to be cleared: 16 rows of 6 x 2048 have 6 of them
+    const uint64_t clear = OP == ROWS_SPREAD ? (uint64_t)a.n * a.pieces / 4096 + 1 : 0;
+    a.tail = (uint32_t)(clear < 1024 ? clear : 1024);
     // Results of more than half of what the second caches hold (8 x 4 MB) go past them, and what they come from is read as something that nobody reads again soon (32 768 x 8 x 4096
     // bf16 combined: 486 us, 432 so; dropout of 65 536 x 8192 with a residual 537 | 499; 4096 x 8 x 2048 33.2 | 29.2, and with the kernel that reads the result 38.5 | 38.6, of
     // 1024 rows 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows of 4099 sorted: 535 us, 667
@@ -615,6 +626,7 @@ static int take_rows(const evt_rows *r, int64_t nx, int64_t no, int32_t flags, R
     ARGCHK(r->x_stride >= 0 && r->residual_stride >= 0, "strides must not be negative");
     ARGCHK(nx <= 0 || no <= 0 || (r->x && r->out), "rows and out must not be NULL");
     ARGCHK((uintptr_t)r->x % size == 0 && (uintptr_t)r->out % size == 0 && (uintptr_t)r->residual % size == 0, "rows must be aligned to their type");
+    ARGCHK((uintptr_t)r->seed_dev % 8 == 0, "seed_dev must be aligned to its type");
     ARGCHK(no <= 1 || r->out_stride >= r->nfeats, "out_stride must be at least nfeats");
     a.x = r->x;
     a.xs = r->x_stride;

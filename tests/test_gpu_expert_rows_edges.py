@@ -345,3 +345,19 @@ def test_single_rows(evt, H, dtype, rows):
     assert torch.equal(y.cpu(), x[torch.tensor(source) // top])
     out = evt.combine_rows(y, plan, w, residual=res.cuda())
     plain.close("combine", out, *plain.combine(y.cpu(), plan.place.cpu(), w.cpu(), res, 0.0, 0, 0))
+
+
+@pytest.mark.parametrize("dtype", list(plain.TYPES))
+@pytest.mark.parametrize("V", [40, 48, 49, 70, 96, 130, 160, 192, 193, 300, 384, 385, 600, 768, 769, 1200, 1536, 1537, 3000])
+def test_choices_of_every_length(evt, V, dtype):
+    """Every number of lanes and of scores a lane, lists of 2, 4, 8 and 16 and longer choices, with many equal scores."""
+    gen = torch.Generator().manual_seed(V)
+    x = (torch.randn(9, V, generator=gen) * 3).round() / 2
+    x[1, V // 3:] = -math.inf
+    x[2, :V - 3] = -math.inf
+    x = x.to(plain.TYPES[dtype])
+    for top in (1, 2, 3, 4, 5, 8, 9, 12, 16, 17, 33):
+        ids, w = evt.route_rows(x.cuda(), top, renormalize=top % 2 == 0, temperature=0.9)
+        want, ww, tol = plain.route(x, top, top % 2 == 0, 0.9)
+        assert torch.equal(ids.cpu(), want), (top, ids.cpu(), want)
+        plain.close("weights", w, ww, tol)

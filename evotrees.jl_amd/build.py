@@ -32,7 +32,7 @@ def _compile(src):
 
 
 def build(verbose=False):
-    with ThreadPoolExecutor(max_workers=8) as ex:
+    with ThreadPoolExecutor(max_workers=4) as ex:
         results = list(ex.map(_compile, SOURCES))
     objs = [r[0] for r in results]
     if verbose:

@@ -20,8 +20,8 @@ this package's losses, these are returned, not recorded: results never require a
 a result: a tensor like it, which counts as changed in place.
 
 Wrong arguments raise ValueError or TypeError before anything is queued; what a call refuses in the library raises EvtError."""
-import ctypes as C
 import operator
+import struct
 
 from . import _lib
 from . import class_losses as _scores
@@ -30,6 +30,10 @@ __all__ = ["RowPlan", "route_rows", "route_rows_grad", "plan_rows", "sort_rows",
 
 _TRUSTED = 2  # EVT_STATIC_TRUSTED: the tensors say where they are
 _MOST = 4096  # experts
+# an evt_rows (_lib.EvtRows) and an evt_scores (_lib.EvtScores) as bytes, a third of the time that a ctypes structure takes
+_rows_bytes = struct.Struct("@PqPqPqqiidQPI4x").pack
+_scores_bytes = struct.Struct("@PqPqqiid").pack
+_NONE = (0, 0)  # no residual
 _makers = {}  # by device and type
 _entries = {}  # by name
 
@@ -158,8 +162,11 @@ class _Rows:
             raise ValueError("the features of a row of %s must lie side by side, got strides %s" % (name, v.stride()))
         return v.data_ptr(), v.stride(0) if rows > 1 else self.feats
 
-    def result(self, out, rows):
+    def result(self, out, rows, like=None):
+        """The tensor that a result goes to; `like`, where it is contiguous, makes one sooner."""
         if out is None:
+            if like is not None and like.is_contiguous():
+                return _scores._like(like)
             return _make(self.device, self.x.dtype, (rows, self.feats), self.x.device)
         self.like("out", out, rows)
         if rows > 1 and out.stride(0) < self.feats:
@@ -177,12 +184,13 @@ class _Rows:
             raise ValueError("the plan is on %s, the rows are on %s" % (plan._on, self.x.device))
         return n
 
-    def args(self, out, rows, residual, p, seed, layer):
+    def args(self, out, rows, res, p, seed, layer):
+        """The call's evt_rows; res: address and row stride of the residual."""
         x, n = self.x, self.rows
         p = float(p)
         if not 0.0 <= p < 1.0:
             raise ValueError("p must be in [0, 1), got %s" % p)
-        at, seed_at = 0, None
+        at = seed_at = 0
         if p:
             if isinstance(seed, _scores._torch.Tensor):
                 seed_at = _check("seed", seed if seed.dim() else seed.view(1), (1,), (_scores._torch.int64,), self.device, x.device)
@@ -191,9 +199,8 @@ class _Rows:
             layer = _whole("layer", layer, 0, 0xFFFFFFFF)
         else:
             layer = 0
-        res = (None, 0) if residual is None else self.like("residual", residual, out.shape[0])
-        return _lib.EvtRows(x.data_ptr(), x.stride(0) if n > 1 else self.feats, out.data_ptr(), out.stride(0) if out.shape[0] > 1 else self.feats, res[0], res[1],
-                            rows, self.feats, self.kind, p, at, seed_at, layer)
+        return _rows_bytes(x.data_ptr(), x.stride(0) if n > 1 else self.feats, out.data_ptr(), out.stride(0) if out.shape[0] > 1 else self.feats, res[0], res[1],
+                           rows, self.feats, self.kind, p, at, seed_at, layer)
 
     def run(self, name, *args):
         _queue(name, self.device, self.x.device, *args)
@@ -210,8 +217,8 @@ def _route(scores, top, temperature):
 
 def _evt_scores(call, grad):
     x, rows = call.x, call.rows
-    return _lib.EvtScores(x.data_ptr(), x.stride(0) if rows > 1 else call.classes, None if grad is None else grad.data_ptr(),
-                          0 if grad is None else grad.stride(0) if rows > 1 else call.classes, rows, call.classes, call.kind, call.temperature)
+    return _scores_bytes(x.data_ptr(), x.stride(0) if rows > 1 else call.classes, 0 if grad is None else grad.data_ptr(),
+                         0 if grad is None else grad.stride(0) if rows > 1 else call.classes, rows, call.classes, call.kind, call.temperature)
 
 
 def route_rows(scores, top, renormalize=True, temperature=1.0):
@@ -223,7 +230,7 @@ def route_rows(scores, top, renormalize=True, temperature=1.0):
     torch = _scores._torch
     experts = _make(call.device, torch.int32, (call.rows, top), call.x.device)
     weights = _make(call.device, torch.float32, (call.rows, top), call.x.device)
-    _queue("evt_route_rows", call.device, call.x.device, C.byref(_evt_scores(call, None)), top, 1 if renormalize else 0, experts.data_ptr(), weights.data_ptr())
+    _queue("evt_route_rows", call.device, call.x.device, _evt_scores(call, None), top, 1 if renormalize else 0, experts.data_ptr(), weights.data_ptr())
     return experts, weights
 
 
@@ -237,7 +244,7 @@ def route_rows_grad(scores, experts, weights, dweights, renormalize=True, temper
     ids_at = call.check("experts", experts, shape, _scores._INTS)
     w_at, dw_at = call.check("weights", weights, shape, _scores._F32S), call.check("dweights", dweights, shape, _scores._F32S)
     grad = call.gradient(True, out)
-    _queue("evt_route_rows_grad", call.device, call.x.device, C.byref(_evt_scores(call, grad)), top, 1 if renormalize else 0, ids_at, _scores._INTS[experts.dtype],
+    _queue("evt_route_rows_grad", call.device, call.x.device, _evt_scores(call, grad), top, 1 if renormalize else 0, ids_at, _scores._INTS[experts.dtype],
            w_at, dw_at)
     if out is not None and not out.is_inference():
         _scores._changed(out)
@@ -276,7 +283,7 @@ def sort_rows(x, plan, out=None):
     call = _Rows("x", x)
     n = call.plan(plan, False)
     y = call.result(out, n)
-    call.run("evt_sort_rows", C.byref(call.args(y, call.rows, None, 0.0, 0, 0)), plan._at, plan.offsets_at, plan.top, plan.experts)
+    call.run("evt_sort_rows", call.args(y, call.rows, _NONE, 0.0, 0, 0), plan._at, plan.offsets_at, plan.top, plan.experts)
     return y
 
 
@@ -288,8 +295,9 @@ def combine_rows(y, plan, weights=None, residual=None, p=0.0, seed=None, layer=0
     call = _Rows("y", y)
     call.plan(plan, True)
     w_at = None if weights is None else _check("weights", weights, (plan.rows, plan.top), _scores._F32S, call.device, y.device)
-    z = call.result(out, plan.rows)
-    call.run("evt_combine_rows", C.byref(call.args(z, plan.rows, residual, p, seed, layer)), plan._at, w_at, plan.top)
+    res = _NONE if residual is None else call.like("residual", residual, plan.rows)
+    z = call.result(out, plan.rows, residual)
+    call.run("evt_combine_rows", call.args(z, plan.rows, res, p, seed, layer), plan._at, w_at, plan.top)
     return z
 
 
@@ -312,7 +320,7 @@ def combine_rows_grad(dout, y, plan, weights, p=0.0, seed=None, layer=0):
         if not n:
             y_at = (None, 0)
     dy = call.result(None, n)
-    call.run("evt_combine_rows_grad", C.byref(call.args(dy, call.rows, None, p, seed, layer)), y_at[0], y_at[1], plan._at, plan.offsets_at, w_at, dw_at, plan.top,
+    call.run("evt_combine_rows_grad", call.args(dy, call.rows, _NONE, p, seed, layer), y_at[0], y_at[1], plan._at, plan.offsets_at, w_at, dw_at, plan.top,
              plan.experts)
     return dy, dweights
 
@@ -324,6 +332,7 @@ def drop_rows(x, p, seed, layer=0, residual=None, out=None):
     layer: a whole number that keeps a program's uses of one seed apart.  Which values are dropped depends on seed, layer, row and column alone (include/evotrees_hip.h says how); no
     mask is stored, and the gradient by x is drop_rows(dout, p, seed, layer).  What is dropped is 0 also where x is infinite or no number.  `out` may be x or the residual."""
     call = _Rows("x", x)
-    z = call.result(out, call.rows)
-    call.run("evt_drop_rows", C.byref(call.args(z, call.rows, residual, p, seed, layer)))
+    res = _NONE if residual is None else call.like("residual", residual, call.rows)
+    z = call.result(out, call.rows, x)
+    call.run("evt_drop_rows", call.args(z, call.rows, res, p, seed, layer))
     return z

@@ -159,3 +159,14 @@ def test_entry_points_refuse(evt):
     for name, args in (("evt_route_rows", (scores(nrows=0), 2, 1, None, None, 2)), ("evt_sort_rows", (rows(nrows=0), None, None, 2, 3, 2)),
                        ("evt_combine_rows", (rows(nrows=0), None, None, 2, 2)), ("evt_drop_rows", (rows(nrows=0, x=None, out=None), 2))):
         assert _code(evt, name, *args)[0] == 0
+
+
+def test_bytes_are_the_structures(evt):
+    import sys
+    rows = sys.modules[evt.RowPlan.__module__]
+    v = (1 << 40, 2, 1 << 41, 3, 1 << 42, 4, 5, 6, 7, 0.5, 2 ** 64 - 1, 1 << 43, 2 ** 32 - 1)
+    r = evt._lib.EvtRows.from_buffer_copy(rows._rows_bytes(*v))
+    assert tuple(getattr(r, f[0]) for f in r._fields_) == v and C.sizeof(r) == len(rows._rows_bytes(*v))
+    v = (1 << 40, 2, 1 << 41, 3, 4, 5, 6, 0.25)
+    r = evt._lib.EvtScores.from_buffer_copy(rows._scores_bytes(*v))
+    assert tuple(getattr(r, f[0]) for f in r._fields_) == v and C.sizeof(r) == len(rows._scores_bytes(*v))

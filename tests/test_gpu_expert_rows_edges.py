@@ -361,3 +361,46 @@ def test_choices_of_every_length(evt, V, dtype):
         want, ww, tol = plain.route(x, top, top % 2 == 0, 0.9)
         assert torch.equal(ids.cpu(), want), (top, ids.cpu(), want)
         plain.close("weights", w, ww, tol)
+
+
+@pytest.mark.parametrize("dtype", list(plain.TYPES))
+@pytest.mark.parametrize("H", [70_001, 1_000_003])
+def test_very_long_rows(evt, H, dtype):
+    rows, top, t = 3, 2, plain.TYPES[dtype]
+    gen = torch.Generator().manual_seed(H)
+    ids = torch.tensor([[1, 0], [-1, 1], [0, 2]])
+    plan = evt.plan_rows(ids.cuda(), 3)
+    place = plan.place.cpu()
+    x, res, y = (torch.randn(n, H, generator=gen).to(t) for n in (rows, rows, rows * top))
+    w = torch.rand(rows, top, generator=gen)
+    want = torch.zeros(rows * top, H, dtype=t)
+    for r in range(rows):
+        for j in range(top):
+            if place[r, j] >= 0:
+                want[place[r, j]] = x[r]
+    assert torch.equal(evt.sort_rows(x.cuda(), plan).cpu(), want)
+    plain.close("combine", evt.combine_rows(y.cuda(), plan, w.cuda(), residual=res.cuda(), p=0.2, seed=8, layer=1), *plain.combine(y, place, w, res, 0.2, 8, 1))
+    dy, dw = evt.combine_rows_grad(x.cuda(), y.cuda(), plan, w.cuda(), p=0.2, seed=8, layer=1)
+    want_y, want_w = plain.combine_grad(x, y, place, w, 0.2, 8, 1)
+    plain.close("dy", dy, *want_y)
+    plain.close("dweights", dw, *want_w)
+    plain.close("drop", evt.drop_rows(x.cuda(), 0.2, 8, layer=1), *plain.drop(x, 0.2, 8, 1, None))
+
+
+def test_many_experts_a_row(evt):
+    """A model's trees as routers: two hundred entries a row."""
+    rows, top, experts, H = 40, 203, 31, 37
+    ids, gen = torch.randint(-1, experts, (rows, top), generator=torch.Generator().manual_seed(1)), torch.Generator().manual_seed(2)
+    plan = evt.plan_rows(ids.cuda(), experts)
+    place, source, offsets = plain.plan(ids, experts)
+    assert plan.place.reshape(-1).tolist() == place and plan.source.tolist() == source and plan.offsets.tolist() == offsets
+    place = plan.place.cpu()
+    x, y, w = torch.randn(rows, H, generator=gen), torch.randn(rows * top, H, generator=gen), torch.rand(rows, top, generator=gen)
+    n = offsets[-1]
+    sorted_rows = evt.sort_rows(x.cuda(), plan).cpu()
+    assert torch.equal(sorted_rows[:n], x[torch.tensor(source[:n]) // top]) and (sorted_rows[n:] == 0).all()
+    plain.close("combine", evt.combine_rows(y.cuda(), plan, w.cuda()), *plain.combine(y, place, w, None, 0.0, 0, 0))
+    dy, dw = evt.combine_rows_grad(x.cuda(), y.cuda(), plan, w.cuda())
+    want_y, want_w = plain.combine_grad(x, y, place, w, 0.0, 0, 0)
+    plain.close("dy", dy, *want_y)
+    plain.close("dweights", dw, *want_w)

@@ -329,8 +329,8 @@ def drop_rows(x, p, seed, layer=0, residual=None, out=None):
     """residual + dropout(x): each value is 0 with probability p and x / (1 - p) otherwise (p in multiples of 2^-32).
 
     seed: a whole number, or an int64 tensor of one element on the rows' GPU, read when the work runs, so that a replayed graph draws anew when its program changed it.
-    layer: a whole number that keeps a program's uses of one seed apart.  Which values are dropped depends on seed, layer, row and column alone (include/evotrees_hip.h says how); no
-    mask is stored, and the gradient by x is drop_rows(dout, p, seed, layer).  What is dropped is 0 also where x is infinite or no number.  `out` may be x or the residual."""
+    layer: a whole number that keeps a program's uses of one seed apart.  Which values are dropped depends on seed, layer, row, column and the number of features alone (include/evotrees_hip.h
+    says how); no mask is stored, and the gradient by x is drop_rows(dout, p, seed, layer).  What is dropped is 0 also where x is infinite or no number.  `out` may be x or the residual."""
     call = _Rows("x", x)
     res = _NONE if residual is None else call.like("residual", residual, call.rows)
     z = call.result(out, call.rows, x)

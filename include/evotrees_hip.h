@@ -494,7 +494,7 @@ int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype, int64_t n
  * Dropout: an element of row r and column c has 32 random bits; drop(v) is 0 - whatever v is - where they are below t = p 2^32 (rounded) and
  * v 2^32 / (2^32 - t) elsewhere.  The bits come from SplitMix64 as a row sample's do (evt_draw_mask): with key = output number `layer` (from 0) of the generator started at the seed,
  * their upper half is bits 16 (c % 4) .. of output number r ceil(nfeats / 4) + c / 4 of the generator started at key, their lower half the same bits of the same
- * output of the one started at ~key.  No mask is stored: the same seed, layer, r and c give the same bits, in the gradient as well. */
+ * output of the one started at ~key.  No mask is stored: the same seed, layer, r, c and nfeats give the same bits, in the gradient as well. */
 typedef struct {
     const void *x;
     int64_t x_stride;

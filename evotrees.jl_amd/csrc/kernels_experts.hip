@@ -592,8 +592,8 @@ static void launch_plan(hipStream_t s, PlanArgs &a) {
         hipLaunchKernelGGL((k_plan_place<4, PLAN_ALONE, false>), dim3(1), block, place_lds, s, a);
         return;
     }
-    const bool small = a.n <= 1 << 20;
-    const int chunk = small ? 1024 : 4096;
+    const int chunk = EVT_PLAN_BLOCK(a.n);
+    const bool small = chunk == 1024;
     a.nb = (int)((a.n + chunk - 1) / chunk);
     const dim3 grid(a.nb);
     const bool few = small && a.nb * a.E <= 2048;

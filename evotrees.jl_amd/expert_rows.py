@@ -271,8 +271,8 @@ def plan_rows(experts, n_experts):
     if device < 0:
         raise ValueError("experts must be on a GPU, got %s" % on)
     # the tables, and what the call works in behind them
-    kept = 2 * n + n_experts + 1
-    plan = RowPlan(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + ((n + 1023) // 1024 + 1) * n_experts,), on))
+    kept, block = 2 * n + n_experts + 1, 1024 if n <= 1 << 20 else 4096
+    plan = RowPlan(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + ((n + block - 1) // block + 1) * n_experts,), on))
     _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, plan._at + 4 * kept)
     return plan
 

@@ -484,7 +484,8 @@ int evt_route_rows_grad(void *stream, const void *scores /* evt_scores */, int32
  * 0 .. nexperts - 1 is none, and one may come twice in a row.  Entry i = row * top + j of an expert stands behind its expert's entries of lower i:
  *   place[i] = its place in that order (-1: none),  source[place[i]] = i (-1 behind the last),  expert e has the places offsets[e] .. offsets[e + 1] - 1
  * (nexperts + 1 numbers).  work: EVT_PLAN_WORK(nrows * top, nexperts) int32 that the call may write. */
-#define EVT_PLAN_WORK(n, nexperts) ((((int64_t)(n) + 1023) / 1024 + 1) * (int64_t)(nexperts))
+#define EVT_PLAN_BLOCK(n) ((n) <= 1 << 20 ? 1024 : 4096) /* entries of a block */
+#define EVT_PLAN_WORK(n, nexperts) ((((int64_t)(n) + EVT_PLAN_BLOCK(n) - 1) / EVT_PLAN_BLOCK(n) + 1) * (int64_t)(nexperts))
 int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype, int64_t nrows, int32_t top, int32_t nexperts, int32_t *place, int32_t *source,
                   int32_t *offsets, int32_t *work, int32_t flags);
 

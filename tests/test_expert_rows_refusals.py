@@ -170,3 +170,14 @@ def test_bytes_are_the_structures(evt):
     v = (1 << 40, 2, 1 << 41, 3, 4, 5, 6, 0.25)
     r = evt._lib.EvtScores.from_buffer_copy(rows._scores_bytes(*v))
     assert tuple(getattr(r, f[0]) for f in r._fields_) == v and C.sizeof(r) == len(rows._scores_bytes(*v))
+
+
+def test_work_of_the_tables_is_the_headers(evt):
+    """plan_rows' share of its tensor, by the macro's own text."""
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "evotrees_hip.h")) as f:
+        header = f.read()
+    assert re.search(r"EVT_PLAN_BLOCK\(n\) \(\(n\) <= 1 << 20 \? 1024 : 4096\)", header)
+    with open(evt.RowPlan.__init__.__code__.co_filename) as f:
+        assert "1024 if n <= 1 << 20 else 4096" in f.read()

@@ -404,3 +404,21 @@ def test_many_experts_a_row(evt):
     want_y, want_w = plain.combine_grad(x, y, place, w, 0.0, 0, 0)
     plain.close("dy", dy, *want_y)
     plain.close("dweights", dw, *want_w)
+
+
+@pytest.mark.parametrize("n", [1 << 20, (1 << 20) + 1, (1 << 20) + 4097])
+@pytest.mark.parametrize("experts", [5, 700, 2049])
+def test_tables_around_the_large_blocks(evt, n, experts):
+    """Both block sizes, joined sources and single ones, entries without an expert; against a stable sort."""
+    gen = torch.Generator().manual_seed(n + experts)
+    ids = (torch.rand(n, generator=gen) ** 3 * experts).long()
+    ids[torch.rand(n, generator=gen) < 0.05] = -1
+    plan = evt.plan_rows(ids.cuda(), experts)
+    key = torch.where(ids < 0, experts, ids)
+    order = torch.argsort(key, stable=True)
+    count = int((ids >= 0).sum())
+    place = torch.empty_like(order)
+    place[order] = torch.arange(n)
+    assert torch.equal(plan.place.cpu()[:, 0].long(), torch.where(ids < 0, -1, place))
+    assert torch.equal(plan.source.cpu().long(), torch.where(torch.arange(n) < count, order, -1))
+    assert plan.offsets.tolist() == [0] + torch.bincount(key, minlength=experts + 1)[:experts].cumsum(0).tolist()

@@ -385,7 +385,8 @@ __global__ __launch_bounds__(256) void k_route_grad(RouteArgs a) {
             total += f[k];
         }
         total = lanes_sum<G>(total);
-        const float factor = total == 0.0f ? 0.0f : -mean * a.inv_t / total;
+        // a row of -inf has no shares; what makes its gradient NaN does so all the same
+        const float factor = total == 0.0f && mean == mean ? 0.0f : -mean * a.inv_t / total;
         T *g = (T *)a.g + row * a.gs;
 #pragma unroll
         for (int i = 0; i < NV; i++) {

@@ -684,8 +684,8 @@ extern "C" int evt_sort_rows(void *stream, const void *rows, const int32_t *plac
     TRY(take_places(r->nrows, top, nexperts, place, a));
     TRY(take_rows(r, r->nrows, a.n, flags, a));
     ARGCHK(!r->residual && r->p == 0.0, "sorted rows have no residual and no dropout");
-    ARGCHK(top > 1 || r->x != r->out, "sorted rows must lie apart from the rows");
     if (a.N == 0) return EVT_OK;
+    ARGCHK(top > 1 || r->x != r->out, "sorted rows must lie apart from the rows");
     ARGCHK(offsets, "offsets must not be NULL");
     TRY(check_device(flags, place, offsets));
     a.count = offsets + nexperts;
@@ -700,8 +700,8 @@ extern "C" int evt_combine_rows(void *stream, const void *rows, const int32_t *p
     RowArgs a = {};
     TRY(take_places(r->nrows, top, 1, place, a));
     TRY(take_rows(r, a.n, r->nrows, flags, a));
-    ARGCHK(top > 1 || r->x != r->out, "combined rows must lie apart from the experts' rows");
     if (a.N == 0) return EVT_OK;
+    ARGCHK(top > 1 || r->x != r->out, "combined rows must lie apart from the experts' rows");
     TRY(check_device(flags, place, weights));
     a.w = weights;
     return launch_rows<ROWS_COMBINE>((hipStream_t)stream, a, r->dtype);
@@ -719,9 +719,9 @@ extern "C" int evt_combine_rows_grad(void *stream, const void *rows, const void 
     ARGCHK(!r->residual, "the gradient takes no residual");
     ARGCHK((y != nullptr) == (dweights != nullptr) && (!y || weights), "y and dweights come together, and with weights");
     ARGCHK(y_stride >= 0 && (uintptr_t)y % size_of(r->dtype) == 0, "y must be aligned to its type, its stride not negative");
+    if (a.N == 0) return EVT_OK;
     ARGCHK(top > 1 || r->x != r->out, "the experts' gradients must lie apart from the rows'");
     ARGCHK(apart({y, y_stride, a.n}, {r->out, r->out_stride, a.n}, a.H, size_of(r->dtype)), "the experts' gradients must lie apart from y");
-    if (a.N == 0) return EVT_OK;
     ARGCHK(offsets, "offsets must not be NULL");
     TRY(check_device(flags, y, place, offsets, weights, dweights));
     a.count = offsets + nexperts;

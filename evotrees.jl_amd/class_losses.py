@@ -30,7 +30,7 @@ _entries = {}  # by name
 
 def _load():
     """torch, the codes of its types and what a call needs of it; imported with the first call, a fit needs none."""
-    global _torch, _FLOATS, _INTS, _F32S, _I32S, _like, _device, _stream, _changed
+    global _torch, _FLOATS, _INTS, _F32S, _I32S, _like, _device, _stream, _changed, _wrapped
     import torch
     _F32S = {torch.float32: _F32}
     _FLOATS = {torch.float32: _F32, torch.bfloat16: _BF16, torch.float16: _F16}
@@ -41,7 +41,13 @@ def _load():
     _changed = torch.autograd.graph.increment_version
     # the current stream's handle without a Stream object around it, 1.1 us less a call
     _stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda index: torch.cuda.current_stream(index).cuda_stream)
+    _wrapped = getattr(getattr(torch._C, "_functorch", None), "is_functorch_wrapped_tensor", lambda t: False)
     _torch = torch
+
+
+def _lasts(t):
+    """Whether a tensor can make others for later calls: one that a tracer's mode or a function transform made is theirs, and has no memory when they have ended."""
+    return type(t) is _torch.Tensor and not _wrapped(t)
 
 
 def _bad(name, v, x, shape, kinds):
@@ -115,8 +121,9 @@ class _Call:
         """A float32 tensor on the call's device, by way of one that is there: 0.3 us less than torch.empty with a type and a device."""
         make = _makers.get(self.device)
         if make is None:
-            make = _torch.empty(0, dtype=_torch.float32, device=self.x.device).new_empty
-            if self.device >= 0:
+            one = _torch.empty(0, dtype=_torch.float32, device=self.x.device)
+            make = one.new_empty
+            if self.device >= 0 and _lasts(one):
                 _makers[self.device] = make
         return make(shape)
 

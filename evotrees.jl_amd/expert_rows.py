@@ -48,8 +48,9 @@ def _make(device, dtype, shape, on):
     """A tensor by way of one that is there: less time than torch.empty with a type and a device."""
     make = _makers.get((device, dtype))
     if make is None:
-        make = _scores._torch.empty(0, dtype=dtype, device=on).new_empty
-        if device >= 0:
+        one = _scores._torch.empty(0, dtype=dtype, device=on)
+        make = one.new_empty
+        if device >= 0 and _scores._lasts(one):
             _makers[(device, dtype)] = make
     return make(shape)
 

@@ -17,7 +17,8 @@ a layer's that a router chooses for a language model's token, or a model of its 
 Rows are (rows, features) tensors of float32, bfloat16 or float16 whose features lie side by side (`x.stride(1) == 1`); rows may be any distance apart.  Weights and
 their gradients are contiguous float32.  All tensors of a call are on one GPU; the work is queued on that GPU's current stream and nothing waits for it.  As the gradients of
 this package's losses, these are returned, not recorded: results never require a gradient, and a call is its own backward pass's part as shown above.  `out` takes
-a result: a tensor like it, which counts as changed in place.
+a result: a tensor like it, which counts as changed in place.  It shares no memory with what the call reads but where a call says so; columns of one matrix, with equal
+strides, share none.
 
 Wrong arguments raise ValueError or TypeError before anything is queued; what a call refuses in the library raises EvtError."""
 import operator

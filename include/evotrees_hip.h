@@ -471,7 +471,7 @@ int evt_preference_loss(void *stream, const void *scores /* evt_scores */, const
  *   weights[i, j] = exp(z_ej) / sum of exp(z) over the row's chosen (renormalize 1) or over all of its experts (0).
  * A score of -inf is an expert that cannot be chosen: a row with fewer others has the id -1 and the weight 0 in what is left.  A NaN (the best of all scores)
  * or +inf makes its row's weights NaN.  experts, weights: nrows x top.  grad is not used.
- * The gradient, from what the choice returned and the weights' gradient dweights, written to grad (which may be the scores' own memory, as above):
+ * The gradient, from what the choice returned and the weights' gradient dweights, written to grad (the scores' own memory, as above, or apart from it):
  *   renormalize 1: grad[i, c] = sum over j with e_j == c of w_j (dw_j - m) / temperature,  m = sum_j w_j dw_j;
  *   renormalize 0: grad[i, c] = (sum over j with e_j == c of w_j dw_j - q_c m) / temperature,  q = softmax(z).
  * A negative id has no part in it, whatever stands at its weight and slope.  A NaN among the others, an id of nclass or more, or with renormalize 0 a NaN or +inf
@@ -491,6 +491,7 @@ int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype, int64_t n
 
 /* Rows of nfeats values (EVT_F32, EVT_BF16 or EVT_F16, alike in a call), a row's side by side, rows a stride of elements apart (any alignment; 0: one row
  * for all, where it is only read).  Products and sums have 32 bits, a value is rounded once.  Elements between nfeats and out_stride stay as they are.
+ * `apart`: no byte in common, and one range of addresses behind the other, or rows of equal strides side by side, as columns of one matrix are.
  *
  * Dropout: an element of row r and column c has 32 random bits; drop(v) is 0 - whatever v is - where they are below t = p 2^32 (rounded) and
  * v 2^32 / (2^32 - t) elsewhere.  The bits come from SplitMix64 as a row sample's do (evt_draw_mask): with key = output number `layer` (from 0) of the generator started at the seed,

@@ -19,3 +19,39 @@ def test_no_rows(evt, top, dtype):
     dx = evt.combine_rows(dy, plan, residual=out)
     assert y.shape == out.shape == dy.shape == dx.shape == (0, 5) and dw.shape == (0, top) and evt.combine_rows_grad(out, None, plan, None)[1] is None
     assert evt.route_rows_grad(scores, ids, w, dw).shape == (0, 7)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,top", [(1, 2), (5, 3), (64, 2), (201, 8), (513, 1), (4099, 2)])
+def test_columns_of_one_matrix(evt, H, top, dtype):
+    """x, residual and result side by side in the same rows: the results of tensors of their own, and nothing else is written."""
+    rows, experts, gen = 37, 7, torch.Generator().manual_seed(H)
+    n = rows * top
+    ids = torch.randint(-1, experts, (rows, top), generator=gen).cuda()
+    plan = evt.plan_rows(ids, experts)
+    w = torch.rand(rows, top, generator=gen).cuda()
+    first = torch.randn(n, 3 * H + 2, generator=gen).to(dtype).cuda()
+
+    def columns():
+        buf = first.clone()
+        return buf, buf[:, :H], buf[:, H:2 * H], buf[:, 2 * H + 1:3 * H + 1]
+
+    def check(call, *shapes):
+        """call(a, b, out) with rows that these tensors have, out one of the three places."""
+        for at in range(3):
+            buf, *cols = columns()
+            a, b = (c[:m] for c, m in zip([c for i, c in enumerate(cols) if i != at], shapes))
+            out = cols[at][:shapes[2]]
+            want = call(a.clone(), b.clone(), None)
+            expected = buf.clone()
+            expected[:shapes[2], out.storage_offset():out.storage_offset() + H] = want
+            assert call(a, b, out) is out and torch.equal(buf, expected)
+
+    check(lambda a, b, out: evt.sort_rows(a, plan, out=out), rows, rows, n)
+    check(lambda a, b, out: evt.combine_rows(a, plan, w, residual=b, p=0.3, seed=2, out=out), n, rows, rows)
+    check(lambda a, b, out: evt.drop_rows(a, 0.3, 2, residual=b, out=out), n, n, n)
+    if 1 < H <= 4096:
+        shape = (n, min(H, 3))
+        e, we = torch.randint(0, H, shape, generator=gen).cuda(), torch.rand(shape, generator=gen).cuda()
+        for renormalize in (True, False):
+            check(lambda a, b, out: evt.route_rows_grad(a, e, we, we, renormalize=renormalize, out=out), n, n, n)

@@ -35,17 +35,22 @@ struct Extent { // rows in memory, in elements
     const void *p;
     int64_t stride, rows;
 };
-// Two matrices' rows of `width` values have no byte in common: one lies behind the other, or both are columns of one matrix, whose rows are equally far apart.  Rows at
-// two strides that reach into each other's range count as lying on each other.
-static bool apart(Extent a, Extent b, int64_t width, int size) {
-    if (!a.p || !b.p || !a.rows || !b.rows) return true;
-    const uintptr_t a0 = (uintptr_t)a.p, b0 = (uintptr_t)b.p;
-    const uintptr_t a1 = a0 + ((a.rows - 1) * a.stride + width) * size, b1 = b0 + ((b.rows - 1) * b.stride + width) * size;
-    if (a1 <= b0 || b1 <= a0) return true;
+struct Bytes {
+    uintptr_t at;
+    uint64_t stride, rows, width;
+    uintptr_t end() const { return at + (rows - 1) * stride + width; }
+};
+// No byte in common: one lies behind the other, or they are columns of one matrix, whose rows are equally far apart.  Rows at two strides that reach into each other's range
+// count as lying on each other.
+static bool apart(Bytes a, Bytes b) {
+    if (!a.at || !b.at || !a.rows || !b.rows || a.end() <= b.at || b.end() <= a.at) return true;
     if ((a.rows > 1 && b.rows > 1 && a.stride != b.stride) || (a.rows == 1 && b.rows == 1)) return false;
-    const uint64_t stride = (uint64_t)(a.rows > 1 ? a : b).stride * size, bytes = (uint64_t)width * size;
-    if (stride < 2 * bytes) return false;
-    const uint64_t gap = (a0 < b0 ? b0 - a0 : a0 - b0) % stride; // from a row of the one to the next of the other
-    return gap >= bytes && stride - gap >= bytes;
+    const uint64_t stride = (a.rows > 1 ? a : b).stride;
+    if (stride < a.width + b.width) return false;
+    const uint64_t gap = a.at < b.at ? (b.at - a.at) % stride : (stride - (a.at - b.at) % stride) % stride; // from a row of a's to the next of b's
+    return gap >= a.width && gap + b.width <= stride;
 }
+static Bytes bytes_of(Extent e, int64_t width, int size) { return {(uintptr_t)e.p, (uint64_t)e.stride * size, (uint64_t)e.rows, (uint64_t)width * size}; }
+static Bytes bytes_of(const void *p, int64_t bytes) { return {(uintptr_t)p, 0, bytes > 0, (uint64_t)bytes}; }
+static bool apart(Extent a, Extent b, int64_t width, int size) { return apart(bytes_of(a, width, size), bytes_of(b, width, size)); }
 static bool same(Extent a, Extent b) { return a.p == b.p && (a.rows <= 1 || a.stride == b.stride); }

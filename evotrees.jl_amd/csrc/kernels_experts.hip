@@ -622,6 +622,11 @@ extern "C" int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype
     a.n = nrows * top;
     ARGCHK(a.n == 0 || (experts && place && source && work), "experts, place, source and work must not be NULL");
     TRY(check_device(flags, experts, place, source, offsets, work));
+    const int64_t n = a.n * 4;
+    const Bytes all[] = {bytes_of(place, n), bytes_of(source, n), bytes_of(offsets, (nexperts + 1) * (int64_t)4), bytes_of(work, a.n ? EVT_PLAN_WORK(a.n, nexperts) * 4 : 0),
+                         bytes_of(experts, id_dtype == EVT_I64 ? 2 * n : n)};
+    for (int i = 0; i < 4; i++)
+        for (int j = i + 1; j < 5; j++) ARGCHK(apart(all[i], all[j]), "place, source, offsets, work and experts must lie apart from each other");
     a.ids = experts;
     a.id64 = id_dtype == EVT_I64;
     a.E = nexperts;
@@ -676,6 +681,18 @@ static int take_places(int64_t nrows, int32_t top, int32_t nexperts, const int32
     return EVT_OK;
 }
 
+// What a call writes lies apart from the tables that it reads: a row may be written before another thread has read its places
+static bool clear_of_tables(Bytes out, const evt_rows *r, const RowArgs &a, const int32_t *offsets, int32_t nexperts, const float *weights) {
+    const int64_t n = (int64_t)a.n * 4;
+    return apart(out, bytes_of(a.place, n)) && apart(out, bytes_of(weights, n)) && apart(out, bytes_of(offsets, (nexperts + 1) * (int64_t)4)) &&
+           apart(out, bytes_of(a.drop ? r->seed_dev : nullptr, 8));
+}
+static int check_tables(const evt_rows *r, int64_t no, const RowArgs &a, const int32_t *offsets, int32_t nexperts, const float *weights) {
+    ARGCHK(clear_of_tables(bytes_of({r->out, r->out_stride, no}, a.H, size_of(r->dtype)), r, a, offsets, nexperts, weights),
+           "out must lie apart from place, offsets, weights and the seed");
+    return EVT_OK;
+}
+
 extern "C" int evt_sort_rows(void *stream, const void *rows, const int32_t *place, const int32_t *offsets, int32_t top, int32_t nexperts, int32_t flags) {
     return guarded([&]() -> int {
     const evt_rows *const r = static_cast<const evt_rows *>(rows);
@@ -688,6 +705,7 @@ extern "C" int evt_sort_rows(void *stream, const void *rows, const int32_t *plac
     ARGCHK(top > 1 || r->x != r->out, "sorted rows must lie apart from the rows");
     ARGCHK(offsets, "offsets must not be NULL");
     TRY(check_device(flags, place, offsets));
+    TRY(check_tables(r, a.n, a, offsets, nexperts, nullptr));
     a.count = offsets + nexperts;
     return launch_rows<ROWS_SPREAD>((hipStream_t)stream, a, r->dtype);
     });
@@ -703,6 +721,7 @@ extern "C" int evt_combine_rows(void *stream, const void *rows, const int32_t *p
     if (a.N == 0) return EVT_OK;
     ARGCHK(top > 1 || r->x != r->out, "combined rows must lie apart from the experts' rows");
     TRY(check_device(flags, place, weights));
+    TRY(check_tables(r, a.N, a, nullptr, 0, weights));
     a.w = weights;
     return launch_rows<ROWS_COMBINE>((hipStream_t)stream, a, r->dtype);
     });
@@ -724,6 +743,12 @@ extern "C" int evt_combine_rows_grad(void *stream, const void *rows, const void 
     ARGCHK(apart({y, y_stride, a.n}, {r->out, r->out_stride, a.n}, a.H, size_of(r->dtype)), "the experts' gradients must lie apart from y");
     ARGCHK(offsets, "offsets must not be NULL");
     TRY(check_device(flags, y, place, offsets, weights, dweights));
+    TRY(check_tables(r, a.n, a, offsets, nexperts, weights));
+    const Bytes slopes = bytes_of(dweights, (int64_t)a.n * 4);
+    const int size = size_of(r->dtype);
+    ARGCHK(clear_of_tables(slopes, r, a, offsets, nexperts, weights) && apart(slopes, bytes_of({r->x, r->x_stride, a.N}, a.H, size)) &&
+               apart(slopes, bytes_of({y, y_stride, a.n}, a.H, size)) && apart(slopes, bytes_of({r->out, r->out_stride, a.n}, a.H, size)),
+           "dweights must lie apart from the rows and the tables");
     a.count = offsets + nexperts;
     a.y = y;
     a.ys = y_stride;
@@ -741,6 +766,7 @@ extern "C" int evt_drop_rows(void *stream, const void *rows, int32_t flags) {
     RowArgs a = {};
     TRY(take_rows(r, r->nrows, r->nrows, flags, a));
     if (a.N == 0) return EVT_OK;
+    TRY(check_tables(r, a.N, a, nullptr, 0, nullptr));
     return launch_rows<ROWS_DROP>((hipStream_t)stream, a, r->dtype);
     });
 }

@@ -66,3 +66,48 @@ def test_columns_of_one_matrix(evt):
     # half-precision columns
     assert apart(says("evt_drop_rows", rows(evt, x=base, x_stride=16, out=base + 16, out_stride=16, dtype=10)))
     assert not apart(says("evt_drop_rows", rows(evt, x=base, x_stride=16, out=base + 14, out_stride=16, dtype=10)))
+
+
+def test_results_on_tables(evt):
+    """A result that lies on what the call reads beside its rows would be written before another thread has read that."""
+    x, out, place, w, offsets, seed, dw, y = (AT + 512 * i for i in range(8))  # 4 rows of 8 values, 2 experts each of 3; sorted rows are 256 bytes
+    given = dict(x=x, out=out)
+
+    def refused(name, *args):
+        rc, error = call(evt, name, *args, TRUSTED)
+        return rc == evt._lib.EVT_ERR_ARG and "apart" in error, error
+
+    for at in (out, out - 28, out + 252):  # 8 entries of 4 bytes
+        for name, args in (("evt_sort_rows", (rows(evt, **given), at, offsets, 2, 3)), ("evt_combine_rows", (rows(evt, x=x, out=out, nrows=8), at, w, 1)),
+                           ("evt_combine_rows", (rows(evt, x=x, out=out, nrows=8), place, at, 1)), ("evt_combine_rows_grad", (rows(evt, **given), y, 8, at, offsets, w, dw, 2, 3)),
+                           ("evt_combine_rows_grad", (rows(evt, **given), y, 8, place, offsets, at, dw, 2, 3)), ("evt_combine_rows_grad", (rows(evt, **given), y, 8, place, offsets, w, at, 2, 3)),
+                           ("evt_route_rows", (scores(evt, x=out, nrows=8), 1, 1, at, w)), ("evt_route_rows", (scores(evt, x=out, nrows=8), 1, 1, place, at)),
+                           ("evt_route_rows_grad", (scores(evt, x=x, grad=out, nrows=8), 1, 1, at, 4, w, dw)), ("evt_route_rows_grad", (scores(evt, x=x, grad=out, nrows=8), 1, 1, place, 4, at, dw)),
+                           ("evt_route_rows_grad", (scores(evt, x=x, grad=out, nrows=8), 1, 0, place, 4, w, at))):
+            no, error = refused(name, *args)
+            assert no, (name, at - out, error)
+    no, error = refused("evt_route_rows_grad", scores(evt, x=x, grad=out, nrows=8), 1, 1, out - 60, 5, w, dw)  # ids of 8 bytes
+    assert no, error
+    for at in (out - 12, out + 252):
+        no, error = refused("evt_sort_rows", rows(evt, **given), place, at, 2, 3)
+        assert no, error
+    for at in (out, out + 120):
+        for name, args in (("evt_drop_rows", (rows(evt, x=x, out=out, p=0.5, seed_dev=at),)), ("evt_combine_rows", (rows(evt, x=x, out=out, p=0.5, seed_dev=at), place, w, 2)),
+                           ("evt_combine_rows_grad", (rows(evt, x=x, out=out, p=0.5, seed_dev=at), None, 0, place, offsets, w, None, 2, 3))):
+            no, error = refused(name, *args)
+            assert no, (name, error)
+    for at in (x, x + 124, y, y + 252, place, place + 28, w - 28, offsets + 12, offsets - 28, seed + 4):
+        no, error = refused("evt_combine_rows_grad", rows(evt, x=x, out=out, p=0.5, seed_dev=seed), y, 8, place, offsets, w, at, 2, 3)
+        assert no and "dweights" in error, (at, error)
+    no, error = refused("evt_route_rows", scores(evt, x=x), 2, 1, w + 28, w)
+    assert no, error
+    work = 4 * 2 * 3  # one block's counts and the totals
+    tables = dict(ids=x, place=out, source=place, offsets=w, work=seed)
+    for first, size in (("place", 32), ("source", 32), ("offsets", 16), ("work", work)):
+        for second in tables:
+            if first != second:
+                for kind in (4, 5):
+                    t = dict(tables)
+                    t[second] = t[first] + size - 4
+                    no, error = refused("evt_plan_rows", t["ids"], kind, 4, 2, 3, t["place"], t["source"], t["offsets"], t["work"])
+                    assert no, (first, second, error)

@@ -55,3 +55,40 @@ def test_columns_of_one_matrix(evt, H, top, dtype):
         e, we = torch.randint(0, H, shape, generator=gen).cuda(), torch.rand(shape, generator=gen).cuda()
         for renormalize in (True, False):
             check(lambda a, b, out: evt.route_rows_grad(a, e, we, we, renormalize=renormalize, out=out), n, n, n)
+
+
+def test_results_on_tables(evt):
+    """Refused where they lie on what the call reads, taken where they only touch it."""
+    rows, top, H, experts = 40, 8, 8, 11
+    n = rows * top
+    gen = torch.Generator().manual_seed(1)
+    memory = torch.zeros(3 * n * H + 64, device="cuda")
+    at = [0]
+
+    def place(*shape):
+        """A tensor that starts where the last one ended."""
+        size = torch.Size(shape).numel()
+        at[0] += size
+        return memory[at[0] - size:at[0]].view(shape)
+
+    w, out, x, y, seed = place(rows, top), place(rows, H), place(rows, H), place(n, H), memory[-2:].view(torch.int64)
+    for t in (w, x, y):
+        t.copy_(torch.randn(t.shape, generator=gen))
+    seed.fill_(77)
+    ids = torch.randint(-1, experts, (rows, top), generator=gen).cuda()
+    plan = evt.plan_rows(ids, experts)
+    assert evt.combine_rows(y, plan, w, residual=x, p=0.3, seed=seed, out=out) is out
+    assert torch.equal(out, evt.combine_rows(y.clone(), plan, w.clone(), residual=x.clone(), p=0.3, seed=77))
+    assert torch.equal(evt.drop_rows(x, 0.3, seed, out=out), evt.drop_rows(x, 0.3, 77))
+    scores = torch.randn(rows, H, generator=gen).cuda()
+    e, v = evt.route_rows(scores, top)
+    tables = plan._tables[:2 * n].view(torch.float32)
+    for call in (lambda: evt.combine_rows(y, plan, w, out=w), lambda: evt.combine_rows(y, plan, w, out=memory[n - 1:n - 1 + rows * H].view(rows, H)),
+                 lambda: evt.combine_rows(y, plan, w, p=0.5, seed=seed, out=memory[-1 - rows * H:-1].view(rows, H)),
+                 lambda: evt.drop_rows(x[:1], 0.5, seed, out=memory[-H - 1:-1].view(1, H)), lambda: evt.combine_rows(y, plan, w, out=tables[:rows * H].view(rows, H)),
+                 lambda: evt.route_rows_grad(scores, e, v, v.clone(), out=v), lambda: evt.route_rows_grad(scores, e, v.clone(), v, renormalize=False, out=v),
+                 lambda: evt.route_rows_grad(scores, e, v, v, out=e.view(torch.float32))):
+        before = memory.clone()
+        with pytest.raises(evt.EvtError, match="apart"):
+            call()
+        assert torch.equal(memory, before)

@@ -20,6 +20,17 @@ static int check_device(int32_t flags, P... ptrs) {
     for (const void *p : all) ARGCHK(!p || on_device(p), "rows through experts take device memory only");
     return EVT_OK;
 }
+// Tables and weights lie at multiples of their type's size: a scalar load takes no other address, and reads what lies in front instead
+template <typename... P>
+static int check_aligned(P... ptrs) {
+    const void *all[] = {(const void *)ptrs...};
+    for (const void *p : all) ARGCHK((uintptr_t)p % 4 == 0, "tables and weights must be aligned to their type");
+    return EVT_OK;
+}
+static int check_ids(const void *ids, int32_t id_dtype) {
+    ARGCHK((uintptr_t)ids % (id_dtype == EVT_I64 ? 8 : 4) == 0, "experts must be aligned to their type");
+    return EVT_OK;
+}
 #define TRY(call)                        \
     do {                                 \
         const int _r = (call);           \

@@ -621,6 +621,8 @@ extern "C" int evt_plan_rows(void *stream, const void *experts, int32_t id_dtype
     PlanArgs a = {};
     a.n = nrows * top;
     ARGCHK(a.n == 0 || (experts && place && source && work), "experts, place, source and work must not be NULL");
+    TRY(check_ids(experts, id_dtype));
+    TRY(check_aligned(place, source, offsets, work));
     TRY(check_device(flags, experts, place, source, offsets, work));
     const int64_t n = a.n * 4;
     const Bytes all[] = {bytes_of(place, n), bytes_of(source, n), bytes_of(offsets, (nexperts + 1) * (int64_t)4), bytes_of(work, a.n ? EVT_PLAN_WORK(a.n, nexperts) * 4 : 0),
@@ -704,6 +706,7 @@ extern "C" int evt_sort_rows(void *stream, const void *rows, const int32_t *plac
     if (a.N == 0) return EVT_OK;
     ARGCHK(top > 1 || r->x != r->out, "sorted rows must lie apart from the rows");
     ARGCHK(offsets, "offsets must not be NULL");
+    TRY(check_aligned(place, offsets));
     TRY(check_device(flags, place, offsets));
     TRY(check_tables(r, a.n, a, offsets, nexperts, nullptr));
     a.count = offsets + nexperts;
@@ -720,6 +723,7 @@ extern "C" int evt_combine_rows(void *stream, const void *rows, const int32_t *p
     TRY(take_rows(r, a.n, r->nrows, flags, a));
     if (a.N == 0) return EVT_OK;
     ARGCHK(top > 1 || r->x != r->out, "combined rows must lie apart from the experts' rows");
+    TRY(check_aligned(place, weights));
     TRY(check_device(flags, place, weights));
     TRY(check_tables(r, a.N, a, nullptr, 0, weights));
     a.w = weights;
@@ -742,6 +746,7 @@ extern "C" int evt_combine_rows_grad(void *stream, const void *rows, const void 
     ARGCHK(top > 1 || r->x != r->out, "the experts' gradients must lie apart from the rows'");
     ARGCHK(apart({y, y_stride, a.n}, {r->out, r->out_stride, a.n}, a.H, size_of(r->dtype)), "the experts' gradients must lie apart from y");
     ARGCHK(offsets, "offsets must not be NULL");
+    TRY(check_aligned(place, offsets, weights, dweights));
     TRY(check_device(flags, y, place, offsets, weights, dweights));
     TRY(check_tables(r, a.n, a, offsets, nexperts, weights));
     const Bytes slopes = bytes_of(dweights, (int64_t)a.n * 4);

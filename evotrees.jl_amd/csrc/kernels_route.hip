@@ -599,6 +599,7 @@ extern "C" int evt_route_rows(void *stream, const void *scores, int32_t top, int
     TRY(take_route(s, top, renormalize, flags, a));
     if (a.N == 0) return EVT_OK;
     ARGCHK(experts && weights, "experts and weights must not be NULL");
+    TRY(check_aligned(experts, weights));
     TRY(check_device(flags, s->x, experts, weights));
     const Bytes x = bytes_of({s->x, s->row_stride, a.N}, a.V, size_of(s->dtype)), ids = bytes_of(experts, a.N * top * 4), w = bytes_of(weights, a.N * top * 4);
     ARGCHK(apart(ids, x) && apart(w, x) && apart(ids, w), "experts and weights must lie apart from the scores and from each other");
@@ -622,6 +623,8 @@ extern "C" int evt_route_rows_grad(void *stream, const void *scores, int32_t top
     ARGCHK(a.N == 1 || s->grad_stride >= s->nclass, "grad_stride must be at least nclass");
     const Extent x = {s->x, s->row_stride, a.N}, g = {s->grad, s->grad_stride, a.N};
     ARGCHK(same(x, g) || apart(x, g, a.V, size), "grad must be the scores' own memory, row for row, or lie apart from them");
+    TRY(check_ids(experts, id_dtype));
+    TRY(check_aligned(weights, dweights));
     TRY(check_device(flags, s->x, s->grad, experts, weights, dweights));
     const Bytes grad = bytes_of(g, a.V, size);
     const int64_t n = a.N * top * 4;

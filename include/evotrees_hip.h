@@ -464,7 +464,7 @@ int evt_preference_loss(void *stream, const void *scores /* evt_scores */, const
  * No counterpart in the reference: what a model of several experts does with its rows - a language model's tokens between two layers, or a table's rows at the
  * leaves of a tree (evt_predict_leaf_idx) - around the experts' own products.  Stateless and device-only, in the manner of the losses above: device pointers of the
  * current device, the caller's stream, nothing allocated, copied, waited for or kept; calls may overlap and be captured.  Results do not depend on the
- * grid or the order of blocks: equal calls give equal bits.  What a call writes lies apart from all else that it is given, but where it may be a call's rows themselves.
+ * grid or the order of blocks: equal calls give equal bits.  Tables, ids and weights are aligned to their type.  What a call writes lies apart from all else that it is given, but where it may be a call's rows themselves.
  *
  * The choice of experts: the `top` best scores of each of nrows rows of nclass experts' scores (1 .. 4096; top 1 .. 64, at most nclass), the best first; of equal
  * scores the lower expert's comes first.  With z = x / temperature and e_j the chosen

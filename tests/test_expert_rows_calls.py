@@ -86,7 +86,7 @@ def test_results_on_tables(evt):
                            ("evt_route_rows_grad", (scores(evt, x=x, grad=out, nrows=8), 1, 0, place, 4, w, at))):
             no, error = refused(name, *args)
             assert no, (name, at - out, error)
-    no, error = refused("evt_route_rows_grad", scores(evt, x=x, grad=out, nrows=8), 1, 1, out - 60, 5, w, dw)  # ids of 8 bytes
+    no, error = refused("evt_route_rows_grad", scores(evt, x=x, grad=out, nrows=8), 1, 1, out - 56, 5, w, dw)  # ids of 8 bytes
     assert no, error
     for at in (out - 12, out + 252):
         no, error = refused("evt_sort_rows", rows(evt, **given), place, at, 2, 3)
@@ -108,6 +108,28 @@ def test_results_on_tables(evt):
             if first != second:
                 for kind in (4, 5):
                     t = dict(tables)
-                    t[second] = t[first] + size - 4
+                    t[second] = t[first] + size - (8 if second == "ids" and kind == 5 else 4)
                     no, error = refused("evt_plan_rows", t["ids"], kind, 4, 2, 3, t["place"], t["source"], t["offsets"], t["work"])
                     assert no, (first, second, error)
+
+
+def test_tables_are_aligned(evt):
+    """A scalar load takes the four bytes below an address that is no multiple of four."""
+    x, out, place, w, offsets, source, dw, y = (AT + 512 * i for i in range(8))
+    given = rows(evt, x=x, out=out)
+    calls = {"evt_route_rows": ((scores(evt, x=x), 2, 1, place, w), (3, 4)), "evt_sort_rows": ((given, place, offsets, 2, 3), (1, 2)),
+             "evt_combine_rows": ((rows(evt, x=x, out=out, nrows=2), place, w, 2), (1, 2)), "evt_combine_rows_grad": ((given, y, 8, place, offsets, w, dw, 2, 3), (3, 4, 5, 6)),
+             "evt_plan_rows": ((x, 4, 4, 2, 3, place, source, offsets, w), (0, 5, 6, 7, 8)), "evt_route_rows_grad": ((scores(evt, x=x, grad=out), 2, 1, place, 4, w, dw), (3, 5, 6))}
+    wide = {"evt_plan_rows": 1, "evt_route_rows_grad": 4}  # where a call takes the type of its ids
+    for name, (args, at) in calls.items():
+        for k in at:
+            for off in (1, 2, 3):
+                wrong = list(args)
+                wrong[k] += off
+                rc, error = call(evt, name, *wrong, TRUSTED)
+                assert rc == evt._lib.EVT_ERR_ARG and "aligned" in error, (name, k, off, error)
+        if name in wide:
+            wrong = list(args)
+            wrong[wide[name]], wrong[at[0]] = 5, wrong[at[0]] + 4
+            rc, error = call(evt, name, *wrong, TRUSTED)
+            assert rc == evt._lib.EVT_ERR_ARG and "aligned" in error, (name, error)

@@ -111,9 +111,24 @@ class RowPlan:
     __slots__ = ("rows", "top", "experts", "device", "offsets_at", "_on", "_tables", "_at")
 
     def __init__(self, rows, top, experts, device, on, tables):
+        torch = _torch()
+        if not isinstance(tables, torch.Tensor) or tables.dtype != torch.int32:
+            raise TypeError("the tables must be one int32 tensor")
+        if tables.get_device() != device:
+            raise ValueError("the plan is on %s, its tables are on %s" % ("cuda:%d" % device if device >= 0 else on, tables.device))
+        rows, top, experts = _whole("rows", rows, 0, 0x7FFFFFFF), _whole("top", top, 1, 0x7FFFFFFF), _whole("experts", experts, 1, _MOST)
+        if tables.dim() != 1 or not tables.is_contiguous() or tables.storage_offset() or tables.shape[0] < 2 * rows * top + experts + 1:
+            raise ValueError("the tables must be a vector of its own memory, place, source and offsets one behind the other, got shape %s" % (tuple(tables.shape),))
+        self._hold(rows, top, experts, device, on, tables)
+
+    def _hold(self, rows, top, experts, device, on, tables):
         self.rows, self.top, self.experts, self.device, self._on, self._tables = rows, top, experts, device, on, tables
         self._at = tables.data_ptr()
         self.offsets_at = self._at + 8 * rows * top
+
+    def __reduce__(self):
+        """A copy has its own tables, at their own address."""
+        return _plan_again, (self.rows, self.top, self.experts, self._tables)
 
     @property
     def place(self):
@@ -127,6 +142,10 @@ class RowPlan:
     @property
     def offsets(self):
         return self._tables.as_strided((self.experts + 1,), (1,), 2 * self.rows * self.top)
+
+
+def _plan_again(rows, top, experts, tables):
+    return RowPlan(rows, top, experts, tables.get_device(), tables.device, tables)
 
 
 class _Rows:
@@ -274,7 +293,8 @@ def plan_rows(experts, n_experts):
         raise ValueError("experts must be on a GPU, got %s" % on)
     # the tables, and what the call works in behind them
     kept, block = 2 * n + n_experts + 1, 1024 if n <= 1 << 20 else 4096
-    plan = RowPlan(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + ((n + block - 1) // block + 1) * n_experts,), on))
+    plan = RowPlan.__new__(RowPlan)
+    plan._hold(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + ((n + block - 1) // block + 1) * n_experts,), on))
     _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, plan._at + 4 * kept)
     return plan
 

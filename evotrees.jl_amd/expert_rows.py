@@ -291,11 +291,19 @@ def plan_rows(experts, n_experts):
     at = _check("experts", experts, experts.shape, _scores._INTS, device, on)
     if device < 0:
         raise ValueError("experts must be on a GPU, got %s" % on)
-    # the tables, and what the call works in behind them
+    # The tables, and what the call works in behind them: a second tensor costs a call 1.5 us.  A large one would stay as long as the plan, which a layer's backward pass still needs, and
+    # goes when the work is queued.
     kept, block = 2 * n + n_experts + 1, 1024 if n <= 1 << 20 else 4096
+    more = ((n + block - 1) // block + 1) * n_experts
     plan = RowPlan.__new__(RowPlan)
-    plan._hold(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + ((n + block - 1) // block + 1) * n_experts,), on))
-    _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, plan._at + 4 * kept)
+    if more <= 16384 or more <= kept >> 3:
+        plan._hold(rows, top, n_experts, device, on, _make(device, torch.int32, (kept + more,), on))
+        work_at = plan._at + 4 * kept
+    else:
+        plan._hold(rows, top, n_experts, device, on, _make(device, torch.int32, (kept,), on))
+        work = _make(device, torch.int32, (more,), on)
+        work_at = work.data_ptr()
+    _queue("evt_plan_rows", device, on, at, _scores._INTS[experts.dtype], rows, top, n_experts, plan._at, plan._at + 4 * n, plan.offsets_at, work_at)
     return plan
 
 

@@ -92,3 +92,32 @@ def test_results_on_tables(evt):
         with pytest.raises(evt.EvtError, match="apart"):
             call()
         assert torch.equal(memory, before)
+
+
+def test_memory_of_a_plan(evt):
+    """Tables of many experts, eagerly and in a graph: what the call works in goes to the next one, and the plan keeps its tables alone."""
+    rows, top, experts, H = 20000, 2, 4096, 33
+    gen = torch.Generator().manual_seed(3)
+    ids, x = torch.randint(-1, experts, (rows, top), generator=gen).cuda(), torch.randn(rows, H, generator=gen).cuda()
+    other = torch.randint(0, experts, (rows, top), generator=gen).cuda()
+    evt.plan_rows(ids, experts)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    plan = evt.plan_rows(ids, experts)
+    tables = 4 * (2 * rows * top + experts + 1)
+    assert torch.cuda.memory_allocated() - before <= tables + 65536
+    wanted = [[t.clone() for t in (p.place, p.source, p.offsets, evt.sort_rows(x, p))] for p in (evt.plan_rows(ids, experts), evt.plan_rows(other, experts))]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        plans = [evt.plan_rows(i, experts) for i in (ids, other)]
+        outs = [[p.place, p.source, p.offsets, evt.sort_rows(x, p)] for p in plans]
+    for _ in range(4):
+        for out in outs:
+            for t in out:
+                t.zero_()
+        g.replay()
+        eager = [evt.plan_rows(i, experts) for i in (other, ids)]
+        for out, want in zip(outs, wanted):
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert torch.equal(eager[0].source, wanted[1][1]) and torch.equal(eager[1].source, wanted[0][1])
+    assert torch.equal(plan.place, wanted[0][0]) and torch.equal(plan.source, wanted[0][1])

@@ -1,7 +1,11 @@
 """A plan's tables: what a copy of a plan has, and tables that are none.  No GPU needed."""
 import copy
+import ctypes as C
 import io
+import os
 import pickle
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -46,3 +50,49 @@ def test_tables_that_are_none(evt):
             evt.RowPlan(*sizes, -1, cpu, whole)
     with pytest.raises(TypeError):
         evt.RowPlan(4.0, 2, 5, -1, cpu, whole)
+
+
+def _work_of(tmp_path):
+    """EVT_PLAN_WORK as a C compiler has it."""
+    source, built = tmp_path / "work.c", tmp_path / "work.so"
+    source.write_text('#include "evotrees_hip.h"\nint64_t work(int64_t n, int32_t experts) { return EVT_PLAN_WORK(n, experts); }\n')
+    subprocess.run(["gcc", "-shared", "-fPIC", "-I", os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include"), "-o", str(built), str(source)], check=True)
+    f = C.CDLL(str(built)).work
+    f.argtypes, f.restype = [C.c_int64, C.c_int32], C.c_int64
+    return f
+
+
+def test_memory_of_a_plan(evt, monkeypatch, tmp_path):
+    """What plan_rows allocates is the tables and EVT_PLAN_WORK behind them or by itself, and a plan keeps little more than its tables."""
+    rows_module = sys.modules[evt.RowPlan.__module__]
+    work_of, queued, made = _work_of(tmp_path), [], []
+
+    class Memory(torch.Tensor):
+        """On a GPU, as far as its checks see."""
+        def get_device(self):
+            return 0
+
+    def make(device, dtype, shape, on):
+        assert device == 0 and dtype == torch.int32
+        made.append(torch.empty(shape, dtype=dtype))
+        return made[-1]
+
+    monkeypatch.setattr(rows_module, "_make", make)
+    monkeypatch.setattr(rows_module, "_queue", lambda name, device, on, *args: queued.append((name, args)))
+    for rows, top in ((0, 3), (1, 1), (16, 6), (1024, 1), (1025, 1), (341, 3), (4096, 8), (32768, 8), (131072, 8), (131072 * 8, 1), (131072 * 8 + 1, 1), (262144, 8)):
+        for experts in (1, 7, 64, 128, 1000, 4096):
+            del queued[:], made[:]
+            n = rows * top
+            plan = evt.plan_rows(torch.zeros(rows, top, dtype=torch.int32).as_subclass(Memory), experts)
+            (name, args), = queued
+            at, _, r, k, e, place, source, offsets, work = args
+            assert name == "evt_plan_rows" and (r, k, e) == (rows, top, experts)
+            first, size = made[0].data_ptr(), 4 * made[0].numel()
+            assert (place, source, offsets) == (first, first + 4 * n, first + 8 * n)
+            needed = 4 * work_of(n, experts)
+            if len(made) == 1:
+                assert work == offsets + 4 * (experts + 1) and work + needed == first + size
+            else:
+                assert len(made) == 2 and size == 8 * n + 4 * (experts + 1) and work == made[1].data_ptr() and needed == 4 * made[1].numel()
+            kept = plan._tables.numel() * 4
+            assert kept <= max(8 * n + 4 * (experts + 1) + 65536, (8 * n + 4 * (experts + 1)) * 9 // 8), (rows, top, experts, kept)

@@ -1,4 +1,6 @@
 """Rows through experts in calls that lie at the edge of what is allowed: empty batches, memory that is shared, more rows than a launch has, threads."""
+import threading
+
 import pytest
 import torch
 
@@ -121,3 +123,80 @@ def test_memory_of_a_plan(evt):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
         assert torch.equal(eager[0].source, wanted[1][1]) and torch.equal(eager[1].source, wanted[0][1])
     assert torch.equal(plan.place, wanted[0][0]) and torch.equal(plan.source, wanted[0][1])
+
+
+@pytest.mark.parametrize("H,top", [(3, 1), (9, 2)])
+def test_more_rows_than_a_launch_has(evt, H, top):
+    """Places and weights by the absolute row, what no entry has cleared once: rows on both sides of the 2^24th, where the second launch begins, with and without experts."""
+    rows, experts = 17_000_000, 5
+    gen = torch.Generator(device="cuda").manual_seed(H)
+    ids = torch.randint(0, experts, (rows, top), generator=gen, device="cuda")
+    ids[(1 << 24) - 700:(1 << 24) + 300] = -1
+    ids[rows - 1000:] = -1
+    plan = evt.plan_rows(ids, experts)
+    place, n = plan.place.long(), rows * top
+    valid, count = place >= 0, int(plan.offsets[-1])
+    assert count == n - 2000 * top and torch.equal(valid, ids >= 0)
+    x = torch.randn(rows, H, generator=gen, device="cuda").half()
+    out = torch.full((n, H), 7.0, dtype=torch.float16, device="cuda")
+    evt.sort_rows(x, plan, out=out)
+    source = plan.source.long()
+    assert torch.equal(out[:count], x[source[:count] // top]) and bool((out[count:] == 0).all())
+    y = torch.randn(n, H, generator=gen, device="cuda").half()
+    w = torch.rand(rows, top, generator=gen, device="cuda")
+    sums, sizes = torch.zeros(rows, H, dtype=torch.float64, device="cuda"), torch.zeros(rows, H, dtype=torch.float64, device="cuda")
+    for j in range(top):
+        part = torch.where(valid[:, j, None], w[:, j, None].double() * y[place[:, j].clamp(min=0)].double(), 0.0)
+        sums += part
+        sizes += part.abs()
+    got = evt.combine_rows(y, plan, w).double()
+    # two 32-bit steps an entry, and the result's half step, the smallest numbers' included
+    assert bool(((got - sums).abs() <= sums.abs() * 2.0 ** -11 + 2.0 ** -25 + 2 * top * 1.01 * 2.0 ** -24 * sizes).all())
+    del sums, sizes, got
+    dy, dw = evt.combine_rows_grad(x, y, plan, w)
+    assert bool((dy[count:] == 0).all()) and bool((dw[~valid] == 0).all())
+    for j in range(top):
+        at = place[:, j].clamp(min=0)
+        assert torch.equal(dy[at][valid[:, j]], (w[:, j, None] * x.float()).half()[valid[:, j]])  # one product, one rounding
+        terms = x.double() * y[at].double()
+        assert bool(((dw[:, j].double() - terms.sum(1)).abs() <= 1.01 * 2.0 ** -24 * (H + 6) * terms.abs().sum(1))[valid[:, j]].all())
+
+
+def test_threads(evt):
+    """Four threads on their own streams, twenty turns each, all of which have to come to an end."""
+    gen = torch.Generator().manual_seed(8)
+    given = []
+    for rows, experts, top, H, dtype in ((9000, 64, 4, 130, torch.bfloat16), (100, 8, 2, 4096, torch.float32), (1500, 1000, 8, 65, torch.float16), (3000, 4096, 1, 512, torch.float32)):
+        given.append((torch.randn(rows, experts, generator=gen).cuda(), torch.randn(rows, H, generator=gen).to(dtype).cuda(), top, experts))
+
+    def step(scores, x, top, experts):
+        ids, w = evt.route_rows(scores, top)
+        plan = evt.plan_rows(ids, experts)
+        y = evt.sort_rows(x, plan)
+        out = evt.combine_rows(y, plan, w, residual=x, p=0.2, seed=4)
+        dy, dw = evt.combine_rows_grad(out, y, plan, w, p=0.2, seed=4)
+        return ids, w, plan.place, plan.source, y, out, dy, dw, evt.route_rows_grad(scores, ids, w, dw)
+
+    wanted = [[t.clone() for t in step(*g)] for g in given]
+    torch.cuda.synchronize()
+    turns, wrong = [0] * len(given), []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got = step(*given[k])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, wanted[k])):
+                        wrong.append("another result in thread %d" % k)
+                    turns[k] += 1
+        except BaseException as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(len(given))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong and turns == [20] * len(given), (wrong, turns)

@@ -4,6 +4,8 @@ import threading
 import pytest
 import torch
 
+import expert_rows_plain as plain
+
 pytestmark = pytest.mark.gpu
 
 
@@ -200,3 +202,78 @@ def test_threads(evt):
     for t in threads:
         t.join()
     assert not wrong and turns == [20] * len(given), (wrong, turns)
+
+
+def test_in_autograd_functions(evt):
+    """The gradients that the calls return, as a program records them: those of a composition of plain operations in 64 bits, at every leaf."""
+    rows, experts, top, H, p, seed = 23, 6, 2, 17, 0.25, 12
+
+    class Route(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, scores):
+            ids, w = evt.route_rows(scores, top)
+            ctx.save_for_backward(scores, ids, w)
+            ctx.mark_non_differentiable(ids)
+            return ids, w
+
+        @staticmethod
+        def backward(ctx, _, dw):
+            scores, ids, w = ctx.saved_tensors
+            return evt.route_rows_grad(scores, ids, w, dw.contiguous())
+
+    class Sort(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x, plan):
+            ctx.plan = plan
+            return evt.sort_rows(x, plan)
+
+        @staticmethod
+        def backward(ctx, dy):
+            return evt.combine_rows(dy.contiguous(), ctx.plan), None
+
+    class Combine(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, y, w, x, plan):
+            ctx.plan = plan
+            ctx.save_for_backward(y, w)
+            return evt.combine_rows(y, plan, w, residual=x, p=p, seed=seed)
+
+        @staticmethod
+        def backward(ctx, dout):
+            y, w = ctx.saved_tensors
+            return (*evt.combine_rows_grad(dout.contiguous(), y, ctx.plan, w, p=p, seed=seed), dout, None)
+
+    gen = torch.Generator().manual_seed(5)
+    leaves = [torch.randn(s, generator=gen) for s in ((rows, experts), (rows, H), (experts, H))]
+    dout = torch.randn(rows, H, generator=gen)
+    scores, x, scale = (t.cuda().requires_grad_() for t in leaves)
+    assert not any(t.requires_grad for t in (*evt.route_rows(scores, top), evt.drop_rows(x, p, seed)))
+    ids, w = Route.apply(scores)
+    plan = evt.plan_rows(ids, experts)
+    expert = ids.reshape(-1)[plan.source.long()].long()
+    out = Combine.apply(Sort.apply(x, plan) * scale[expert], w, x, plan)
+    got = torch.autograd.grad(out, (scores, x, scale), dout.cuda())
+
+    s64, x64, k64 = (t.double().requires_grad_() for t in leaves)
+    chosen = ids.cpu().long()
+    w64 = torch.softmax(s64.gather(1, chosen), 1)
+    total = sum(w64[:, j, None] * k64[chosen[:, j]] * x64 for j in range(top))
+    gone = plain.bits(rows, H, seed, 0) < plain.threshold(p)
+    want_out = x64 + torch.where(gone, 0.0, total * (2.0 ** 32 / (2 ** 32 - plain.threshold(p))))
+    want = torch.autograd.grad(want_out, (s64, x64, k64), dout.double())
+    # two hundred 32-bit roundings of sums whose terms' sizes add up to less than 40: 46 of dout w x / (1 - p) at most, or a row's 17 of dout scale x / (1 - p)
+    for name, a, b in (("out", out, want_out.detach()), ("scores", got[0], want[0]), ("x", got[1], want[1]), ("scale", got[2], want[2])):
+        plain.close(name, a, b, torch.full_like(b, 200 * plain.U * 40))
+
+
+def test_leaves_of_a_tree(evt):
+    """A column of predict_leaf_idx, as the module's documentation takes it to the GPU."""
+    gen = torch.Generator().manual_seed(6)
+    X = torch.randn(500, 3, generator=gen, dtype=torch.float64).numpy()
+    m = evt.fit(evt.EvoTreeRegressor(nrounds=2, max_depth=3, nbins=16), x_train=X, y_train=X[:, 0] + X[:, 1])
+    leaf = evt.predict_leaf_idx(m, X)
+    k = leaf.shape[1] - 1
+    ids = torch.from_numpy(leaf[:, k].astype("int64")).cuda()
+    plan = evt.plan_rows(ids, int(leaf[:, k].max()) + 1)
+    place, source, offsets = plain.plan(ids.cpu()[:, None], plan.experts)
+    assert plan.place.reshape(-1).tolist() == place and plan.source.tolist() == source and plan.offsets.tolist() == offsets and offsets[-1] == 500

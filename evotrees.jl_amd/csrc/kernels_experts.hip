@@ -2,7 +2,7 @@
 // include/evotrees_hip.h).
 //
 // All of it moves bytes, in pieces of sixteen: of what is read or written in order memory is the bound, of scattered rows a little less of it (262 144 rows of 4096 bf16
-// sorted: of one expert 6.06 TB/s, of 8 5.59, of 64 5.24, of 512 5.20).  Products and sums are 32-bit, and a value is rounded once, when it is written.
+// sorted: of one expert 6.16 TB/s, of 8 5.67, of 64 5.33, of 512 5.30).  Products and sums are 32-bit, and a value is rounded once, when it is written.
 #include "experts.h"
 
 // ---- the tables of rows by expert ------------------------------------------------------------
@@ -96,7 +96,8 @@ enum { PLAN_ALONE, PLAN_BLOCKS, PLAN_SUMS };
 // Every entry's place: the experts before its own, its expert's entries of the blocks before, of the wavefronts before, and of its wavefront's before it.  The last are found by
 // comparing the experts' bits over the wavefront, 64 consecutive entries at a time, without atomics: many entries of one expert would queue up at one word.
 // JOIN: a block's entries are put in order in shared memory, so that what goes to the source's places in a row goes there together: four bytes by themselves are a request each (1 000 000 x
-// 8 of 64 experts 74 us, 61 so; of 1000 152 | 113; blocks of 1024 entries have too few of an expert: 32 768 x 8 of 64 11.0 | 11.6).
+// 8 of 64 experts 67 us, 56 so; of 1000 142 | 109; of few experts it is no gain: 262 144 x 8 of 8 24.7 | 25.9).  Blocks of 1024 entries are not joined: with few of them that costs (2048 x 8 of
+// 256 11.0 us, 11.5 joined, 32 768 x 8 of 64 11.4 | 11.6), with many it would give a tenth, which is left (131 072 x 8 of 64 17.3 | 15.7, of 256 22.2 | 20.1, of 1000 38.3 | 37.2).
 template <int ITEMS, int FROM, bool JOIN>
 __global__ __launch_bounds__(256) void k_plan_place(PlanArgs a) {
     constexpr int W = 4, THREADS = 64 * W;
@@ -534,9 +535,10 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
     const uint64_t clear = OP == ROWS_SPREAD ? (uint64_t)a.n * a.pieces / 4096 + 1 : 0;
     a.tail = (uint32_t)(clear < 1024 ? clear : 1024);
     // Results of more than half of what the second caches hold (8 x 4 MB) go past them, and what they come from is read as something that nobody reads again soon (32 768 x 8 x 4096
-    // bf16 combined: 486 us, 432 so; dropout of 65 536 x 8192 with a residual 537 | 499; 4096 x 8 x 2048 33.2 | 29.2, and with the kernel that reads the result 38.5 | 38.6, of
-    // 1024 rows 12.7 | 13.1).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows of 4099 sorted: 535 us, 667
-    // so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 33.9), and gradients are no sooner done (908 | 911)
+    // bf16 combined: 486 us, 432 so; dropout of 65 536 x 8192 with a residual 537 | 499; 4096 x 8 x 2048 33.2 | 29.2).  With the kernel that reads the result behind it, combined rows with a
+    // residual gain as much (4096 x 8 x 2048, 17 MB, 42.2 us, 39.0 so; 8192 x 8 x 4096 164 | 148; 32 768 x 8 x 4096 618 | 557), dropout alone loses what its reader then fetches from memory
+    // (4096 x 2048 14.5 | 15.7, 16 384 x 4096 88 | 100, 32 768 x 8192 359 | 363).  Not what goes to scattered places: parts of lines would leave the second cache before their neighbours come (rows of 4099 sorted: 535 us, 667
+    // so), not rows that pieces do not divide (200 003 x 97 f32 combined 37.7 | 42.3, of 100 37.9 | 33.9), and gradients are no sooner done (909 | 910)
     const bool past = OP != ROWS_SPREAD && (double)a.N * a.H * sizeof(T) > 16e6 && (uintptr_t)a.out % 16 == 0 && a.os % E == 0 && a.H % E == 0;
     // Wavefronts of one row, whose places and weights are scalars, from 512 pieces on (32 768 x 8 x 4096 bf16 combined with a residual: 467 us with the rows' pieces behind each
     // other, 462 so; of 4099 sorted 531 | 507); below, lanes without a piece cost more than that gives (65 536 x 4 x 520 combined: 62.5 | 74.6, dropout with a residual 34.8 | 43.8)
@@ -554,8 +556,8 @@ static void launch_rows_typed(hipStream_t s, RowArgs &a) {
             else if (a.pieces <= 32) launch_dot_as<T, 32, false>(s, a, rows);
             else if (a.pieces <= 64) launch_dot_as<T, 64, false>(s, a, rows);
             else {
-                // blocks of up to 8 wavefronts in as many turns as it takes (32 768 rows of 8 x 4099 bf16 with dropout: 1033 us by 4, 1004 so, 1220 by 16; 16 rows of 8 x 16 384
-                // 14.5 | 10.3 | 10.4)
+                // blocks of up to 8 wavefronts in as many turns as it takes (by 4, 6, 8 and 16: 32 768 rows of 8 x 4099 bf16 with dropout 1033, 990, 1004, 1220 us, 65 536 of 4 x 1391 359, 351, 364,
+                // 363, 16 rows of 8 x 16 384 14.5, 11.9, 10.3, 10.4: few long rows decide for 8, batches of odd rows lose 1 to 4 %)
                 const int turns = (a.parts + 7) / 8;
                 launch_dot_as<T, 0, false>(s, a, rows, 64 * ((a.parts + turns - 1) / turns));
             }
@@ -578,10 +580,11 @@ static int launch_rows(hipStream_t s, RowArgs &a, int dtype) {
     return EVT_OK;
 }
 
-// One block for the smallest (16 x 6 of 64 experts: 3.0 us on the device, by a block of 1024 threads 6.2; 512 x 8: 7.8 us, by two launches 7.7).  Then a launch that
-// counts, in blocks of 1024 entries (131 072 x 2: 10.1 us, of 4096 17.8; 131 072 x 8 22 | 25), from 2^20 entries on of 4096 (262 144 x 8 of 256 experts 29.9 us, of 1024 36.9, of
-// 64 experts 26.0 | 22.6; 2 000 000 x 1 of 1023 45 | 63), and one that finds the places.  Up to 2048 counts each of its blocks adds up what is before it by itself (2048 x 8 of
-// 64: 9.0 us, 10.1 with a launch for the sums; of 4096 counts, 8192 x 8 of 64: 12.2 | 10.3).
+// One block for the smallest (16 x 6 of 64 experts: 3.0 us on the device).  Then a launch that counts, in blocks of 1024 entries up to 2^20 of them (131 072 x 2 of 64 experts: 11.3 us, of 4096
+// 21.1; 131 072 x 8 of 256 22.2 | 27.3) and of 4096 beyond (262 144 x 8 of 256 29.6 us, of 1024 32.8; of 1000 41.6 | 62.0; 2 000 000 x 1 of 1023 41.0 | 58.1), and one that finds the places.  The
+// number of experts, which this does not look at, moves that limit: 131 072 x 8 of 1000 take 38.3 us in blocks of 1024 and 33.5 in blocks of 4096, 262 144 x 8 of 64 27.0 us in blocks of
+// 4096 and 23.3 in blocks of 1024, of 8 25.9 | 18.7.  Up to 2048 counts each block that finds places adds up what is before it by itself (2048 x 8 of 64: 9.3 us, 10.3 with a launch for the
+// sums; 16 384 x 8 of 16 10.3 | 10.0; of 4096 counts, 8192 x 8 of 64: 12.5 | 10.5).
 static void launch_plan(hipStream_t s, PlanArgs &a) {
     a.bits = 0;
     while ((1 << a.bits) < a.E) a.bits++;

@@ -513,7 +513,7 @@ static void launch_route_typed(hipStream_t s, const RouteArgs &a) {
     if (V <= 2048) return launch_route_as<T, 64, 32>(s, a);
     launch_route_as<T, 64, 64>(s, a);
 }
-// Sixteen values of the gradient a lane
+// Sixteen values of the gradient a lane, of more than 1024 classes 32 or 64
 template <typename T, int G, int N>
 static void launch_grad_as(hipStream_t s, const RouteArgs &a) {
     constexpr int ROWS = 256 / G;

@@ -3,7 +3,8 @@ dropout, and the gradients of these (the C entry points evt_route_rows, evt_rout
 evt_drop_rows; include/evotrees_hip.h has the formulas).
 
 They stand beside the losses over rows of class scores, the partition of rows by node (update_nodes_idx!, src/fit-utils.jl) and the random sample of rows: an expert may be
-a layer's that a router chooses for a language model's token, or a model of its own at a leaf that predict_leaf_idx finds for a table's row.  They have no counterpart in the reference.
+a layer's that a router chooses for a language model's token, or a model of its own at a leaf that predict_leaf_idx finds for a table's row: a column of what that returns, uint32
+on the host, goes to the GPU as int32 or int64, torch.from_numpy(leaf[:, k].astype("int64")).cuda().  They have no counterpart in the reference.
 
     experts, weights = route_rows(scores, 8)                    # (rows, 8) each
     plan = plan_rows(experts, n_experts)
@@ -16,7 +17,8 @@ a layer's that a router chooses for a language model's token, or a model of its 
 
 Rows are (rows, features) tensors of float32, bfloat16 or float16 whose features lie side by side (`x.stride(1) == 1`); rows may be any distance apart.  Weights and
 their gradients are contiguous float32.  All tensors of a call are on one GPU; the work is queued on that GPU's current stream and nothing waits for it.  As the gradients of
-this package's losses, these are returned, not recorded: results never require a gradient, and a call is its own backward pass's part as shown above.  `out` takes
+this package's losses, these are returned, not recorded: a call reads the values of its tensors, whether they require a gradient or carry a tangent or not, its results never do, and
+the backward pass is the program's to write, as shown above or in a torch.autograd.Function.  `out` takes
 a result: a tensor like it, which counts as changed in place.  It shares no memory with what the call reads but where a call says so; columns of one matrix, with equal
 strides, share none.
 

@@ -277,3 +277,26 @@ def test_leaves_of_a_tree(evt):
     plan = evt.plan_rows(ids, int(leaf[:, k].max()) + 1)
     place, source, offsets = plain.plan(ids.cpu()[:, None], plan.experts)
     assert plan.place.reshape(-1).tolist() == place and plan.source.tolist() == source and plan.offsets.tolist() == offsets and offsets[-1] == 500
+
+
+@pytest.mark.parametrize("mode", [torch.inference_mode, torch.no_grad])
+def test_a_layer_without_gradients(evt, mode):
+    """Scores that are one row in memory, results in place, tensors made in that mode and read outside of it."""
+    rows, experts, top, H = 30, 20, 3, 50
+    gen = torch.Generator().manual_seed(9)
+    one, x = torch.randn(1, experts, generator=gen), torch.randn(rows, H, generator=gen)
+    with mode():
+        scores, held = one.cuda().expand(rows, experts), x.cuda()
+        ids, w = evt.route_rows(scores, top, renormalize=False)
+        plan = evt.plan_rows(ids, experts)
+        y = evt.sort_rows(held, plan)
+        out = evt.combine_rows(y, plan, w, residual=held, out=held)
+        grads = evt.route_rows_grad(scores, ids, w, w, renormalize=False)
+    assert out is held
+    want, ww, tol = plain.route(one.expand(rows, experts), top, False, 1.0)
+    assert torch.equal(ids.cpu(), want)
+    plain.close("weights", w, ww, tol)
+    plain.close("out", out, *plain.combine(y.cpu(), plan.place.cpu(), w.cpu(), x, 0.0, 0, 0))
+    plain.close("grad", grads, *plain.route_grad(one.expand(rows, experts), want, w.cpu(), w.cpu(), False, 1.0))
+    again = evt.plan_rows(ids.clone(), experts)  # outside
+    assert torch.equal(again.place, plan.place) and not again.place.is_inference()
